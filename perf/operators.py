@@ -93,6 +93,8 @@ def draw(rng):
                 Sq = _log(rng, 1, 12000)
                 kind = rng.choice(["full", "causal", "prefix", "docs"])
                 Sk = Sq if kind == "docs" or rng.random() < 0.6 else _log(rng, max(1, Sq // 8), Sq * 4)
+                if train:       # a row of one key has no gradient but dv: keep more than such rows
+                    Sq, Sk = max(Sq, 4), max(Sk, 4)
                 B = max(1, _log(rng, 1, 64) if Sq <= 1024 else rng.randint(1, 3))
                 c = _attn("", dtype, train, B, Sq, Sk, Hq, Hk, D, causal=kind in ("causal", "prefix") or (kind == "docs" and cap > 0),
                           prefix=max(1, Sk // rng.randint(2, 5)) if kind == "prefix" else 0,
