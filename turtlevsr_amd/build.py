@@ -30,8 +30,9 @@ def hipcc() -> str:
 
 
 def _flags():
+    # packed fp32 arithmetic off: some forms of it have given wrong results on gfx950 now and then
     return ["-O3", "-std=c++17", "-fPIC", f"--offload-arch={ARCH}", "-munsafe-fp-atomics",
-            "-I", CSRC, "-I", os.path.join(REPO, "include")]
+            "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops", "-I", CSRC, "-I", os.path.join(REPO, "include")]
 
 
 def _compile(src: str, force: bool) -> str:
