@@ -1,0 +1,856 @@
+"""Token attention operators (turtlevsr_amd/token_ops.py): axial_rope, qk_norm_rope, attention, paged_attention
+against their definitions in fp64, gradients included, at the sizes and masks where such kernels go wrong.
+
+Tolerances are error bounds of the algorithm, element by element. u = eps / 2 of the type is one rounding. Scores are
+fp32 sums of D products: their error E is at most (D / 2 + 8) 2^-23 of the largest sum of |q k|, and p's relative error
+is E. With A = p |v|: |o - ref| <= (2 u + E) A (p rounded once, o rounded once). Likewise dv over p^T |do|; dq and dk add
+the absolute errors of dP and delta times p, through |k| and |q|: both are fp32 sums of D products, and delta = do . o takes
+the o that the rounded p gave (u A, before o's own rounding, whose remainder the kernel keeps: 2 u^2), so its error is
+(u + 2 u^2 + E) |do| . A besides.
+"""
+import math
+import os
+import re
+
+import pytest
+import torch
+
+from turtlevsr_amd import _lib, token_ops as T
+
+DEV = "cuda"
+DTYPES = [torch.float32, torch.bfloat16, torch.float16]
+REPO = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+
+
+def unit(dt):
+    return torch.finfo(dt).eps / 2
+
+
+def randn(*shape, dtype=torch.float32, seed=0, dev=DEV):
+    g = torch.Generator(device=dev).manual_seed(seed * 7919 + sum(shape))
+    return torch.randn(*shape, device=dev, generator=g).to(dtype)
+
+
+def within(got, ref, tol, what):
+    got = got.detach().double()
+    assert got.shape == ref.shape, what
+    assert torch.isfinite(got).all(), f"{what}: not finite"
+    bad = (got - ref).abs() > tol
+    if bad.any():
+        i = tuple(int(x) for x in bad.nonzero()[0])
+        t = tol.expand_as(ref)[i]
+        raise AssertionError(f"{what}: {int(bad.sum())} of {bad.numel()} out of bounds, first at {i}: {got[i]} for {ref[i]} (+- {t})")
+
+
+# -------------------------------------------------------------------------------------------------
+# definitions in fp64
+# -------------------------------------------------------------------------------------------------
+
+def rope_ref(x, pos, axes, base=10000.0, inverse=False):
+    B, S, H, D = x.shape
+    p = pos.double().expand(B, S, len(axes))
+    y = x.clone()
+    c = 0
+    for a, d in enumerate(axes):
+        for i in range(d // 2):
+            th = p[:, :, a] * base ** (-2.0 * i / d) * (-1 if inverse else 1)
+            co, si = th.cos()[:, :, None], th.sin()[:, :, None]
+            x0, x1 = x[..., c], x[..., c + 1]
+            y[..., c], y[..., c + 1] = x0 * co - x1 * si, x0 * si + x1 * co
+            c += 2
+    return y
+
+
+def visible_ref(B, Sq, Sk, causal=False, prefix=None, q_doc=None, k_doc=None, dev=DEV):
+    i, j = torch.arange(Sq, device=dev)[:, None] + (Sk - Sq), torch.arange(Sk, device=dev)[None]
+    vis = torch.ones(B, Sq, Sk, dtype=torch.bool, device=dev)
+    if causal:
+        vis &= (j <= i)[None]
+        if prefix is not None:
+            pre = torch.as_tensor(prefix, device=dev).expand(B)
+            vis |= j[None] < pre[:, None, None]
+    if q_doc is not None:
+        k_doc = q_doc if k_doc is None else k_doc
+        vis &= (q_doc[:, :, None] == k_doc[:, None, :]) & (q_doc[:, :, None] >= 0)
+    return vis
+
+
+def attn_ref(q, k, v, vis, scale=None, softcap=0.0, slopes=None, do=None, dist=None):
+    """Results and their error bounds from fp64 matrices: {"o": (ref, tol), "dq": ...}."""
+    dt = q.dtype
+    B, Sq, Hq, D = q.shape
+    Sk, Hk = k.shape[1], k.shape[2]
+    G = Hq // Hk
+    u = unit(dt)
+    scale = D ** -0.5 if scale is None else scale
+    # what no query may see is not part of the definition
+    seen = vis.any(1)[:, :, None, None]
+    rows = vis.any(2)[:, None, :, None]
+    f = lambda t: t.detach().double().permute(0, 2, 1, 3)
+    Q = torch.where(rows, f(q), 0.0)
+    K, V = (torch.where(seen.permute(0, 2, 1, 3), f(t), 0.0).repeat_interleave(G, 1) for t in (k, v))
+    raw = Q @ K.transpose(2, 3) * scale
+    mag = (Q.abs() @ K.abs().transpose(2, 3)).max() * abs(scale)
+    E = (D / 2 + 8) * 2.0 ** -23 * float(mag) + 2.0 ** -20
+    s = softcap * torch.tanh(raw / softcap) if softcap else raw
+    if softcap:
+        E += softcap * 2.0 ** -22
+    if slopes is not None:
+        if dist is None:
+            dist = (torch.arange(Sq, device=q.device)[:, None] + (Sk - Sq) - torch.arange(Sk, device=q.device)[None]).abs().double()[None, None]
+        pen = slopes.double().view(1, Hq, 1, 1) * dist
+        s = s - pen
+        E += float(torch.where(vis[:, None], pen, 0.0).max()) * 2.0 ** -22
+    m = vis[:, None]
+    s = s.masked_fill(~m, -math.inf)
+    p = torch.softmax(torch.where(rows, s, 0.0), -1) * rows * m
+    o = p @ V
+    out = {"o": (o, (2 * u + E) * (p @ V.abs()) + 1e-30)}
+    if do is not None:
+        g = torch.where(rows, f(do), 0.0)
+        dp = g @ V.transpose(2, 3)
+        delta = (g * o).sum(-1, keepdim=True)
+        dcap = 1 - torch.tanh(raw / softcap) ** 2 if softcap else 1.0
+        pd = p * (dp - delta)
+        ds = pd * dcap * scale
+        e32 = (D / 2 + 8) * 2.0 ** -23
+        edp = e32 * (g.abs() @ V.abs().transpose(2, 3))
+        edl = (e32 + u + 2 * u * u + 2 * E) * (g.abs() * (p @ V.abs())).sum(-1, keepdim=True)
+        eds = ((u + E + 2.0 ** -20) * pd.abs() + p * (edp + edl) + (2.0 ** -24 if dt == torch.float16 else 0.0) * m * rows) * abs(scale)
+        dq, dqt = ds @ K, eds @ K.abs() * (1 + 2 * u)
+        sums = lambda t: t.view(B, Hk, G, Sk, D).sum(2)
+        dk, dkt = sums(ds.transpose(2, 3) @ Q), sums(eds.transpose(2, 3) @ Q.abs()) * (1 + 2 * u)
+        dv, dvt = sums(p.transpose(2, 3) @ g), (2 * u + E) * sums(p.transpose(2, 3) @ g.abs())
+        floor = 2.0 ** -24 if dt == torch.float16 else 1e-30
+        out.update(dq=(dq, dqt + u * dq.abs() + floor), dk=(dk, dkt + u * dk.abs() + floor), dv=(dv, dvt + floor))
+    return {n: (a.permute(0, 2, 1, 3), b.permute(0, 2, 1, 3)) for n, (a, b) in out.items()}
+
+
+def check_attention(q, k, v, do=None, **kw):
+    vis = visible_ref(q.shape[0], q.shape[1], k.shape[1], kw.get("causal", False), kw.get("prefix"), kw.get("q_doc"), kw.get("k_doc"))
+    ref = attn_ref(q, k, v, vis, kw.get("scale"), kw.get("softcap", 0.0), kw.get("slopes"), do)
+    if do is None:
+        within(T.attention(q, k, v, **kw), *ref["o"], "o")
+        return
+    q, k, v = (t.detach().requires_grad_(True) for t in (q, k, v))
+    o = T.attention(q, k, v, **kw)
+    within(o, *ref["o"], "o")
+    for n, g in zip(("dq", "dk", "dv"), torch.autograd.grad(o, (q, k, v), do)):
+        within(g, *ref[n], n)
+
+
+# -------------------------------------------------------------------------------------------------
+# refusals and the C surface (no GPU)
+# -------------------------------------------------------------------------------------------------
+
+def test_token_exports_match_header():
+    hdr = open(os.path.join(REPO, "include", "turtle_token.h")).read()
+    declared = set(re.findall(r"\b(turtle_token_[a-z0-9_]+)\s*\(", hdr))
+    assert len(declared) == 8
+    L = _lib.lib()
+    for s in declared:
+        assert hasattr(L, s), s
+    T.lib()
+
+
+def test_c_entries_refuse_bad_arguments():
+    """Every entry returns an error for missing pointers and sizes out of range; none launches anything."""
+    L = T.lib()
+    s, ax = T._Side(), T._axes_table((8, 8, 8), 1e4)
+    assert L.turtle_token_rope(s, None, ax, None, 0, 0, 1, 1, 64, 0, 1, None) == -1
+    assert L.turtle_token_norm_rope_fwd(s, s, ax, None, 0, 0, 1, 1, 64, 1e-6, 1, None) == -1
+    assert L.turtle_token_norm_rope_bwd(s, s, ax, None, 0, 0, 1, 1, 64, 1e-6, None, None, 0, 1, None) == -1
+    assert L.turtle_token_norm_rope_workspace(0, 64) == 0
+    a, g = T._Attn(), T._Grads()
+    assert L.turtle_token_attn_fwd(a, 1, None) == -1 and L.turtle_token_attn_bwd(g, 1, None) == -1
+    assert L.turtle_token_attn_fwd(None, 1, None) == -1 and L.turtle_token_attn_bwd(None, 1, None) == -1
+    assert L.turtle_token_attn_workspace(a, 1) == 0 and L.turtle_token_attn_workspace(None, 1) == 0
+    a.B, a.Sq, a.Sk, a.Hq, a.Hk, a.D = 1, 1, 100, 4, 3, 64            # heads not a multiple
+    assert L.turtle_token_attn_fwd(a, 1, None) == -1
+    a.Hk, a.Sq, a.Hq = 1, 1 << 29, 4                                  # 2^31 rows
+    assert L.turtle_token_attn_workspace(a, 1) == 0 and L.turtle_token_attn_fwd(a, 1, None) == -1
+
+
+def _cpu(*shape, dtype=torch.bfloat16):
+    return torch.zeros(*shape, dtype=dtype)
+
+
+def test_rope_refusals():
+    x, pos = _cpu(2, 5, 3, 64), torch.zeros(5, 3, dtype=torch.int32)
+    ok = (16, 24, 24)
+    with pytest.raises(RuntimeError, match="ROCm device"):
+        T.axial_rope(x, pos, ok)
+    with pytest.raises(ValueError, match="S, heads, D"):
+        T.axial_rope(x[0], pos, ok)
+    with pytest.raises(TypeError):
+        T.axial_rope(x.double(), pos, ok)
+    with pytest.raises(ValueError, match="multiple of 8"):
+        T.axial_rope(x[..., :60], pos, (8, 8, 8))
+    with pytest.raises(ValueError, match="multiple of 8"):
+        T.axial_rope(_cpu(2, 5, 3, 136), pos, (8, 8, 8))
+    for axes in [(16, 24, 26), (15, 8, 8), (), (8,) * 5, (-2, 8, 8)]:
+        with pytest.raises(ValueError, match="axes"):
+            T.axial_rope(x, pos, axes)
+    with pytest.raises(ValueError, match="base"):
+        T.axial_rope(x, pos, ok, base=0.5)
+    with pytest.raises(TypeError, match="pos"):
+        T.axial_rope(x, pos.float(), ok)
+    for shape in [(5, 2), (4, 3), (3, 5, 3)]:
+        with pytest.raises(ValueError, match="pos"):
+            T.axial_rope(x, torch.zeros(*shape, dtype=torch.int64), ok)
+    k = _cpu(2, 5, 1, 64)
+    with pytest.raises(RuntimeError, match="ROCm device"):
+        T.qk_norm_rope(x, k, pos, None, None, ok)
+    with pytest.raises(ValueError, match="does not match"):
+        T.qk_norm_rope(x, k[:, :4], pos, None, None, ok)
+    with pytest.raises(TypeError, match="k is"):
+        T.qk_norm_rope(x, k.float(), pos, None, None, ok)
+    with pytest.raises(ValueError, match="q_weight"):
+        T.qk_norm_rope(x, k, pos, torch.zeros(32), None, ok)
+    with pytest.raises(TypeError, match="k_weight"):
+        T.qk_norm_rope(x, k, pos, None, torch.zeros(64, dtype=torch.int32), ok)
+    with pytest.raises(ValueError, match="eps"):
+        T.qk_norm_rope(x, k, pos, None, None, ok, eps=-1.0)
+
+
+def test_attention_refusals():
+    q, k = _cpu(2, 5, 4, 64), _cpu(2, 7, 2, 64)
+    with pytest.raises(RuntimeError, match="ROCm device"):
+        T.attention(q, k, k)
+    with pytest.raises(ValueError, match="not a multiple"):
+        T.attention(q, _cpu(2, 7, 3, 64), _cpu(2, 7, 3, 64))
+    with pytest.raises(ValueError, match="one shape"):
+        T.attention(q, k, k[:, :6])
+    with pytest.raises(ValueError, match="sequences"):
+        T.attention(q, k[:1], k[:1])
+    with pytest.raises(TypeError):
+        T.attention(q, k, k.float())
+    with pytest.raises(ValueError, match="prefix"):
+        T.attention(q, k, k, prefix=3)
+    with pytest.raises(ValueError, match="prefix"):
+        T.attention(q, k, k, causal=True, prefix=torch.zeros(3, dtype=torch.int32))
+    with pytest.raises(TypeError, match="prefix"):
+        T.attention(q, k, k, causal=True, prefix=torch.zeros(2))
+    with pytest.raises(ValueError, match="k_doc"):
+        T.attention(q, k, k, q_doc=torch.zeros(2, 5, dtype=torch.int32))
+    with pytest.raises(ValueError, match="k_doc"):
+        T.attention(q, k, k, k_doc=torch.zeros(2, 7, dtype=torch.int32))
+    with pytest.raises(TypeError, match="q_doc"):
+        T.attention(q, k, k, q_doc=torch.zeros(2, 5), k_doc=torch.zeros(2, 7))
+    for c in (-1.0, float("nan"), float("inf")):
+        with pytest.raises(ValueError, match="softcap"):
+            T.attention(q, k, k, softcap=c)
+    with pytest.raises(ValueError, match="scale"):
+        T.attention(q, k, k, scale=float("inf"))
+    with pytest.raises(ValueError, match="slopes"):
+        T.attention(q, k, k, slopes=torch.zeros(2))
+    with pytest.raises(TypeError, match="slopes"):
+        T.attention(q, k, k, slopes=torch.zeros(4, dtype=torch.int32))
+    with pytest.raises(ValueError, match="no gradient"):
+        T.attention(q, k, k, slopes=torch.zeros(4, requires_grad=True))
+
+
+def test_paged_refusals():
+    q, pool = _cpu(2, 1, 4, 64), _cpu(6, 16, 2, 64)
+    tab, kl = torch.zeros(2, 3, dtype=torch.int32), torch.zeros(2, dtype=torch.int32)
+    with pytest.raises(RuntimeError, match="ROCm device"):
+        T.paged_attention(q, pool, pool, tab, kl)
+    with pytest.raises(ValueError, match="block_table"):
+        T.paged_attention(q, pool, pool, tab[0], kl)
+    with pytest.raises(TypeError, match="block_table"):
+        T.paged_attention(q, pool, pool, tab.long(), kl)
+    with pytest.raises(TypeError, match="kv_lens"):
+        T.paged_attention(q, pool, pool, tab, kl.long())
+    with pytest.raises(ValueError, match="kv_lens"):
+        T.paged_attention(q, pool, pool, tab, kl[:1])
+    with pytest.raises(ValueError, match="q_lens"):
+        T.paged_attention(q, pool, pool, tab, kl, q_lens=kl[:1])
+    with pytest.raises(ValueError, match="one shape"):
+        T.paged_attention(q, pool, pool[:5], tab, kl)
+    with pytest.raises(RuntimeError, match="no gradient"):
+        T.paged_attention(q.requires_grad_(True), pool, pool, tab, kl)
+
+
+# -------------------------------------------------------------------------------------------------
+# rotation and norm
+# -------------------------------------------------------------------------------------------------
+
+def _grid(S, naxis, t0=0):
+    g = torch.Generator().manual_seed(S)
+    p = torch.randint(0, 50, (S, naxis), generator=g)
+    p[:, 0] += t0
+    return p.to(DEV)
+
+
+ROPES = [(1, 1, 1, (8,), 8, 0), (2, 7, 3, (2, 4, 2), 8, 5), (1, 33, 2, (16, 24, 24), 64, 100003), (3, 19, 5, (8, 16, 12), 40, -70000),
+         (2, 130, 9, (32, 48, 48), 128, 2000000000), (1, 5, 17, (0, 10, 0, 14), 24, 3), (1, 300, 1, (20,), 96, 1 << 20)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("B,S,H,axes,D,t0", ROPES)
+def test_axial_rope_matches_definition(dt, B, S, H, axes, D, t0):
+    """|y - ref| <= u |ref| + the angle's and functions' error (2^-20 in 16-bit types, 2^-22 in fp32) of the pair."""
+    x, dy = randn(B, S, H, D, dtype=dt, seed=1), randn(B, S, H, D, dtype=dt, seed=2)
+    err = 2.0 ** -22 if dt == torch.float32 else 2.0 ** -18
+    for pos in (_grid(S, len(axes), t0).to(torch.int32), torch.stack([_grid(S, len(axes), t0 + b) for b in range(B)]).long()):
+        leaf = x.detach().requires_grad_(True)
+        y = T.axial_rope(leaf, pos, axes)
+        (dx,) = torch.autograd.grad(y, leaf, dy)
+        for got, src, inv in ((y, x, False), (dx, dy, True)):
+            ref = rope_ref(src.double(), pos, axes, inverse=inv)
+            pair = src.double().abs()
+            pair = pair + pair.view(B, S, H, D // 2, 2).flip(-1).reshape(B, S, H, D)
+            within(got, ref, unit(dt) * ref.abs() + (err + unit(dt) * 2.0 ** -8) * pair, "dx" if inv else "y")
+        n = sum(axes)
+        assert torch.equal(y.detach()[..., n:], x[..., n:])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("B,S,Hq,Hk,axes,D", [(1, 1, 1, 1, (8,), 8), (2, 65, 4, 2, (16, 24, 24), 64), (3, 41, 6, 2, (8, 16, 12), 40),
+                                               (1, 700, 9, 3, (32, 48, 48), 128), (2, 257, 16, 16, (2, 2, 2), 16)])
+def test_qk_norm_rope_matches_definition(dt, B, S, Hq, Hk, axes, D):
+    """fp32 arithmetic, results rounded once: |y - ref| <= u |ref| + 2^-18 (16-bit) or 2^-20 of the pair's magnitude;
+    dx in terms of the magnitudes that cancel in it; dw is a sum of N terms in fp32: 2^-20 of the sum of |terms|
+    (blocked partial sums: under 64 roundings a path)."""
+    eps = 1e-6
+    err = 2.0 ** -20 if dt == torch.float32 else 2.0 ** -18
+    pos = _grid(S, len(axes), 1234)
+    qkv = randn(B, S, Hq + 2 * Hk, D, dtype=dt, seed=3)
+    wq, wk = 1 + 0.2 * randn(D, seed=4), 1 + 0.2 * randn(D, seed=5)
+    g = [randn(B, S, h, D, dtype=dt, seed=6 + h) for h in (Hq, Hk)]
+    q, k = qkv[:, :, :Hq].detach().requires_grad_(True), qkv[:, :, Hq:Hq + Hk].detach().requires_grad_(True)
+    lw = [w.clone().requires_grad_(True) for w in (wq, wk)]
+    out = T.qk_norm_rope(q, k, pos, *lw, axes, eps=eps)
+    grads = torch.autograd.grad(out, (q, k, *lw), g)
+    for n, x, w, y, dy, dx, dw in (("q", q, wq, out[0], g[0], grads[0], grads[2]), ("k", k, wk, out[1], g[1], grads[1], grads[3])):
+        X, W, H = x.detach().double(), w.double(), x.shape[2]
+        r = 1 / (X.pow(2).mean(-1, keepdim=True) + eps).sqrt()
+        swap = lambda t: t.abs() + t.abs().view(B, S, H, D // 2, 2).flip(-1).reshape(B, S, H, D)
+        ref = rope_ref(X * r * W, pos, axes)
+        within(y, ref, unit(dt) * ref.abs() + err * swap(X * r * W), n)
+        dz = rope_ref(dy.double(), pos, axes, inverse=True)
+        gw = dz * W
+        m = (gw * X * r).mean(-1, keepdim=True)
+        ref = r * (gw - X * r * m)
+        mag = r * (swap(dy.double()) * W.abs() + (X * r).abs() * (swap(dy.double()) * (W * X * r).abs()).mean(-1, keepdim=True))
+        within(dx, ref, unit(dt) * ref.abs() + err * mag, "d" + n)
+        terms = dz * X * r
+        within(dw, terms.sum((0, 1, 2)), err * (swap(dy.double()) * (X * r).abs()).sum((0, 1, 2)), "dw " + n)
+    assert torch.equal(T.qk_norm_rope(q, k, pos, wq, wk, axes)[0], out[0])
+
+
+@pytest.mark.gpu
+def test_qk_norm_rope_partial_gains_and_repeat():
+    """None for a gain is a gain of one; a gain in bf16 gets a bf16 gradient; repeats are bit-identical."""
+    q, k = randn(2, 100, 4, 64, dtype=torch.bfloat16, seed=1), randn(2, 100, 2, 64, dtype=torch.bfloat16, seed=2)
+    pos = _grid(100, 3)
+    one = torch.ones(64, device=DEV)
+    a = T.qk_norm_rope(q, k, pos, None, one, (16, 24, 24))
+    b = T.qk_norm_rope(q, k, pos, one, None, (16, 24, 24))
+    assert all(torch.equal(x, y) for x, y in zip(a, b))
+    w = one.bfloat16().requires_grad_(True)
+    ql = q.detach().requires_grad_(True)
+    runs = []
+    for _ in range(3):
+        y = T.qk_norm_rope(ql, k, pos, w, None, (16, 24, 24))
+        runs.append(torch.autograd.grad(y[0], (ql, w), a[0]))
+    assert runs[0][1].dtype == torch.bfloat16
+    for r in runs[1:]:
+        assert all(torch.equal(x, y) for x, y in zip(r, runs[0]))
+
+
+@pytest.mark.gpu
+def test_rope_empty_and_unaligned():
+    pos = _grid(6, 3)
+    for shape in [(0, 6, 2, 64), (2, 0, 2, 64)]:
+        x = torch.zeros(*shape, device=DEV, requires_grad=True)
+        y = T.axial_rope(x, pos[:shape[1]], (16, 24, 24))
+        assert y.shape == x.shape
+        q, k = T.qk_norm_rope(x, x, pos[:shape[1]], torch.ones(64, device=DEV, requires_grad=True), None, (16, 24, 24))
+        (q.sum() + k.sum()).backward()
+        assert x.grad.shape == x.shape
+    # rows that do not start at 16 bytes, heads before tokens, a transposed channel axis: same values
+    x = randn(2, 6, 2, 64, dtype=torch.bfloat16)
+    want = T.axial_rope(x, pos, (16, 24, 24))
+    odd = torch.empty(x.numel() + 1, dtype=x.dtype, device=DEV)[1:].view(x.shape).copy_(x)
+    swapped = x.transpose(1, 2).contiguous().transpose(1, 2)
+    chan = x.transpose(2, 3).contiguous().transpose(2, 3)
+    for y in (odd, swapped, chan):
+        assert torch.equal(T.axial_rope(y, pos, (16, 24, 24)), want)
+
+
+# -------------------------------------------------------------------------------------------------
+# attention
+# -------------------------------------------------------------------------------------------------
+
+SIZES = [(1, 1, 1, 1, 1, 8), (2, 1, 5, 2, 1, 64), (1, 2, 64, 4, 4, 64), (1, 33, 65, 2, 2, 40), (2, 64, 64, 4, 2, 64), (1, 129, 127, 3, 1, 128),
+         (1, 31, 200, 8, 1, 16), (2, 200, 31, 2, 2, 96), (1, 257, 511, 2, 1, 72)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("B,Sq,Sk,Hq,Hk,D", SIZES)
+@pytest.mark.parametrize("kind", ["full", "causal", "prefix", "bias_cap"])
+def test_attention_and_gradients(dt, B, Sq, Sk, Hq, Hk, D, kind):
+    q, k, v = (randn(B, s, h, D, dtype=dt, seed=i) for i, (s, h) in enumerate(((Sq, Hq), (Sk, Hk), (Sk, Hk))))
+    do = randn(B, Sq, Hq, D, dtype=dt, seed=9)
+    kw = {"full": {}, "causal": dict(causal=True), "prefix": dict(causal=True, prefix=torch.tensor([Sk // 3 + b for b in range(B)], device=DEV)),
+          "bias_cap": dict(softcap=2.0, slopes=torch.linspace(0.01, 0.5, Hq, device=DEV))}[kind]
+    check_attention(q, k, v, do, **kw)
+
+
+def _docs(B, S, seed, pad):
+    g = torch.Generator().manual_seed(seed)
+    n = torch.randint(1, max(2, S // 4), (B, S), generator=g)
+    d = torch.zeros(B, S, dtype=torch.int64)
+    for b in range(B):
+        ids = torch.repeat_interleave(torch.arange(S), n[b])[:S - pad]
+        d[b, :S - pad] = ids
+        d[b, S - pad:] = -1
+    return d.to(DEV)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("B,S,Hq,Hk,D,pad,causal", [(1, 1, 1, 1, 64, 0, False), (2, 70, 4, 2, 64, 9, False), (1, 300, 2, 1, 128, 70, True),
+                                                     (1, 700, 2, 2, 64, 0, False), (3, 20, 2, 1, 32, 20, True), (1, 1100, 1, 1, 48, 130, True)])
+def test_attention_documents_hide_padding_that_holds_nan(dt, B, S, Hq, Hk, D, pad, causal):
+    q, k, v = (randn(B, S, h, D, dtype=dt, seed=i) for i, h in enumerate((Hq, Hk, Hk)))
+    do = randn(B, S, Hq, D, dtype=dt, seed=9)
+    doc = _docs(B, S, S, pad)
+    for t in (q, k, v, do):
+        t[doc < 0] = float("nan")
+    if pad:
+        q[:, -1], v[:, -1] = float("inf"), float("-inf")
+    check_attention(q, k, v, do, q_doc=doc, causal=causal, softcap=0.0 if S == 70 else 3.0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16])
+def test_attention_documents_out_of_order_and_cross(dt):
+    """Numbers in any order, query numbers that no key has, keys against another clip's queries."""
+    q, k, v = randn(2, 150, 4, 64, dtype=dt, seed=1), randn(2, 333, 2, 64, dtype=dt, seed=2), randn(2, 333, 2, 64, dtype=dt, seed=3)
+    g = torch.Generator().manual_seed(4)
+    qd = torch.randint(-1, 5, (2, 150), generator=g).to(DEV)
+    kd = torch.randint(-1, 4, (2, 333), generator=g).to(DEV, torch.int32)
+    check_attention(q, k, v, randn(2, 150, 4, 64, dtype=dt, seed=5), q_doc=qd, k_doc=kd)
+    qd[0], kd[1] = 7, 9                        # nothing matches at all
+    check_attention(q, k, v, randn(2, 150, 4, 64, dtype=dt, seed=5), q_doc=qd, k_doc=kd)
+    # few rows over many tiles of documents
+    q1, qd1 = q[:, :3].contiguous(), torch.tensor([[2, 0, 3], [1, 1, 6]], device=DEV)
+    kd2 = torch.arange(333, device=DEV).div(60, rounding_mode="floor").expand(2, 333)
+    check_attention(q1, k, v, randn(2, 3, 4, 64, dtype=dt, seed=6), q_doc=qd1, k_doc=kd2)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("Sq,Sk", [(1, 9000), (5, 3001), (40, 5000), (700, 2100)])
+@pytest.mark.parametrize("dt", DTYPES)
+def test_attention_few_rows_over_many_keys(dt, Sq, Sk):
+    """The keys split over blocks and joined."""
+    q, k, v = randn(1, Sq, 4, 64, dtype=dt, seed=1), randn(1, Sk, 2, 64, dtype=dt, seed=2), randn(1, Sk, 2, 64, dtype=dt, seed=3)
+    do = randn(1, Sq, 4, 64, dtype=dt, seed=4)
+    check_attention(q, k, v, do)
+    check_attention(q, k, v, do, causal=True, slopes=torch.tensor([0.3, 0.02, 0.001, 0.0], device=DEV))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", DTYPES)
+def test_attention_large_scores_and_scales(dt):
+    """Scores in the hundreds (a one-hot softmax), a negative scale, a scale of zero, one key far above the rest late."""
+    q, k, v = randn(1, 100, 2, 64, dtype=dt, seed=1), randn(1, 300, 2, 64, dtype=dt, seed=2), randn(1, 300, 2, 64, dtype=dt, seed=3)
+    do = randn(1, 100, 2, 64, dtype=dt, seed=4)
+    for scale in (3.0, -0.125, 0.0):
+        check_attention(q, k, v, do, scale=scale)
+    k2 = k.clone()
+    k2[:, 290] *= 16
+    check_attention(q, k2, v, do)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16])
+def test_attention_strides_and_broadcast(dt):
+    """Slices of a channels-last projection, heads-first layouts, a key shared by expand (its gradient is the sum), a
+    gradient that arrives expanded."""
+    B, H, W, heads, D = 2, 6, 7, 2, 64
+    S = H * W
+    qkv = randn(B, 3 * heads * D, H, W, dtype=dt, seed=1).to(memory_format=torch.channels_last)
+    q, k, v = qkv.permute(0, 2, 3, 1).reshape(B, S, 3, heads, D).unbind(2)
+    assert q.data_ptr() == qkv.data_ptr()
+    do = randn(B, S, heads, D, dtype=dt, seed=2)
+    check_attention(q, k, v, do)
+    hf = lambda t: t.transpose(1, 2).contiguous().transpose(1, 2)
+    check_attention(hf(q), hf(k), hf(v), hf(do))
+    k1 = randn(1, S, heads, D, dtype=dt, seed=3).requires_grad_(True)
+    o = T.attention(q, k1.expand(B, -1, -1, -1), v)
+    (gk,) = torch.autograd.grad(o, k1, do)
+    kf = k1.detach().expand(B, -1, -1, -1).contiguous().requires_grad_(True)
+    (gf,) = torch.autograd.grad(T.attention(q, kf, v), kf, do)
+    assert torch.equal(gk, gf.sum(0, keepdim=True))
+    ql = q.detach().requires_grad_(True)
+    (a,) = torch.autograd.grad(T.attention(ql, k, v).sum(), ql)
+    (b,) = torch.autograd.grad(T.attention(ql, k, v), ql, torch.ones_like(do))
+    assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+def test_attention_rows_past_32_bit_offsets():
+    """Token strides that put the last keys 5 GB behind the first."""
+    S, D, stride = 40001, 64, 65536
+    big = torch.empty(S * stride, dtype=torch.bfloat16, device=DEV)
+    k = big.as_strided((1, S, 1, D), (0, stride, D, 1))
+    v = big.as_strided((1, S, 1, D), (0, stride, D, 1), D)
+    k.copy_(randn(1, S, 1, D, dtype=torch.bfloat16, seed=1))
+    v.copy_(randn(1, S, 1, D, dtype=torch.bfloat16, seed=2))
+    q = randn(1, 3, 2, D, dtype=torch.bfloat16, seed=3)
+    do = randn(1, 3, 2, D, dtype=torch.bfloat16, seed=4)
+    check_attention(q, k, v, do)
+
+
+@pytest.mark.gpu
+def test_attention_no_tokens():
+    for Sq, Sk in ((0, 5), (5, 0), (0, 0)):
+        q, k = torch.zeros(2, Sq, 2, 64, device=DEV, requires_grad=True), torch.ones(2, Sk, 2, 64, device=DEV, requires_grad=True)
+        o = T.attention(q, k, k)
+        assert o.shape == q.shape and not o.any()
+        o.sum().backward()
+        assert q.grad.shape == q.shape and k.grad.shape == k.shape and not q.grad.any() and not k.grad.any()
+
+
+@pytest.mark.gpu
+def test_attention_gradient_against_differences():
+    """fp32: the directional derivative of sum(do o) along random directions, by central differences in fp64 of the
+    definition and from the kernel's gradients."""
+    B, Sq, Sk, Hq, Hk, D = 1, 9, 14, 2, 1, 16
+    q, k, v = (randn(B, s, h, D, seed=i) for i, (s, h) in enumerate(((Sq, Hq), (Sk, Hk), (Sk, Hk))))
+    do, kw = randn(B, Sq, Hq, D, seed=5), dict(causal=True, softcap=1.5)
+    leaves = [t.requires_grad_(True) for t in (q, k, v)]
+    grads = torch.autograd.grad(T.attention(*leaves, **kw), leaves, do)
+
+    def value(ts):
+        qd, kd, vd = (t.double().transpose(1, 2) for t in ts)
+        z = qd @ kd.repeat_interleave(Hq // Hk, 1).transpose(2, 3) * D ** -0.5
+        z = 1.5 * torch.tanh(z / 1.5)
+        z = z.masked_fill(~visible_ref(B, Sq, Sk, True)[:, None], -math.inf)
+        return float((torch.softmax(z, -1) @ vd.repeat_interleave(Hq // Hk, 1) * do.double().transpose(1, 2)).sum())
+
+    for i in range(3):
+        d = randn(*leaves[i].shape, seed=20 + i).double()
+        h = 1e-5
+        at = lambda s: [t.detach().double() + (s * h * d if j == i else 0) for j, t in enumerate(leaves)]
+        diff = (value(at(1)) - value(at(-1))) / (2 * h)
+        got = float((grads[i].double() * d).sum())
+        assert abs(got - diff) <= 1e-5 * float((grads[i].double() * d).abs().sum()) + 1e-7
+
+
+@pytest.mark.gpu
+def test_attention_repeats_bit_for_bit_and_only_wanted_gradients():
+    q, k, v = (randn(2, 500, h, 64, dtype=torch.bfloat16, seed=h) for h in (4, 2, 2))
+    do = randn(2, 500, 4, 64, dtype=torch.bfloat16, seed=9)
+    leaves = [t.requires_grad_(True) for t in (q, k, v)]
+    first = torch.autograd.grad(T.attention(*leaves, causal=True), leaves, do)
+    for _ in range(3):
+        again = torch.autograd.grad(T.attention(*leaves, causal=True), leaves, do)
+        assert all(torch.equal(a, b) for a, b in zip(first, again))
+    (dq,) = torch.autograd.grad(T.attention(q, k.detach(), v.detach(), causal=True), q, do)
+    (dv,) = torch.autograd.grad(T.attention(q.detach(), k.detach(), v, causal=True), v, do)
+    assert torch.equal(dq, first[0]) and torch.equal(dv, first[2])
+
+
+# -------------------------------------------------------------------------------------------------
+# pages
+# -------------------------------------------------------------------------------------------------
+
+def _pages(B, lens, page, Hk, D, dt, spare=2, seed=0):
+    """(k_pages, v_pages, table, dense k, dense v): random page order; everything past a length is NaN."""
+    M = max(1, max(-(-n // page) for n in lens))
+    n = B * M + spare
+    kp, vp = (torch.full((n, page, Hk, D), float("nan"), dtype=dt, device=DEV) for _ in range(2))
+    table = torch.randperm(n, generator=torch.Generator().manual_seed(seed))[:B * M].reshape(B, M).to(torch.int32)
+    k, v = randn(B, max(1, max(lens)), Hk, D, dtype=dt, seed=seed + 1), randn(B, max(1, max(lens)), Hk, D, dtype=dt, seed=seed + 2)
+    for b in range(B):
+        for j in range(0, lens[b], page):
+            e = min(page, lens[b] - j)
+            kp[table[b, j // page], :e], vp[table[b, j // page], :e] = k[b, j:j + e], v[b, j:j + e]
+        table[b, -(-lens[b] // page):] = -1
+    return kp, vp, table.to(DEV), k, v
+
+
+def check_paged(q, kp, vp, table, kl, k, v, ql=None, hidden=None, **kw):
+    """hidden: bool [B, keys], keys that nobody sees (bad pages)."""
+    B, Sq = q.shape[:2]
+    klt = torch.tensor(kl, dtype=torch.int32, device=DEV)
+    qlt = None if ql is None else torch.tensor(ql, dtype=torch.int32, device=DEV)
+    got = T.paged_attention(q, kp, vp, table, klt, q_lens=qlt, **kw)
+    i, j = torch.arange(Sq, device=DEV), torch.arange(k.shape[1], device=DEV)
+    nq = torch.tensor([Sq] * B if ql is None else ql, device=DEV).clamp(0, Sq)
+    at = i[None] + (klt.long() - nq)[:, None]
+    vis = (j[None, None] < klt.long()[:, None, None]) & (i[None, :, None] < nq[:, None, None])
+    if kw.get("causal", True):
+        vis &= j[None, None] <= at[:, :, None]
+    if hidden is not None:
+        vis &= ~hidden[:, None]
+    dist = (at[:, :, None] - j).abs().double()[:, None]
+    ref = attn_ref(q, k, v, vis, kw.get("scale"), kw.get("softcap", 0.0), kw.get("slopes"), dist=dist)
+    within(got, *ref["o"], "o")
+    return got
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("page,D", [(1, 64), (16, 64), (7, 40), (64, 128), (100, 64), (256, 96)])
+def test_paged_single_tokens(dt, page, D):
+    lens = [1, 2, 63, 64, 65, 301, 777, 0]
+    kp, vp, table, k, v = _pages(len(lens), lens, page, 2, D, dt, seed=page)
+    q = randn(len(lens), 1, 8, D, dtype=dt, seed=5)
+    check_paged(q, kp, vp, table, lens, k, v)
+    check_paged(q, kp, vp, table, lens, k, v, causal=False, softcap=2.0, slopes=torch.linspace(0, 0.3, 8, device=DEV))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("Sq,causal", [(5, True), (37, True), (200, True), (200, False), (130, True)])
+def test_paged_chunks_of_ragged_lengths(dt, Sq, causal):
+    lens, ql = [Sq, 400, 3 * Sq, 1, 0, 350], [Sq, Sq, max(1, Sq // 2), 1, 0, 0]
+    kp, vp, table, k, v = _pages(6, lens, 48, 2, 64, dt, seed=Sq)
+    q = randn(6, Sq, 4, 64, dtype=dt, seed=6)
+    for b in range(6):
+        q[b, ql[b]:] = float("nan")
+    check_paged(q, kp, vp, table, lens, k, v, ql, causal=causal)
+
+
+@pytest.mark.gpu
+def test_paged_long_history_is_split_and_pool_passes_32_bits():
+    """One token over 20000 keys on pages at the far end of a pool of 6 GB; 2 sequences whose first is tiny."""
+    page, Hk, D = 256, 4, 128
+    n = 6 * (1 << 30) // (page * Hk * D * 2)
+    kp = torch.empty(n, page, Hk, D, dtype=torch.bfloat16, device=DEV)
+    vp = torch.empty(n, page, Hk, D, dtype=torch.bfloat16, device=DEV)
+    lens = [3, 20000]
+    M = -(-lens[1] // page)
+    k, v = randn(2, lens[1], Hk, D, dtype=torch.bfloat16, seed=1), randn(2, lens[1], Hk, D, dtype=torch.bfloat16, seed=2)
+    table = torch.stack([torch.arange(M), n - 1 - torch.arange(M)]).to(DEV, torch.int32)
+    for b in range(2):
+        pad = torch.zeros(M * page - lens[1], Hk, D, dtype=torch.bfloat16, device=DEV)
+        kp[table[b].long()] = torch.cat((k[b], pad)).view(M, page, Hk, D)
+        vp[table[b].long()] = torch.cat((v[b], pad)).view(M, page, Hk, D)
+    check_paged(randn(2, 1, 16, D, dtype=torch.bfloat16, seed=3), kp, vp, table, lens, k, v)
+
+
+def test_paged_bad_pages_are_outside_the_pools_on_paper():
+    """The kernel takes a page number as unsigned and compares it with the pool's size before any address is made:
+    -1, the pool's size and the extremes all fail that comparison."""
+    for bad in (-1, 10, 2 ** 31 - 1, -2 ** 31):
+        assert (bad & 0xffffffff) >= 10
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("Sq", [1, 50])
+def test_paged_bad_pages_and_lengths(Sq):
+    """Page numbers outside the pools hide their keys; lengths past the table's room are cut to it."""
+    page, lens = 16, [100, 64]
+    kp, vp, table, k, v = _pages(2, lens, page, 1, 64, torch.bfloat16, seed=3)
+    hidden = torch.zeros(2, 100, dtype=torch.bool, device=DEV)
+    for b, j, bad in ((0, 0, -1), (0, 3, kp.shape[0]), (1, 2, 2 ** 31 - 1), (1, 1, -2 ** 31)):
+        table[b, j] = bad
+        hidden[b, j * page:(j + 1) * page] = True
+    q = randn(2, Sq, 2, 64, dtype=torch.bfloat16, seed=4)
+    check_paged(q, kp, vp, table, lens, k, v, hidden=hidden, causal=False)
+    check_paged(q, kp, vp, table, lens, k, v, hidden=hidden)
+    cut = table[:, :4].contiguous()               # room for 64 keys of 100
+    hidden[:, 64:] = True
+    check_paged(q, kp, vp, cut, lens, k, v, hidden=hidden, causal=False)
+    none = T.paged_attention(q, kp, vp, table, torch.tensor([-5, 0], dtype=torch.int32, device=DEV))
+    assert not none.any()
+
+
+@pytest.mark.gpu
+def test_paged_equals_attention_on_a_dense_history():
+    """A chunk over pages gives what attention gives for the same rows (both causal with the last query at the last key)."""
+    kp, vp, table, k, v = _pages(2, [300, 300], 64, 2, 64, torch.float32, seed=1)
+    q = randn(2, 40, 4, 64, seed=2)
+    a = T.attention(q, k, v, causal=True)
+    b = T.paged_attention(q, kp, vp, table, torch.tensor([300, 300], dtype=torch.int32, device=DEV))
+    within(b, a.double(), torch.full((1,), 1e-5, dtype=torch.float64, device=DEV), "o")
+
+
+# -------------------------------------------------------------------------------------------------
+# together, streams, graphs
+# -------------------------------------------------------------------------------------------------
+
+def _block(qkv, pos, wq, wk, heads, D, **kw):
+    """The attention of a transformer block over a channels-last map [B, 3 heads D, H, W]."""
+    B, _, H, W = qkv.shape
+    q, k, v = qkv.permute(0, 2, 3, 1).reshape(B, H * W, 3, heads, D).unbind(2)
+    q, k = T.qk_norm_rope(q, k, pos, wq, wk, (D // 4 // 2 * 2, D // 8 * 2, D // 8 * 2))
+    return T.attention(q, k, v, **kw), k, v
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16])
+def test_block_trains_through_all_operators(dt):
+    """Norm, rotation and attention in one graph: the gradients of the map and the gains against autograd on the fp64
+    definitions. Tolerance: the chain rounds q', k' (u each, which moves scores by u sum|q k| scale) and every gradient
+    once, so a relative error (Frobenius) under 16 u plus the fp32 arithmetic's 1e-5."""
+    B, H, W, heads, D = 2, 5, 9, 2, 64
+    ax = (D // 4 // 2 * 2, D // 8 * 2, D // 8 * 2)
+    qkv = randn(B, 3 * heads * D, H, W, dtype=dt, seed=1).to(memory_format=torch.channels_last).requires_grad_(True)
+    pos = _grid(H * W, 3)
+    wq, wk = (1 + 0.1 * randn(D, seed=2)).requires_grad_(True), (1 + 0.1 * randn(D, seed=3)).requires_grad_(True)
+    do = randn(B, H * W, heads, D, dtype=dt, seed=4)
+    o, _, _ = _block(qkv, pos, wq, wk, heads, D, causal=True, prefix=9)
+    got = torch.autograd.grad(o, (qkv, wq, wk), do)
+
+    x, a, b = (t.detach().double().requires_grad_(True) for t in (qkv, wq, wk))
+    q, k, v = x.permute(0, 2, 3, 1).reshape(B, H * W, 3, heads, D).unbind(2)
+    def nr(t, w):
+        z = t / (t.pow(2).mean(-1, keepdim=True) + 1e-6).sqrt() * w
+        c, parts = 0, []
+        for i, d in enumerate(ax):
+            th = pos[:, i, None].double() * 10000.0 ** (-torch.arange(0, d, 2, device=DEV, dtype=torch.float64) / d)
+            z0, z1 = z[..., c:c + d:2], z[..., c + 1:c + d:2]
+            co, si = th.cos()[:, None], th.sin()[:, None]
+            parts.append(torch.stack((z0 * co - z1 * si, z0 * si + z1 * co), -1).flatten(-2))
+            c += d
+        return torch.cat(parts + [z[..., c:]], -1)
+    q, k = nr(q, a).transpose(1, 2), nr(k, b).transpose(1, 2)
+    s = (q @ k.transpose(2, 3) * D ** -0.5).masked_fill(~visible_ref(B, H * W, H * W, True, 9)[:, None], -math.inf)
+    ref = (torch.softmax(s, -1) @ v.transpose(1, 2)).transpose(1, 2)
+    want = torch.autograd.grad(ref, (x, a, b), do.double())
+    tol = 16 * unit(dt) + 1e-5
+    for n, g, r in zip(("o", "dqkv", "dwq", "dwk"), (o, *got), (ref, *want)):
+        rel = float((g.detach().double() - r.detach()).norm() / r.detach().norm())
+        assert rel <= tol, (n, rel)
+
+
+@pytest.mark.gpu
+def test_serving_frames_over_a_paged_history():
+    """Frame by frame with a page for each frame equals the whole clip at once: tokens of a frame see all of their own
+    and of earlier frames (a document per prefix is the frame-causal mask, here by keys up to the frame's end)."""
+    heads, D, n, frames = 2, 64, 30, 4
+    qkv = randn(1, frames * n, 3, heads, D, dtype=torch.bfloat16, seed=1)
+    pos = torch.stack((torch.arange(frames).repeat_interleave(n), torch.arange(n).repeat(frames)), 1).to(DEV)
+    w = 1 + 0.1 * randn(D, seed=2)
+    q, k = T.qk_norm_rope(qkv[:, :, 0], qkv[:, :, 1], pos, w, w, (32, 32))
+    v = qkv[:, :, 2]
+    kp, vp = torch.full((6, n, heads, D), float("nan"), dtype=torch.bfloat16, device=DEV), torch.full((6, n, heads, D), float("nan"), dtype=torch.bfloat16, device=DEV)
+    table = torch.tensor([[4, 0, 5, 2]], dtype=torch.int32, device=DEV)
+    for f in range(frames):
+        sl = slice(f * n, (f + 1) * n)
+        qf, kf = T.qk_norm_rope(qkv[:, sl, 0], qkv[:, sl, 1], pos[sl], w, w, (32, 32))
+        assert torch.equal(qf, q[:, sl]) and torch.equal(kf, k[:, sl])
+        kp[table[0, f].long()], vp[table[0, f].long()] = kf[0], v[0, sl]
+        o = T.paged_attention(qf, kp, vp, table, torch.tensor([(f + 1) * n], dtype=torch.int32, device=DEV), causal=False)
+        e = (f + 1) * n
+        ref = attn_ref(q[:, sl], k[:, :e], v[:, :e], torch.ones(1, n, e, dtype=torch.bool, device=DEV))
+        within(o, *ref["o"], f"frame {f}")
+
+
+@pytest.mark.gpu
+def test_operators_on_another_stream():
+    q, k, v = (randn(1, 300, 2, 64, dtype=torch.bfloat16, seed=i) for i in range(3))
+    pos = _grid(300, 3)
+    want = T.attention(*T.qk_norm_rope(q, k, pos, None, None, (16, 24, 24)), v)
+    st = torch.cuda.Stream()
+    st.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(st):
+        got = T.attention(*T.qk_norm_rope(q, k, pos, None, None, (16, 24, 24)), v)
+    torch.cuda.current_stream().wait_stream(st)
+    assert torch.equal(got, want)
+
+
+@pytest.mark.gpu
+def test_inference_in_a_graph_follows_its_inputs():
+    """A captured step - rotation, cache write, paged attention, dense attention with documents - replayed with other
+    tokens, lengths, tables and documents, with eager work between the replays."""
+    B, heads, D, page, M = 3, 2, 64, 16, 8
+    kp, vp = torch.zeros(B * M, page, heads, D, dtype=torch.bfloat16, device=DEV), torch.zeros(B * M, page, heads, D, dtype=torch.bfloat16, device=DEV)
+    x = randn(B, 1, 3, heads, D, dtype=torch.bfloat16, seed=1)
+    pos = torch.zeros(B, 1, 1, dtype=torch.int32, device=DEV)
+    table = torch.arange(B * M, device=DEV, dtype=torch.int32).view(B, M)
+    lens = torch.ones(B, dtype=torch.int32, device=DEV)
+    seq = randn(1, 600, 3, heads, D, dtype=torch.bfloat16, seed=2)
+    doc = torch.zeros(1, 600, dtype=torch.int32, device=DEV)
+
+    def step():
+        q, k = T.qk_norm_rope(x[:, :, 0], x[:, :, 1], pos, None, None, (64,))
+        slot = table.gather(1, (pos[:, :, 0] // page).long()).long() * page + pos[:, :, 0] % page
+        kp.view(-1, heads, D).index_copy_(0, slot[:, 0], k[:, 0])
+        vp.view(-1, heads, D).index_copy_(0, slot[:, 0], x[:, 0, 2])
+        return T.paged_attention(q, kp, vp, table, lens), T.attention(seq[:, :, 0], seq[:, :, 1], seq[:, :, 2], q_doc=doc)
+
+    with torch.no_grad():
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            step()
+        torch.cuda.current_stream().wait_stream(side)
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = step()
+        for n in range(20):
+            x.copy_(randn(B, 1, 3, heads, D, dtype=torch.bfloat16, seed=100 + n))
+            pos.fill_(n)
+            lens.fill_(n + 1)
+            doc.copy_((torch.arange(600, device=DEV) // (50 + 10 * n))[None])
+            g.replay()
+            got = [t.clone() for t in out]
+            torch.cuda.synchronize()
+            want = step()
+            assert all(torch.equal(a, b) for a, b in zip(got, want)), n
+
+
+@pytest.mark.gpu
+def test_training_step_in_a_graph():
+    """Forward and backward captured together, replayed on other data; two graphs of their own do not disturb each other."""
+    def make(seed):
+        leaves = [randn(1, 333, 2, 64, dtype=torch.bfloat16, seed=seed + i).requires_grad_(True) for i in range(3)]
+        w = torch.ones(64, device=DEV, requires_grad=True)
+        do, pos = randn(1, 333, 2, 64, dtype=torch.bfloat16, seed=seed + 5), _grid(333, 2)
+
+        def step():
+            q, k = T.qk_norm_rope(leaves[0], leaves[1], pos, w, None, (32, 32))
+            o = T.attention(q, k, leaves[2], causal=True, softcap=5.0)
+            return (o.detach(),) + torch.autograd.grad(o, (*leaves, w), do)
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            step()
+        torch.cuda.current_stream().wait_stream(side)
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = step()
+        return leaves, do, g, out, step
+    a, b = make(1), make(50)
+    for n in range(4):
+        for leaves, do, g, out, step in (a, b):
+            with torch.no_grad():
+                for i, t in enumerate(leaves):
+                    t.copy_(randn(*t.shape, dtype=t.dtype, seed=200 + n * 10 + i))
+        a[2].replay()
+        b[2].replay()
+        torch.cuda.synchronize()
+        for leaves, do, g, out, step in (a, b):
+            got = [t.detach().clone() for t in out]
+            assert all(torch.equal(x, y.detach()) for x, y in zip(got, step()))
+
+
+@pytest.mark.gpu
+def test_op_set_takes_the_autocast_type():
+    """HipOps, the training graph's op set: fp32 tensors under bf16 autocast give the bf16 call's results."""
+    from turtlevsr_amd.train_ops import HipOps
+    q, k, v = (randn(1, 50, 2, 64, seed=i) for i in range(3))
+    b = [t.bfloat16() for t in (q, k, v)]
+    pos = _grid(50, 3)
+    ax = (16, 24, 24)
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        x = HipOps.axial_rope(q, pos, ax)
+        y = HipOps.qk_norm_rope(q, k, pos, None, None, ax)
+        z = HipOps.attention(q, k, v, causal=True)
+        table, lens = torch.zeros(1, 1, dtype=torch.int32, device=DEV), torch.tensor([50], dtype=torch.int32, device=DEV)
+        p = HipOps.paged_attention(q, b[1], b[2], table, lens)
+    assert torch.equal(x, T.axial_rope(b[0], pos, ax))
+    assert all(torch.equal(a, c) for a, c in zip(y, T.qk_norm_rope(b[0], b[1], pos, None, None, ax)))
+    assert torch.equal(z, T.attention(*b, causal=True)) and torch.equal(p, T.paged_attention(b[0], b[1], b[2], table, lens))
+    assert HipOps.attention(q, k, v).dtype == torch.float32

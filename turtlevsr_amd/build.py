@@ -18,7 +18,7 @@ REPO = os.path.dirname(PKG)
 CSRC = os.path.join(PKG, "csrc")
 OBJ = os.path.join(PKG, "build")
 LIB = os.path.join(PKG, "lib", "libturtle_hip.so")
-SOURCES = ["gemm.hip", "gemm2.hip", "gemm3.hip", "gemm5.hip", "spatial.hip", "attn.hip", "sab.hip", "fused.hip", "fused2.hip", "dwgemm.hip", "tilepd.hip", "gffn.hip", "gemm8.hip", "gemm9.hip", "gemm_f32.hip", "gemm_sk.hip", "ffn.hip", "t0.hip", "train_ops.hip", "turtle.cpp"]
+SOURCES = ["gemm.hip", "gemm2.hip", "gemm3.hip", "gemm5.hip", "spatial.hip", "attn.hip", "sab.hip", "fused.hip", "fused2.hip", "dwgemm.hip", "tilepd.hip", "gffn.hip", "gemm8.hip", "gemm9.hip", "gemm_f32.hip", "gemm_sk.hip", "ffn.hip", "t0.hip", "train_ops.hip", "token.hip", "token_attn.hip", "turtle.cpp"]
 ARCH = os.environ.get("TURTLE_OFFLOAD_ARCH", "gfx950")
 
 
@@ -39,7 +39,7 @@ def _compile(src: str, force: bool) -> str:
     obj = os.path.join(OBJ, src + ".o")
     path = os.path.join(CSRC, src)
     deps = [path] + [os.path.join(CSRC, h) for h in os.listdir(CSRC) if h.endswith(".h")]
-    deps.append(os.path.join(REPO, "include", "turtle_hip.h"))
+    deps += [os.path.join(REPO, "include", h) for h in ("turtle_hip.h", "turtle_train.h", "turtle_token.h")]
     if not force and os.path.exists(obj) and os.path.getmtime(obj) >= max(os.path.getmtime(d) for d in deps):
         return obj
     cmd = [hipcc()] + _flags() + ["-x", "hip", "-c", path, "-o", obj]

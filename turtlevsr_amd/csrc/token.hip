@@ -1,0 +1,405 @@
+// Rotary positions over several axes, alone and behind a per-head RMS norm, forward and backward
+// (include/turtle_token.h).
+//
+//   z = x r w, r = 1 / sqrt(mean(x^2) + eps)          (norm of a (token, head) row over its D channels)
+//   y = R z: channel pair i of the row turns by pos[axis_i] f_i
+//   backward: dz = R^T dy, g = dz w, dx = r (g - x r^2 mean(g x)), dw = sum over rows of dz x r
+//
+// Bound: HBM - x in, y out (backward: x, dy in, dx out) and nothing in between. A row of D channels sits on
+// D / 8 lanes (rounded up to a power of two), 8 channels a lane, so the norm's sums are a few DPP steps. A
+// thread keeps ONE token and channel chunk and walks over the heads of q and k: the angles (4 pairs a lane) are
+// computed once for all of them.
+//
+// Angles: f_i is a 64-bit fixed-point number of revolutions per position, so pos * f_i wraps exactly and
+// position 10^6 is as precise as position 0 (fp32 products would be off by 0.06 rad there).
+#include "common.h"
+#include "../../include/turtle_token.h"
+
+#include <algorithm>
+
+namespace turtle {
+namespace {
+
+typedef turtle_token_side Side;
+typedef turtle_token_axes Axes;
+
+constexpr int NTHR = 256;
+constexpr int UF = 4;             // rows a thread has in flight, forward
+constexpr int UB = 2;             // ... backward (two inputs each)
+constexpr int MAXB = 1024;        // blocks of the backward: its dw partials are one row of 2 D floats a block
+
+TURTLE_DEV void ld8(const float* p, float (&v)[8]) {
+  const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
+  v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+}
+TURTLE_DEV void ld8(const bf16* p, float (&v)[8]) {
+  const uint4 q = *reinterpret_cast<const uint4*>(p);
+  const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) { v[2 * i] = __uint_as_float(w[i] << 16); v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u); }
+}
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+TURTLE_DEV void ld8(const f16* p, float (&v)[8]) {
+  const f16x8 q = *reinterpret_cast<const f16x8*>(p);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = (float)q[i];
+}
+TURTLE_DEV void st8(float* p, const float (&v)[8]) {
+  *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+  *reinterpret_cast<float4*>(p + 4) = make_float4(v[4], v[5], v[6], v[7]);
+}
+TURTLE_DEV void st8(bf16* p, const float (&v)[8]) {
+  bf16x8 o;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) o[i] = (bf16)v[i];
+  *reinterpret_cast<bf16x8*>(p) = o;
+}
+TURTLE_DEV void st8(f16* p, const float (&v)[8]) {
+  f16x8 o;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) o[i] = (f16)v[i];
+  *reinterpret_cast<f16x8*>(p) = o;
+}
+
+// sine and cosine of hi / 2^32 revolutions. 16-bit results: the hardware functions (they take revolutions; their
+// error is far under the results' rounding). fp32: the nearest quarter turn is split off exactly, the rest, at
+// most pi / 4, goes through the Taylor polynomials up to x^9 and x^10 (truncation under 4e-9).
+template <typename T>
+TURTLE_DEV void sincos_rev(uint32_t hi, float& s, float& c) {
+  if constexpr (sizeof(T) == 2) {
+    const float t = (float)(int32_t)hi * 2.3283064365386963e-10f;
+    s = __builtin_amdgcn_sinf(t);
+    c = __builtin_amdgcn_cosf(t);
+  } else {
+    const uint32_t q = (hi + 0x20000000u) >> 30;
+    const float x = (float)(int32_t)(hi - (q << 30)) * (6.283185307179586f * 2.3283064365386963e-10f), u = x * x;
+    const float sx = x * fmaf(u, fmaf(u, fmaf(u, fmaf(u, 1.f / 362880.f, -1.f / 5040.f), 1.f / 120.f), -1.f / 6.f), 1.f);
+    const float cx = fmaf(u, fmaf(u, fmaf(u, fmaf(u, fmaf(u, -1.f / 3628800.f, 1.f / 40320.f), -1.f / 720.f), 1.f / 24.f), -0.5f), 1.f);
+    const float a = (q & 1) ? cx : sx, b = (q & 1) ? sx : cx;
+    s = (q & 2) ? -a : a;
+    c = ((q + 1) & 2) ? -b : b;
+  }
+}
+
+// sum over aligned groups of 2^LB lanes (LB <= 4), in every lane of the group
+template <int LB>
+TURTLE_DEV float row_sum(float v) {
+  if constexpr (LB >= 1) v += __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), 0xB1, 0xF, 0xF, true));    // lane ^ 1
+  if constexpr (LB >= 2) v += __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), 0x4E, 0xF, 0xF, true));    // lane ^ 2
+  if constexpr (LB >= 3) v += __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), 0x141, 0xF, 0xF, true));   // mirror of 8
+  if constexpr (LB >= 4) v += __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), 0x140, 0xF, 0xF, true));   // mirror of 16
+  return v;
+}
+
+struct RopeArgs {
+  Side s[2];
+  Axes ax;
+  const void* pos;
+  int64_t pos_b, S, N;       // N = B * S tokens
+  int D, hs;                 // hs: threads (a power of two) that share a token's heads
+  int pos64;
+  float eps, sign;
+  float* part;               // backward: [gridDim.x][2][D] or NULL
+};
+
+// a lane's place: its chunk of 8 channels, its share of the heads, its token within the block's step
+struct Place {
+  int c, h0, tok, step;
+  bool on;
+  template <int LB>
+  TURTLE_DEV static Place of(const RopeArgs& a) {
+    Place p;
+    const int slot = threadIdx.x >> LB;
+    p.c = (threadIdx.x & ((1 << LB) - 1)) * 8;
+    p.on = p.c < a.D;
+    p.h0 = slot & (a.hs - 1);
+    p.tok = slot / a.hs;
+    p.step = (NTHR >> LB) / a.hs;
+    return p;
+  }
+};
+
+struct Turn {
+  uint64_t f[4];
+  int ax[4];
+  bool rot[4];
+  float s[4], c[4];
+  TURTLE_DEV void init(const Axes& t, int c0) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int p = (c0 >> 1) + i;
+      rot[i] = p < t.npair;
+      f[i] = rot[i] ? t.freq[p] : 0;
+      ax[i] = rot[i] ? t.axis[p] : 0;
+    }
+  }
+  template <typename T>
+  TURTLE_DEV void at(const RopeArgs& a, int64_t n) {
+    const int64_t b = a.pos_b ? n / a.S : 0;
+    const int64_t o = a.pos_b ? b * a.pos_b + (n - b * a.S) * a.ax.naxis : (n % a.S) * a.ax.naxis;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int64_t p = a.pos64 ? reinterpret_cast<const int64_t*>(a.pos)[o + ax[i]] : (int64_t)reinterpret_cast<const int32_t*>(a.pos)[o + ax[i]];
+      sincos_rev<T>((uint32_t)(((uint64_t)p * f[i]) >> 32), s[i], c[i]);
+    }
+  }
+  // channels that are not rotated pass unchanged, whatever they hold
+  TURTLE_DEV void apply(float (&v)[8], float sign) const {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float x0 = v[2 * i], x1 = v[2 * i + 1], sn = s[i] * sign;
+      v[2 * i] = rot[i] ? x0 * c[i] - x1 * sn : x0;
+      v[2 * i + 1] = rot[i] ? x0 * sn + x1 * c[i] : x1;
+    }
+  }
+};
+
+template <typename T, bool NORM, int LB>
+__global__ __launch_bounds__(NTHR) void rope_kernel(RopeArgs a) {
+  const Place p = Place::of<LB>(a);
+  const int HT = a.s[0].H + a.s[1].H;
+  Turn tn;
+  tn.init(a.ax, p.c);
+  float w[2][8];
+  if constexpr (NORM) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) w[i][e] = (p.on && a.s[i].w) ? a.s[i].w[p.c + e] : 1.f;
+  }
+  const float invD = 1.f / (float)a.D;
+  for (int64_t n = (int64_t)blockIdx.x * p.step + p.tok; n < a.N; n += (int64_t)gridDim.x * p.step) {
+    const int64_t b = n / a.S, t = n - b * a.S;
+    tn.at<T>(a, n);
+    for (int h0 = p.h0; h0 < HT; h0 += UF * a.hs) {
+      float v[UF][8];
+#pragma unroll
+      for (int u = 0; u < UF; ++u) {
+        const int h = h0 + u * a.hs, k = h >= a.s[0].H ? 1 : 0;
+        if (h < HT && p.on) {
+          const Side& sd = a.s[k];
+          ld8(reinterpret_cast<const T*>(sd.x) + b * sd.sb + t * sd.ss + (int64_t)(h - (k ? a.s[0].H : 0)) * sd.sh + p.c, v[u]);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[u][e] = 0.f;
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < UF; ++u) {
+        const int h = h0 + u * a.hs, k = h >= a.s[0].H ? 1 : 0;
+        if constexpr (NORM) {
+          float ss = 0.f;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) ss = fmaf(v[u][e], v[u][e], ss);
+          const float r = 1.f / sqrtf(fmaf(row_sum<LB>(ss), invD, a.eps));
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[u][e] *= r * (k ? w[1][e] : w[0][e]);
+        }
+        tn.apply(v[u], a.sign);
+        if (h < HT && p.on) st8(reinterpret_cast<T*>(a.s[k].y) + (n * a.s[k].H + (h - (k ? a.s[0].H : 0))) * a.D + p.c, v[u]);
+      }
+    }
+  }
+}
+
+template <typename T, int LB>
+__global__ __launch_bounds__(NTHR) void norm_rope_bwd_kernel(RopeArgs a) {
+  const Place p = Place::of<LB>(a);
+  const int HT = a.s[0].H + a.s[1].H;
+  Turn tn;
+  tn.init(a.ax, p.c);
+  float w[2][8], dw[2][8];
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) { w[i][e] = (p.on && a.s[i].w) ? a.s[i].w[p.c + e] : 1.f; dw[i][e] = 0.f; }
+  const float invD = 1.f / (float)a.D;
+  for (int64_t n = (int64_t)blockIdx.x * p.step + p.tok; n < a.N; n += (int64_t)gridDim.x * p.step) {
+    const int64_t b = n / a.S, t = n - b * a.S;
+    tn.at<T>(a, n);
+    for (int h0 = p.h0; h0 < HT; h0 += UB * a.hs) {
+      float x[UB][8], g[UB][8];
+#pragma unroll
+      for (int u = 0; u < UB; ++u) {
+        const int h = h0 + u * a.hs, k = h >= a.s[0].H ? 1 : 0;
+        if (h < HT && p.on) {
+          const Side& sd = a.s[k];
+          const int64_t hl = h - (k ? a.s[0].H : 0);
+          ld8(reinterpret_cast<const T*>(sd.x) + b * sd.sb + t * sd.ss + hl * sd.sh + p.c, x[u]);
+          ld8(reinterpret_cast<const T*>(sd.dy) + b * sd.gb + t * sd.gs + hl * sd.gh + p.c, g[u]);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) x[u][e] = g[u][e] = 0.f;
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < UB; ++u) {
+        const int h = h0 + u * a.hs, k = h >= a.s[0].H ? 1 : 0;
+        tn.apply(g[u], -1.f);
+        float ss = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) ss = fmaf(x[u][e], x[u][e], ss);
+        const float sum = row_sum<LB>(ss);
+        const float r = h < HT ? 1.f / sqrtf(fmaf(sum, invD, a.eps)) : 0.f;
+        float dot = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          x[u][e] *= r;
+          const float d = g[u][e] * x[u][e];
+          dw[0][e] += k ? 0.f : d;
+          dw[1][e] += k ? d : 0.f;
+          g[u][e] *= k ? w[1][e] : w[0][e];
+          dot = fmaf(g[u][e], x[u][e], dot);
+        }
+        const float m = row_sum<LB>(dot) * invD;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) g[u][e] = r * (g[u][e] - x[u][e] * m);
+        if (h < HT && p.on) st8(reinterpret_cast<T*>(a.s[k].y) + (n * a.s[k].H + (h - (k ? a.s[0].H : 0))) * a.D + p.c, g[u]);
+      }
+    }
+  }
+  if (!a.part) return;
+  // the block's dw: over its slots in a fixed order
+  __shared__ float red[NTHR * 8];
+  for (int k = 0; k < 2; ++k) {
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < 8; ++e) red[threadIdx.x * 8 + e] = dw[k][e];
+    __syncthreads();
+    if ((int)threadIdx.x < a.D) {
+      float s = 0.f;
+      for (int i = 0; i < (NTHR >> LB); ++i) s += red[(i << LB) * 8 + threadIdx.x];
+      a.part[((int64_t)blockIdx.x * 2 + k) * a.D + threadIdx.x] = s;
+    }
+  }
+}
+
+// dw[c] = sum over the blocks' partials: 8 columns of 2 D a block, 32 threads a column
+__global__ __launch_bounds__(NTHR) void dw_sum_kernel(const float* __restrict__ part, float* __restrict__ dw, int nblk, int cols) {
+  __shared__ float red[NTHR];
+  const int col = blockIdx.x * 8 + (threadIdx.x & 7), r0 = threadIdx.x >> 3;
+  float s = 0.f;
+  for (int r = r0; r < nblk; r += 32) s += part[(int64_t)r * cols + col];
+  red[threadIdx.x] = s;
+  __syncthreads();
+  if (threadIdx.x < 8) {
+    float t = 0.f;
+    for (int i = 0; i < 32; ++i) t += red[i * 8 + threadIdx.x];
+    dw[col] = t;
+  }
+}
+
+bool side_ok(const Side* s, int D, int es, bool bwd) {
+  auto al = [&](int64_t st) { return (st * es) % 16 == 0; };
+  if (!s->x || !s->y || s->H <= 0 || ((uintptr_t)s->x | (uintptr_t)s->y) % 16 || !al(s->sb) || !al(s->ss) || !al(s->sh)) return false;
+  return !bwd || (s->dy && (uintptr_t)s->dy % 16 == 0 && al(s->gb) && al(s->gs) && al(s->gh));
+}
+
+// channel lanes of a row: log2 of D / 8 rounded up to a power of two
+int lane_bits(int D) { int lb = 0; while ((8 << lb) < D) ++lb; return lb; }
+
+bool fill(RopeArgs& r, const Side* a, const Side* b, const Axes* axes, const void* pos, int64_t pos_b, int pos64, int64_t B, int64_t S,
+          int D, int dtype, bool bwd, int unroll) {
+  if (!a || !axes || !pos || B <= 0 || S <= 0 || D <= 0 || D % 8 || D > 128 || dtype < 0 || dtype > 2) return false;
+  const int es = dtype == 0 ? 4 : 2;
+  if (!side_ok(a, D, es, bwd) || (b && b->x && !side_ok(b, D, es, bwd))) return false;
+  if (axes->npair < 0 || 2 * axes->npair > D || axes->naxis < 1 || axes->naxis > 4) return false;
+  for (int i = 0; i < axes->npair; ++i)
+    if (axes->axis[i] >= axes->naxis) return false;
+  r = RopeArgs{};
+  r.s[0] = *a;
+  if (b && b->x) r.s[1] = *b;
+  r.ax = *axes;
+  r.pos = pos; r.pos_b = pos_b; r.pos64 = pos64;
+  r.S = S; r.N = B * S; r.D = D;
+  // heads dealt so that a thread has about `unroll` rows: they share its angles and are in flight together
+  const int slots = NTHR >> lane_bits(D), HT = r.s[0].H + r.s[1].H;
+  int hs = 1;
+  while (hs < slots && hs * unroll < HT) hs *= 2;
+  r.hs = hs;
+  return true;
+}
+
+unsigned blocks_for(const RopeArgs& r) {
+  const int64_t step = (NTHR >> lane_bits(r.D)) / r.hs;
+  return (unsigned)std::min<int64_t>((r.N + step - 1) / step, 1 << 16);
+}
+
+template <typename T, bool NORM>
+void launch_rope(const RopeArgs& r, hipStream_t st) {
+  const unsigned g = blocks_for(r);
+  switch (lane_bits(r.D)) {
+    case 0: rope_kernel<T, NORM, 0><<<g, NTHR, 0, st>>>(r); break;
+    case 1: rope_kernel<T, NORM, 1><<<g, NTHR, 0, st>>>(r); break;
+    case 2: rope_kernel<T, NORM, 2><<<g, NTHR, 0, st>>>(r); break;
+    case 3: rope_kernel<T, NORM, 3><<<g, NTHR, 0, st>>>(r); break;
+    default: rope_kernel<T, NORM, 4><<<g, NTHR, 0, st>>>(r); break;
+  }
+}
+template <typename T>
+void launch_bwd(const RopeArgs& r, unsigned g, hipStream_t st) {
+  switch (lane_bits(r.D)) {
+    case 0: norm_rope_bwd_kernel<T, 0><<<g, NTHR, 0, st>>>(r); break;
+    case 1: norm_rope_bwd_kernel<T, 1><<<g, NTHR, 0, st>>>(r); break;
+    case 2: norm_rope_bwd_kernel<T, 2><<<g, NTHR, 0, st>>>(r); break;
+    case 3: norm_rope_bwd_kernel<T, 3><<<g, NTHR, 0, st>>>(r); break;
+    default: norm_rope_bwd_kernel<T, 4><<<g, NTHR, 0, st>>>(r); break;
+  }
+}
+
+}  // namespace
+}  // namespace turtle
+
+using namespace turtle;
+
+extern "C" {
+
+int turtle_token_rope(const turtle_token_side* a, const turtle_token_side* b, const turtle_token_axes* axes, const void* pos,
+                      int64_t pos_b, int pos64, int64_t B, int64_t S, int D, int inverse, int dtype, void* stream) {
+  RopeArgs r;
+  if (!fill(r, a, b, axes, pos, pos_b, pos64, B, S, D, dtype, false, UF)) return -1;
+  r.sign = inverse ? -1.f : 1.f;
+  hipStream_t st = (hipStream_t)stream;
+  if (dtype == 0) launch_rope<float, false>(r, st);
+  else if (dtype == 1) launch_rope<bf16, false>(r, st);
+  else launch_rope<f16, false>(r, st);
+  return (int)hipGetLastError();
+}
+
+int turtle_token_norm_rope_fwd(const turtle_token_side* a, const turtle_token_side* b, const turtle_token_axes* axes,
+                               const void* pos, int64_t pos_b, int pos64, int64_t B, int64_t S, int D, float eps, int dtype,
+                               void* stream) {
+  RopeArgs r;
+  if (!fill(r, a, b, axes, pos, pos_b, pos64, B, S, D, dtype, false, UF)) return -1;
+  r.sign = 1.f;
+  r.eps = eps;
+  hipStream_t st = (hipStream_t)stream;
+  if (dtype == 0) launch_rope<float, true>(r, st);
+  else if (dtype == 1) launch_rope<bf16, true>(r, st);
+  else launch_rope<f16, true>(r, st);
+  return (int)hipGetLastError();
+}
+
+size_t turtle_token_norm_rope_workspace(int64_t tokens, int D) {
+  if (tokens <= 0 || D <= 0) return 0;
+  return (size_t)std::min<int64_t>(tokens, MAXB) * 2 * D * sizeof(float);
+}
+
+int turtle_token_norm_rope_bwd(const turtle_token_side* a, const turtle_token_side* b, const turtle_token_axes* axes,
+                               const void* pos, int64_t pos_b, int pos64, int64_t B, int64_t S, int D, float eps, float* dw,
+                               void* ws, size_t ws_bytes, int dtype, void* stream) {
+  RopeArgs r;
+  if (!fill(r, a, b, axes, pos, pos_b, pos64, B, S, D, dtype, true, UB)) return -1;
+  const unsigned g = std::min<unsigned>(blocks_for(r), MAXB);
+  if (dw && (!ws || ws_bytes < (size_t)g * 2 * D * sizeof(float))) return -1;
+  r.eps = eps;
+  r.part = dw ? (float*)ws : nullptr;
+  hipStream_t st = (hipStream_t)stream;
+  if (dtype == 0) launch_bwd<float>(r, g, st);
+  else if (dtype == 1) launch_bwd<bf16>(r, g, st);
+  else launch_bwd<f16>(r, g, st);
+  if (dw) dw_sum_kernel<<<2 * D / 8, NTHR, 0, st>>>((const float*)ws, dw, (int)g, 2 * D);
+  return (int)hipGetLastError();
+}
+
+}  // extern "C"

@@ -1097,3 +1097,25 @@ class HipOps:
         """[b, heads, ch, ch] Gram of the L2-normalised (over HW) q and k, the first / second half of
         qk's channels (``sink`` as in conv1x1)."""
         return _NormGram.apply(_act(qk), heads, sink)
+
+    # token attention (turtlevsr_amd/token_ops.py): the same calls with activations in the autocast dtype
+
+    @staticmethod
+    def axial_rope(x, pos, axes, base: float = 10000.0):
+        from . import token_ops
+        return token_ops.axial_rope(_act(x), pos, axes, base)
+
+    @staticmethod
+    def qk_norm_rope(q, k, pos, q_weight, k_weight, axes, base: float = 10000.0, eps: float = 1e-6):
+        from . import token_ops
+        return token_ops.qk_norm_rope(_act(q), _act(k), pos, q_weight, k_weight, axes, base, eps)
+
+    @staticmethod
+    def attention(q, k, v, **kw):
+        from . import token_ops
+        return token_ops.attention(_act(q), _act(k), _act(v), **kw)
+
+    @staticmethod
+    def paged_attention(q, k_pages, v_pages, block_table, kv_lens, **kw):
+        from . import token_ops
+        return token_ops.paged_attention(_act(q).to(k_pages.dtype), k_pages, v_pages, block_table, kv_lens, **kw)
