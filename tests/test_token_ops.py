@@ -156,19 +156,25 @@ def test_token_exports_match_header():
 def test_c_entries_refuse_bad_arguments():
     """Every entry returns an error for missing pointers and sizes out of range; none launches anything."""
     L = T.lib()
-    s, ax = T._Side(), T._axes_table((8, 8, 8), 1e4)
+    s, ax = bytes(T._SIDE.size), T._axes_table((8, 8, 8), 1e4)
     assert L.turtle_token_rope(s, None, ax, None, 0, 0, 1, 1, 64, 0, 1, None) == -1
     assert L.turtle_token_norm_rope_fwd(s, s, ax, None, 0, 0, 1, 1, 64, 1e-6, 1, None) == -1
     assert L.turtle_token_norm_rope_bwd(s, s, ax, None, 0, 0, 1, 1, 64, 1e-6, None, None, 0, 1, None) == -1
     assert L.turtle_token_norm_rope_workspace(0, 64) == 0
-    a, g = T._Attn(), T._Grads()
-    assert L.turtle_token_attn_fwd(a, 1, None) == -1 and L.turtle_token_attn_bwd(g, 1, None) == -1
+
+    def args(B, Sq, Sk, Hq, Hk, D):
+        a = [0] * (len(T._ATTN.unpack(bytes(T._ATTN.size))))
+        a[12:18] = B, Sq, Sk, Hq, Hk, D
+        return T._ATTN.pack(*a)
+    none = args(0, 0, 0, 0, 0, 0)
+    assert L.turtle_token_attn_fwd(none, 1, None) == -1 and L.turtle_token_attn_bwd(none + bytes(T._GRADS.size), 1, None) == -1
     assert L.turtle_token_attn_fwd(None, 1, None) == -1 and L.turtle_token_attn_bwd(None, 1, None) == -1
-    assert L.turtle_token_attn_workspace(a, 1) == 0 and L.turtle_token_attn_workspace(None, 1) == 0
-    a.B, a.Sq, a.Sk, a.Hq, a.Hk, a.D = 1, 1, 100, 4, 3, 64            # heads not a multiple
-    assert L.turtle_token_attn_fwd(a, 1, None) == -1
-    a.Hk, a.Sq, a.Hq = 1, 1 << 29, 4                                  # 2^31 rows
-    assert L.turtle_token_attn_workspace(a, 1) == 0 and L.turtle_token_attn_fwd(a, 1, None) == -1
+    assert L.turtle_token_attn_workspace(none, 1) == 0 and L.turtle_token_attn_workspace(None, 1) == 0
+    assert L.turtle_token_attn_fwd(args(1, 1, 100, 4, 3, 64), 1, None) == -1           # heads not a multiple
+    assert L.turtle_token_attn_fwd(args(1, 1, 100, 4, 1, 60), 1, None) == -1           # channels
+    assert L.turtle_token_attn_fwd(args(1, 1, 100, 4, 1, 64), 1, None) == -1           # no tensors
+    big = args(1, 1 << 29, 100, 4, 1, 64)                                              # 2^31 rows
+    assert L.turtle_token_attn_workspace(big, 1) == 0 and L.turtle_token_attn_fwd(big, 1, None) == -1
 
 
 def _cpu(*shape, dtype=torch.bfloat16):

@@ -1,0 +1,396 @@
+// Token attention: capped, biased and masked softmax(q k^T) v over clips of tokens, its backward, and the same
+// forward over a paged cache (include/turtle_token.h).
+//
+// Rows. The G = Hq / Hk query heads that share a key head are rows of ONE problem: row m = i G + g is query i of
+// head hk G + g, so keys and values are read once for all of them and a single new token of 8 sharing heads still
+// fills 8 of a wave's 32 columns.
+//
+// One pass, everything in registers. A wave owns 32 rows. It computes S^T = K Q^T with 32x32 matrix instructions
+// (keys x rows): a lane then holds scores of ONE row (row = lane & 31), so the softmax's running maximum, sum and
+// rescaling factor are one register each and the maximum over keys is in-lane but for one exchange with lane ^ 32.
+// The probabilities leave the accumulator layout as the B operand of O^T = V^T P^T: 8 consecutive accumulator
+// registers of a lane are the keys 16 s + {4 h .. 4 h + 3, 8 + 4 h .. 8 + 4 h + 3} (h = lane >> 5), and any order of
+// the contraction is right as long as V^T is read in the same one - which is what the transposing LDS read gives in
+// two 4-key pieces. Nothing is exchanged through memory between the two products.
+//
+// Tiles of BN keys of K and V go HBM -> LDS by LDS-DMA, two buffers, the next tile in flight behind the current
+// one's products. LDS rows are not padded (the DMA writes lane-linear): 16-byte chunk c of row r sits at chunk
+// c ^ swz(r), applied on the DMA's source address, so that both the row reads (K: 32 rows, one chunk) and the
+// transposing reads (V: 4 rows, 4 chunks) touch distinct banks.
+//
+// Backward, two kernels and no atomics, so results do not depend on the launch's order:
+//   dk, dv: a wave owns 32 keys and walks over the rows: S = Q K^T, dP = dO V^T (rows x keys, lane = key), then
+//           dV^T += dO^T P and dK^T += Q^T dS with the same register-to-operand step as above;
+//   dq:     a wave owns 32 rows and walks over the keys: S^T, dP^T (lane = row), dQ^T += K^T dS^T.
+//   delta_i = do_i . o_i uses o with its rounding remainder (o_lo): a row whose few keys make dP - delta cancel
+//   would otherwise get 16-bit noise as its gradient.
+//
+// What is rounded: p and dS to the inputs' type as operands of the second products (fp16: p times 2^10, so that
+// 1 / 10^4 keeps its bits), results at the end; scores, maxima, sums and accumulators are fp32.
+#pragma once
+#include "common.h"
+#include "../../include/turtle_token.h"
+
+#include <algorithm>
+#include <type_traits>
+
+
+namespace turtle {
+namespace {
+
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+typedef __attribute__((address_space(3))) char lds_char;
+
+__device__ __attribute__((aligned(64))) uint4 g_zero_ta[4];   // source of rows and channels that are not there
+
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr int RT = 64;            // tokens of a document-range tile
+
+template <typename T> TURTLE_DEV f32x16 mma(uint4 a, uint4 b, f32x16 c);
+template <> TURTLE_DEV f32x16 mma<bf16>(uint4 a, uint4 b, f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+template <> TURTLE_DEV f32x16 mma<f16>(uint4 a, uint4 b, f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+// fp32: a 16-byte chunk pair is 8 channels, contracted two at a time in the order (e, 4 + e)
+template <> TURTLE_DEV f32x16 mma<float>(uint4 a, uint4 b, f32x16 c) {
+  c = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(a.x), __uint_as_float(b.x), c, 0, 0, 0);
+  c = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(a.y), __uint_as_float(b.y), c, 0, 0, 0);
+  c = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(a.z), __uint_as_float(b.z), c, 0, 0, 0);
+  return __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(a.w), __uint_as_float(b.w), c, 0, 0, 0);
+}
+
+// accumulator register r of a 32x32 tile: its row (0..31) is acc_row(r) + 4 (lane >> 5)
+constexpr TURTLE_DEV int acc_row(int r) { return 8 * (r >> 2) + (r & 3); }
+
+TURTLE_DEV f32x16 zero16() {
+  f32x16 z;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) z[i] = 0.f;
+  return z;
+}
+
+// combine over lane ^ 32
+TURTLE_DEV float half_max(float v) { return fmaxf(v, __shfl_xor(v, 32, 64)); }
+TURTLE_DEV float half_sum(float v) { return v + __shfl_xor(v, 32, 64); }
+
+TURTLE_DEV uint32_t lds_addr(const char* p) { return (uint32_t)(uintptr_t)(const lds_char*)p; }
+
+// 64 lanes x 16 B -> LDS (see gemm9.hip): inline asm, because the compiler would drain a builtin DMA before every
+// LDS read; waited for by vm_wait
+TURTLE_DEV void dma16(const void* gp, uint32_t lds_wave_base) {
+  unsigned keep;
+  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off\n\ts_mov_b32 m0, %0"
+               : "=&s"(keep) : "v"(gp), "s"(lds_wave_base) : "memory");
+}
+// at most N vector-memory operations of this wave still in flight
+template <int N>
+TURTLE_DEV void vm_wait() {
+  static_assert(N >= 0 && N < 64, "vmcnt range");
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+// all of this wave's LDS accesses done, then the block's barrier
+TURTLE_DEV void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+// A tile of rows of DP channels (zero past D) in LDS
+template <typename T, int DP>
+struct Rows {
+  static constexpr int ES = sizeof(T), ROWB = DP * ES, CH = ROWB / 16, STEPS = ROWB / 32;
+  static constexpr int DT = DP / 32;
+  // the chunk exchange of row r: bijective over 16 rows (row reads), and over 4 rows in steps of 4 chunks
+  // (transposing reads); 128-byte rows alternate between the two halves of the banks by themselves
+  TURTLE_DEV static int swz(int r) {
+    if constexpr (CH == 8) return (((r >> 1) & 1) << 2) | ((r >> 2) & 3);
+    else return ((r & 3) << 2) | ((r >> 2) & 3);
+  }
+  // row r's 16-byte chunk c
+  TURTLE_DEV static uint4 chunk(const char* t, int r, int c) { return *reinterpret_cast<const uint4*>(t + r * ROWB + ((c ^ swz(r)) << 4)); }
+  // acc[w] = (32 rows from r0)(channels) x frag[w]: frag is the B operand's STEPS chunks
+  template <int RW>
+  TURTLE_DEV static void times(const char* t, int r0, const uint4 (&frag)[RW][STEPS], f32x16 (&acc)[RW], int lane) {
+#pragma unroll
+    for (int w = 0; w < RW; ++w) acc[w] = zero16();
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s) {
+      const uint4 x = chunk(t, r0 + (lane & 31), 2 * s + (lane >> 5));
+#pragma unroll
+      for (int w = 0; w < RW; ++w) acc[w] = mma<T>(x, frag[w][s], acc[w]);
+    }
+  }
+  // acc[w][dt] += (rows r0 .. r0 + 15)^T (channels 32 dt ..) x p[w]: p = 8 accumulator registers' values of those rows.
+  // TWO: p in two terms (its rounding and the remainder), for products that keep p's fp32 value (16-bit types)
+  template <int RW, bool TWO>
+  TURTLE_DEV static void t_times(const char* t, int r0, const float (&p)[RW][8], f32x16 (&acc)[RW][DT], int lane) {
+    const int h = lane >> 5;
+    if constexpr (ES == 2) {
+      uint4 hi[RW], lo[RW];
+#pragma unroll
+      for (int w = 0; w < RW; ++w) {
+        hi[w] = pack(p[w]);
+        if constexpr (TWO) lo[w] = rest(p[w], hi[w]);
+      }
+      const int li = lane & 15, row = r0 + 4 * h + (li >> 2), sub = ((lane >> 4) & 1) * 2 + ((li & 3) >> 1);
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) {
+        const char* a = t + row * ROWB + (((dt * 4 + sub) ^ swz(row)) << 4) + (li & 1) * 8;
+        const char* b = t + (row + 8) * ROWB + (((dt * 4 + sub) ^ swz(row + 8)) << 4) + (li & 1) * 8;
+        const uint2 x = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)a));
+        const uint2 y = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)b));
+        const uint4 v = make_uint4(x.x, x.y, y.x, y.y);
+#pragma unroll
+        for (int w = 0; w < RW; ++w) {
+          acc[w][dt] = mma<T>(v, hi[w], acc[w][dt]);
+          if constexpr (TWO) acc[w][dt] = mma<T>(v, lo[w], acc[w][dt]);
+        }
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int row = r0 + acc_row(e) + 4 * h;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) {
+          const int d = dt * 32 + (lane & 31);
+          const float v = *reinterpret_cast<const float*>(t + row * ROWB + (((d >> 2) ^ swz(row)) << 4) + (d & 3) * 4);
+#pragma unroll
+          for (int w = 0; w < RW; ++w) acc[w][dt] = __builtin_amdgcn_mfma_f32_32x32x2f32(v, p[w][e], acc[w][dt], 0, 0, 0);
+        }
+      }
+    }
+  }
+  TURTLE_DEV static uint4 rest(const float (&p)[8], uint4 hi) {
+    typedef T tx8 __attribute__((ext_vector_type(8)));
+    const tx8 h = __builtin_bit_cast(tx8, hi);
+    float r[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) r[i] = p[i] - (float)h[i];
+    return pack(r);
+  }
+  TURTLE_DEV static uint4 pack(const float (&p)[8]) {
+    typedef T tx8 __attribute__((ext_vector_type(8)));
+    tx8 o;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) o[i] = (T)p[i];
+    if constexpr (ES == 2) return __builtin_bit_cast(uint4, o);
+    else return make_uint4(0, 0, 0, 0);
+  }
+  // one global row as the B operand: this lane's STEPS chunks (zero when p is null or past D channels)
+  TURTLE_DEV static void frag(const T* p, int D, uint4 (&f)[STEPS], int lane) {
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s) {
+      const int d = (2 * s + (lane >> 5)) * (16 / ES);
+      f[s] = (p && d < D) ? *reinterpret_cast<const uint4*>(p + d) : make_uint4(0, 0, 0, 0);
+    }
+  }
+  // DMA of N rows of two tensors (LDS tiles t0, t1) by NT threads: src(r, p0, p1) sets the addresses of row r's first
+  // channels, or null
+  template <int N, int NT, typename F>
+  TURTLE_DEV static void load2(char* t0, char* t1, int tid, int D, F src) {
+    static_assert(N * CH % NT == 0, "whole DMA instructions");
+    const uint32_t b0 = lds_addr(t0) + (uint32_t)(tid & ~63) * 16, b1 = lds_addr(t1) + (uint32_t)(tid & ~63) * 16;
+#pragma unroll
+    for (int i = 0; i < N * CH / NT; ++i) {
+      const int ci = i * NT + tid, r = ci / CH, c = ((ci % CH) ^ swz(r)) * 16;
+      const char *p0 = nullptr, *p1 = nullptr;
+      if (c < D * ES) src(r, p0, p1);
+      dma16(p0 ? (const void*)(p0 + c) : (const void*)g_zero_ta, __builtin_amdgcn_readfirstlane(b0 + (uint32_t)i * NT * 16));
+      dma16(p1 ? (const void*)(p1 + c) : (const void*)g_zero_ta, __builtin_amdgcn_readfirstlane(b1 + (uint32_t)i * NT * 16));
+    }
+  }
+  template <int N, int NT> static constexpr int loads2() { return 2 * (N * CH / NT); }
+  // 4 consecutive channels d0 .. d0 + 3 of a dense result row
+  TURTLE_DEV static void put4(T* p, const float (&v)[4]) {
+    if constexpr (ES == 4) *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+    else {
+      typedef T tx4 __attribute__((ext_vector_type(4)));
+      tx4 o;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) o[i] = (T)v[i];
+      *reinterpret_cast<tx4*>(p) = o;
+    }
+  }
+};
+
+struct Args {
+  const void *q, *k, *v;
+  int64_t qb, qs, qh, kb, ks, kh, vb, vs, vh;
+  int B, Sq, Sk, Hq, Hk, G, D, M;         // M = Sq * G rows of a (sequence, key head)
+  float scale, scale2, cap, icap, cap2;   // scale2 = scale log2 e; cap2 = cap log2 e; icap = scale / cap
+  const float* slopes;
+  const int *prefix, *qdoc, *kdoc;
+  const int4 *qr, *kr;                    // document ranges of RT-token tiles
+  int nqr, nkr;
+  int causal;
+  int page, npages, maxpages;
+  uint32_t pmul, psh;                     // j / page = mulhi(j, pmul) >> psh (page > 1)
+  const int *table, *kv_lens, *q_lens;
+  void *o, *olo;
+  float* lse;
+  int mtiles, nsplit, total, lds_win;
+  float *part, *plse;                     // [nsplit][B Hk][M][D], [nsplit][B Hk][M]
+  // backward
+  const void* dout;
+  int64_t gb, gs, gh;
+  void *dq, *dk, *dv;
+  const float* delta;
+};
+
+// work item of a block: consecutive items on one XCD (blocks are dealt to the 8 XCDs in turn), so that the tiles
+// of one key head share an L2
+TURTLE_DEV int xcd_item(int total) {
+  const int chunk = (total + 7) >> 3;
+  const int i = (int)(blockIdx.x >> 3);
+  return i < chunk ? (int)(blockIdx.x & 7) * chunk + i : total;
+}
+
+// One row's (query's) place and rules, in the lane that owns it
+struct Row {
+  int pos;       // its place among the keys
+  int doc;
+  float slope2;
+  bool on;
+};
+
+TURTLE_DEV Row row_of(const Args& a, int b, int hk, int m, int off, int nq) {
+  Row r;
+  const int i = m / a.G, g = m - i * a.G;
+  r.on = m < a.M && i < nq;
+  r.pos = i + off;
+  r.doc = (a.qdoc && r.on) ? a.qdoc[(int64_t)b * a.Sq + i] : 0;
+  if (r.doc < 0) r.on = false;
+  r.slope2 = (a.slopes && r.on) ? a.slopes[hk * a.G + g] * LOG2E : 0.f;
+  return r;
+}
+
+// tanh for the cap. 16-bit inputs: 1 - 2 / (e^2x + 1), absolute error ~1e-7, under the scores' own rounding there;
+// fp32: the library's, which keeps its relative error for small x
+template <typename T>
+TURTLE_DEV float cap_tanh(float x) {
+  if constexpr (sizeof(T) == 4) return tanhf(x);
+  else return 1.f - 2.f * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(2.f * LOG2E * x));
+}
+
+// document range of tokens [t0, t1): {lo, hi, 1 if all are the same valid number, 1 if any is invalid}
+TURTLE_DEV int4 doc_range(const int4* ranges, int nr, int t0, int t1) {
+  int4 x = make_int4(0x7fffffff, -1, 1, 0);
+  for (int r = t0 / RT; r <= (t1 - 1) / RT && r < nr; ++r) {
+    const int4 y = ranges[r];
+    x.x = min(x.x, y.x); x.y = max(x.y, y.y); x.z &= y.z; x.w |= y.w;
+  }
+  if (x.x != x.y) x.z = 0;
+  return x;
+}
+
+// A walk over tiles of UNIT tokens that may hold a document of [lo, hi]: 64 tiles are looked up at a time, a lane each.
+// Of the tile it stops at: mixed = not every pair of it with a pure tile of document `pure` (-1: none) is visible;
+// holes = it has tokens without a document.
+struct DocWalk {
+  const int4* ranges;     // of this sequence; null: every tile, all visible
+  int nr, lo, hi, pure;
+  uint64_t act, mix, hole;
+  int base;
+  bool mixed, holes;
+  TURTLE_DEV void init(const int4* r, int n, int4 mine) {
+    ranges = r; nr = n; lo = mine.x; hi = mine.y; pure = mine.z ? mine.x : -1;
+    base = -1; act = mix = hole = 0; mixed = holes = false;
+  }
+  // the first tile >= t (in steps of STRIDE), or `end`; G rows share a token, there are ntok tokens
+  template <int UNIT, int STRIDE>
+  TURTLE_DEV int next(int t, int end, int G, int ntok, int lane) {
+    if (!ranges) return min(t, end);
+    while (t < end) {
+      if (base < 0 || t >= base + 64 * STRIDE) {
+        base = t;
+        const int tt = t + lane * STRIDE;
+        int4 x = make_int4(0x7fffffff, -1, 0, 0);
+        if (tt < end) x = doc_range(ranges, nr, tt * UNIT / G, min((tt * UNIT + UNIT - 1) / G + 1, ntok));
+        act = __ballot(x.x <= hi && x.y >= lo);
+        mix = __ballot(!(x.z && x.x == pure));
+        hole = __ballot(x.w != 0);
+      }
+      const int at = (t - base) / STRIDE;
+      const uint64_t left = act >> at;
+      if (left) {
+        const int k = at + __builtin_ctzll(left);
+        mixed = (mix >> k) & 1;
+        holes = (hole >> k) & 1;
+        return base + k * STRIDE;
+      }
+      t = base + 64 * STRIDE;
+    }
+    return end;
+  }
+};
+
+// -------------------------------------------------------------------------------------------------
+// host
+// -------------------------------------------------------------------------------------------------
+typedef turtle_token_attn_args In;
+
+bool rows16(const void* p, int64_t sb, int64_t ss, int64_t sh, int es) {
+  return p && (uintptr_t)p % 16 == 0 && sb * es % 16 == 0 && ss * es % 16 == 0 && sh * es % 16 == 0;
+}
+
+bool sizes_ok(const In* x, int dtype) {
+  if (!x || dtype < 0 || dtype > 2 || x->B <= 0 || x->Sq <= 0 || x->Hq <= 0 || x->Hk <= 0 || x->Hq % x->Hk) return false;
+  if (x->D <= 0 || x->D % 8 || x->D > 128) return false;
+  const int64_t G = x->Hq / x->Hk;
+  if ((int64_t)x->Sq * G >= (1ll << 30) || (int64_t)x->B * x->Hk >= (1ll << 24)) return false;
+  if (x->table) {
+    if (x->page <= 0 || x->npages < 0 || x->maxpages <= 0 || (int64_t)x->page * x->maxpages >= (1ll << 30)) return false;
+  } else if (x->Sk <= 0 || x->Sk >= (1 << 30)) {
+    return false;
+  }
+  return true;
+}
+
+// keys that a sequence can have
+int64_t key_room(const In* x) { return x->table ? (int64_t)x->page * x->maxpages : x->Sk; }
+
+bool fill(Args& a, const In* x, int dtype) {
+  if (!sizes_ok(x, dtype)) return false;
+  const int es = dtype == 0 ? 4 : 2;
+  if (!rows16(x->q, x->qb, x->qs, x->qh, es) || !rows16(x->k, x->kb, x->ks, x->kh, es) || !rows16(x->v, x->vb, x->vs, x->vh, es)) return false;
+  if (!x->o || (uintptr_t)x->o % 16 || (uintptr_t)x->o_lo % 16) return false;
+  if (x->prefix && !x->causal) return false;
+  if ((x->qdoc != nullptr) != (x->kdoc != nullptr)) return false;
+  if (x->qdoc && !x->ranges) return false;
+  if (x->table && (!x->kv_lens || x->qdoc || x->prefix)) return false;
+  a = Args{};
+  a.q = x->q; a.k = x->k; a.v = x->v;
+  a.qb = x->qb; a.qs = x->qs; a.qh = x->qh; a.kb = x->kb; a.ks = x->ks; a.kh = x->kh; a.vb = x->vb; a.vs = x->vs; a.vh = x->vh;
+  a.B = x->B; a.Sq = x->Sq; a.Sk = x->table ? 0 : x->Sk; a.Hq = x->Hq; a.Hk = x->Hk; a.G = x->Hq / x->Hk; a.D = x->D; a.M = x->Sq * a.G;
+  a.scale = x->scale; a.scale2 = x->scale * LOG2E; a.cap = x->softcap;
+  if (x->softcap > 0.f) { a.icap = x->scale / x->softcap; a.cap2 = x->softcap * LOG2E; }
+  a.slopes = x->slopes; a.prefix = x->prefix; a.qdoc = x->qdoc; a.kdoc = x->kdoc; a.causal = x->causal;
+  a.nqr = (x->Sq + RT - 1) / RT; a.nkr = x->table ? 0 : (x->Sk + RT - 1) / RT;
+  a.qr = (const int4*)x->ranges; a.kr = a.qr ? a.qr + (int64_t)x->B * a.nqr : nullptr;
+  a.page = x->page; a.npages = x->npages; a.maxpages = x->maxpages; a.table = x->table; a.kv_lens = x->kv_lens; a.q_lens = x->q_lens;
+  if (x->table && x->page > 1) {
+    // j / page for j < 2^30: with l = ceil(log2 page), floor(j m / 2^(31 + l)) for m = floor(2^(31 + l) / page) + 1 is exact
+    int l = 0;
+    while ((1ll << l) < x->page) ++l;
+    a.pmul = (uint32_t)((1ull << (31 + l)) / (uint64_t)x->page + 1);
+    a.psh = (uint32_t)(l - 1);
+  }
+  a.o = x->o; a.olo = dtype == 0 ? nullptr : x->o_lo; a.lse = x->lse;
+  return true;
+}
+
+template <typename K>
+int launch(K kernel, int64_t total, int threads, int lds, Args& a, hipStream_t st) {
+  if (total <= 0 || total >= (1ll << 30)) return -1;
+  a.total = (int)total;
+  if (lds > 64 * 1024) {
+    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+    if (e != hipSuccess) return (int)e;
+  }
+  kernel<<<dim3((unsigned)((total + 7) / 8 * 8)), dim3(threads), lds, st>>>(a);
+  return (int)hipGetLastError();
+}
+
+}  // namespace
+}  // namespace turtle

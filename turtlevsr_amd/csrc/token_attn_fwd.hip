@@ -1,0 +1,471 @@
+// Token attention, forward: dense and paged (token_attn.h holds the method and the shared parts).
+//
+// Four shapes of one kernel, chosen by the number of rows M = Sq G of a (sequence, key head):
+//   M <= 32 (new tokens)        the block's waves take the key tiles in turn, each with its own LDS buffers and no
+//                               block barrier, and join at the end: the call is bound by reading K and V once
+//   M <= 64, or <= 256 keys     2 waves x 32 rows
+//   otherwise                   4 waves x 32 or x 64 rows: 64 rows read every K and V tile from LDS once for two
+//                               row groups, which halves the LDS traffic that bounds the 32-row form; it is taken
+//                               when its blocks still fill the chip
+// The first two have matrix instructions to spare and multiply p in two terms (TWO): with few keys, p's rounding
+// would be as large an error as the result's own.
+#include "token_attn.h"
+
+namespace turtle {
+namespace {
+
+template <typename T, int DP, int NW, int RW, bool WK> struct Fwd {
+  typedef Rows<T, DP> R;
+  static constexpr int NT = NW * 64;
+  static constexpr int WROWS = 32 * RW;               // rows of a wave
+  static constexpr int BM = WK ? WROWS : NW * WROWS;  // rows of a block
+  static constexpr int BN = (WK || sizeof(T) == 4) ? 32 : 64;
+  static constexpr int TILE = BN * R::ROWB;
+  static constexpr int BUF = 4 * TILE;                // two stages of K and V
+  static constexpr int LT = WK ? 64 : NT;             // threads that load a tile
+  static constexpr int NLD = R::template loads2<BN, LT>();
+  static constexpr int WIN = 256;                     // page numbers a wave keeps at hand
+  static constexpr bool TWO = sizeof(T) == 2 && (WK || NW == 2);
+  static int lds(bool paged, int64_t keys) {
+    const int buf = WK ? NW * BUF : (keys <= BN ? BUF / 2 : BUF);
+    const int join = WK ? (2 * NW * 32 + R::DT * 16 * 64) * 4 : 0;
+    return (buf > join ? buf : join) + (paged ? NW * WIN * 4 : 0);
+  }
+};
+
+// sum of 8 probabilities as the product takes them (16-bit: the rounded ones, two at a time)
+template <typename T> TURTLE_DEV float sum8(const float (&p)[8], float l) {
+  float a = 0.f, b = 0.f;
+#pragma unroll
+  for (int e = 0; e < 8; e += 2) { a += p[e]; b += p[e + 1]; }
+  return l + (a + b);
+}
+
+template <typename T, int DP, int NW, int RW, bool WK, bool PAGED>
+__global__ __launch_bounds__(NW * 64) void attn_fwd_kernel(Args a) {
+  typedef Fwd<T, DP, NW, RW, WK> F;
+  typedef Rows<T, DP> R;
+  constexpr int BN = F::BN, KT = BN / 32, DT = R::DT, STEP = WK ? NW : 1;
+  // fp16: p is scaled by 2^6; with p at most 2^8 over the running maximum (below) that stays under the type's 2^16
+  constexpr float POFF = std::is_same<T, f16>::value ? 6.f : 0.f;
+  constexpr float SLACK = 8.f;
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
+
+  const int item = xcd_item(a.total);
+  if (item >= a.total) return;
+  const int mt = a.mtiles - 1 - item % a.mtiles, rest = item / a.mtiles;   // causal: the longest tiles first
+  const int sp = rest % a.nsplit, bh = rest / a.nsplit, b = bh / a.Hk, hk = bh - b * a.Hk;
+
+  int kn = a.Sk, nq = a.Sq, off = a.Sk - a.Sq;
+  if constexpr (PAGED) {
+    const int64_t room = (int64_t)a.page * a.maxpages;
+    const int kl = a.kv_lens[b];
+    nq = a.q_lens ? min(max(a.q_lens[b], 0), a.Sq) : a.Sq;
+    off = kl - nq;
+    kn = max(0, (int)min((int64_t)kl, room));
+  }
+  const int m0 = mt * F::BM, mend = min(a.M, nq * a.G), m1 = min(m0 + F::BM, mend);   // rows of this block that exist: [m0, m1)
+  const int pre = (!PAGED && a.prefix) ? a.prefix[b] : 0;
+  const int mw = m0 + (WK ? 0 : wave * F::WROWS), mw1 = min(mw + F::WROWS, mend);     // ... of this wave
+  int mrow[RW];
+  Row row[RW];
+#pragma unroll
+  for (int w = 0; w < RW; ++w) {
+    mrow[w] = mw + w * 32 + (lane & 31);
+    row[w] = row_of(a, b, hk, mrow[w], off, nq);
+  }
+
+  // key tiles this block walks over
+  int kend = kn;
+  if (a.causal) kend = min(kn, max((m1 - 1) / a.G + off + 1, pre));
+  if (m1 <= m0) kend = 0;
+  int t1 = (max(kend, 0) + BN - 1) / BN, t0 = 0;
+  if (a.nsplit > 1) {
+    const int per = (t1 + a.nsplit - 1) / a.nsplit;
+    t0 = min(t1, sp * per);
+    t1 = min(t1, t0 + per);
+  }
+  DocWalk dw;
+  dw.init(nullptr, 0, make_int4(0, 0, 0, 0));
+  if (!PAGED && a.qdoc && m1 > m0)
+    dw.init(a.kr + (int64_t)b * a.nkr, a.nkr, doc_range(a.qr + (int64_t)b * a.nqr, a.nqr, m0 / a.G, (m1 - 1) / a.G + 1));
+  // what this wave's rows see whole: keys before `whole`; and at all: keys before `some`
+  const int whole = a.causal ? max(mw / a.G + off + 1, pre) : 0x7fffffff;
+  const int some = mw1 <= mw ? 0 : (a.causal ? max((mw1 - 1) / a.G + off + 1, pre) : 0x7fffffff);
+
+  uint4 qf[RW][R::STEPS];
+#pragma unroll
+  for (int w = 0; w < RW; ++w) {
+    const int i = mrow[w] / a.G, g = mrow[w] - i * a.G;
+    R::frag(row[w].on ? reinterpret_cast<const T*>(a.q) + (int64_t)b * a.qb + (int64_t)i * a.qs + (int64_t)(hk * a.G + g) * a.qh : nullptr,
+            a.D, qf[w], lane);
+  }
+
+  char* buf = smem + (WK ? wave * F::BUF : 0);
+  const char* kbase = reinterpret_cast<const char*>(a.k) + ((PAGED ? 0 : (int64_t)b * a.kb) + (int64_t)hk * a.kh) * R::ES;
+  const char* vbase = reinterpret_cast<const char*>(a.v) + ((PAGED ? 0 : (int64_t)b * a.vb) + (int64_t)hk * a.vh) * R::ES;
+  // page numbers: this wave's window of the sequence's table, read from LDS - a global read per tile would have to
+  // wait, in order, behind the tiles in flight
+  int* win = reinterpret_cast<int*>(smem + a.lds_win) + wave * F::WIN;
+  int wbase = 0, wend = 0;
+  auto page_of = [&](int key) { return a.page == 1 ? key : (int)(__umulhi((uint32_t)key, a.pmul) >> a.psh); };
+  // starts tile t's copy into dst; returns which of its keys are seen at all (bit = key within the tile)
+  auto issue = [&](int t, char* dst) -> uint64_t {
+    const int k0 = t * BN;
+    if constexpr (PAGED) {
+      const int p0 = page_of(k0), p1 = page_of(min(k0 + BN, kn) - 1);
+      if (p0 < wbase || p1 >= wend) {
+        wbase = p0;
+        wend = p0 + F::WIN;
+#pragma unroll
+        for (int e = 0; e < F::WIN / 64; ++e) {
+          const int p = p0 + e * 64 + lane;
+          win[e * 64 + lane] = p < a.maxpages ? a.table[(int64_t)b * a.maxpages + p] : -1;
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      }
+      R::template load2<BN, F::LT>(dst, dst + F::TILE, WK ? lane : tid, a.D, [&](int r, const char*& p0, const char*& p1) {
+        const int key = k0 + r;
+        if (key >= kn) return;
+        const int pg = page_of(key), id = win[pg - wbase], in = key - pg * a.page;
+        if ((uint32_t)id >= (uint32_t)a.npages) return;
+        p0 = kbase + ((int64_t)id * a.kb + (int64_t)in * a.ks) * R::ES;
+        p1 = vbase + ((int64_t)id * a.vb + (int64_t)in * a.vs) * R::ES;
+      });
+      const int key = k0 + (lane & (BN - 1));
+      bool ok = key < kn;
+      if (ok) ok = (uint32_t)win[page_of(key) - wbase] < (uint32_t)a.npages;
+      return __ballot(ok);
+    } else {
+      const bool holes = dw.holes;
+      R::template load2<BN, F::LT>(dst, dst + F::TILE, WK ? lane : tid, a.D, [&](int r, const char*& p0, const char*& p1) {
+        const int key = k0 + r;
+        if (key >= kn || (holes && a.kdoc[(int64_t)b * a.Sk + key] < 0)) return;
+        p0 = kbase + (int64_t)key * a.ks * R::ES;
+        p1 = vbase + (int64_t)key * a.vs * R::ES;
+      });
+      return ~0ull;
+    }
+  };
+
+  f32x16 acc[RW][DT];
+  float mx[RW], l[RW];
+#pragma unroll
+  for (int w = 0; w < RW; ++w) {
+#pragma unroll
+    for (int i = 0; i < DT; ++i) acc[w][i] = zero16();
+    mx[w] = -INFINITY;
+    l[w] = 0.f;
+  }
+
+  auto next = [&](int t) { return dw.template next<BN, STEP>(t, t1, 1, a.Sk, lane); };
+  int t = next(WK ? t0 + wave : t0), par = 0;
+  uint64_t seen = ~0ull;
+  if (t < t1) seen = issue(t, buf);
+  bool mixed = dw.mixed;
+  while (t < t1) {
+    const int tn = next(t + STEP);
+    uint64_t seen_n = ~0ull;
+    if (tn < t1) {
+      seen_n = issue(tn, buf + (par ^ 1) * 2 * F::TILE);
+      vm_wait<F::NLD>();
+    } else {
+      vm_wait<0>();
+    }
+    if constexpr (!WK) lds_barrier();
+    const char* kt = buf + par * 2 * F::TILE;
+    const char* vt = kt + F::TILE;
+    const int k0 = t * BN;
+
+    if (k0 < some) {
+      f32x16 s[KT][RW];
+#pragma unroll
+      for (int j = 0; j < KT; ++j) R::template times<RW>(kt, j * 32, qf, s[j], lane);
+
+      const bool caus = k0 + BN > whole, holes = PAGED && (BN == 32 ? (uint32_t)seen != ~0u : seen != ~0ull);
+      const bool masked = mixed || caus || k0 + BN > kn || holes;
+      float mul = a.scale2;
+      if (masked || a.cap > 0.f || a.slopes || a.scale2 <= 0.f) {
+        mul = 1.f;
+        int kd = 0;
+        if (mixed) { const int key = k0 + (lane & (BN - 1)); kd = key < kn ? a.kdoc[(int64_t)b * a.Sk + key] : -1; }
+#pragma unroll
+        for (int j = 0; j < KT; ++j)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const int kk = j * 32 + acc_row(r) + 4 * h, key = k0 + kk;
+            int kdoc = 0;
+            if (mixed) kdoc = __shfl(kd, kk, 64);          // every lane gives its number
+#pragma unroll
+            for (int w = 0; w < RW; ++w) {
+              float x = s[j][w][r];
+              x = a.cap > 0.f ? a.cap2 * cap_tanh<T>(x * a.icap) : x * a.scale2;
+              if (a.slopes) x -= row[w].slope2 * fabsf((float)(row[w].pos - key));
+              if (masked) {
+                bool vis = key < kn;
+                if (mixed) vis = vis && kdoc == row[w].doc;
+                if (caus) vis = vis && (key <= row[w].pos || key < pre);
+                if (holes) vis = vis && ((seen >> kk) & 1);
+                x = vis ? x : -INFINITY;
+              }
+              s[j][w][r] = x;
+            }
+          }
+      }
+
+      // running maximum; the accumulators are only rescaled when it grew by more than 2^SLACK in some row
+#pragma unroll
+      for (int w = 0; w < RW; ++w) {
+        float tm = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < KT; ++j)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) tm = fmaxf(tm, s[j][w][r]);
+        const float mn = fmaxf(mx[w], half_max(tm) * mul);
+        if (__any(mn > mx[w] + SLACK)) {
+          const float al = __builtin_amdgcn_exp2f(mx[w] - (mn == -INFINITY ? 0.f : mn));
+          mx[w] = mn;
+          l[w] *= al;
+#pragma unroll
+          for (int i = 0; i < DT; ++i)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) acc[w][i][r] *= al;
+        }
+        const float sh = POFF - (mx[w] == -INFINITY ? 0.f : mx[w]);
+#pragma unroll
+        for (int j = 0; j < KT; ++j)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) s[j][w][r] = __builtin_amdgcn_exp2f(fmaf(s[j][w][r], mul, sh));
+      }
+#pragma unroll
+      for (int j = 0; j < KT; ++j)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          float p[RW][8];
+#pragma unroll
+          for (int w = 0; w < RW; ++w) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) p[w][e] = s[j][w][8 * u + e];
+            l[w] = sum8<T>(p[w], l[w]);
+          }
+          R::template t_times<RW, F::TWO>(vt, j * 32 + u * 16, p, acc, lane);
+        }
+    }
+    if constexpr (!WK) lds_barrier();
+    else asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    par ^= 1;
+    t = tn;
+    seen = seen_n;
+    mixed = dw.mixed;
+  }
+#pragma unroll
+  for (int w = 0; w < RW; ++w) l[w] = half_sum(l[w]);
+
+  if constexpr (WK) {
+    // join the waves: their (max, sum), then the rescaled accumulators summed through LDS in wave order
+    float* ml = reinterpret_cast<float*>(smem);
+    float* sum = ml + 2 * NW * 32;
+    __syncthreads();
+    if (h == 0) { ml[wave * 32 + lane] = mx[0]; ml[(NW + wave) * 32 + lane] = l[0]; }
+    __syncthreads();
+    float mall = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) mall = fmaxf(mall, ml[w * 32 + (lane & 31)]);
+    const float mb = mall == -INFINITY ? 0.f : mall;
+    l[0] = 0.f;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) l[0] += ml[(NW + w) * 32 + (lane & 31)] * __builtin_amdgcn_exp2f(ml[w * 32 + (lane & 31)] - mb);
+    const float f = __builtin_amdgcn_exp2f(mx[0] - mb);
+    mx[0] = mall;
+    for (int w = 0; w < NW; ++w) {
+      if (wave == w) {
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            float* p = sum + (dt * 16 + r) * 64 + lane;
+            *p = (w ? *p : 0.f) + acc[0][dt][r] * f;
+          }
+      }
+      __syncthreads();
+    }
+    // every wave takes its share of the channels
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[0][dt][r] = sum[(dt * 16 + r) * 64 + lane];
+  }
+
+#pragma unroll
+  for (int w = 0; w < RW; ++w) {
+    if (mrow[w] >= a.M) continue;
+    const float inv = (l[w] > 0.f && row[w].on) ? 1.f / l[w] : 0.f;
+    const float lse = inv > 0.f ? mx[w] + log2f(l[w]) - POFF : INFINITY;
+    const int i = mrow[w] / a.G, g = mrow[w] - i * a.G;
+    const bool first = (!WK || wave == 0) && h == 0;
+    const int64_t pi = ((int64_t)sp * a.B * a.Hk + bh) * a.M + mrow[w];
+    const int64_t oi = (((int64_t)b * a.Sq + i) * a.Hq + hk * a.G + g) * a.D;
+    if (first && a.nsplit > 1) a.plse[pi] = lse;
+    if (first && a.nsplit <= 1 && a.lse) a.lse[(int64_t)bh * a.M + mrow[w]] = lse;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) {
+      if (WK && dt % NW != wave) continue;
+#pragma unroll
+      for (int q4 = 0; q4 < 4; ++q4) {
+        const int d = dt * 32 + 8 * q4 + 4 * h;
+        if (d >= a.D) continue;
+        float v[4], lo[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) { v[e] = acc[w][dt][4 * q4 + e] * inv; lo[e] = v[e] - to_f((T)v[e]); }
+        if (a.nsplit > 1) {
+          *reinterpret_cast<float4*>(a.part + pi * a.D + d) = make_float4(v[0], v[1], v[2], v[3]);
+        } else {
+          R::put4(reinterpret_cast<T*>(a.o) + oi + d, v);
+          if (a.olo) R::put4(reinterpret_cast<T*>(a.olo) + oi + d, lo);
+        }
+      }
+    }
+  }
+}
+
+__global__ __launch_bounds__(256) void doc_range_kernel(const int* __restrict__ qdoc, const int* __restrict__ kdoc, int4* qr, int4* kr, int B,
+                                                        int Sq, int Sk, int nqr, int nkr) {
+  const int w = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+  if (w >= B * (nqr + nkr)) return;
+  const bool isq = w < B * nqr;
+  const int u = isq ? w : w - B * nqr, n = isq ? nqr : nkr, S = isq ? Sq : Sk;
+  const int b = u / n, t = u - b * n, i = t * RT + lane;
+  const int d = i < S ? (isq ? qdoc : kdoc)[(int64_t)b * S + i] : -1;
+  int lo = d < 0 ? 0x7fffffff : d, hi = d < 0 ? -1 : d;
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) { lo = min(lo, __shfl_xor(lo, o, 64)); hi = max(hi, __shfl_xor(hi, o, 64)); }
+  const bool bad = __any(i < S && d < 0), whole = __all(i >= S || d >= 0);
+  if (lane == 0) (isq ? qr : kr)[(int64_t)b * n + t] = make_int4(lo, hi, whole && lo == hi ? 1 : 0, bad ? 1 : 0);
+}
+
+// results of the splits -> o: 4 channels a thread
+template <typename T>
+__global__ __launch_bounds__(256) void attn_join_kernel(Args a) {
+  const int c4 = a.D / 4;
+  const int64_t n = (int64_t)a.B * a.Hk * a.M, stride = n;
+  const int64_t u = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (u >= n * c4) return;
+  const int64_t r = u / c4;
+  const int d = (int)(u - r * c4) * 4;
+  float mx = -INFINITY;
+  for (int s = 0; s < a.nsplit; ++s) {
+    const float x = a.plse[s * stride + r];
+    if (x != INFINITY) mx = fmaxf(mx, x);
+  }
+  float v[4] = {0.f, 0.f, 0.f, 0.f}, l = 0.f;
+  for (int s = 0; s < a.nsplit; ++s) {
+    const float x = a.plse[s * stride + r];
+    if (x == INFINITY) continue;
+    const float w = __builtin_amdgcn_exp2f(x - mx);
+    const float4 p = *reinterpret_cast<const float4*>(a.part + (s * stride + r) * a.D + d);
+    l += w;
+    v[0] = fmaf(w, p.x, v[0]); v[1] = fmaf(w, p.y, v[1]); v[2] = fmaf(w, p.z, v[2]); v[3] = fmaf(w, p.w, v[3]);
+  }
+  const float inv = l > 0.f ? 1.f / l : 0.f;
+  float lo[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) { v[e] *= inv; lo[e] = v[e] - to_f((T)v[e]); }
+  const int64_t bh = r / a.M, m = r - bh * a.M, b = bh / a.Hk, hk = bh - b * a.Hk, i = m / a.G, g = m - i * a.G;
+  const int64_t oi = ((b * a.Sq + i) * a.Hq + hk * a.G + g) * a.D + d;
+  Rows<T, 64>::put4(reinterpret_cast<T*>(a.o) + oi, v);
+  if (a.olo) Rows<T, 64>::put4(reinterpret_cast<T*>(a.olo) + oi, lo);
+  if (a.lse && d == 0) a.lse[r] = l > 0.f ? mx + log2f(l) : INFINITY;
+}
+
+struct Plan { int kind, nsplit; int64_t mtiles; };      // kind: 0 new tokens, 1 two waves, 2 four waves, 3 four waves x 64 rows
+
+Plan plan_of(const In* x, int dtype) {
+  const int64_t M = (int64_t)x->Sq * (x->Hq / x->Hk), bh = (int64_t)x->B * x->Hk, room = key_room(x);
+  Plan p;
+  int bm;
+  if (M <= 32) { p.kind = 0; bm = 32; }
+  else if (dtype != 0 && (M <= 64 || room <= 256)) { p.kind = 1; bm = 64; }
+  else if (dtype != 0 && (M + 255) / 256 * bh >= 256) { p.kind = 3; bm = 256; }
+  else { p.kind = 2; bm = 128; }
+  p.mtiles = (M + bm - 1) / bm;
+  // too few blocks to fill the 256 CUs: the keys are split over blocks too, 512 at least each, and joined by a second
+  // kernel
+  const int64_t want = std::max<int64_t>(1, 256 / (p.mtiles * bh)), most = std::max<int64_t>(1, room / 512);
+  p.nsplit = (int)std::min<int64_t>({want, most, 64});
+  return p;
+}
+
+size_t ranges_bytes(const In* x) {
+  if (!x->qdoc) return 0;
+  return (size_t)x->B * ((x->Sq + RT - 1) / RT + (x->Sk + RT - 1) / RT) * sizeof(int4);
+}
+size_t ws_bytes(const In* x, int dtype) {
+  const Plan p = plan_of(x, dtype);
+  if (p.nsplit <= 1) return 0;
+  return (size_t)p.nsplit * x->B * x->Sq * x->Hq * (x->D + 1) * sizeof(float);
+}
+
+template <typename T, int DP, int NW, int RW, bool WK, bool PAGED>
+int run(Args& a, const Plan& p, int64_t keys, hipStream_t st) {
+  typedef Fwd<T, DP, NW, RW, WK> F;
+  const int lds = F::lds(PAGED, keys);
+  a.lds_win = lds - (PAGED ? NW * F::WIN * 4 : 0);
+  return launch(attn_fwd_kernel<T, DP, NW, RW, WK, PAGED>, p.mtiles * a.B * a.Hk * p.nsplit, F::NT, lds, a, st);
+}
+
+template <typename T, int DP, bool PAGED>
+int fwd(Args& a, const Plan& p, int64_t keys, hipStream_t st) {
+  constexpr int WK = sizeof(T) == 4 && DP == 128 ? 2 : 4;
+  a.mtiles = (int)p.mtiles;
+  a.nsplit = p.nsplit;
+  int rc;
+  if (p.kind == 0) rc = run<T, DP, WK, 1, true, PAGED>(a, p, keys, st);
+  else if (sizeof(T) == 4 || p.kind == 2) rc = run<T, DP, 4, 1, false, PAGED>(a, p, keys, st);
+  else if (p.kind == 1) rc = run<T, DP, sizeof(T) == 4 ? 4 : 2, 1, false, PAGED>(a, p, keys, st);
+  else rc = run<T, DP, 4, sizeof(T) == 4 ? 1 : 2, false, PAGED>(a, p, keys, st);
+  if (rc || p.nsplit <= 1) return rc;
+  const int64_t n = (int64_t)a.B * a.Hk * a.M * (a.D / 4);
+  attn_join_kernel<T><<<(unsigned)((n + 255) / 256), 256, 0, st>>>(a);
+  return (int)hipGetLastError();
+}
+
+template <typename T>
+int fwd_any(Args& a, const Plan& p, int64_t keys, hipStream_t st) {
+  const bool paged = a.table != nullptr;
+  if (a.D <= 64) return paged ? fwd<T, 64, true>(a, p, keys, st) : fwd<T, 64, false>(a, p, keys, st);
+  return paged ? fwd<T, 128, true>(a, p, keys, st) : fwd<T, 128, false>(a, p, keys, st);
+}
+
+}  // namespace
+}  // namespace turtle
+
+using namespace turtle;
+
+extern "C" {
+
+size_t turtle_token_attn_ranges(const turtle_token_attn_args* a) { return a ? ranges_bytes(a) : 0; }
+size_t turtle_token_attn_workspace(const turtle_token_attn_args* a, int dtype) { return sizes_ok(a, dtype) ? ws_bytes(a, dtype) : 0; }
+
+int turtle_token_attn_fwd(const turtle_token_attn_args* x, int dtype, void* stream) {
+  Args a;
+  if (!fill(a, x, dtype)) return -1;
+  const Plan p = plan_of(x, dtype);
+  if (p.nsplit > 1) {
+    if (!x->ws || x->ws_bytes < ws_bytes(x, dtype) || (uintptr_t)x->ws % 16) return -1;
+    a.part = (float*)x->ws;
+    a.plse = a.part + (size_t)p.nsplit * x->B * x->Sq * x->Hq * x->D;
+  }
+  hipStream_t st = (hipStream_t)stream;
+  if (x->qdoc) {
+    const int n = x->B * (a.nqr + a.nkr);
+    doc_range_kernel<<<(n + 3) / 4, 256, 0, st>>>(x->qdoc, x->kdoc, (int4*)a.qr, (int4*)a.kr, x->B, x->Sq, x->Sk, a.nqr, a.nkr);
+    const int rc = (int)hipGetLastError();
+    if (rc) return rc;
+  }
+  if (dtype == 0) return fwd_any<float>(a, p, key_room(x), st);
+  if (dtype == 1) return fwd_any<bf16>(a, p, key_room(x), st);
+  return fwd_any<f16>(a, p, key_room(x), st);
+}
+
+}  // extern "C"

@@ -21,38 +21,22 @@ from __future__ import annotations
 
 import ctypes as C
 import functools
+import struct
 
 import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .train_ops import _check, _dt, _p, _stream
+from .train_ops import _check, _dt
 
 MAX_D = 128
 
-
-class _Axes(C.Structure):
-    _fields_ = [("freq", C.c_uint64 * 64), ("axis", C.c_uint8 * 64), ("npair", C.c_int32), ("naxis", C.c_int32)]
-
-
-class _Side(C.Structure):
-    _fields_ = [("x", C.c_void_p), ("dy", C.c_void_p), ("y", C.c_void_p), ("w", C.c_void_p)] + \
-               [(n, C.c_int64) for n in ("sb", "ss", "sh", "gb", "gs", "gh")] + [("H", C.c_int32), ("pad", C.c_int32)]
-
-
-class _Attn(C.Structure):
-    _fields_ = [(n, C.c_void_p) for n in ("q", "k", "v")] + \
-               [(n, C.c_int64) for n in ("qb", "qs", "qh", "kb", "ks", "kh", "vb", "vs", "vh")] + \
-               [(n, C.c_int32) for n in ("B", "Sq", "Sk", "Hq", "Hk", "D")] + [("scale", C.c_float), ("softcap", C.c_float)] + \
-               [(n, C.c_void_p) for n in ("slopes", "prefix", "qdoc", "kdoc")] + \
-               [(n, C.c_int32) for n in ("causal", "page", "npages", "maxpages")] + \
-               [(n, C.c_void_p) for n in ("table", "kv_lens", "q_lens", "o", "o_lo", "lse", "ranges", "ws")] + [("ws_bytes", C.c_size_t)]
-
-
-class _Grads(C.Structure):
-    _fields_ = [("f", _Attn), ("dout", C.c_void_p)] + [(n, C.c_int64) for n in ("gb", "gs", "gh")] + \
-               [(n, C.c_void_p) for n in ("dq", "dk", "dv", "delta")]
-
+# the argument blocks of include/turtle_token.h, packed in one go (a small call is bound by its host work)
+_SIDE = struct.Struct("@4P6q2i")
+_AXES = struct.Struct("@64Q64B2i")
+_ATTN = struct.Struct("@3P9q6i2f4P4i8PN")
+_GRADS = struct.Struct("@P3q4P")
+_NO_SIDE = bytes(_SIDE.size)
 
 _bound = None
 
@@ -62,19 +46,19 @@ def lib():
     if _bound is not None:
         return _bound
     L = _lib.lib()
-    vp, i64, ci, sz, P = C.c_void_p, C.c_int64, C.c_int, C.c_size_t, C.POINTER
-    rope = [P(_Side), P(_Side), P(_Axes), vp, i64, ci, i64, i64, ci]
+    vp, i64, ci, sz, blk = C.c_void_p, C.c_int64, C.c_int, C.c_size_t, C.c_char_p
+    rope = [blk, blk, blk, vp, i64, ci, i64, i64, ci]
     L.turtle_token_rope.argtypes = rope + [ci, ci, vp]
     L.turtle_token_norm_rope_fwd.argtypes = rope + [C.c_float, ci, vp]
     L.turtle_token_norm_rope_workspace.argtypes = [i64, ci]
     L.turtle_token_norm_rope_workspace.restype = sz
     L.turtle_token_norm_rope_bwd.argtypes = rope + [C.c_float, vp, vp, sz, ci, vp]
-    L.turtle_token_attn_ranges.argtypes = [P(_Attn)]
+    L.turtle_token_attn_ranges.argtypes = [blk]
     L.turtle_token_attn_ranges.restype = sz
-    L.turtle_token_attn_workspace.argtypes = [P(_Attn), ci]
+    L.turtle_token_attn_workspace.argtypes = [blk, ci]
     L.turtle_token_attn_workspace.restype = sz
-    L.turtle_token_attn_fwd.argtypes = [P(_Attn), ci, vp]
-    L.turtle_token_attn_bwd.argtypes = [P(_Grads), ci, vp]
+    L.turtle_token_attn_fwd.argtypes = [blk, ci, vp]
+    L.turtle_token_attn_bwd.argtypes = [blk, ci, vp]
     _bound = L
     return L
 
@@ -83,18 +67,29 @@ def lib():
 # arguments
 # -------------------------------------------------------------------------------------------------
 
-def _tokens(t, name: str) -> torch.Tensor:
+def _ptr(t) -> int:
+    return 0 if t is None else t.data_ptr()
+
+
+def _tokens(t) -> torch.Tensor:
     """``t`` itself when the kernels can read it: channels contiguous, rows at multiples of 16 bytes; else a copy."""
-    es = t.element_size()
-    ok = t.data_ptr() % 16 == 0 and (t.shape[3] == 1 or t.stride(3) == 1)
-    for i in range(3):
-        ok = ok and (t.shape[i] == 1 or (t.stride(i) * es) % 16 == 0)
-    return t if ok else t.clone(memory_format=torch.contiguous_format)
+    if t.data_ptr() % 16 == 0:
+        if t.is_contiguous():
+            return t
+        n, st, per = t.shape, t.stride(), 16 // t.element_size()
+        if st[3] == 1 and (st[0] % per == 0 or n[0] == 1) and (st[1] % per == 0 or n[1] == 1) and (st[2] % per == 0 or n[2] == 1):
+            return t
+    return t.clone(memory_format=torch.contiguous_format)
 
 
 def _strides(t):
     """(batch, token, head) strides in elements; 0 along a dimension of one (it may have any stride)."""
-    return tuple(t.stride(i) if t.shape[i] > 1 else 0 for i in range(3))
+    n, st = t.shape, t.stride()
+    return (st[0] if n[0] > 1 else 0, st[1] if n[1] > 1 else 0, st[2] if n[2] > 1 else 0)
+
+
+def _stream(t) -> int:
+    return torch._C._cuda_getCurrentRawStream(t.device.index)
 
 
 def _check_tokens(t, name: str, D=None):
@@ -155,20 +150,17 @@ def _scale(scale, D: int) -> float:
     return s
 
 
-class _on:
-    """The tensors' device as the current one (a no-op where it already is)."""
+def _run(t, what: str, entry, *args):
+    """One library call on ``t``'s device (made the current one where it is not) and its current stream."""
+    if torch.cuda.current_device() == t.device.index:
+        _check(entry(*args, _stream(t)), what)
+    else:
+        with torch.cuda.device(t.device):
+            _check(entry(*args, _stream(t)), what)
 
-    def __init__(self, t):
-        self.to = None if torch.cuda.current_device() == t.device.index else torch.cuda.device(t.device)
 
-    def __enter__(self):
-        if self.to is not None:
-            self.to.__enter__()
-
-    def __exit__(self, *e):
-        if self.to is not None:
-            self.to.__exit__(*e)
-        return False
+def _wants_grad(*ts) -> bool:
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)
 
 
 # -------------------------------------------------------------------------------------------------
@@ -179,15 +171,13 @@ class _on:
 def _axes_table(axes, base: float):
     """Every rotated pair's axis and its revolutions per unit of position in 64-bit fixed point: with it
     pos * freq mod 2^64 is the exact angle, however far the position."""
-    t = _Axes()
+    freq, axis = [0] * 64, [0] * 64
     i = 0
     for a, d in enumerate(axes):
         for j in range(0, d, 2):
-            f = base ** (-j / d) / 6.283185307179586476925
-            t.freq[i], t.axis[i] = int(f * 2.0 ** 64), a
+            freq[i], axis[i] = int(base ** (-j / d) / 6.283185307179586476925 * 2.0 ** 64), a
             i += 1
-    t.npair, t.naxis = i, len(axes)
-    return t
+    return _AXES.pack(*freq, *axis, i, len(axes))
 
 
 def _axes(axes, base, D: int):
@@ -197,7 +187,7 @@ def _axes(axes, base, D: int):
     base = float(base)
     if not 1.0 <= base < float("inf"):
         raise ValueError(f"base = {base}, must be at least 1")
-    return _axes_table(ax, base)
+    return _axes_table(ax, base), len(ax)
 
 
 def _pos(pos, B: int, S: int, naxis: int, like):
@@ -212,21 +202,20 @@ def _pos(pos, B: int, S: int, naxis: int, like):
 
 
 def _side(x, y, w=None, dy=None):
-    s = _Side()
-    if x is None:
-        return s
-    s.x, s.y, s.H = x.data_ptr(), y.data_ptr(), x.shape[2]
-    s.sb, s.ss, s.sh = _strides(x)
-    if w is not None:
-        s.w = w.data_ptr()
-    if dy is not None:
-        s.dy = dy.data_ptr()
-        s.gb, s.gs, s.gh = _strides(dy)
-    return s
+    return _SIDE.pack(x.data_ptr(), _ptr(dy), y.data_ptr(), _ptr(w), *_strides(x), *((0, 0, 0) if dy is None else _strides(dy)), x.shape[2], 0)
 
 
 def _dense(x):
     return torch.empty(x.shape, dtype=x.dtype, device=x.device)
+
+
+def _turn(x, pos, pos_b, pos64, tab, inverse):
+    x = _tokens(x)
+    y = _dense(x)
+    B, S, H, D = x.shape
+    if B and S:
+        _run(x, "token_rope", lib().turtle_token_rope, _side(x, y), _NO_SIDE, tab, pos.data_ptr(), pos_b, pos64, B, S, D, inverse, _dt(x))
+    return y
 
 
 class _Rope(torch.autograd.Function):
@@ -234,24 +223,12 @@ class _Rope(torch.autograd.Function):
     def forward(ctx, x, pos, pos_b, pos64, tab):
         ctx.save_for_backward(pos)
         ctx.rest = (pos_b, pos64, tab)
-        return _Rope.turn(x, pos, pos_b, pos64, tab, 0)
-
-    @staticmethod
-    def turn(x, pos, pos_b, pos64, tab, inverse):
-        x = _tokens(x, "x")
-        y = _dense(x)
-        B, S, _, D = x.shape
-        if x.numel():
-            with _on(x):
-                _check(lib().turtle_token_rope(_side(x, y), None, tab, _p(pos), pos_b, pos64, B, S, D, inverse, _dt(x), _stream(x)),
-                       "token_rope")
-        return y
+        return _turn(x, pos, pos_b, pos64, tab, 0)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        (pos,) = ctx.saved_tensors
-        return _Rope.turn(dy, pos, *ctx.rest, 1), None, None, None, None
+        return _turn(dy, ctx.saved_tensors[0], *ctx.rest, 1), None, None, None, None
 
 
 def axial_rope(x, pos, axes, base: float = 10000.0):
@@ -264,50 +241,57 @@ def axial_rope(x, pos, axes, base: float = 10000.0):
     distance); axes one to four even numbers. Returns a dense tensor of x's type."""
     _check_tokens(x, "x")
     B, S, _, D = x.shape
-    tab = _axes(axes, base, D)
-    p, pos_b, pos64 = _pos(pos, B, S, tab.naxis, x)
+    tab, naxis = _axes(axes, base, D)
+    p, pos_b, pos64 = _pos(pos, B, S, naxis, x)
     _device(x)
-    return _Rope.apply(x, p, pos_b, pos64, tab)
+    return _Rope.apply(x, p, pos_b, pos64, tab) if _wants_grad(x) else _turn(x, p, pos_b, pos64, tab, 0)
+
+
+def _gain(w):
+    return None if w is None else w.detach().float().contiguous()
+
+
+def _norm_turn(q, k, wq, wk, pos, pos_b, pos64, tab, eps):
+    """(q', k') from readable q, k and fp32 gains."""
+    yq, yk = _dense(q), _dense(k)
+    B, S, _, D = q.shape
+    if B and S:
+        _run(q, "token_norm_rope_fwd", lib().turtle_token_norm_rope_fwd, _side(q, yq, wq), _side(k, yk, wk), tab, pos.data_ptr(), pos_b,
+             pos64, B, S, D, eps, _dt(q))
+    return yq, yk
 
 
 class _QkNormRope(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, wq, wk, pos, pos_b, pos64, tab, eps):
-        q, k = _tokens(q, "q"), _tokens(k, "k")
-        yq, yk = _dense(q), _dense(k)
-        B, S, _, D = q.shape
-        w = [None if t is None else t.detach().float().contiguous() for t in (wq, wk)]
-        if q.numel():
-            with _on(q):
-                _check(lib().turtle_token_norm_rope_fwd(_side(q, yq, w[0]), _side(k, yk, w[1]), tab, _p(pos), pos_b, pos64, B, S, D, eps,
-                                                        _dt(q), _stream(q)), "token_norm_rope_fwd")
-        ctx.save_for_backward(q, k, pos, *[t for t in w if t is not None])
-        ctx.has_w = [t is not None for t in w]
-        ctx.w_dt = [None if t is None else t.dtype for t in (wq, wk)]
-        ctx.rest = (pos_b, pos64, tab, eps)
-        return yq, yk
+    def forward(ctx, q, k, wq, wk, *rest):
+        q, k = _tokens(q), _tokens(k)
+        gq, gk = _gain(wq), _gain(wk)
+        ctx.save_for_backward(q, k, rest[0], gq, gk)
+        ctx.rest = rest[1:]
+        ctx.w_dt = (None if wq is None else wq.dtype, None if wk is None else wk.dtype)
+        return _norm_turn(q, k, gq, gk, *rest)
 
     @staticmethod
     @once_differentiable
-    def backward(ctx, gq, gk):
-        q, k, pos, *ws = ctx.saved_tensors
-        w = [ws.pop(0) if has else None for has in ctx.has_w]
+    def backward(ctx, dyq, dyk):
+        q, k, pos, wq, wk = ctx.saved_tensors
         pos_b, pos64, tab, eps = ctx.rest
         B, S, _, D = q.shape
-        gq, gk = _tokens(gq, "dq"), _tokens(gk, "dk")
+        dyq, dyk = _tokens(dyq), _tokens(dyk)
         dq, dk = _dense(q), _dense(k)
-        want = any(ctx.has_w[i] and ctx.needs_input_grad[2 + i] for i in range(2))
-        dw = torch.zeros(2, D, dtype=torch.float32, device=q.device) if want and not q.numel() else \
-            (torch.empty(2, D, dtype=torch.float32, device=q.device) if want else None)
-        if q.numel():
-            L = lib()
-            n = int(L.turtle_token_norm_rope_workspace(B * S, D)) if want else 0
-            ws = torch.empty(n, dtype=torch.uint8, device=q.device) if n else None
-            with _on(q):
-                _check(L.turtle_token_norm_rope_bwd(_side(q, dq, w[0], gq), _side(k, dk, w[1], gk), tab, _p(pos), pos_b, pos64, B, S, D,
-                                                    eps, _p(dw), _p(ws), n, _dt(q), _stream(q)), "token_norm_rope_bwd")
-        g = [dw[i].to(ctx.w_dt[i]) if want and ctx.has_w[i] else None for i in range(2)]
-        return dq, dk, g[0], g[1], None, None, None, None, None
+        need = [w is not None and n for w, n in zip((wq, wk), ctx.needs_input_grad[2:4])]
+        L, buf, dw, ws, n = lib(), None, 0, 0, 0
+        if need[0] or need[1]:                    # the two gains' gradients, then the kernel's partial sums
+            n = L.turtle_token_norm_rope_workspace(B * S, D) if B and S else 0
+            buf = torch.empty(2 * D + n // 4, dtype=torch.float32, device=q.device)
+            dw = buf.data_ptr()
+            ws = dw + 8 * D
+        if B and S:
+            _run(q, "token_norm_rope_bwd", L.turtle_token_norm_rope_bwd, _side(q, dq, wq, dyq), _side(k, dk, wk, dyk), tab, pos.data_ptr(),
+                 pos_b, pos64, B, S, D, eps, dw, ws, n, _dt(q))
+        elif buf is not None:
+            buf.zero_()
+        return (dq, dk) + tuple(buf[i * D:(i + 1) * D].to(ctx.w_dt[i]) if need[i] else None for i in range(2)) + (None,) * 5
 
 
 def qk_norm_rope(q, k, pos, q_weight, k_weight, axes, base: float = 10000.0, eps: float = 1e-6):
@@ -335,82 +319,98 @@ def qk_norm_rope(q, k, pos, q_weight, k_weight, axes, base: float = 10000.0, eps
     eps = float(eps)
     if not 0.0 <= eps < float("inf"):
         raise ValueError(f"eps = {eps}, must be finite and not negative")
-    tab = _axes(axes, base, D)
-    p, pos_b, pos64 = _pos(pos, B, S, tab.naxis, q)
+    tab, naxis = _axes(axes, base, D)
+    rest = (*_pos(pos, B, S, naxis, q), tab, eps)
     _device(q)
-    return _QkNormRope.apply(q, k, q_weight, k_weight, p, pos_b, pos64, tab, eps)
+    if _wants_grad(q, k, q_weight, k_weight):
+        return _QkNormRope.apply(q, k, q_weight, k_weight, *rest)
+    return _norm_turn(_tokens(q), _tokens(k), _gain(q_weight), _gain(k_weight), *rest)
 
 
 # -------------------------------------------------------------------------------------------------
 # attention
 # -------------------------------------------------------------------------------------------------
 
-def _set(a, **kw):
-    for n, v in kw.items():
-        setattr(a, n, v.data_ptr() if isinstance(v, torch.Tensor) else v)
+def _attn_block(q, k, v, rules, masks, o, Sk, pages=(0, 0, 0), cache=(None, None, None), lo=0, lse=0, ranges=0, ws=0, ws_bytes=0):
+    """turtle_token_attn_args. rules: (scale, softcap, causal); masks: (slopes, prefix, q_doc, k_doc)."""
+    scale, softcap, causal = rules
+    B, Sq, Hq, D = q.shape
+    return _ATTN.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), *_strides(q), *_strides(k), *_strides(v), B, Sq, Sk, Hq, k.shape[2], D,
+                      scale, softcap, *map(_ptr, masks), causal, *pages, *map(_ptr, cache), o.data_ptr(), lo, lse, ranges, ws, ws_bytes)
 
 
-def _attn_args(q, k, v, scale, softcap, causal, slopes, prefix, q_doc, k_doc):
-    a = _Attn()
-    (a.qb, a.qs, a.qh), (a.kb, a.ks, a.kh), (a.vb, a.vs, a.vh) = _strides(q), _strides(k), _strides(v)
-    a.B, a.Sq, a.Hq, a.D = q.shape
-    a.Sk, a.Hk = k.shape[1], k.shape[2]
-    _set(a, q=q, k=k, v=v, scale=scale, softcap=softcap, causal=int(causal), slopes=slopes, prefix=prefix, qdoc=q_doc, kdoc=k_doc)
-    return a
+def _attn_forward(q, k, v, rules, masks, grad):
+    """(o, aux) of readable, non-empty q, k, v; aux (or None): what the backward needs besides - o's rounding remainder
+    (16-bit types), the rows' softmax sums, room for their deltas, the document ranges - in one buffer."""
+    o = _dense(q)
+    n, Sk, dt = q.shape[0] * q.shape[1] * q.shape[2], k.shape[1], _dt(q)
+    lo = lse = ranges = 0
+    aux = None
+    docs = masks[2] is not None
+    if grad or docs:
+        nr = lib().turtle_token_attn_ranges(_attn_block(q, k, v, rules, masks, o, Sk)) if docs else 0
+        parts = _aux_parts(n, q.shape[3], dt, nr) if grad else (0, 0, 0, 0, nr)
+        aux = torch.empty(parts[4], dtype=torch.uint8, device=q.device)
+        p = aux.data_ptr()
+        ranges = p + parts[3] if docs else 0
+        if grad:
+            lo, lse = (p if dt else 0), p + parts[1]
+    ws, nws = _attn_workspace(_attn_block(q, k, v, rules, masks, o, Sk), dt, q)
+    blk = _attn_block(q, k, v, rules, masks, o, Sk, lo=lo, lse=lse, ranges=ranges, ws=_ptr(ws), ws_bytes=nws)
+    _run(q, "token_attn_fwd", lib().turtle_token_attn_fwd, blk, dt)
+    return o, aux
 
 
-def _workspace(a, dt: int, dev):
-    n = int(lib().turtle_token_attn_workspace(a, dt))
-    ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
-    _set(a, ws=ws, ws_bytes=n)
-    return ws
+def _aux_parts(n: int, D: int, dt: int, nr: int):
+    """Byte offsets of (remainder, sums, deltas, ranges, end) for n rows."""
+    a = 2 * n * D if dt else 0
+    b = a + 4 * n
+    c = (b + 4 * n + 15) // 16 * 16
+    return 0, a, b, c, c + nr
+
+
+def _attn_workspace(blk, dt: int, like):
+    n = lib().turtle_token_attn_workspace(blk, dt)
+    return (torch.empty(n, dtype=torch.uint8, device=like.device), n) if n else (None, 0)
+
+
+class _NoKeys(torch.autograd.Function):
+    """Attention where there are no keys, or no queries: zeros, and zero gradients."""
+
+    @staticmethod
+    def forward(ctx, q, k, v):
+        ctx.save_for_backward(q, k, v)
+        return torch.zeros(q.shape, dtype=q.dtype, device=q.device)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, do):
+        return tuple(torch.zeros(t.shape, dtype=t.dtype, device=t.device) for t in ctx.saved_tensors)
 
 
 class _Attention(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, v, scale, softcap, causal, slopes, prefix, q_doc, k_doc):
-        q, k, v = _tokens(q, "q"), _tokens(k, "k"), _tokens(v, "v")
-        ctx.rest = (scale, softcap, causal)
-        opt = (slopes, prefix, q_doc, k_doc)
-        if q.numel() == 0 or k.numel() == 0:
-            ctx.save_for_backward(q, k, v)
-            return torch.zeros(q.shape, dtype=q.dtype, device=q.device)
-        a = _attn_args(q, k, v, *ctx.rest, *opt)
-        grad = any(ctx.needs_input_grad[:3])
-        o = _dense(q)
-        lo = _dense(q) if grad and q.dtype != torch.float32 else None
-        lse = torch.empty(q.shape[0] * q.shape[1] * q.shape[2], dtype=torch.float32, device=q.device) if grad else None
-        n = int(lib().turtle_token_attn_ranges(a))
-        ranges = torch.empty(n, dtype=torch.uint8, device=q.device) if n else None
-        _set(a, o=o, o_lo=lo, lse=lse, ranges=ranges)
-        dt = _dt(q)
-        ws = _workspace(a, dt, q.device)      # noqa: F841  (alive until the launch)
-        with _on(q):
-            _check(lib().turtle_token_attn_fwd(a, dt, _stream(q)), "token_attn_fwd")
-        if grad:
-            ctx.save_for_backward(q, k, v, o, lse, lo, ranges, *opt)
+    def forward(ctx, q, k, v, rules, *masks):
+        q, k, v = _tokens(q), _tokens(k), _tokens(v)
+        o, aux = _attn_forward(q, k, v, rules, masks, True)
+        ctx.save_for_backward(q, k, v, o, aux, *masks)
+        ctx.rules = rules
         return o
 
     @staticmethod
     @once_differentiable
     def backward(ctx, do):
-        q, k, v, *saved = ctx.saved_tensors
+        q, k, v, o, aux, *masks = ctx.saved_tensors
         need = ctx.needs_input_grad
-        if not saved:
-            return tuple(torch.zeros_like(t) if n else None for t, n in zip((q, k, v), need)) + (None,) * 7
-        o, lse, lo, ranges, *opt = saved
-        do = _tokens(do.to(q.dtype), "do")
-        g = _Grads()
-        g.f = _attn_args(q, k, v, *ctx.rest, *opt)
-        _set(g.f, o=o, o_lo=lo, lse=lse, ranges=ranges)
+        do = _tokens(do)
+        n, dt, p = q.shape[0] * q.shape[1] * q.shape[2], _dt(q), aux.data_ptr()
+        _, lse, delta, ranges, _ = _aux_parts(n, q.shape[3], dt, 0)
         dq = _dense(q) if need[0] else None
         dk, dv = (_dense(k), _dense(v)) if need[1] or need[2] else (None, None)
-        delta = torch.empty_like(lse)
-        g.gb, g.gs, g.gh = _strides(do)
-        _set(g, dout=do, dq=dq, dk=dk, dv=dv, delta=delta)
-        with _on(q):
-            _check(lib().turtle_token_attn_bwd(g, _dt(q), _stream(q)), "token_attn_bwd")
-        return (dq, dk if need[1] else None, dv if need[2] else None) + (None,) * 7
+        blk = _attn_block(q, k, v, ctx.rules, masks, o, k.shape[1], lo=p if dt else 0, lse=p + lse, ranges=p + ranges if masks[2] is not None else 0)
+        blk += _GRADS.pack(do.data_ptr(), *_strides(do), _ptr(dq), _ptr(dk), _ptr(dv), p + delta)
+        _run(q, "token_attn_bwd", lib().turtle_token_attn_bwd, blk, dt)
+        return (dq, dk if need[1] else None, dv if need[2] else None) + (None,) * 5
 
 
 def _check_qkv(q, k, v):
@@ -460,7 +460,12 @@ def attention(q, k, v, *, scale=None, softcap: float = 0.0, slopes=None, causal:
         k_doc = q_doc if k_doc is None else _ints(k_doc, (B, Sk), "k_doc", q)
     scale, softcap, slopes = _scale(scale, D), _cap(softcap), _slopes(slopes, Hq, q)
     _device(q)
-    return _Attention.apply(q, k, v, scale, softcap, bool(causal), slopes, prefix, q_doc, k_doc)
+    rules, masks = (scale, softcap, 1 if causal else 0), (slopes, prefix, q_doc, k_doc)
+    if B == 0 or Sq == 0 or Sk == 0:
+        return _NoKeys.apply(q, k, v)
+    if _wants_grad(q, k, v):
+        return _Attention.apply(q, k, v, rules, *masks)
+    return _attn_forward(_tokens(q), _tokens(k), _tokens(v), rules, masks, False)[0]
 
 
 def paged_attention(q, k_pages, v_pages, block_table, kv_lens, *, q_lens=None, scale=None, softcap: float = 0.0, slopes=None,
@@ -492,15 +497,10 @@ def paged_attention(q, k_pages, v_pages, block_table, kv_lens, *, q_lens=None, s
     _device(q)
     if q.numel() == 0 or k_pages.numel() == 0 or block_table.numel() == 0:
         return torch.zeros(q.shape, dtype=q.dtype, device=q.device)
-    q, kp, vp = _tokens(q, "q"), _tokens(k_pages, "k_pages"), _tokens(v_pages, "v_pages")
-    table, kv_lens = block_table.contiguous(), kv_lens.contiguous()
-    q_lens = None if q_lens is None else q_lens.contiguous()
-    a = _attn_args(q, kp, vp, scale, softcap, causal, slopes, None, None, None)
-    o = _dense(q)
-    a.Sk = 0
-    _set(a, o=o, page=kp.shape[1], npages=kp.shape[0], maxpages=table.shape[1], table=table, kv_lens=kv_lens, q_lens=q_lens)
-    dt = _dt(q)
-    ws = _workspace(a, dt, q.device)          # noqa: F841  (alive until the launch)
-    with _on(q):
-        _check(lib().turtle_token_attn_fwd(a, dt, _stream(q)), "token_attn_fwd")
+    q, kp, vp = _tokens(q), _tokens(k_pages), _tokens(v_pages)
+    cache = (block_table.contiguous(), kv_lens.contiguous(), None if q_lens is None else q_lens.contiguous())
+    rules, masks, pages = (scale, softcap, 1 if causal else 0), (slopes, None, None, None), (kp.shape[1], kp.shape[0], block_table.shape[1])
+    o, dt = _dense(q), _dt(q)
+    ws, nws = _attn_workspace(_attn_block(q, kp, vp, rules, masks, o, 0, pages, cache), dt, q)
+    _run(q, "token_attn_fwd", lib().turtle_token_attn_fwd, _attn_block(q, kp, vp, rules, masks, o, 0, pages, cache, ws=_ptr(ws), ws_bytes=nws), dt)
     return o
