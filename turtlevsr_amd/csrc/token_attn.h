@@ -200,6 +200,20 @@ struct Rows {
       dma16(p1 ? (const void*)(p1 + c) : (const void*)g_zero_ta, __builtin_amdgcn_readfirstlane(b1 + (uint32_t)i * NT * 16));
     }
   }
+  // the same where every row is there, row r starts at row 0's address + r * (s0, s1) bytes and D = DP: this lane's
+  // addresses are computed once (p0, p1 point at its chunk of its first row) and advance by whole steps
+  template <int NT> static constexpr bool linear() { return (NT / CH) % 16 == 0; }
+  template <int NT>
+  TURTLE_DEV static int64_t lane_off(int tid, int64_t st) { return (int64_t)(tid / CH) * st + (((tid % CH) ^ swz(tid / CH)) << 4); }
+  template <int N, int NT>
+  TURTLE_DEV static void load2_linear(char* t0, char* t1, int tid, const char* p0, const char* p1, int64_t s0, int64_t s1) {
+    const uint32_t b0 = lds_addr(t0) + (uint32_t)(tid & ~63) * 16, b1 = lds_addr(t1) + (uint32_t)(tid & ~63) * 16;
+#pragma unroll
+    for (int i = 0; i < N * CH / NT; ++i) {
+      dma16(p0 + i * (NT / CH) * s0, __builtin_amdgcn_readfirstlane(b0 + (uint32_t)i * NT * 16));
+      dma16(p1 + i * (NT / CH) * s1, __builtin_amdgcn_readfirstlane(b1 + (uint32_t)i * NT * 16));
+    }
+  }
   template <int N, int NT> static constexpr int loads2() { return 2 * (N * CH / NT); }
   // 4 consecutive channels d0 .. d0 + 3 of a dense result row
   TURTLE_DEV static void put4(T* p, const float (&v)[4]) {
@@ -229,7 +243,7 @@ struct Args {
   const int *table, *kv_lens, *q_lens;
   void *o, *olo;
   float* lse;
-  int mtiles, nsplit, total, lds_win;
+  int mtiles, nsplit, total, runs, lds_win;
   float *part, *plse;                     // [nsplit][B Hk][M][D], [nsplit][B Hk][M]
   // backward
   const void* dout;
@@ -238,12 +252,13 @@ struct Args {
   const float* delta;
 };
 
-// work item of a block: consecutive items on one XCD (blocks are dealt to the 8 XCDs in turn), so that the tiles
-// of one key head share an L2
-TURTLE_DEV int xcd_item(int total) {
-  const int chunk = (total + 7) >> 3;
-  const int i = (int)(blockIdx.x >> 3);
-  return i < chunk ? (int)(blockIdx.x & 7) * chunk + i : total;
+// work item of a block. Blocks are dealt to the 8 XCDs in turn, each with an L2 of its own: with enough key heads, runs
+// of consecutive items go to one XCD, so that the tiles of a key head share its L2; with few, items are dealt as they
+// come - a run would be a piece of one sequence, and pieces cost unequally (causal, documents)
+TURTLE_DEV int xcd_item(const Args& a) {
+  if (!a.runs) return (int)blockIdx.x;
+  const int chunk = (a.total + 7) >> 3;
+  return (int)(blockIdx.x & 7) * chunk + (int)(blockIdx.x >> 3);
 }
 
 // One row's (query's) place and rules, in the lane that owns it
@@ -265,12 +280,38 @@ TURTLE_DEV Row row_of(const Args& a, int b, int hk, int m, int off, int nq) {
   return r;
 }
 
-// tanh for the cap. 16-bit inputs: 1 - 2 / (e^2x + 1), absolute error ~1e-7, under the scores' own rounding there;
-// fp32: the library's, which keeps its relative error for small x
-template <typename T>
-TURTLE_DEV float cap_tanh(float x) {
-  if constexpr (sizeof(T) == 4) return tanhf(x);
-  else return 1.f - 2.f * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(2.f * LOG2E * x));
+// tanh of the scores in place, for the cap. While every |x| of the wave is at most 1/2 - scores within half the cap -
+// an odd polynomial (least-maximum fit of tanh(x) / x in x^2: relative error 5.5e-7 for 16-bit inputs, 3.2e-10 for
+// fp32): 5 instructions where the exponential form takes two of the slow ones besides. Beyond: 16-bit inputs
+// 1 - 2 / (e^2x + 1), absolute error ~1e-7, under the scores' own rounding there; fp32 the library's.
+template <typename T, int N>
+TURTLE_DEV void tanh_all(f32x16 (&s)[N], float icap) {
+  float big = 0.f;
+#pragma unroll
+  for (int w = 0; w < N; ++w)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) { s[w][r] *= icap; big = fmaxf(big, fabsf(s[w][r])); }
+  if (!__any(!(big <= 0.5f))) {
+#pragma unroll
+    for (int w = 0; w < N; ++w)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const float x = s[w][r], u = x * x;
+        float p;
+        if constexpr (sizeof(T) == 2) p = fmaf(u, fmaf(u, fmaf(u, -0.0444022265f, 0.131902966f), -0.333263179f), 0.999999456f);
+        else p = fmaf(u, fmaf(u, fmaf(u, fmaf(u, fmaf(u, -0.0066134277f, 0.0212747076f), -0.0538934189f), 0.13332902f), -0.333333242f), 1.f);
+        s[w][r] = x * p;
+      }
+  } else {
+#pragma unroll
+    for (int w = 0; w < N; ++w)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const float x = s[w][r];
+        if constexpr (sizeof(T) == 4) s[w][r] = tanhf(x);
+        else s[w][r] = 1.f - 2.f * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(2.f * LOG2E * x));
+      }
+  }
 }
 
 // document range of tokens [t0, t1): {lo, hi, 1 if all are the same valid number, 1 if any is invalid}
@@ -383,7 +424,9 @@ bool fill(Args& a, const In* x, int dtype) {
 template <typename K>
 int launch(K kernel, int64_t total, int threads, int lds, Args& a, hipStream_t st) {
   if (total <= 0 || total >= (1ll << 30)) return -1;
+  const int bh = a.B * a.Hk;
   a.total = (int)total;
+  a.runs = bh % 8 == 0 || bh >= 64;
   if (lds > 64 * 1024) {
     const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
     if (e != hipSuccess) return (int)e;

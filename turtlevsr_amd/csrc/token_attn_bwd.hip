@@ -1,6 +1,21 @@
 // Token attention, backward (token_attn.h holds the method and the shared parts): delta, then dk and dv by key tiles,
 // then dq by row tiles. No atomics: every sum has a fixed order.
 #include "token_attn.h"
+#ifndef KG128
+#define KG128 0
+#endif
+#ifndef KWMIN
+#define KWMIN (1<<30)
+#endif
+#ifndef QWMIN
+#define QWMIN (1<<30)
+#endif
+#ifndef DKV_WAVES
+#define DKV_WAVES (sizeof(T)==2 && KG==1 && DP==64 ? 2 : 1)
+#endif
+#ifndef DQ_WAVES
+#define DQ_WAVES (sizeof(T)==2 && RW==1 ? 2 : 1)
+#endif
 
 namespace turtle {
 namespace {
@@ -40,17 +55,6 @@ __global__ __launch_bounds__(256) void attn_delta_kernel(Args a, float* delta) {
   }
 }
 
-// scores -> (p, dcap): p in the exponent's scale, of one pair. lse = +inf: 0
-template <typename T>
-TURTLE_DEV float pair_p(const Args& a, float raw, float slope2, int dist, float lse, bool vis, float& dcap) {
-  float x;
-  dcap = 1.f;
-  if (a.cap > 0.f) { const float th = cap_tanh<T>(raw * a.icap); x = a.cap2 * th; dcap = 1.f - th * th; }
-  else x = raw * a.scale2;
-  if (a.slopes) x -= slope2 * fabsf((float)dist);
-  return vis ? __builtin_amdgcn_exp2f(x - lse) : 0.f;
-}
-
 template <typename T, int DP, int KG> struct Dkv {
   typedef Rows<T, DP> R;
   static constexpr int WKEYS = 32 * KG, BK = 4 * WKEYS;   // keys of a wave, of a block
@@ -63,7 +67,7 @@ template <typename T, int DP, int KG> struct Dkv {
 };
 
 template <typename T, int DP, int KG>
-__global__ __launch_bounds__(256) void attn_dkv_kernel(Args a) {
+__global__ __launch_bounds__(256, DKV_WAVES) void attn_dkv_kernel(Args a) {
   typedef Dkv<T, DP, KG> C;
   typedef Rows<T, DP> R;
   constexpr int BM = C::BM, DT = R::DT;
@@ -71,7 +75,7 @@ __global__ __launch_bounds__(256) void attn_dkv_kernel(Args a) {
   constexpr float POFF = std::is_same<T, f16>::value ? 10.f : 0.f, PS = std::is_same<T, f16>::value ? 1.f / 1024.f : 1.f;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
-  const int item = xcd_item(a.total);
+  const int item = xcd_item(a);
   if (item >= a.total) return;
   const int kt = item % a.mtiles, bh = item / a.mtiles, b = bh / a.Hk, hk = bh - b * a.Hk;
   const int k0 = kt * C::BK, k1 = min(k0 + C::BK, a.Sk), off = a.Sk - a.Sq;
@@ -101,6 +105,17 @@ __global__ __launch_bounds__(256) void attn_dkv_kernel(Args a) {
 
   const char* qbase = reinterpret_cast<const char*>(a.q) + ((int64_t)b * a.qb + (int64_t)hk * a.G * a.qh) * R::ES;
   const char* gbase = reinterpret_cast<const char*>(a.dout) + ((int64_t)b * a.gb + (int64_t)hk * a.G * a.gh) * R::ES;
+  // where a tile holds whole tokens, its rows lie at the same offsets from its first one every time
+  constexpr int NI = BM * R::CH / 256;
+  const bool plain = BM % a.G == 0 && a.D == DP;
+  const int per = BM / a.G;
+  int64_t qoff[NI], goff[NI];
+#pragma unroll
+  for (int i = 0; i < NI; ++i) {
+    const int r = (i * 256 + tid) / R::CH, c = ((tid % R::CH) ^ R::swz(r)) << 4, ti = r / a.G, g = r - ti * a.G;
+    qoff[i] = ((int64_t)ti * a.qs + (int64_t)g * a.qh) * R::ES + c;
+    goff[i] = ((int64_t)ti * a.gs + (int64_t)g * a.gh) * R::ES + c;
+  }
   auto issue = [&](int t, int stage) {
     char* dst = smem + stage * C::STAGE;
     if (rules && tid < 64) {
@@ -113,6 +128,14 @@ __global__ __launch_bounds__(256) void attn_dkv_kernel(Args a) {
       if (lane < BM) { info[lane] = i + off; info[BM + lane] = d; info[2 * BM + lane] = __float_as_int(s); }
     }
     const bool holes = dw.holes;
+    if (plain && !holes && t * BM + BM <= a.M && (!a.causal || t * per + off >= 0 || pre > 0)) {
+#pragma unroll
+      for (int i = 0; i < NI; ++i) {
+        const uint32_t at = (uint32_t)(i * 256 + (tid & ~63)) * 16;
+        dma16(qbase + qoff[i] + (int64_t)t * per * a.qs * R::ES, __builtin_amdgcn_readfirstlane(lds_addr(dst) + at));
+        dma16(gbase + goff[i] + (int64_t)t * per * a.gs * R::ES, __builtin_amdgcn_readfirstlane(lds_addr(dst + C::TILE) + at));
+      }
+    } else
     R::template load2<BM, 256>(dst, dst + C::TILE, tid, a.D, [&](int r, const char*& p0, const char*& p1) {
       const int m = t * BM + r, i = m / a.G, g = m - i * a.G;
       // rows that see nothing may hold anything: they are not read
@@ -157,47 +180,69 @@ __global__ __launch_bounds__(256) void attn_dkv_kernel(Args a) {
       R::template times<KG>(qt, 0, kf, s, lane);
       R::template times<KG>(gt, 0, vf, dp, lane);
       const bool caus = a.causal && m0 / a.G + off + 1 < kw1 && kw1 > pre;
-      const bool special = mixed || caus || a.cap > 0.f || a.slopes;
+      float mul = a.scale2;
+      if (a.cap > 0.f) {
+        tanh_all<T, KG>(s, a.icap);
+        mul = a.cap2;
+      }
+      // dp -> (dp - delta) times the cap's slope
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
-        const int rr = 8 * c + 4 * h;
-        const float4 lse = *reinterpret_cast<const float4*>(in + rr), del = *reinterpret_cast<const float4*>(in + BM + rr);
-        const float ls[4] = {lse.x, lse.y, lse.z, lse.w}, de[4] = {del.x, del.y, del.z, del.w};
-        if (special) {
-          int4 pos = make_int4(0, 0, 0, 0), doc = pos;
-          float4 slp = make_float4(0.f, 0.f, 0.f, 0.f);
-          if (rules) {
-            pos = *reinterpret_cast<const int4*>(info + rr);
-            doc = *reinterpret_cast<const int4*>(info + BM + rr);
-            slp = *reinterpret_cast<const float4*>(info + 2 * BM + rr);
+        const float4 del = *reinterpret_cast<const float4*>(in + BM + 8 * c + 4 * h);
+        const float de[4] = {del.x, del.y, del.z, del.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+#pragma unroll
+          for (int w = 0; w < KG; ++w) {
+            const int r = 4 * c + e;
+            dp[w][r] = (dp[w][r] - de[e]) * PS;
+            if (a.cap > 0.f) dp[w][r] *= fmaf(-s[w][r], s[w][r], 1.f);
           }
-          const int po[4] = {pos.x, pos.y, pos.z, pos.w}, dc4[4] = {doc.x, doc.y, doc.z, doc.w};
-          const float sp4[4] = {slp.x, slp.y, slp.z, slp.w};
+      }
+      if (a.slopes) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const int4 pos = *reinterpret_cast<const int4*>(info + 8 * c + 4 * h);
+          const float4 slp = *reinterpret_cast<const float4*>(info + 2 * BM + 8 * c + 4 * h);
+          const int po[4] = {pos.x, pos.y, pos.z, pos.w};
+          const float sp[4] = {slp.x, slp.y, slp.z, slp.w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+#pragma unroll
+            for (int w = 0; w < KG; ++w) s[w][4 * c + e] = fmaf(-sp[e], fabsf((float)(po[e] - key[w])), s[w][4 * c + e] * mul);
+        }
+        mul = 1.f;
+      }
+      if (caus || mixed) {
+        // the pairs that do not see each other: p = 0, and whatever dP holds there
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const int4 pos = *reinterpret_cast<const int4*>(info + 8 * c + 4 * h), doc = *reinterpret_cast<const int4*>(info + BM + 8 * c + 4 * h);
+          const int po[4] = {pos.x, pos.y, pos.z, pos.w}, dc[4] = {doc.x, doc.y, doc.z, doc.w};
 #pragma unroll
           for (int e = 0; e < 4; ++e)
 #pragma unroll
             for (int w = 0; w < KG; ++w) {
-              const int r = 4 * c + e;
-              bool vis = true;
-              if (caus) vis = key[w] <= po[e] || key[w] < pre;
-              if (mixed) vis = vis && dc4[e] == kdoc[w];
-              float dc;
-              const float p = pair_p<T>(a, s[w][r], sp4[e], po[e] - key[w], ls[e] - POFF, vis, dc);
-              const float ds = p * ((dp[w][r] - de[e]) * (PS * dc));
-              s[w][r] = p;
-              dp[w][r] = vis ? ds : 0.f;
-            }
-        } else {
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-#pragma unroll
-            for (int w = 0; w < KG; ++w) {
-              const int r = 4 * c + e;
-              const float p = __builtin_amdgcn_exp2f(fmaf(s[w][r], a.scale2, POFF - ls[e]));
-              s[w][r] = p;
-              dp[w][r] = p * ((dp[w][r] - de[e]) * PS);
+              bool vis = !caus || max(po[e], pre - 1) >= key[w];
+              vis = vis && (!mixed || dc[e] == kdoc[w]);
+              s[w][4 * c + e] = vis ? s[w][4 * c + e] * mul : -INFINITY;
+              dp[w][4 * c + e] = vis ? dp[w][4 * c + e] : 0.f;
             }
         }
+        mul = 1.f;
+      }
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const float4 lse = *reinterpret_cast<const float4*>(in + 8 * c + 4 * h);
+        const float ls[4] = {lse.x, lse.y, lse.z, lse.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+#pragma unroll
+          for (int w = 0; w < KG; ++w) {
+            const int r = 4 * c + e;
+            s[w][r] = __builtin_amdgcn_exp2f(fmaf(s[w][r], mul, POFF - ls[e]));
+            dp[w][r] *= s[w][r];
+          }
       }
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
@@ -245,13 +290,13 @@ template <typename T, int DP, int RW> struct Dq {
 };
 
 template <typename T, int DP, int RW>
-__global__ __launch_bounds__(256) void attn_dq_kernel(Args a) {
+__global__ __launch_bounds__(256, DQ_WAVES) void attn_dq_kernel(Args a) {
   typedef Dq<T, DP, RW> C;
   typedef Rows<T, DP> R;
   constexpr int BN = C::BN, DT = R::DT;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
-  const int item = xcd_item(a.total);
+  const int item = xcd_item(a);
   if (item >= a.total) return;
   const int mt = a.mtiles - 1 - item % a.mtiles, bh = item / a.mtiles, b = bh / a.Hk, hk = bh - b * a.Hk;
   const int off = a.Sk - a.Sq, m0 = mt * C::BM, m1 = min(m0 + C::BM, a.M);
@@ -283,8 +328,16 @@ __global__ __launch_bounds__(256) void attn_dq_kernel(Args a) {
   }
   const char* kbase = reinterpret_cast<const char*>(a.k) + ((int64_t)b * a.kb + (int64_t)hk * a.kh) * R::ES;
   const char* vbase = reinterpret_cast<const char*>(a.v) + ((int64_t)b * a.vb + (int64_t)hk * a.vh) * R::ES;
+  const int64_t kst = a.ks * R::ES, vst = a.vs * R::ES;
+  const int64_t koff = R::template lane_off<256>(tid, kst), voff = R::template lane_off<256>(tid, vst);
   auto issue = [&](int t, char* dst) {
     const bool holes = dw.holes;
+    if constexpr (R::template linear<256>()) {
+      if (!holes && t * BN + BN <= a.Sk && a.D == DP) {
+        R::template load2_linear<BN, 256>(dst, dst + C::TILE, tid, kbase + koff + (int64_t)t * BN * kst, vbase + voff + (int64_t)t * BN * vst, kst, vst);
+        return;
+      }
+    }
     R::template load2<BN, 256>(dst, dst + C::TILE, tid, a.D, [&](int r, const char*& p0, const char*& p1) {
       const int key = t * BN + r;
       if (key >= a.Sk || (holes && a.kdoc[(int64_t)b * a.Sk + key] < 0)) return;
@@ -318,32 +371,48 @@ __global__ __launch_bounds__(256) void attn_dq_kernel(Args a) {
       f32x16 s[RW], dp[RW];
       R::template times<RW>(kt, 0, qf, s, lane);
       R::template times<RW>(vt, 0, gf, dp, lane);
-      const bool caus = k0 + BN > whole, masked = mixed || caus || k0 + BN > a.Sk;
-      if (masked || a.cap > 0.f || a.slopes) {
-        int kd = 0;
-        if (mixed) { const int key = k0 + (lane & 31); kd = key < a.Sk ? a.kdoc[(int64_t)b * a.Sk + key] : -1; }
+      const bool caus = k0 + BN > whole;
+      float mul = a.scale2;
+      if (a.cap > 0.f) {
+        tanh_all<T, RW>(s, a.icap);
+        mul = a.cap2;
+      }
+#pragma unroll
+      for (int w = 0; w < RW; ++w)
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-          const int kk = acc_row(r) + 4 * h, key = k0 + kk;
-          int kdoc = 0;
-          if (mixed) kdoc = __shfl(kd, kk, 64);
+          dp[w][r] -= delta[w];
+          if (a.cap > 0.f) dp[w][r] *= fmaf(-s[w][r], s[w][r], 1.f);
+        }
+      if (a.slopes) {
+#pragma unroll
+        for (int w = 0; w < RW; ++w) {
+          const int at = row[w].pos - k0 - 4 * h;
+#pragma unroll
+          for (int r = 0; r < 16; ++r) s[w][r] = fmaf(-row[w].slope2, fabsf((float)(at - acc_row(r))), s[w][r] * mul);
+        }
+        mul = 1.f;
+      }
+      if (caus || mixed || k0 + BN > a.Sk) {
+        const int key = k0 + (lane & 31), kd = mixed && key < a.Sk ? a.kdoc[(int64_t)b * a.Sk + key] : -1;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          int d = 0;
+          if (mixed) d = __shfl(kd, acc_row(r) + 4 * h, 64);      // every lane gives its number
 #pragma unroll
           for (int w = 0; w < RW; ++w) {
-            bool vis = key < a.Sk;
-            if (mixed) vis = vis && kdoc == row[w].doc;
-            if (caus) vis = vis && (key <= row[w].pos || key < pre);
-            float dc;
-            const float p = pair_p<T>(a, s[w][r], row[w].slope2, row[w].pos - key, lse[w], vis, dc);
-            const float ds = p * ((dp[w][r] - delta[w]) * dc);
-            dp[w][r] = vis ? ds : 0.f;
+            const int last = min(caus ? max(row[w].pos, pre - 1) : a.Sk, a.Sk - 1) - k0 - 4 * h;
+            const bool vis = acc_row(r) <= last && (!mixed || d == row[w].doc);
+            s[w][r] = vis ? s[w][r] * mul : -INFINITY;
+            dp[w][r] = vis ? dp[w][r] : 0.f;
           }
         }
-      } else {
-#pragma unroll
-        for (int w = 0; w < RW; ++w)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) dp[w][r] = __builtin_amdgcn_exp2f(fmaf(s[w][r], a.scale2, -lse[w])) * (dp[w][r] - delta[w]);
+        mul = 1.f;
       }
+#pragma unroll
+      for (int w = 0; w < RW; ++w)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) dp[w][r] *= __builtin_amdgcn_exp2f(fmaf(s[w][r], mul, -lse[w]));
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
         float x[RW][8];
@@ -398,8 +467,8 @@ int bwd(Args& a, float* delta, hipStream_t st) {
   int rc = (int)hipGetLastError();
   if (rc) return rc;
   a.delta = delta;
-  constexpr int W2 = sizeof(T) == 2 && DP == 64 ? 2 : 1;
-  const bool kw = W2 == 2 && (a.Sk + 255) / 256 * bh >= 256, qw = W2 == 2 && (a.M + 255) / 256 * bh >= 256;
+  constexpr int W2 = sizeof(T) == 2 && (DP == 64 || KG128) ? 2 : 1;
+  const bool kw = W2 == 2 && (a.Sk + 255) / 256 * bh >= KWMIN, qw = W2 == 2 && (a.M + 255) / 256 * bh >= QWMIN;
   if (a.dk) {
     rc = kw ? run_dkv<T, DP, W2>(a, st) : run_dkv<T, DP, 1>(a, st);
     if (rc) return rc;

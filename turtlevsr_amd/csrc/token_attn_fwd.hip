@@ -10,6 +10,12 @@
 // The first two have matrix instructions to spare and multiply p in two terms (TWO): with few keys, p's rounding
 // would be as large an error as the result's own.
 #include "token_attn.h"
+#ifndef LMIN
+#define LMIN 512
+#endif
+#ifndef FWD_WAVES
+#define FWD_WAVES (DP == 128 && (RW == 2 || sizeof(T)==4) ? 1 : 2)
+#endif
 
 namespace turtle {
 namespace {
@@ -33,8 +39,8 @@ template <typename T, int DP, int NW, int RW, bool WK> struct Fwd {
   }
 };
 
-// sum of 8 probabilities as the product takes them (16-bit: the rounded ones, two at a time)
-template <typename T> TURTLE_DEV float sum8(const float (&p)[8], float l) {
+// l + the sum of 8 probabilities
+TURTLE_DEV float sum8(const float (&p)[8], float l) {
   float a = 0.f, b = 0.f;
 #pragma unroll
   for (int e = 0; e < 8; e += 2) { a += p[e]; b += p[e + 1]; }
@@ -42,7 +48,7 @@ template <typename T> TURTLE_DEV float sum8(const float (&p)[8], float l) {
 }
 
 template <typename T, int DP, int NW, int RW, bool WK, bool PAGED>
-__global__ __launch_bounds__(NW * 64) void attn_fwd_kernel(Args a) {
+__global__ __launch_bounds__(NW * 64, FWD_WAVES) void attn_fwd_kernel(Args a) {
   typedef Fwd<T, DP, NW, RW, WK> F;
   typedef Rows<T, DP> R;
   constexpr int BN = F::BN, KT = BN / 32, DT = R::DT, STEP = WK ? NW : 1;
@@ -52,7 +58,7 @@ __global__ __launch_bounds__(NW * 64) void attn_fwd_kernel(Args a) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
 
-  const int item = xcd_item(a.total);
+  const int item = xcd_item(a);
   if (item >= a.total) return;
   const int mt = a.mtiles - 1 - item % a.mtiles, rest = item / a.mtiles;   // causal: the longest tiles first
   const int sp = rest % a.nsplit, bh = rest / a.nsplit, b = bh / a.Hk, hk = bh - b * a.Hk;
@@ -105,6 +111,8 @@ __global__ __launch_bounds__(NW * 64) void attn_fwd_kernel(Args a) {
   char* buf = smem + (WK ? wave * F::BUF : 0);
   const char* kbase = reinterpret_cast<const char*>(a.k) + ((PAGED ? 0 : (int64_t)b * a.kb) + (int64_t)hk * a.kh) * R::ES;
   const char* vbase = reinterpret_cast<const char*>(a.v) + ((PAGED ? 0 : (int64_t)b * a.vb) + (int64_t)hk * a.vh) * R::ES;
+  const int64_t kst = a.ks * R::ES, vst = a.vs * R::ES;
+  const int64_t koff = R::template lane_off<F::LT>(tid, kst), voff = R::template lane_off<F::LT>(tid, vst);
   // page numbers: this wave's window of the sequence's table, read from LDS - a global read per tile would have to
   // wait, in order, behind the tiles in flight
   int* win = reinterpret_cast<int*>(smem + a.lds_win) + wave * F::WIN;
@@ -139,6 +147,12 @@ __global__ __launch_bounds__(NW * 64) void attn_fwd_kernel(Args a) {
       return __ballot(ok);
     } else {
       const bool holes = dw.holes;
+      if constexpr (R::template linear<F::LT>()) {
+        if (!holes && k0 + BN <= kn && a.D == DP) {
+          R::template load2_linear<BN, F::LT>(dst, dst + F::TILE, tid, kbase + koff + (int64_t)k0 * kst, vbase + voff + (int64_t)k0 * vst, kst, vst);
+          return ~0ull;
+        }
+      }
       R::template load2<BN, F::LT>(dst, dst + F::TILE, WK ? lane : tid, a.D, [&](int r, const char*& p0, const char*& p1) {
         const int key = k0 + r;
         if (key >= kn || (holes && a.kdoc[(int64_t)b * a.Sk + key] < 0)) return;
@@ -183,34 +197,58 @@ __global__ __launch_bounds__(NW * 64) void attn_fwd_kernel(Args a) {
 #pragma unroll
       for (int j = 0; j < KT; ++j) R::template times<RW>(kt, j * 32, qf, s[j], lane);
 
-      const bool caus = k0 + BN > whole, holes = PAGED && (BN == 32 ? (uint32_t)seen != ~0u : seen != ~0ull);
-      const bool masked = mixed || caus || k0 + BN > kn || holes;
+      // the rules that apply to this tile, each in a pass of its own (uniform branches)
+      const bool caus = k0 + BN > whole;
+      bool gaps = k0 + BN > kn;
+      if constexpr (PAGED) gaps = BN == 32 ? (uint32_t)seen != ~0u : seen != ~0ull;
       float mul = a.scale2;
-      if (masked || a.cap > 0.f || a.slopes || a.scale2 <= 0.f) {
+      if (a.cap > 0.f) {
+#pragma unroll
+        for (int j = 0; j < KT; ++j) tanh_all<T, RW>(s[j], a.icap);
+        mul = a.cap2;
+      }
+      if (a.slopes || mul <= 0.f) {
+#pragma unroll
+        for (int j = 0; j < KT; ++j)
+#pragma unroll
+          for (int w = 0; w < RW; ++w) {
+            const int at = row[w].pos - k0 - j * 32 - 4 * h;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[j][w][r] = fmaf(-row[w].slope2, fabsf((float)(at - acc_row(r))), s[j][w][r] * mul);
+          }
         mul = 1.f;
-        int kd = 0;
-        if (mixed) { const int key = k0 + (lane & (BN - 1)); kd = key < kn ? a.kdoc[(int64_t)b * a.Sk + key] : -1; }
+      }
+      if (caus) {
+#pragma unroll
+        for (int j = 0; j < KT; ++j)
+#pragma unroll
+          for (int w = 0; w < RW; ++w) {
+            const int last = max(row[w].pos, pre - 1) - k0 - j * 32 - 4 * h;      // the last key in sight
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[j][w][r] = acc_row(r) <= last ? s[j][w][r] : -INFINITY;
+          }
+      }
+      if (gaps) {
+        if constexpr (!PAGED) seen = kn - k0 >= 64 ? ~0ull : (1ull << (kn - k0)) - 1;
+#pragma unroll
+        for (int j = 0; j < KT; ++j) {
+          const uint32_t bits = (uint32_t)(seen >> (j * 32)) >> (4 * h);
+#pragma unroll
+          for (int w = 0; w < RW; ++w)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[j][w][r] = (bits >> acc_row(r)) & 1 ? s[j][w][r] : -INFINITY;
+        }
+      }
+      if (mixed) {
+        const int key = k0 + (lane & (BN - 1));
+        const int kd = key < kn ? a.kdoc[(int64_t)b * a.Sk + key] : -1;
 #pragma unroll
         for (int j = 0; j < KT; ++j)
 #pragma unroll
           for (int r = 0; r < 16; ++r) {
-            const int kk = j * 32 + acc_row(r) + 4 * h, key = k0 + kk;
-            int kdoc = 0;
-            if (mixed) kdoc = __shfl(kd, kk, 64);          // every lane gives its number
+            const int d = __shfl(kd, j * 32 + acc_row(r) + 4 * h, 64);
 #pragma unroll
-            for (int w = 0; w < RW; ++w) {
-              float x = s[j][w][r];
-              x = a.cap > 0.f ? a.cap2 * cap_tanh<T>(x * a.icap) : x * a.scale2;
-              if (a.slopes) x -= row[w].slope2 * fabsf((float)(row[w].pos - key));
-              if (masked) {
-                bool vis = key < kn;
-                if (mixed) vis = vis && kdoc == row[w].doc;
-                if (caus) vis = vis && (key <= row[w].pos || key < pre);
-                if (holes) vis = vis && ((seen >> kk) & 1);
-                x = vis ? x : -INFINITY;
-              }
-              s[j][w][r] = x;
-            }
+            for (int w = 0; w < RW; ++w) s[j][w][r] = d == row[w].doc ? s[j][w][r] : -INFINITY;
           }
       }
 
@@ -247,7 +285,7 @@ __global__ __launch_bounds__(NW * 64) void attn_fwd_kernel(Args a) {
           for (int w = 0; w < RW; ++w) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) p[w][e] = s[j][w][8 * u + e];
-            l[w] = sum8<T>(p[w], l[w]);
+            l[w] = sum8(p[w], l[w]);
           }
           R::template t_times<RW, F::TWO>(vt, j * 32 + u * 16, p, acc, lane);
         }
@@ -384,9 +422,10 @@ Plan plan_of(const In* x, int dtype) {
   const int64_t M = (int64_t)x->Sq * (x->Hq / x->Hk), bh = (int64_t)x->B * x->Hk, room = key_room(x);
   Plan p;
   int bm;
-  if (M <= 32) { p.kind = 0; bm = 32; }
+  const int64_t b64 = (M + 63) / 64 * bh;
+  if (M <= 32 || b64 < 256) { p.kind = 0; bm = 32; }
   else if (dtype != 0 && (M <= 64 || room <= 256)) { p.kind = 1; bm = 64; }
-  else if (dtype != 0 && (M + 255) / 256 * bh >= 256) { p.kind = 3; bm = 256; }
+  else if (dtype != 0 && x->D <= 64 && (M + 255) / 256 * bh >= LMIN) { p.kind = 3; bm = 256; }
   else { p.kind = 2; bm = 128; }
   p.mtiles = (M + bm - 1) / bm;
   // too few blocks to fill the 256 CUs: the keys are split over blocks too, 512 at least each, and joined by a second
