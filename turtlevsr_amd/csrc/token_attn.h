@@ -13,8 +13,8 @@
 // the contraction is right as long as V^T is read in the same one - which is what the transposing LDS read gives in
 // two 4-key pieces. Nothing is exchanged through memory between the two products.
 //
-// Tiles of BN keys of K and V go HBM -> LDS by LDS-DMA, two buffers, the next tile in flight behind the current
-// one's products. LDS rows are not padded (the DMA writes lane-linear): 16-byte chunk c of row r sits at chunk
+// Tiles of BN keys of K and V go HBM -> LDS by LDS-DMA into a ring of NS slots, NS - 1 tiles in flight behind the
+// current one's products; one barrier a tile (it frees the slot of the tile before). LDS rows are not padded (the DMA writes lane-linear): 16-byte chunk c of row r sits at chunk
 // c ^ swz(r), applied on the DMA's source address, so that both the row reads (K: 32 rows, one chunk) and the
 // transposing reads (V: 4 rows, 4 chunks) touch distinct banks.
 //
@@ -92,6 +92,13 @@ template <int N>
 TURTLE_DEV void vm_wait() {
   static_assert(N >= 0 && N < 64, "vmcnt range");
   asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+// at most N tiles of NLD operations each still in flight, N known at run time
+template <int NLD, int MOST>
+TURTLE_DEV void vm_wait_tiles(int n) {
+  if constexpr (MOST <= 0) vm_wait<0>();
+  else if (n >= MOST) vm_wait<NLD * MOST>();
+  else vm_wait_tiles<NLD, MOST - 1>(n);
 }
 // all of this wave's LDS accesses done, then the block's barrier
 TURTLE_DEV void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
@@ -200,20 +207,24 @@ struct Rows {
       dma16(p1 ? (const void*)(p1 + c) : (const void*)g_zero_ta, __builtin_amdgcn_readfirstlane(b1 + (uint32_t)i * NT * 16));
     }
   }
-  // the same where every row is there, row r starts at row 0's address + r * (s0, s1) bytes and D = DP: this lane's
-  // addresses are computed once (p0, p1 point at its chunk of its first row) and advance by whole steps
-  template <int NT> static constexpr bool linear() { return (NT / CH) % 16 == 0; }
-  template <int NT>
-  TURTLE_DEV static int64_t lane_off(int tid, int64_t st) { return (int64_t)(tid / CH) * st + (((tid % CH) ^ swz(tid / CH)) << 4); }
-  template <int N, int NT>
-  TURTLE_DEV static void load2_linear(char* t0, char* t1, int tid, const char* p0, const char* p1, int64_t s0, int64_t s1) {
-    const uint32_t b0 = lds_addr(t0) + (uint32_t)(tid & ~63) * 16, b1 = lds_addr(t1) + (uint32_t)(tid & ~63) * 16;
+  // The same where every row is there, row r starts at row 0's address + r st bytes and D = DP. A lane's chunk within
+  // its rows depends on the instruction only through the exchange, with a period of NV instructions: its NV offsets
+  // are computed once, a tile costs one base address.
+  template <int NT> struct Lin {
+    static constexpr int RPI = NT / CH, NV = RPI >= 16 ? 1 : 16 / RPI;
+    int64_t off[NV];
+    TURTLE_DEV void init(int tid, int64_t st) {
 #pragma unroll
-    for (int i = 0; i < N * CH / NT; ++i) {
-      dma16(p0 + i * (NT / CH) * s0, __builtin_amdgcn_readfirstlane(b0 + (uint32_t)i * NT * 16));
-      dma16(p1 + i * (NT / CH) * s1, __builtin_amdgcn_readfirstlane(b1 + (uint32_t)i * NT * 16));
+      for (int i = 0; i < NV; ++i) off[i] = (int64_t)(tid / CH) * st + (((tid % CH) ^ swz(i * RPI + tid / CH)) << 4);
     }
-  }
+    template <int N>
+    TURTLE_DEV void load(char* t, int tid, const char* p, int64_t st) const {
+      const uint32_t b0 = lds_addr(t) + (uint32_t)(tid & ~63) * 16;
+#pragma unroll
+      for (int i = 0; i < N * CH / NT; ++i)
+        dma16(p + i * RPI * st + off[i % NV], __builtin_amdgcn_readfirstlane(b0 + (uint32_t)i * NT * 16));
+    }
+  };
   template <int N, int NT> static constexpr int loads2() { return 2 * (N * CH / NT); }
   // 4 consecutive channels d0 .. d0 + 3 of a dense result row
   TURTLE_DEV static void put4(T* p, const float (&v)[4]) {

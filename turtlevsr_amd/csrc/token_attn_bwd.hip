@@ -1,20 +1,26 @@
 // Token attention, backward (token_attn.h holds the method and the shared parts): delta, then dk and dv by key tiles,
 // then dq by row tiles. No atomics: every sum has a fixed order.
 #include "token_attn.h"
-#ifndef KG128
-#define KG128 0
-#endif
-#ifndef KWMIN
-#define KWMIN (1<<30)
-#endif
-#ifndef QWMIN
-#define QWMIN (1<<30)
-#endif
 #ifndef DKV_WAVES
-#define DKV_WAVES (sizeof(T)==2 && KG==1 && DP==64 ? 2 : 1)
+#define DKV_WAVES (sizeof(T)==2 && DP==64 ? 2 : 1)
 #endif
 #ifndef DQ_WAVES
 #define DQ_WAVES (sizeof(T)==2 && RW==1 ? 2 : 1)
+#endif
+#ifndef DKV_NS64
+#define DKV_NS64 4
+#endif
+#ifndef DKV_NS128
+#define DKV_NS128 4
+#endif
+#ifndef DQ_NS64
+#define DQ_NS64 4
+#endif
+#ifndef DQ_NS128
+#define DQ_NS128 (sizeof(T)==4?3:4)
+#endif
+#ifndef WKMAX
+#define WKMAX 128
 #endif
 
 namespace turtle {
@@ -55,22 +61,49 @@ __global__ __launch_bounds__(256) void attn_delta_kernel(Args a, float* delta) {
   }
 }
 
-template <typename T, int DP, int KG> struct Dkv {
+// WK: for small grids - the block's NW waves own the same 32 keys and take the row tiles in turn, each with its own
+// ring and no barriers, and join at the end
+template <typename T, int DP, int NW, bool WK> struct Dkv {
   typedef Rows<T, DP> R;
-  static constexpr int WKEYS = 32 * KG, BK = 4 * WKEYS;   // keys of a wave, of a block
+  static constexpr int NT = NW * 64, LT = WK ? 64 : NT;
+  static constexpr int BK = WK ? 32 : NW * 32;            // keys of a block
   static constexpr int BM = 32;                           // rows of a tile
+  static constexpr int NS = WK ? 2 : (DP == 64 ? DKV_NS64 : DKV_NS128);
   static constexpr int TILE = BM * R::ROWB;
-  static constexpr int STAGE = 2 * TILE + 64 * 4;         // Q, dO, 32 softmax sums and 32 deltas
   static constexpr int INFO = 3 * BM * 4;                 // place, document, slope of each row
-  static constexpr int LDS = 2 * STAGE + 2 * INFO;
-  static constexpr int NLD = R::template loads2<BM, 256>() + 1;
+  static constexpr int SLOT = 2 * TILE + 64 * 4 + INFO;   // Q, dO, 32 softmax sums and 32 deltas
+  static constexpr int JOIN = R::DT * 16 * 64 * 4;
+  static constexpr int LDS = NS * SLOT * (WK ? NW : 1) > JOIN ? NS * SLOT * (WK ? NW : 1) : JOIN;
+  static constexpr int NLD = R::template loads2<BM, LT>() + 1;
 };
 
-template <typename T, int DP, int KG>
-__global__ __launch_bounds__(256, DKV_WAVES) void attn_dkv_kernel(Args a) {
-  typedef Dkv<T, DP, KG> C;
+// sum of the waves' accumulators through LDS, in wave order; every wave gets it
+template <int NW, int DT>
+TURTLE_DEV void join_waves(f32x16 (&acc)[DT], float* sum, int wave, int lane) {
+  __syncthreads();
+  for (int w = 0; w < NW; ++w) {
+    if (wave == w) {
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          float* p = sum + (dt * 16 + r) * 64 + lane;
+          *p = (w ? *p : 0.f) + acc[dt][r];
+        }
+    }
+    __syncthreads();
+  }
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) acc[dt][r] = sum[(dt * 16 + r) * 64 + lane];
+}
+
+template <typename T, int DP, int NW, bool WK>
+__global__ __launch_bounds__(NW * 64, DKV_WAVES) void attn_dkv_kernel(Args a) {
+  typedef Dkv<T, DP, NW, WK> C;
   typedef Rows<T, DP> R;
-  constexpr int BM = C::BM, DT = R::DT;
+  constexpr int BM = C::BM, DT = R::DT, KG = 1, NS = C::NS, STEP = WK ? NW : 1;
   // fp16: p times 2^10 as operand of dv (p of 10^4 keys would lose bits below the type's normal range)
   constexpr float POFF = std::is_same<T, f16>::value ? 10.f : 0.f, PS = std::is_same<T, f16>::value ? 1.f / 1024.f : 1.f;
   extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -79,7 +112,7 @@ __global__ __launch_bounds__(256, DKV_WAVES) void attn_dkv_kernel(Args a) {
   if (item >= a.total) return;
   const int kt = item % a.mtiles, bh = item / a.mtiles, b = bh / a.Hk, hk = bh - b * a.Hk;
   const int k0 = kt * C::BK, k1 = min(k0 + C::BK, a.Sk), off = a.Sk - a.Sq;
-  const int kw = k0 + wave * C::WKEYS, kw1 = min(kw + C::WKEYS, a.Sk);
+  const int kw = k0 + (WK ? 0 : wave * 32), kw1 = min(kw + 32, a.Sk);
   const int pre = a.prefix ? a.prefix[b] : 0;
   int key[KG], kdoc[KG];
   bool kon[KG];
@@ -106,37 +139,38 @@ __global__ __launch_bounds__(256, DKV_WAVES) void attn_dkv_kernel(Args a) {
   const char* qbase = reinterpret_cast<const char*>(a.q) + ((int64_t)b * a.qb + (int64_t)hk * a.G * a.qh) * R::ES;
   const char* gbase = reinterpret_cast<const char*>(a.dout) + ((int64_t)b * a.gb + (int64_t)hk * a.G * a.gh) * R::ES;
   // where a tile holds whole tokens, its rows lie at the same offsets from its first one every time
-  constexpr int NI = BM * R::CH / 256;
+  constexpr int NI = BM * R::CH / C::LT;
+  const int ltid = WK ? lane : tid;
+  char* ring = smem + (WK ? wave * NS * C::SLOT : 0);
   const bool plain = BM % a.G == 0 && a.D == DP;
   const int per = BM / a.G;
   int64_t qoff[NI], goff[NI];
 #pragma unroll
   for (int i = 0; i < NI; ++i) {
-    const int r = (i * 256 + tid) / R::CH, c = ((tid % R::CH) ^ R::swz(r)) << 4, ti = r / a.G, g = r - ti * a.G;
+    const int r = (i * C::LT + ltid) / R::CH, c = ((ltid % R::CH) ^ R::swz(r)) << 4, ti = r / a.G, g = r - ti * a.G;
     qoff[i] = ((int64_t)ti * a.qs + (int64_t)g * a.qh) * R::ES + c;
     goff[i] = ((int64_t)ti * a.gs + (int64_t)g * a.gh) * R::ES + c;
   }
-  auto issue = [&](int t, int stage) {
-    char* dst = smem + stage * C::STAGE;
-    if (rules && tid < 64) {
+  auto issue = [&](int t, char* dst) {
+    if (rules && ltid < 64) {
       const int m = t * BM + (lane & 31), i = m / a.G, g = m - i * a.G;
       float s = 0.f;
       if (a.slopes) s = a.G <= 64 ? __shfl(sl, g, 64) : a.slopes[hk * a.G + g] * LOG2E;
       int d = 0;
       if (dw.mixed) d = m < a.M ? a.qdoc[(int64_t)b * a.Sq + i] : -1;
-      int* info = reinterpret_cast<int*>(smem + 2 * C::STAGE + stage * C::INFO);
+      int* info = reinterpret_cast<int*>(dst + 2 * C::TILE + 256);
       if (lane < BM) { info[lane] = i + off; info[BM + lane] = d; info[2 * BM + lane] = __float_as_int(s); }
     }
     const bool holes = dw.holes;
     if (plain && !holes && t * BM + BM <= a.M && (!a.causal || t * per + off >= 0 || pre > 0)) {
 #pragma unroll
       for (int i = 0; i < NI; ++i) {
-        const uint32_t at = (uint32_t)(i * 256 + (tid & ~63)) * 16;
+        const uint32_t at = (uint32_t)(i * C::LT + (ltid & ~63)) * 16;
         dma16(qbase + qoff[i] + (int64_t)t * per * a.qs * R::ES, __builtin_amdgcn_readfirstlane(lds_addr(dst) + at));
         dma16(gbase + goff[i] + (int64_t)t * per * a.gs * R::ES, __builtin_amdgcn_readfirstlane(lds_addr(dst + C::TILE) + at));
       }
     } else
-    R::template load2<BM, 256>(dst, dst + C::TILE, tid, a.D, [&](int r, const char*& p0, const char*& p1) {
+    R::template load2<BM, C::LT>(dst, dst + C::TILE, ltid, a.D, [&](int r, const char*& p0, const char*& p1) {
       const int m = t * BM + r, i = m / a.G, g = m - i * a.G;
       // rows that see nothing may hold anything: they are not read
       if (m >= a.M || (a.causal && i + off < 0 && pre <= 0) || (holes && a.qdoc[(int64_t)b * a.Sq + i] < 0)) return;
@@ -155,23 +189,32 @@ __global__ __launch_bounds__(256, DKV_WAVES) void attn_dkv_kernel(Args a) {
 #pragma unroll
     for (int i = 0; i < DT; ++i) { dk[w][i] = zero16(); dv[w][i] = zero16(); }
 
-  auto next = [&](int t) { return dw.template next<BM, 1>(t, t1, a.G, a.Sq, lane); };
-  int t = next(t0), par = 0;
-  if (t < t1) issue(t, 0);
-  bool mixed = dw.mixed;
-  while (t < t1) {
-    const int tn = next(t + 1);
-    if (tn < t1) {
-      issue(tn, par ^ 1);
-      vm_wait<C::NLD>();
+  struct Tile { int t; bool mixed; } q[NS];
+  auto next = [&](int t) { return dw.template next<BM, STEP>(t, t1, a.G, a.Sq, lane); };
+  int slot = 0, fly = 0;
+  auto fetch = [&](Tile& x, int t, int into) {
+    x.t = next(t);
+    x.mixed = dw.mixed;
+    if (x.t < t1) { issue(x.t, ring + into * C::SLOT); ++fly; }
+  };
+#pragma unroll
+  for (int i = 0; i < NS - 1; ++i) fetch(q[i], i ? q[i - 1].t + STEP : (WK ? t0 + wave : t0), i);
+  while (q[0].t < t1) {
+    const int last = slot ? slot - 1 : NS - 1;
+    if constexpr (WK) {
+      fetch(q[NS - 1], q[NS - 2].t + STEP, last);
+      vm_wait_tiles<C::NLD, NS - 1>(fly - 1);
     } else {
-      vm_wait<0>();
+      vm_wait_tiles<C::NLD, NS - 2>(fly - 1);
+      lds_barrier();
+      fetch(q[NS - 1], q[NS - 2].t + STEP, last);
     }
-    lds_barrier();
-    const char* qt = smem + par * C::STAGE;
+    const char* qt = ring + slot * C::SLOT;
     const char* gt = qt + C::TILE;
     const float* in = reinterpret_cast<const float*>(qt + 2 * C::TILE);
-    const int* info = reinterpret_cast<const int*>(smem + 2 * C::STAGE + par * C::INFO);
+    const int* info = reinterpret_cast<const int*>(qt + 2 * C::TILE + 256);
+    const int t = q[0].t;
+    const bool mixed = q[0].mixed;
     const int m0 = t * BM, m1 = min(m0 + BM, a.M);
     // causal: does any row of the tile see a key of this wave; do all see all of them
     const bool any = !a.causal || (m1 - 1) / a.G + off >= kw || kw < pre;
@@ -255,17 +298,23 @@ __global__ __launch_bounds__(256, DKV_WAVES) void attn_dkv_kernel(Args a) {
         R::template t_times<KG, false>(qt, u * 16, y, dk, lane);
       }
     }
-    lds_barrier();
-    par ^= 1;
-    t = tn;
-    mixed = dw.mixed;
+    if constexpr (WK) asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    --fly;
+    slot = slot + 1 == NS ? 0 : slot + 1;
+#pragma unroll
+    for (int i = 0; i + 1 < NS; ++i) q[i] = q[i + 1];
+  }
+  if constexpr (WK) {
+    join_waves<NW>(dk[0], reinterpret_cast<float*>(smem), wave, lane);
+    join_waves<NW>(dv[0], reinterpret_cast<float*>(smem), wave, lane);
   }
 #pragma unroll
   for (int w = 0; w < KG; ++w) {
     if (key[w] >= a.Sk) continue;
     const int64_t oi = (((int64_t)b * a.Sk + key[w]) * a.Hk + hk) * a.D;
 #pragma unroll
-    for (int dt = 0; dt < DT; ++dt)
+    for (int dt = 0; dt < DT; ++dt) {
+      if (WK && dt % NW != wave) continue;
 #pragma unroll
       for (int q4 = 0; q4 < 4; ++q4) {
         const int d = dt * 32 + 8 * q4 + 4 * h;
@@ -279,28 +328,33 @@ __global__ __launch_bounds__(256, DKV_WAVES) void attn_dkv_kernel(Args a) {
         R::put4(reinterpret_cast<T*>(a.dk) + oi + d, x);
         R::put4(reinterpret_cast<T*>(a.dv) + oi + d, y);
       }
+    }
   }
 }
 
-template <typename T, int DP, int RW> struct Dq {
+template <typename T, int DP, int NW, int RW, bool WK> struct Dq {
   typedef Rows<T, DP> R;
-  static constexpr int WROWS = 32 * RW, BM = 4 * WROWS, BN = 32;
-  static constexpr int TILE = BN * R::ROWB, LDS = 4 * TILE;
-  static constexpr int NLD = R::template loads2<BN, 256>();
+  static constexpr int NT = NW * 64, LT = WK ? 64 : NT;
+  static constexpr int WROWS = 32 * RW, BM = WK ? WROWS : NW * WROWS, BN = 32;
+  static constexpr int NS = WK ? 2 : (DP == 64 ? DQ_NS64 : DQ_NS128);
+  static constexpr int TILE = BN * R::ROWB, SLOT = 2 * TILE;
+  static constexpr int JOIN = R::DT * 16 * 64 * 4;
+  static constexpr int LDS = NS * SLOT * (WK ? NW : 1) > JOIN ? NS * SLOT * (WK ? NW : 1) : JOIN;
+  static constexpr int NLD = R::template loads2<BN, LT>();
 };
 
-template <typename T, int DP, int RW>
-__global__ __launch_bounds__(256, DQ_WAVES) void attn_dq_kernel(Args a) {
-  typedef Dq<T, DP, RW> C;
+template <typename T, int DP, int NW, int RW, bool WK>
+__global__ __launch_bounds__(NW * 64, DQ_WAVES) void attn_dq_kernel(Args a) {
+  typedef Dq<T, DP, NW, RW, WK> C;
   typedef Rows<T, DP> R;
-  constexpr int BN = C::BN, DT = R::DT;
+  constexpr int BN = C::BN, DT = R::DT, NS = C::NS, STEP = WK ? NW : 1;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
   const int item = xcd_item(a);
   if (item >= a.total) return;
   const int mt = a.mtiles - 1 - item % a.mtiles, bh = item / a.mtiles, b = bh / a.Hk, hk = bh - b * a.Hk;
   const int off = a.Sk - a.Sq, m0 = mt * C::BM, m1 = min(m0 + C::BM, a.M);
-  const int mw = m0 + wave * C::WROWS, mw1 = min(mw + C::WROWS, a.M);
+  const int mw = m0 + (WK ? 0 : wave * C::WROWS), mw1 = min(mw + C::WROWS, a.M);
   const int pre = a.prefix ? a.prefix[b] : 0;
   int kend = a.Sk;
   if (a.causal) kend = min(a.Sk, max((m1 - 1) / a.G + off + 1, pre));
@@ -329,16 +383,19 @@ __global__ __launch_bounds__(256, DQ_WAVES) void attn_dq_kernel(Args a) {
   const char* kbase = reinterpret_cast<const char*>(a.k) + ((int64_t)b * a.kb + (int64_t)hk * a.kh) * R::ES;
   const char* vbase = reinterpret_cast<const char*>(a.v) + ((int64_t)b * a.vb + (int64_t)hk * a.vh) * R::ES;
   const int64_t kst = a.ks * R::ES, vst = a.vs * R::ES;
-  const int64_t koff = R::template lane_off<256>(tid, kst), voff = R::template lane_off<256>(tid, vst);
+  const int ltid = WK ? lane : tid;
+  typename R::template Lin<C::LT> klin, vlin;
+  klin.init(ltid, kst);
+  vlin.init(ltid, vst);
+  char* ring = smem + (WK ? wave * NS * C::SLOT : 0);
   auto issue = [&](int t, char* dst) {
     const bool holes = dw.holes;
-    if constexpr (R::template linear<256>()) {
-      if (!holes && t * BN + BN <= a.Sk && a.D == DP) {
-        R::template load2_linear<BN, 256>(dst, dst + C::TILE, tid, kbase + koff + (int64_t)t * BN * kst, vbase + voff + (int64_t)t * BN * vst, kst, vst);
-        return;
-      }
+    if (!holes && t * BN + BN <= a.Sk && a.D == DP) {
+      klin.template load<BN>(dst, ltid, kbase + (int64_t)t * BN * kst, kst);
+      vlin.template load<BN>(dst + C::TILE, ltid, vbase + (int64_t)t * BN * vst, vst);
+      return;
     }
-    R::template load2<BN, 256>(dst, dst + C::TILE, tid, a.D, [&](int r, const char*& p0, const char*& p1) {
+    R::template load2<BN, C::LT>(dst, dst + C::TILE, ltid, a.D, [&](int r, const char*& p0, const char*& p1) {
       const int key = t * BN + r;
       if (key >= a.Sk || (holes && a.kdoc[(int64_t)b * a.Sk + key] < 0)) return;
       p0 = kbase + (int64_t)key * a.ks * R::ES;
@@ -351,22 +408,30 @@ __global__ __launch_bounds__(256, DQ_WAVES) void attn_dq_kernel(Args a) {
 #pragma unroll
     for (int j = 0; j < DT; ++j) dq[w][j] = zero16();
 
-  auto next = [&](int t) { return dw.template next<BN, 1>(t, t1, 1, a.Sk, lane); };
-  int t = next(0), par = 0;
-  if (t < t1) issue(t, smem);
-  bool mixed = dw.mixed;
-  while (t < t1) {
-    const int tn = next(t + 1);
-    if (tn < t1) {
-      issue(tn, smem + (par ^ 1) * 2 * C::TILE);
-      vm_wait<C::NLD>();
+  struct Tile { int t; bool mixed; } q[NS];
+  auto next = [&](int t) { return dw.template next<BN, STEP>(t, t1, 1, a.Sk, lane); };
+  int slot = 0, fly = 0;
+  auto fetch = [&](Tile& x, int t, int into) {
+    x.t = next(t);
+    x.mixed = dw.mixed;
+    if (x.t < t1) { issue(x.t, ring + into * C::SLOT); ++fly; }
+  };
+#pragma unroll
+  for (int i = 0; i < NS - 1; ++i) fetch(q[i], i ? q[i - 1].t + STEP : (WK ? wave : 0), i);
+  while (q[0].t < t1) {
+    const int last = slot ? slot - 1 : NS - 1;
+    if constexpr (WK) {
+      fetch(q[NS - 1], q[NS - 2].t + STEP, last);
+      vm_wait_tiles<C::NLD, NS - 1>(fly - 1);
     } else {
-      vm_wait<0>();
+      vm_wait_tiles<C::NLD, NS - 2>(fly - 1);
+      lds_barrier();
+      fetch(q[NS - 1], q[NS - 2].t + STEP, last);
     }
-    lds_barrier();
-    const char* kt = smem + par * 2 * C::TILE;
+    const char* kt = ring + slot * C::SLOT;
     const char* vt = kt + C::TILE;
-    const int k0 = t * BN;
+    const bool mixed = q[0].mixed;
+    const int k0 = q[0].t * BN;
     if (k0 < some) {
       f32x16 s[RW], dp[RW];
       R::template times<RW>(kt, 0, qf, s, lane);
@@ -423,18 +488,21 @@ __global__ __launch_bounds__(256, DQ_WAVES) void attn_dq_kernel(Args a) {
         R::template t_times<RW, false>(kt, u * 16, x, dq, lane);
       }
     }
-    lds_barrier();
-    par ^= 1;
-    t = tn;
-    mixed = dw.mixed;
+    if constexpr (WK) asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    --fly;
+    slot = slot + 1 == NS ? 0 : slot + 1;
+#pragma unroll
+    for (int i = 0; i + 1 < NS; ++i) q[i] = q[i + 1];
   }
+  if constexpr (WK) join_waves<NW>(dq[0], reinterpret_cast<float*>(smem), wave, lane);
 #pragma unroll
   for (int w = 0; w < RW; ++w) {
     if (mrow[w] >= a.M) continue;
     const int i = mrow[w] / a.G, g = mrow[w] - i * a.G;
     const int64_t oi = (((int64_t)b * a.Sq + i) * a.Hq + hk * a.G + g) * a.D;
 #pragma unroll
-    for (int dt = 0; dt < DT; ++dt)
+    for (int dt = 0; dt < DT; ++dt) {
+      if (WK && dt % NW != wave) continue;
 #pragma unroll
       for (int q4 = 0; q4 < 4; ++q4) {
         const int d = dt * 32 + 8 * q4 + 4 * h;
@@ -444,20 +512,21 @@ __global__ __launch_bounds__(256, DQ_WAVES) void attn_dq_kernel(Args a) {
         for (int e = 0; e < 4; ++e) x[e] = row[w].on ? dq[w][dt][4 * q4 + e] * a.scale : 0.f;
         R::put4(reinterpret_cast<T*>(a.dq) + oi + d, x);
       }
+    }
   }
 }
 
-template <typename T, int DP, int KG>
+template <typename T, int DP, int NW, bool WK>
 int run_dkv(Args& a, hipStream_t st) {
-  typedef Dkv<T, DP, KG> C;
+  typedef Dkv<T, DP, NW, WK> C;
   a.mtiles = (a.Sk + C::BK - 1) / C::BK;
-  return launch(attn_dkv_kernel<T, DP, KG>, (int64_t)a.mtiles * a.B * a.Hk, 256, C::LDS, a, st);
+  return launch(attn_dkv_kernel<T, DP, NW, WK>, (int64_t)a.mtiles * a.B * a.Hk, C::NT, C::LDS, a, st);
 }
-template <typename T, int DP, int RW>
+template <typename T, int DP, int NW, int RW, bool WK>
 int run_dq(Args& a, hipStream_t st) {
-  typedef Dq<T, DP, RW> C;
+  typedef Dq<T, DP, NW, RW, WK> C;
   a.mtiles = (a.M + C::BM - 1) / C::BM;
-  return launch(attn_dq_kernel<T, DP, RW>, (int64_t)a.mtiles * a.B * a.Hk, 256, C::LDS, a, st);
+  return launch(attn_dq_kernel<T, DP, NW, RW, WK>, (int64_t)a.mtiles * a.B * a.Hk, C::NT, C::LDS, a, st);
 }
 
 template <typename T, int DP>
@@ -467,14 +536,15 @@ int bwd(Args& a, float* delta, hipStream_t st) {
   int rc = (int)hipGetLastError();
   if (rc) return rc;
   a.delta = delta;
-  constexpr int W2 = sizeof(T) == 2 && (DP == 64 || KG128) ? 2 : 1;
-  const bool kw = W2 == 2 && (a.Sk + 255) / 256 * bh >= KWMIN, qw = W2 == 2 && (a.M + 255) / 256 * bh >= QWMIN;
+  constexpr int WK = sizeof(T) == 4 && DP == 128 ? 2 : 4;
   if (a.dk) {
-    rc = kw ? run_dkv<T, DP, W2>(a, st) : run_dkv<T, DP, 1>(a, st);
+    const bool few = ((int64_t)a.Sk + 127) / 128 * bh < WKMAX;
+    rc = few ? run_dkv<T, DP, WK, true>(a, st) : run_dkv<T, DP, 4, false>(a, st);
     if (rc) return rc;
   }
   if (!a.dq) return 0;
-  return qw ? run_dq<T, DP, W2>(a, st) : run_dq<T, DP, 1>(a, st);
+  const bool few = ((int64_t)a.M + 127) / 128 * bh < WKMAX;
+  return few ? run_dq<T, DP, WK, 1, true>(a, st) : run_dq<T, DP, 4, 1, false>(a, st);
 }
 
 }  // namespace

@@ -20,22 +20,36 @@
 namespace turtle {
 namespace {
 
+#ifndef NS64
+#define NS64 3
+#endif
+#ifndef BN128
+#define BN128 64
+#endif
+#ifndef NS128
+#define NS128 2
+#endif
+#ifndef NSWK
+#define NSWK 2
+#endif
 template <typename T, int DP, int NW, int RW, bool WK> struct Fwd {
   typedef Rows<T, DP> R;
   static constexpr int NT = NW * 64;
   static constexpr int WROWS = 32 * RW;               // rows of a wave
   static constexpr int BM = WK ? WROWS : NW * WROWS;  // rows of a block
-  static constexpr int BN = (WK || sizeof(T) == 4) ? 32 : 64;
-  static constexpr int TILE = BN * R::ROWB;
-  static constexpr int BUF = 4 * TILE;                // two stages of K and V
+  static constexpr int BN = (WK || sizeof(T) == 4) ? 32 : (DP == 64 ? 64 : BN128);
+  static constexpr int NS = WK ? NSWK : (DP == 64 ? NS64 : NS128);     // slots of the ring
+  static constexpr int TILE = BN * R::ROWB, SLOT = 2 * TILE;
   static constexpr int LT = WK ? 64 : NT;             // threads that load a tile
   static constexpr int NLD = R::template loads2<BN, LT>();
   static constexpr int WIN = 256;                     // page numbers a wave keeps at hand
   static constexpr bool TWO = sizeof(T) == 2 && (WK || NW == 2);
-  static int lds(bool paged, int64_t keys) {
-    const int buf = WK ? NW * BUF : (keys <= BN ? BUF / 2 : BUF);
-    const int join = WK ? (2 * NW * 32 + R::DT * 16 * 64) * 4 : 0;
-    return (buf > join ? buf : join) + (paged ? NW * WIN * 4 : 0);
+  // LDS without the page numbers; a call with fewer tiles than slots takes only those
+  static int lds(int64_t keys) {
+    const int64_t tiles = (keys + BN - 1) / BN;
+    if (!WK) return SLOT * (int)(tiles < NS ? tiles : NS);
+    const int buf = NW * NS * SLOT, join = (2 * NW * 32 + R::DT * 16 * 64) * 4;
+    return buf > join ? buf : join;
   }
 };
 
@@ -108,11 +122,14 @@ __global__ __launch_bounds__(NW * 64, FWD_WAVES) void attn_fwd_kernel(Args a) {
             a.D, qf[w], lane);
   }
 
-  char* buf = smem + (WK ? wave * F::BUF : 0);
+  char* buf = smem + (WK ? wave * F::NS * F::SLOT : 0);
   const char* kbase = reinterpret_cast<const char*>(a.k) + ((PAGED ? 0 : (int64_t)b * a.kb) + (int64_t)hk * a.kh) * R::ES;
   const char* vbase = reinterpret_cast<const char*>(a.v) + ((PAGED ? 0 : (int64_t)b * a.vb) + (int64_t)hk * a.vh) * R::ES;
   const int64_t kst = a.ks * R::ES, vst = a.vs * R::ES;
-  const int64_t koff = R::template lane_off<F::LT>(tid, kst), voff = R::template lane_off<F::LT>(tid, vst);
+  const int ltid = WK ? lane : tid;
+  typename R::template Lin<F::LT> klin, vlin;
+  klin.init(ltid, kst);
+  vlin.init(ltid, vst);
   // page numbers: this wave's window of the sequence's table, read from LDS - a global read per tile would have to
   // wait, in order, behind the tiles in flight
   int* win = reinterpret_cast<int*>(smem + a.lds_win) + wave * F::WIN;
@@ -133,7 +150,16 @@ __global__ __launch_bounds__(NW * 64, FWD_WAVES) void attn_fwd_kernel(Args a) {
         }
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
       }
-      R::template load2<BN, F::LT>(dst, dst + F::TILE, WK ? lane : tid, a.D, [&](int r, const char*& p0, const char*& p1) {
+      const int in0 = k0 - p0 * a.page;
+      if (in0 + BN <= a.page && k0 + BN <= kn && a.D == DP) {       // a whole tile of one page
+        const int id = __builtin_amdgcn_readfirstlane(win[p0 - wbase]);
+        if ((uint32_t)id < (uint32_t)a.npages) {
+          klin.template load<BN>(dst, ltid, kbase + (int64_t)id * a.kb * R::ES + in0 * kst, kst);
+          vlin.template load<BN>(dst + F::TILE, ltid, vbase + (int64_t)id * a.vb * R::ES + in0 * vst, vst);
+          return ~0ull;
+        }
+      }
+      R::template load2<BN, F::LT>(dst, dst + F::TILE, ltid, a.D, [&](int r, const char*& p0, const char*& p1) {
         const int key = k0 + r;
         if (key >= kn) return;
         const int pg = page_of(key), id = win[pg - wbase], in = key - pg * a.page;
@@ -147,13 +173,12 @@ __global__ __launch_bounds__(NW * 64, FWD_WAVES) void attn_fwd_kernel(Args a) {
       return __ballot(ok);
     } else {
       const bool holes = dw.holes;
-      if constexpr (R::template linear<F::LT>()) {
-        if (!holes && k0 + BN <= kn && a.D == DP) {
-          R::template load2_linear<BN, F::LT>(dst, dst + F::TILE, tid, kbase + koff + (int64_t)k0 * kst, vbase + voff + (int64_t)k0 * vst, kst, vst);
-          return ~0ull;
-        }
+      if (!holes && k0 + BN <= kn && a.D == DP) {
+        klin.template load<BN>(dst, ltid, kbase + k0 * kst, kst);
+        vlin.template load<BN>(dst + F::TILE, ltid, vbase + k0 * vst, vst);
+        return ~0ull;
       }
-      R::template load2<BN, F::LT>(dst, dst + F::TILE, WK ? lane : tid, a.D, [&](int r, const char*& p0, const char*& p1) {
+      R::template load2<BN, F::LT>(dst, dst + F::TILE, ltid, a.D, [&](int r, const char*& p0, const char*& p1) {
         const int key = k0 + r;
         if (key >= kn || (holes && a.kdoc[(int64_t)b * a.Sk + key] < 0)) return;
         p0 = kbase + (int64_t)key * a.ks * R::ES;
@@ -173,24 +198,35 @@ __global__ __launch_bounds__(NW * 64, FWD_WAVES) void attn_fwd_kernel(Args a) {
     l[w] = 0.f;
   }
 
+  // the walk: tile q[0] is computed on, q[1 ..] are in flight; it ends where q[0] reaches t1
+  constexpr int NS = F::NS;
+  struct Tile { int t; bool mixed; uint64_t seen; } q[NS];
   auto next = [&](int t) { return dw.template next<BN, STEP>(t, t1, 1, a.Sk, lane); };
-  int t = next(WK ? t0 + wave : t0), par = 0;
-  uint64_t seen = ~0ull;
-  if (t < t1) seen = issue(t, buf);
-  bool mixed = dw.mixed;
-  while (t < t1) {
-    const int tn = next(t + STEP);
-    uint64_t seen_n = ~0ull;
-    if (tn < t1) {
-      seen_n = issue(tn, buf + (par ^ 1) * 2 * F::TILE);
-      vm_wait<F::NLD>();
+  int slot = 0, fly = 0;         // slot of q[0]; tiles in flight
+  auto fetch = [&](Tile& x, int t, int into) {
+    x.t = next(t);
+    x.seen = ~0ull;
+    x.mixed = dw.mixed;
+    if (x.t < t1) { x.seen = issue(x.t, buf + into * F::SLOT); ++fly; }
+  };
+#pragma unroll
+  for (int i = 0; i < NS - 1; ++i) fetch(q[i], i ? q[i - 1].t + STEP : (WK ? t0 + wave : t0), i);
+  while (q[0].t < t1) {
+    const int last = slot ? slot - 1 : NS - 1;      // the slot of the tile before
+    // a wave of its own starts the newest tile first; with a block the barrier frees its slot
+    if constexpr (WK) {
+      fetch(q[NS - 1], q[NS - 2].t + STEP, last);
+      vm_wait_tiles<F::NLD, NS - 1>(fly - 1);
     } else {
-      vm_wait<0>();
+      vm_wait_tiles<F::NLD, NS - 2>(fly - 1);
+      lds_barrier();
+      fetch(q[NS - 1], q[NS - 2].t + STEP, last);
     }
-    if constexpr (!WK) lds_barrier();
-    const char* kt = buf + par * 2 * F::TILE;
+    const char* kt = buf + slot * F::SLOT;
     const char* vt = kt + F::TILE;
-    const int k0 = t * BN;
+    const int k0 = q[0].t * BN;
+    const bool mixed = q[0].mixed;
+    uint64_t seen = q[0].seen;
 
     if (k0 < some) {
       f32x16 s[KT][RW];
@@ -290,12 +326,11 @@ __global__ __launch_bounds__(NW * 64, FWD_WAVES) void attn_fwd_kernel(Args a) {
           R::template t_times<RW, F::TWO>(vt, j * 32 + u * 16, p, acc, lane);
         }
     }
-    if constexpr (!WK) lds_barrier();
-    else asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    par ^= 1;
-    t = tn;
-    seen = seen_n;
-    mixed = dw.mixed;
+    if constexpr (WK) asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    --fly;
+    slot = slot + 1 == NS ? 0 : slot + 1;
+#pragma unroll
+    for (int i = 0; i + 1 < NS; ++i) q[i] = q[i + 1];
   }
 #pragma unroll
   for (int w = 0; w < RW; ++w) l[w] = half_sum(l[w]);
@@ -430,7 +465,7 @@ Plan plan_of(const In* x, int dtype) {
   p.mtiles = (M + bm - 1) / bm;
   // too few blocks to fill the 256 CUs: the keys are split over blocks too, 512 at least each, and joined by a second
   // kernel
-  const int64_t want = std::max<int64_t>(1, 256 / (p.mtiles * bh)), most = std::max<int64_t>(1, room / 512);
+  const int64_t want = std::max<int64_t>(1, (p.kind == 0 && dtype != 0 && x->D <= 64 ? 512 : 256) / (p.mtiles * bh)), most = std::max<int64_t>(1, room / 512);
   p.nsplit = (int)std::min<int64_t>({want, most, 64});
   return p;
 }
@@ -448,8 +483,8 @@ size_t ws_bytes(const In* x, int dtype) {
 template <typename T, int DP, int NW, int RW, bool WK, bool PAGED>
 int run(Args& a, const Plan& p, int64_t keys, hipStream_t st) {
   typedef Fwd<T, DP, NW, RW, WK> F;
-  const int lds = F::lds(PAGED, keys);
-  a.lds_win = lds - (PAGED ? NW * F::WIN * 4 : 0);
+  a.lds_win = F::lds(keys);
+  const int lds = a.lds_win + (PAGED ? NW * F::WIN * 4 : 0);
   return launch(attn_fwd_kernel<T, DP, NW, RW, WK, PAGED>, p.mtiles * a.B * a.Hk * p.nsplit, F::NT, lds, a, st);
 }
 
