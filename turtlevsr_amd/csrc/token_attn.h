@@ -116,17 +116,36 @@ struct Rows {
   }
   // row r's 16-byte chunk c
   TURTLE_DEV static uint4 chunk(const char* t, int r, int c) { return *reinterpret_cast<const uint4*>(t + r * ROWB + ((c ^ swz(r)) << 4)); }
-  // acc[w] = (32 rows from r0)(channels) x frag[w]: frag is the B operand's STEPS chunks
-  template <int RW>
-  TURTLE_DEV static void times(const char* t, int r0, const uint4 (&frag)[RW][STEPS], f32x16 (&acc)[RW], int lane) {
+  // acc[j][w] = (rows 32 j .. 32 j + 31)(channels) x frag[w], the KT RW chains of products interleaved: frag is the B
+  // operand's STEPS chunks
+  template <int KT, int RW>
+  TURTLE_DEV static void times(const char* t, const uint4 (&frag)[RW][STEPS], f32x16 (&acc)[KT][RW], int lane) {
 #pragma unroll
-    for (int w = 0; w < RW; ++w) acc[w] = zero16();
+    for (int j = 0; j < KT; ++j)
 #pragma unroll
-    for (int s = 0; s < STEPS; ++s) {
-      const uint4 x = chunk(t, r0 + (lane & 31), 2 * s + (lane >> 5));
+      for (int w = 0; w < RW; ++w) acc[j][w] = zero16();
 #pragma unroll
-      for (int w = 0; w < RW; ++w) acc[w] = mma<T>(x, frag[w][s], acc[w]);
-    }
+    for (int s = 0; s < STEPS; ++s)
+#pragma unroll
+      for (int j = 0; j < KT; ++j) {
+        const uint4 x = chunk(t, j * 32 + (lane & 31), 2 * s + (lane >> 5));
+#pragma unroll
+        for (int w = 0; w < RW; ++w) acc[j][w] = mma<T>(x, frag[w][s], acc[j][w]);
+      }
+  }
+  // the same of two tiles with an operand each
+  template <int KT>
+  TURTLE_DEV static void times2(const char* t0, const char* t1, const uint4 (&f0)[STEPS], const uint4 (&f1)[STEPS], f32x16 (&a0)[KT],
+                                f32x16 (&a1)[KT], int lane) {
+#pragma unroll
+    for (int j = 0; j < KT; ++j) { a0[j] = zero16(); a1[j] = zero16(); }
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s)
+#pragma unroll
+      for (int j = 0; j < KT; ++j) {
+        a0[j] = mma<T>(chunk(t0, j * 32 + (lane & 31), 2 * s + (lane >> 5)), f0[s], a0[j]);
+        a1[j] = mma<T>(chunk(t1, j * 32 + (lane & 31), 2 * s + (lane >> 5)), f1[s], a1[j]);
+      }
   }
   // acc[w][dt] += (rows r0 .. r0 + 15)^T (channels 32 dt ..) x p[w]: p = 8 accumulator registers' values of those rows.
   // TWO: p in two terms (its rounding and the remainder), for products that keep p's fp32 value (16-bit types)
@@ -193,12 +212,12 @@ struct Rows {
     }
   }
   // DMA of N rows of two tensors (LDS tiles t0, t1) by NT threads: src(r, p0, p1) sets the addresses of row r's first
-  // channels, or null
+  // channels, or null. For the odd tile: kept small rather than unrolled
   template <int N, int NT, typename F>
   TURTLE_DEV static void load2(char* t0, char* t1, int tid, int D, F src) {
     static_assert(N * CH % NT == 0, "whole DMA instructions");
     const uint32_t b0 = lds_addr(t0) + (uint32_t)(tid & ~63) * 16, b1 = lds_addr(t1) + (uint32_t)(tid & ~63) * 16;
-#pragma unroll
+#pragma unroll 1
     for (int i = 0; i < N * CH / NT; ++i) {
       const int ci = i * NT + tid, r = ci / CH, c = ((ci % CH) ^ swz(r)) * 16;
       const char *p0 = nullptr, *p1 = nullptr;
@@ -250,7 +269,7 @@ struct Args {
   int nqr, nkr;
   int causal;
   int page, npages, maxpages;
-  uint32_t pmul, psh;                     // j / page = mulhi(j, pmul) >> psh (page > 1)
+  uint32_t pmul, psh, gmul, gsh;          // j / page = mulhi(j, pmul) >> psh (page > 1); m / G likewise
   const int *table, *kv_lens, *q_lens;
   void *o, *olo;
   float* lse;
@@ -272,6 +291,10 @@ TURTLE_DEV int xcd_item(const Args& a) {
   return (int)(blockIdx.x & 7) * chunk + (int)(blockIdx.x >> 3);
 }
 
+TURTLE_DEV int quot(int n, int d, uint32_t mul, uint32_t sh) { return d == 1 ? n : (int)(__umulhi((uint32_t)n, mul) >> sh); }
+// the token of row m
+TURTLE_DEV int token_of(const Args& a, int m) { return quot(m, a.G, a.gmul, a.gsh); }
+
 // One row's (query's) place and rules, in the lane that owns it
 struct Row {
   int pos;       // its place among the keys
@@ -282,7 +305,7 @@ struct Row {
 
 TURTLE_DEV Row row_of(const Args& a, int b, int hk, int m, int off, int nq) {
   Row r;
-  const int i = m / a.G, g = m - i * a.G;
+  const int i = token_of(a, m), g = m - i * a.G;
   r.on = m < a.M && i < nq;
   r.pos = i + off;
   r.doc = (a.qdoc && r.on) ? a.qdoc[(int64_t)b * a.Sq + i] : 0;
@@ -402,6 +425,14 @@ bool sizes_ok(const In* x, int dtype) {
 // keys that a sequence can have
 int64_t key_room(const In* x) { return x->table ? (int64_t)x->page * x->maxpages : x->Sk; }
 
+// n / d for n < 2^30: with l = ceil(log2 d), floor(n m / 2^(31 + l)) for m = floor(2^(31 + l) / d) + 1 is exact
+void reciprocal(int d, uint32_t& mul, uint32_t& sh) {
+  int l = 0;
+  while ((1ll << l) < d) ++l;
+  mul = d > 1 ? (uint32_t)((1ull << (31 + l)) / (uint64_t)d + 1) : 0;
+  sh = d > 1 ? (uint32_t)(l - 1) : 0;
+}
+
 bool fill(Args& a, const In* x, int dtype) {
   if (!sizes_ok(x, dtype)) return false;
   const int es = dtype == 0 ? 4 : 2;
@@ -421,13 +452,8 @@ bool fill(Args& a, const In* x, int dtype) {
   a.nqr = (x->Sq + RT - 1) / RT; a.nkr = x->table ? 0 : (x->Sk + RT - 1) / RT;
   a.qr = (const int4*)x->ranges; a.kr = a.qr ? a.qr + (int64_t)x->B * a.nqr : nullptr;
   a.page = x->page; a.npages = x->npages; a.maxpages = x->maxpages; a.table = x->table; a.kv_lens = x->kv_lens; a.q_lens = x->q_lens;
-  if (x->table && x->page > 1) {
-    // j / page for j < 2^30: with l = ceil(log2 page), floor(j m / 2^(31 + l)) for m = floor(2^(31 + l) / page) + 1 is exact
-    int l = 0;
-    while ((1ll << l) < x->page) ++l;
-    a.pmul = (uint32_t)((1ull << (31 + l)) / (uint64_t)x->page + 1);
-    a.psh = (uint32_t)(l - 1);
-  }
+  if (x->table) reciprocal(x->page, a.pmul, a.psh);
+  reciprocal(a.G, a.gmul, a.gsh);
   a.o = x->o; a.olo = dtype == 0 ? nullptr : x->o_lo; a.lse = x->lse;
   return true;
 }

@@ -2,22 +2,31 @@
 // then dq by row tiles. No atomics: every sum has a fixed order.
 #include "token_attn.h"
 #ifndef DKV_WAVES
-#define DKV_WAVES (sizeof(T)==2 && DP==64 ? 2 : 1)
+#define DKV_WAVES (sizeof(T) == 2 && (DP == 64 || !WK) ? 2 : 1)
 #endif
 #ifndef DQ_WAVES
-#define DQ_WAVES (sizeof(T)==2 && RW==1 ? 2 : 1)
+#define DQ_WAVES (sizeof(T) == 2 ? 2 : 1)
 #endif
 #ifndef DKV_NS64
-#define DKV_NS64 4
+#define DKV_NS64 3
 #endif
 #ifndef DKV_NS128
-#define DKV_NS128 4
+#define DKV_NS128 2
 #endif
 #ifndef DQ_NS64
-#define DQ_NS64 4
+#define DQ_NS64 3
 #endif
 #ifndef DQ_NS128
-#define DQ_NS128 (sizeof(T)==4?3:4)
+#define DQ_NS128 3
+#endif
+#ifndef DKV_MT
+#define DKV_MT 2
+#endif
+#ifndef DKV_VL
+#define DKV_VL 1
+#endif
+#ifndef DQ_KT
+#define DQ_KT 2
 #endif
 #ifndef WKMAX
 #define WKMAX 128
@@ -62,19 +71,21 @@ __global__ __launch_bounds__(256) void attn_delta_kernel(Args a, float* delta) {
 }
 
 // WK: for small grids - the block's NW waves own the same 32 keys and take the row tiles in turn, each with its own
-// ring and no barriers, and join at the end
+// ring and no barriers, and join at the end.
+// 128 channels: the operands of S and dP and the two accumulators would take 192 registers of the 256 that let two
+// waves share a SIMD; V stays in LDS there (VL).
 template <typename T, int DP, int NW, bool WK> struct Dkv {
   typedef Rows<T, DP> R;
   static constexpr int NT = NW * 64, LT = WK ? 64 : NT;
   static constexpr int BK = WK ? 32 : NW * 32;            // keys of a block
-  static constexpr int BM = 32;                           // rows of a tile
+  static constexpr int MT = (sizeof(T) == 2 && DP == 64) ? DKV_MT : 1, BM = 32 * MT;     // rows of a tile
   static constexpr int NS = WK ? 2 : (DP == 64 ? DKV_NS64 : DKV_NS128);
+  static constexpr bool VL = sizeof(T) == 2 && DP == 128 && !WK && DKV_VL;
   static constexpr int TILE = BM * R::ROWB;
-  static constexpr int INFO = 3 * BM * 4;                 // place, document, slope of each row
-  static constexpr int SLOT = 2 * TILE + 64 * 4 + INFO;   // Q, dO, 32 softmax sums and 32 deltas
-  static constexpr int JOIN = R::DT * 16 * 64 * 4;
-  static constexpr int LDS = NS * SLOT * (WK ? NW : 1) > JOIN ? NS * SLOT * (WK ? NW : 1) : JOIN;
-  static constexpr int NLD = R::template loads2<BM, LT>() + 1;
+  static constexpr int SLOT = 2 * TILE + 5 * BM * 4;      // Q, dO; softmax sum, delta, place, document, slope of a row
+  static constexpr int RING = NS * SLOT * (WK ? NW : 1), JOIN = R::DT * 16 * 64 * 4;
+  static constexpr int LDS = (RING > JOIN ? RING : JOIN) + (VL ? BK * R::ROWB : 0);
+  static constexpr int NLD = R::template loads2<BM, LT>() + MT;
 };
 
 // sum of the waves' accumulators through LDS, in wave order; every wave gets it
@@ -103,7 +114,7 @@ template <typename T, int DP, int NW, bool WK>
 __global__ __launch_bounds__(NW * 64, DKV_WAVES) void attn_dkv_kernel(Args a) {
   typedef Dkv<T, DP, NW, WK> C;
   typedef Rows<T, DP> R;
-  constexpr int BM = C::BM, DT = R::DT, KG = 1, NS = C::NS, STEP = WK ? NW : 1;
+  constexpr int BM = C::BM, MT = C::MT, DT = R::DT, NS = C::NS, STEP = WK ? NW : 1;
   // fp16: p times 2^10 as operand of dv (p of 10^4 keys would lose bits below the type's normal range)
   constexpr float POFF = std::is_same<T, f16>::value ? 10.f : 0.f, PS = std::is_same<T, f16>::value ? 1.f / 1024.f : 1.f;
   extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -114,16 +125,17 @@ __global__ __launch_bounds__(NW * 64, DKV_WAVES) void attn_dkv_kernel(Args a) {
   const int k0 = kt * C::BK, k1 = min(k0 + C::BK, a.Sk), off = a.Sk - a.Sq;
   const int kw = k0 + (WK ? 0 : wave * 32), kw1 = min(kw + 32, a.Sk);
   const int pre = a.prefix ? a.prefix[b] : 0;
-  int key[KG], kdoc[KG];
-  bool kon[KG];
-  uint4 kf[KG][R::STEPS], vf[KG][R::STEPS];
+  const int key = kw + (lane & 31), kdoc = (a.kdoc && key < a.Sk) ? a.kdoc[(int64_t)b * a.Sk + key] : 0;
+  const bool kon = key < a.Sk && kdoc >= 0;
+  uint4 kf[R::STEPS], vf[R::STEPS];
+  R::frag(kon ? reinterpret_cast<const T*>(a.k) + (int64_t)b * a.kb + (int64_t)key * a.ks + (int64_t)hk * a.kh : nullptr, a.D, kf, lane);
+  R::frag(kon ? reinterpret_cast<const T*>(a.v) + (int64_t)b * a.vb + (int64_t)key * a.vs + (int64_t)hk * a.vh : nullptr, a.D, vf, lane);
+  // VL: each lane's own chunks, at the places `chunk` reads them from
+  char* vlds = smem + C::LDS - C::BK * R::ROWB + wave * 32 * R::ROWB;
+  if constexpr (C::VL) {
 #pragma unroll
-  for (int w = 0; w < KG; ++w) {
-    key[w] = kw + w * 32 + (lane & 31);
-    kdoc[w] = (a.kdoc && key[w] < a.Sk) ? a.kdoc[(int64_t)b * a.Sk + key[w]] : 0;
-    kon[w] = key[w] < a.Sk && kdoc[w] >= 0;
-    R::frag(kon[w] ? reinterpret_cast<const T*>(a.k) + (int64_t)b * a.kb + (int64_t)key[w] * a.ks + (int64_t)hk * a.kh : nullptr, a.D, kf[w], lane);
-    R::frag(kon[w] ? reinterpret_cast<const T*>(a.v) + (int64_t)b * a.vb + (int64_t)key[w] * a.vs + (int64_t)hk * a.vh : nullptr, a.D, vf[w], lane);
+    for (int s = 0; s < R::STEPS; ++s)
+      *reinterpret_cast<uint4*>(vlds + (lane & 31) * R::ROWB + (((2 * s + h) ^ R::swz(lane & 31)) << 4)) = vf[s];
   }
 
   // rows that may see a key of this block
@@ -139,247 +151,260 @@ __global__ __launch_bounds__(NW * 64, DKV_WAVES) void attn_dkv_kernel(Args a) {
   const char* qbase = reinterpret_cast<const char*>(a.q) + ((int64_t)b * a.qb + (int64_t)hk * a.G * a.qh) * R::ES;
   const char* gbase = reinterpret_cast<const char*>(a.dout) + ((int64_t)b * a.gb + (int64_t)hk * a.G * a.gh) * R::ES;
   // where a tile holds whole tokens, its rows lie at the same offsets from its first one every time
-  constexpr int NI = BM * R::CH / C::LT;
   const int ltid = WK ? lane : tid;
-  char* ring = smem + (WK ? wave * NS * C::SLOT : 0);
+  constexpr int NI = BM * R::CH / C::LT;
   const bool plain = BM % a.G == 0 && a.D == DP;
-  const int per = BM / a.G;
+  const int per = token_of(a, BM);
   int64_t qoff[NI], goff[NI];
 #pragma unroll
   for (int i = 0; i < NI; ++i) {
-    const int r = (i * C::LT + ltid) / R::CH, c = ((ltid % R::CH) ^ R::swz(r)) << 4, ti = r / a.G, g = r - ti * a.G;
+    const int r = (i * C::LT + ltid) / R::CH, c = ((ltid % R::CH) ^ R::swz(r)) << 4, ti = token_of(a, r), g = r - ti * a.G;
     qoff[i] = ((int64_t)ti * a.qs + (int64_t)g * a.qh) * R::ES + c;
     goff[i] = ((int64_t)ti * a.gs + (int64_t)g * a.gh) * R::ES + c;
   }
+  const int64_t qstep = (int64_t)per * a.qs * R::ES, gstep = (int64_t)per * a.gs * R::ES;
+  const float* sums = a.lse + (int64_t)bh * a.M;
+  const float* deltas = a.delta + (int64_t)bh * a.M;
+  char* ring = smem + (WK ? wave * NS * C::SLOT : 0);
   auto issue = [&](int t, char* dst) {
-    if (rules && ltid < 64) {
-      const int m = t * BM + (lane & 31), i = m / a.G, g = m - i * a.G;
+    if (rules && ltid < BM) {
+      const int m = t * BM + ltid, i = token_of(a, m), g = m - i * a.G;
       float s = 0.f;
       if (a.slopes) s = a.G <= 64 ? __shfl(sl, g, 64) : a.slopes[hk * a.G + g] * LOG2E;
       int d = 0;
       if (dw.mixed) d = m < a.M ? a.qdoc[(int64_t)b * a.Sq + i] : -1;
-      int* info = reinterpret_cast<int*>(dst + 2 * C::TILE + 256);
-      if (lane < BM) { info[lane] = i + off; info[BM + lane] = d; info[2 * BM + lane] = __float_as_int(s); }
+      int* info = reinterpret_cast<int*>(dst + 2 * C::TILE) + 2 * BM + ltid;
+      info[0] = i + off;
+      info[BM] = d;
+      info[2 * BM] = __float_as_int(s);
     }
-    const bool holes = dw.holes;
-    if (plain && !holes && t * BM + BM <= a.M && (!a.causal || t * per + off >= 0 || pre > 0)) {
+    const int m0 = t * BM;
+    if (plain && !dw.holes && m0 + BM <= a.M && (!a.causal || t * per + off >= 0 || pre > 0)) {
+      const char *qp = qbase + t * qstep, *gp = gbase + t * gstep;
 #pragma unroll
       for (int i = 0; i < NI; ++i) {
         const uint32_t at = (uint32_t)(i * C::LT + (ltid & ~63)) * 16;
-        dma16(qbase + qoff[i] + (int64_t)t * per * a.qs * R::ES, __builtin_amdgcn_readfirstlane(lds_addr(dst) + at));
-        dma16(gbase + goff[i] + (int64_t)t * per * a.gs * R::ES, __builtin_amdgcn_readfirstlane(lds_addr(dst + C::TILE) + at));
+        dma16(qp + qoff[i], __builtin_amdgcn_readfirstlane(lds_addr(dst) + at));
+        dma16(gp + goff[i], __builtin_amdgcn_readfirstlane(lds_addr(dst + C::TILE) + at));
       }
-    } else
-    R::template load2<BM, C::LT>(dst, dst + C::TILE, ltid, a.D, [&](int r, const char*& p0, const char*& p1) {
-      const int m = t * BM + r, i = m / a.G, g = m - i * a.G;
-      // rows that see nothing may hold anything: they are not read
-      if (m >= a.M || (a.causal && i + off < 0 && pre <= 0) || (holes && a.qdoc[(int64_t)b * a.Sq + i] < 0)) return;
-      p0 = qbase + ((int64_t)i * a.qs + (int64_t)g * a.qh) * R::ES;
-      p1 = gbase + ((int64_t)i * a.gs + (int64_t)g * a.gh) * R::ES;
-    });
-    // every wave writes the same 64 values, so that all count the same number of loads
-    const int m = t * BM + (lane & 31);
-    const float* src = m < a.M ? (h ? a.delta : a.lse) + (int64_t)bh * a.M + m : g_row_pad + h;
-    dma4(src, __builtin_amdgcn_readfirstlane(lds_addr(dst + 2 * C::TILE)));
+    } else {
+      const bool holes = dw.holes;
+      R::template load2<BM, C::LT>(dst, dst + C::TILE, ltid, a.D, [&](int r, const char*& p0, const char*& p1) {
+        const int m = m0 + r, i = token_of(a, m), g = m - i * a.G;
+        // rows that see nothing may hold anything: they are not read
+        if (m >= a.M || (a.causal && i + off < 0 && pre <= 0) || (holes && a.qdoc[(int64_t)b * a.Sq + i] < 0)) return;
+        p0 = qbase + ((int64_t)i * a.qs + (int64_t)g * a.qh) * R::ES;
+        p1 = gbase + ((int64_t)i * a.gs + (int64_t)g * a.gh) * R::ES;
+      });
+    }
+    // every wave writes the same sums and deltas, so that all count the same number of loads
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+      const int e = i * 64 + lane, m = m0 + (e & (BM - 1)), which = e / BM;
+      const float* src = m < a.M ? (which ? deltas : sums) + m : g_row_pad + which;
+      dma4(src, __builtin_amdgcn_readfirstlane(lds_addr(dst + 2 * C::TILE) + i * 256));
+    }
   };
 
-  f32x16 dk[KG][DT], dv[KG][DT];
+  f32x16 dk[1][DT], dv[1][DT];
 #pragma unroll
-  for (int w = 0; w < KG; ++w)
-#pragma unroll
-    for (int i = 0; i < DT; ++i) { dk[w][i] = zero16(); dv[w][i] = zero16(); }
+  for (int i = 0; i < DT; ++i) { dk[0][i] = zero16(); dv[0][i] = zero16(); }
 
-  struct Tile { int t; bool mixed; } q[NS];
-  auto next = [&](int t) { return dw.template next<BM, STEP>(t, t1, a.G, a.Sq, lane); };
-  int slot = 0, fly = 0;
-  auto fetch = [&](Tile& x, int t, int into) {
-    x.t = next(t);
+  // the walk over row tiles: as the forward's over key tiles
+  struct Tile { int t; bool mixed; } q[NS - 1];
+  int tnew = WK ? t0 + wave : t0, fill = NS - 1, fly = 0, into = 0, slot = 0;
+  for (;;) {
+    const bool live = fill == 0;
+    if (live) {
+      if (q[0].t >= t1) break;
+      if constexpr (!WK) {
+        vm_wait_tiles<C::NLD, NS - 2>(fly - 1);
+        lds_barrier();
+      }
+    }
+    Tile x{dw.template next<BM, STEP>(tnew, t1, a.G, a.Sq, lane), false};
     x.mixed = dw.mixed;
     if (x.t < t1) { issue(x.t, ring + into * C::SLOT); ++fly; }
-  };
+    tnew = x.t + STEP;
+    into = into + 1 == NS ? 0 : into + 1;
+    const Tile cur = q[0];
 #pragma unroll
-  for (int i = 0; i < NS - 1; ++i) fetch(q[i], i ? q[i - 1].t + STEP : (WK ? t0 + wave : t0), i);
-  while (q[0].t < t1) {
-    const int last = slot ? slot - 1 : NS - 1;
-    if constexpr (WK) {
-      fetch(q[NS - 1], q[NS - 2].t + STEP, last);
-      vm_wait_tiles<C::NLD, NS - 1>(fly - 1);
-    } else {
-      vm_wait_tiles<C::NLD, NS - 2>(fly - 1);
-      lds_barrier();
-      fetch(q[NS - 1], q[NS - 2].t + STEP, last);
-    }
+    for (int i = 0; i + 2 < NS; ++i) q[i] = q[i + 1];
+    q[NS - 2] = x;
+    if (!live) { --fill; continue; }
+    if constexpr (WK) vm_wait_tiles<C::NLD, NS - 1>(fly - 1);
     const char* qt = ring + slot * C::SLOT;
     const char* gt = qt + C::TILE;
-    const float* in = reinterpret_cast<const float*>(qt + 2 * C::TILE);
-    const int* info = reinterpret_cast<const int*>(qt + 2 * C::TILE + 256);
-    const int t = q[0].t;
-    const bool mixed = q[0].mixed;
-    const int m0 = t * BM, m1 = min(m0 + BM, a.M);
-    // causal: does any row of the tile see a key of this wave; do all see all of them
-    const bool any = !a.causal || (m1 - 1) / a.G + off >= kw || kw < pre;
-    if (any && kw < a.Sk) {
-      f32x16 s[KG], dp[KG];
-      R::template times<KG>(qt, 0, kf, s, lane);
-      R::template times<KG>(gt, 0, vf, dp, lane);
-      const bool caus = a.causal && m0 / a.G + off + 1 < kw1 && kw1 > pre;
+    const float* in = reinterpret_cast<const float*>(qt + 2 * C::TILE) + 4 * h;
+    const int* info = reinterpret_cast<const int*>(in) + 2 * BM;
+    const bool mixed = cur.mixed;
+    // causal: places of the tile's first and last row
+    const int p0 = token_of(a, cur.t * BM) + off, p1 = token_of(a, min(cur.t * BM + BM, a.M) - 1) + off;
+    if ((!a.causal || p1 >= kw || kw < pre) && kw < a.Sk) {
+      f32x16 s[MT], dp[MT];
+      if constexpr (C::VL) {
+        uint4 vl[R::STEPS];
+#pragma unroll
+        for (int i = 0; i < R::STEPS; ++i) vl[i] = R::chunk(vlds, lane & 31, 2 * i + h);
+        R::template times2<MT>(qt, gt, kf, vl, s, dp, lane);
+      } else {
+        R::template times2<MT>(qt, gt, kf, vf, s, dp, lane);
+      }
+      const bool caus = a.causal && p0 + 1 < kw1 && kw1 > pre;
       float mul = a.scale2;
       if (a.cap > 0.f) {
-        tanh_all<T, KG>(s, a.icap);
+        tanh_all<T, MT>(s, a.icap);
         mul = a.cap2;
-      }
-      // dp -> (dp - delta) times the cap's slope
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        const float4 del = *reinterpret_cast<const float4*>(in + BM + 8 * c + 4 * h);
-        const float de[4] = {del.x, del.y, del.z, del.w};
+        for (int j = 0; j < MT; ++j)
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
+          for (int c = 0; c < 4; ++c) {
+            const float4 del = *reinterpret_cast<const float4*>(in + BM + j * 32 + 8 * c);
+            const float de[4] = {del.x, del.y, del.z, del.w};
 #pragma unroll
-          for (int w = 0; w < KG; ++w) {
-            const int r = 4 * c + e;
-            dp[w][r] = (dp[w][r] - de[e]) * PS;
-            if (a.cap > 0.f) dp[w][r] *= fmaf(-s[w][r], s[w][r], 1.f);
+            for (int e = 0; e < 4; ++e) {
+              const int r = 4 * c + e;
+              dp[j][r] = (dp[j][r] - de[e]) * fmaf(-s[j][r] * PS, s[j][r], PS);      // times the cap's slope
+            }
+          }
+      } else {
+#pragma unroll
+        for (int j = 0; j < MT; ++j)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            const float4 del = *reinterpret_cast<const float4*>(in + BM + j * 32 + 8 * c);
+            const float de[4] = {del.x, del.y, del.z, del.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) dp[j][4 * c + e] = (dp[j][4 * c + e] - de[e]) * PS;
           }
       }
       if (a.slopes) {
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          const int4 pos = *reinterpret_cast<const int4*>(info + 8 * c + 4 * h);
-          const float4 slp = *reinterpret_cast<const float4*>(info + 2 * BM + 8 * c + 4 * h);
-          const int po[4] = {pos.x, pos.y, pos.z, pos.w};
-          const float sp[4] = {slp.x, slp.y, slp.z, slp.w};
+        for (int j = 0; j < MT; ++j)
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
+          for (int c = 0; c < 4; ++c) {
+            const int4 pos = *reinterpret_cast<const int4*>(info + j * 32 + 8 * c);
+            const float4 slp = *reinterpret_cast<const float4*>(info + 2 * BM + j * 32 + 8 * c);
+            const int po[4] = {pos.x, pos.y, pos.z, pos.w};
+            const float sp[4] = {slp.x, slp.y, slp.z, slp.w};
 #pragma unroll
-            for (int w = 0; w < KG; ++w) s[w][4 * c + e] = fmaf(-sp[e], fabsf((float)(po[e] - key[w])), s[w][4 * c + e] * mul);
-        }
+            for (int e = 0; e < 4; ++e) s[j][4 * c + e] = fmaf(-sp[e], fabsf((float)(po[e] - key)), s[j][4 * c + e] * mul);
+          }
         mul = 1.f;
       }
       if (caus || mixed) {
-        // the pairs that do not see each other: p = 0, and whatever dP holds there
+        // the pairs that do not see each other: p = 0, whatever dP holds there
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          const int4 pos = *reinterpret_cast<const int4*>(info + 8 * c + 4 * h), doc = *reinterpret_cast<const int4*>(info + BM + 8 * c + 4 * h);
-          const int po[4] = {pos.x, pos.y, pos.z, pos.w}, dc[4] = {doc.x, doc.y, doc.z, doc.w};
+        for (int j = 0; j < MT; ++j)
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
+          for (int c = 0; c < 4; ++c) {
+            const int4 pos = *reinterpret_cast<const int4*>(info + j * 32 + 8 * c), doc = *reinterpret_cast<const int4*>(info + BM + j * 32 + 8 * c);
+            const int po[4] = {pos.x, pos.y, pos.z, pos.w}, dc[4] = {doc.x, doc.y, doc.z, doc.w};
 #pragma unroll
-            for (int w = 0; w < KG; ++w) {
-              bool vis = !caus || max(po[e], pre - 1) >= key[w];
-              vis = vis && (!mixed || dc[e] == kdoc[w]);
-              s[w][4 * c + e] = vis ? s[w][4 * c + e] * mul : -INFINITY;
-              dp[w][4 * c + e] = vis ? dp[w][4 * c + e] : 0.f;
+            for (int e = 0; e < 4; ++e) {
+              const int r = 4 * c + e;
+              const bool vis = (!caus || max(po[e], pre - 1) >= key) && (!mixed || dc[e] == kdoc);
+              s[j][r] = vis ? s[j][r] * mul : -INFINITY;
+              dp[j][r] = vis ? dp[j][r] : 0.f;
             }
-        }
+          }
         mul = 1.f;
       }
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        const float4 lse = *reinterpret_cast<const float4*>(in + 8 * c + 4 * h);
-        const float ls[4] = {lse.x, lse.y, lse.z, lse.w};
+      for (int j = 0; j < MT; ++j)
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
+        for (int c = 0; c < 4; ++c) {
+          const float4 lse = *reinterpret_cast<const float4*>(in + j * 32 + 8 * c);
+          const float ls[4] = {lse.x, lse.y, lse.z, lse.w};
 #pragma unroll
-          for (int w = 0; w < KG; ++w) {
+          for (int e = 0; e < 4; ++e) {
             const int r = 4 * c + e;
-            s[w][r] = __builtin_amdgcn_exp2f(fmaf(s[w][r], mul, POFF - ls[e]));
-            dp[w][r] *= s[w][r];
+            s[j][r] = __builtin_amdgcn_exp2f(fmaf(s[j][r], mul, POFF - ls[e]));
+            dp[j][r] *= s[j][r];
           }
-      }
+        }
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        float x[KG][8], y[KG][8];
+      for (int u = 0; u < 2 * MT; ++u) {
+        float x[1][8], y[1][8];
 #pragma unroll
-        for (int w = 0; w < KG; ++w)
-#pragma unroll
-          for (int e = 0; e < 8; ++e) { x[w][e] = s[w][8 * u + e]; y[w][e] = dp[w][8 * u + e]; }
-        R::template t_times<KG, false>(gt, u * 16, x, dv, lane);
-        R::template t_times<KG, false>(qt, u * 16, y, dk, lane);
+        for (int e = 0; e < 8; ++e) { x[0][e] = s[u >> 1][8 * (u & 1) + e]; y[0][e] = dp[u >> 1][8 * (u & 1) + e]; }
+        R::template t_times<1, false>(gt, u * 16, x, dv, lane);
+        R::template t_times<1, false>(qt, u * 16, y, dk, lane);
       }
     }
     if constexpr (WK) asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     --fly;
     slot = slot + 1 == NS ? 0 : slot + 1;
-#pragma unroll
-    for (int i = 0; i + 1 < NS; ++i) q[i] = q[i + 1];
   }
   if constexpr (WK) {
     join_waves<NW>(dk[0], reinterpret_cast<float*>(smem), wave, lane);
     join_waves<NW>(dv[0], reinterpret_cast<float*>(smem), wave, lane);
   }
+  if (key >= a.Sk) return;
+  const int64_t oi = (((int64_t)b * a.Sk + key) * a.Hk + hk) * a.D;
 #pragma unroll
-  for (int w = 0; w < KG; ++w) {
-    if (key[w] >= a.Sk) continue;
-    const int64_t oi = (((int64_t)b * a.Sk + key[w]) * a.Hk + hk) * a.D;
+  for (int dt = 0; dt < DT; ++dt) {
+    if (WK && dt % NW != wave) continue;
 #pragma unroll
-    for (int dt = 0; dt < DT; ++dt) {
-      if (WK && dt % NW != wave) continue;
+    for (int q4 = 0; q4 < 4; ++q4) {
+      const int d = dt * 32 + 8 * q4 + 4 * h;
+      if (d >= a.D) continue;
+      float x[4], y[4];
 #pragma unroll
-      for (int q4 = 0; q4 < 4; ++q4) {
-        const int d = dt * 32 + 8 * q4 + 4 * h;
-        if (d >= a.D) continue;
-        float x[4], y[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          x[e] = kon[w] ? dk[w][dt][4 * q4 + e] * a.scale : 0.f;
-          y[e] = kon[w] ? dv[w][dt][4 * q4 + e] * PS : 0.f;
-        }
-        R::put4(reinterpret_cast<T*>(a.dk) + oi + d, x);
-        R::put4(reinterpret_cast<T*>(a.dv) + oi + d, y);
+      for (int e = 0; e < 4; ++e) {
+        x[e] = kon ? dk[0][dt][4 * q4 + e] * a.scale : 0.f;
+        y[e] = kon ? dv[0][dt][4 * q4 + e] * PS : 0.f;
       }
+      R::put4(reinterpret_cast<T*>(a.dk) + oi + d, x);
+      R::put4(reinterpret_cast<T*>(a.dv) + oi + d, y);
     }
   }
 }
 
-template <typename T, int DP, int NW, int RW, bool WK> struct Dq {
+template <typename T, int DP, int NW, bool WK> struct Dq {
   typedef Rows<T, DP> R;
   static constexpr int NT = NW * 64, LT = WK ? 64 : NT;
-  static constexpr int WROWS = 32 * RW, BM = WK ? WROWS : NW * WROWS, BN = 32;
+  static constexpr int BM = WK ? 32 : NW * 32;            // rows of a block
+  static constexpr int KT = (sizeof(T) == 2 && DP == 64) ? DQ_KT : 1, BN = 32 * KT;      // keys of a tile
   static constexpr int NS = WK ? 2 : (DP == 64 ? DQ_NS64 : DQ_NS128);
   static constexpr int TILE = BN * R::ROWB, SLOT = 2 * TILE;
-  static constexpr int JOIN = R::DT * 16 * 64 * 4;
-  static constexpr int LDS = NS * SLOT * (WK ? NW : 1) > JOIN ? NS * SLOT * (WK ? NW : 1) : JOIN;
+  static constexpr int RING = NS * SLOT * (WK ? NW : 1), JOIN = R::DT * 16 * 64 * 4;
+  static constexpr int LDS = RING > JOIN ? RING : JOIN;
   static constexpr int NLD = R::template loads2<BN, LT>();
 };
 
-template <typename T, int DP, int NW, int RW, bool WK>
+template <typename T, int DP, int NW, bool WK>
 __global__ __launch_bounds__(NW * 64, DQ_WAVES) void attn_dq_kernel(Args a) {
-  typedef Dq<T, DP, NW, RW, WK> C;
+  typedef Dq<T, DP, NW, WK> C;
   typedef Rows<T, DP> R;
-  constexpr int BN = C::BN, DT = R::DT, NS = C::NS, STEP = WK ? NW : 1;
+  constexpr int BN = C::BN, KT = C::KT, DT = R::DT, NS = C::NS, STEP = WK ? NW : 1;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
   const int item = xcd_item(a);
   if (item >= a.total) return;
   const int mt = a.mtiles - 1 - item % a.mtiles, bh = item / a.mtiles, b = bh / a.Hk, hk = bh - b * a.Hk;
   const int off = a.Sk - a.Sq, m0 = mt * C::BM, m1 = min(m0 + C::BM, a.M);
-  const int mw = m0 + (WK ? 0 : wave * C::WROWS), mw1 = min(mw + C::WROWS, a.M);
+  const int mw = m0 + (WK ? 0 : wave * 32), mw1 = min(mw + 32, a.M);
   const int pre = a.prefix ? a.prefix[b] : 0;
   int kend = a.Sk;
-  if (a.causal) kend = min(a.Sk, max((m1 - 1) / a.G + off + 1, pre));
+  if (a.causal) kend = min(a.Sk, max(token_of(a, m1 - 1) + off + 1, pre));
   const int t1 = (max(kend, 0) + BN - 1) / BN;
   DocWalk dw;
   dw.init(nullptr, 0, make_int4(0, 0, 0, 0));
   if (a.qdoc)
-    dw.init(a.kr + (int64_t)b * a.nkr, a.nkr, doc_range(a.qr + (int64_t)b * a.nqr, a.nqr, m0 / a.G, (m1 - 1) / a.G + 1));
-  const int whole = a.causal ? max(mw / a.G + off + 1, pre) : 0x7fffffff;
-  const int some = mw1 <= mw ? 0 : (a.causal ? max((mw1 - 1) / a.G + off + 1, pre) : 0x7fffffff);
+    dw.init(a.kr + (int64_t)b * a.nkr, a.nkr, doc_range(a.qr + (int64_t)b * a.nqr, a.nqr, token_of(a, m0), token_of(a, m1 - 1) + 1));
+  // what this wave's rows see whole: keys before `whole`; and at all: keys before `some`
+  const int whole = a.causal ? max(token_of(a, mw) + off + 1, pre) : 0x7fffffff;
+  const int some = mw1 <= mw ? 0 : (a.causal ? max(token_of(a, mw1 - 1) + off + 1, pre) : 0x7fffffff);
 
-  int mrow[RW];
-  Row row[RW];
-  float lse[RW], delta[RW];
-  uint4 qf[RW][R::STEPS], gf[RW][R::STEPS];
-#pragma unroll
-  for (int w = 0; w < RW; ++w) {
-    mrow[w] = mw + w * 32 + (lane & 31);
-    row[w] = row_of(a, b, hk, mrow[w], off, a.Sq);
-    const int i = mrow[w] / a.G, g = mrow[w] - i * a.G, hq = hk * a.G + g;
-    R::frag(row[w].on ? reinterpret_cast<const T*>(a.q) + (int64_t)b * a.qb + (int64_t)i * a.qs + (int64_t)hq * a.qh : nullptr, a.D, qf[w], lane);
-    R::frag(row[w].on ? reinterpret_cast<const T*>(a.dout) + (int64_t)b * a.gb + (int64_t)i * a.gs + (int64_t)hq * a.gh : nullptr, a.D, gf[w], lane);
-    lse[w] = row[w].on ? a.lse[(int64_t)bh * a.M + mrow[w]] : INFINITY;
-    delta[w] = row[w].on ? a.delta[(int64_t)bh * a.M + mrow[w]] : 0.f;
-  }
+  const int mrow = mw + (lane & 31);
+  const Row row = row_of(a, b, hk, mrow, off, a.Sq);
+  const int i = token_of(a, mrow), g = mrow - i * a.G, hq = hk * a.G + g;
+  uint4 qf[1][R::STEPS], gf[R::STEPS];
+  R::frag(row.on ? reinterpret_cast<const T*>(a.q) + (int64_t)b * a.qb + (int64_t)i * a.qs + (int64_t)hq * a.qh : nullptr, a.D, qf[0], lane);
+  R::frag(row.on ? reinterpret_cast<const T*>(a.dout) + (int64_t)b * a.gb + (int64_t)i * a.gs + (int64_t)hq * a.gh : nullptr, a.D, gf, lane);
+  const float lse = row.on ? a.lse[(int64_t)bh * a.M + mrow] : INFINITY, delta = row.on ? a.delta[(int64_t)bh * a.M + mrow] : 0.f;
+
   const char* kbase = reinterpret_cast<const char*>(a.k) + ((int64_t)b * a.kb + (int64_t)hk * a.kh) * R::ES;
   const char* vbase = reinterpret_cast<const char*>(a.v) + ((int64_t)b * a.vb + (int64_t)hk * a.vh) * R::ES;
   const int64_t kst = a.ks * R::ES, vst = a.vs * R::ES;
@@ -389,129 +414,121 @@ __global__ __launch_bounds__(NW * 64, DQ_WAVES) void attn_dq_kernel(Args a) {
   vlin.init(ltid, vst);
   char* ring = smem + (WK ? wave * NS * C::SLOT : 0);
   auto issue = [&](int t, char* dst) {
-    const bool holes = dw.holes;
-    if (!holes && t * BN + BN <= a.Sk && a.D == DP) {
-      klin.template load<BN>(dst, ltid, kbase + (int64_t)t * BN * kst, kst);
-      vlin.template load<BN>(dst + C::TILE, ltid, vbase + (int64_t)t * BN * vst, vst);
+    const int k0 = t * BN;
+    if (!dw.holes && k0 + BN <= a.Sk && a.D == DP) {
+      klin.template load<BN>(dst, ltid, kbase + k0 * kst, kst);
+      vlin.template load<BN>(dst + C::TILE, ltid, vbase + k0 * vst, vst);
       return;
     }
+    const bool holes = dw.holes;
     R::template load2<BN, C::LT>(dst, dst + C::TILE, ltid, a.D, [&](int r, const char*& p0, const char*& p1) {
-      const int key = t * BN + r;
+      const int key = k0 + r;
       if (key >= a.Sk || (holes && a.kdoc[(int64_t)b * a.Sk + key] < 0)) return;
-      p0 = kbase + (int64_t)key * a.ks * R::ES;
-      p1 = vbase + (int64_t)key * a.vs * R::ES;
+      p0 = kbase + key * kst;
+      p1 = vbase + key * vst;
     });
   };
-  f32x16 dq[RW][DT];
+  f32x16 dq[1][DT];
 #pragma unroll
-  for (int w = 0; w < RW; ++w)
-#pragma unroll
-    for (int j = 0; j < DT; ++j) dq[w][j] = zero16();
+  for (int j = 0; j < DT; ++j) dq[0][j] = zero16();
 
-  struct Tile { int t; bool mixed; } q[NS];
-  auto next = [&](int t) { return dw.template next<BN, STEP>(t, t1, 1, a.Sk, lane); };
-  int slot = 0, fly = 0;
-  auto fetch = [&](Tile& x, int t, int into) {
-    x.t = next(t);
+  struct Tile { int t; bool mixed; } q[NS - 1];
+  int tnew = WK ? wave : 0, fill = NS - 1, fly = 0, into = 0, slot = 0;
+  for (;;) {
+    const bool live = fill == 0;
+    if (live) {
+      if (q[0].t >= t1) break;
+      if constexpr (!WK) {
+        vm_wait_tiles<C::NLD, NS - 2>(fly - 1);
+        lds_barrier();
+      }
+    }
+    Tile x{dw.template next<BN, STEP>(tnew, t1, 1, a.Sk, lane), false};
     x.mixed = dw.mixed;
     if (x.t < t1) { issue(x.t, ring + into * C::SLOT); ++fly; }
-  };
+    tnew = x.t + STEP;
+    into = into + 1 == NS ? 0 : into + 1;
+    const Tile cur = q[0];
 #pragma unroll
-  for (int i = 0; i < NS - 1; ++i) fetch(q[i], i ? q[i - 1].t + STEP : (WK ? wave : 0), i);
-  while (q[0].t < t1) {
-    const int last = slot ? slot - 1 : NS - 1;
-    if constexpr (WK) {
-      fetch(q[NS - 1], q[NS - 2].t + STEP, last);
-      vm_wait_tiles<C::NLD, NS - 1>(fly - 1);
-    } else {
-      vm_wait_tiles<C::NLD, NS - 2>(fly - 1);
-      lds_barrier();
-      fetch(q[NS - 1], q[NS - 2].t + STEP, last);
-    }
+    for (int j = 0; j + 2 < NS; ++j) q[j] = q[j + 1];
+    q[NS - 2] = x;
+    if (!live) { --fill; continue; }
+    if constexpr (WK) vm_wait_tiles<C::NLD, NS - 1>(fly - 1);
     const char* kt = ring + slot * C::SLOT;
     const char* vt = kt + C::TILE;
-    const bool mixed = q[0].mixed;
-    const int k0 = q[0].t * BN;
+    const int k0 = cur.t * BN;
+    const bool mixed = cur.mixed;
     if (k0 < some) {
-      f32x16 s[RW], dp[RW];
-      R::template times<RW>(kt, 0, qf, s, lane);
-      R::template times<RW>(vt, 0, gf, dp, lane);
-      const bool caus = k0 + BN > whole;
+      f32x16 s[KT], dp[KT];
+      R::template times2<KT>(kt, vt, qf[0], gf, s, dp, lane);
       float mul = a.scale2;
       if (a.cap > 0.f) {
-        tanh_all<T, RW>(s, a.icap);
+        tanh_all<T, KT>(s, a.icap);
         mul = a.cap2;
+#pragma unroll
+        for (int j = 0; j < KT; ++j)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) dp[j][r] = (dp[j][r] - delta) * fmaf(-s[j][r], s[j][r], 1.f);      // times the cap's slope
+      } else {
+#pragma unroll
+        for (int j = 0; j < KT; ++j)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) dp[j][r] -= delta;
       }
-#pragma unroll
-      for (int w = 0; w < RW; ++w)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          dp[w][r] -= delta[w];
-          if (a.cap > 0.f) dp[w][r] *= fmaf(-s[w][r], s[w][r], 1.f);
-        }
       if (a.slopes) {
 #pragma unroll
-        for (int w = 0; w < RW; ++w) {
-          const int at = row[w].pos - k0 - 4 * h;
+        for (int j = 0; j < KT; ++j) {
+          const int at = row.pos - k0 - j * 32 - 4 * h;
 #pragma unroll
-          for (int r = 0; r < 16; ++r) s[w][r] = fmaf(-row[w].slope2, fabsf((float)(at - acc_row(r))), s[w][r] * mul);
+          for (int r = 0; r < 16; ++r) s[j][r] = fmaf(-row.slope2, fabsf((float)(at - acc_row(r))), s[j][r] * mul);
         }
         mul = 1.f;
       }
-      if (caus || mixed || k0 + BN > a.Sk) {
-        const int key = k0 + (lane & 31), kd = mixed && key < a.Sk ? a.kdoc[(int64_t)b * a.Sk + key] : -1;
+      if (k0 + BN > whole || mixed || k0 + BN > a.Sk) {
+        // the last key in sight; the pairs that do not see each other: p = 0, whatever dP holds there
+        const int last = min(a.causal ? max(row.pos, pre - 1) : a.Sk, a.Sk - 1) - k0 - 4 * h;
+        const int key = k0 + (lane & (BN - 1)), kd = mixed && key < a.Sk ? a.kdoc[(int64_t)b * a.Sk + key] : -1;
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          int d = 0;
-          if (mixed) d = __shfl(kd, acc_row(r) + 4 * h, 64);      // every lane gives its number
+        for (int j = 0; j < KT; ++j)
 #pragma unroll
-          for (int w = 0; w < RW; ++w) {
-            const int last = min(caus ? max(row[w].pos, pre - 1) : a.Sk, a.Sk - 1) - k0 - 4 * h;
-            const bool vis = acc_row(r) <= last && (!mixed || d == row[w].doc);
-            s[w][r] = vis ? s[w][r] * mul : -INFINITY;
-            dp[w][r] = vis ? dp[w][r] : 0.f;
+          for (int r = 0; r < 16; ++r) {
+            bool vis = j * 32 + acc_row(r) <= last;
+            if (mixed) { const int d = __shfl(kd, j * 32 + acc_row(r) + 4 * h, 64); vis = vis && d == row.doc; }   // every lane gives its number
+            s[j][r] = vis ? s[j][r] * mul : -INFINITY;
+            dp[j][r] = vis ? dp[j][r] : 0.f;
           }
-        }
         mul = 1.f;
       }
 #pragma unroll
-      for (int w = 0; w < RW; ++w)
+      for (int j = 0; j < KT; ++j)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) dp[w][r] *= __builtin_amdgcn_exp2f(fmaf(s[w][r], mul, -lse[w]));
+        for (int r = 0; r < 16; ++r) dp[j][r] *= __builtin_amdgcn_exp2f(fmaf(s[j][r], mul, -lse));
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        float x[RW][8];
+      for (int u = 0; u < 2 * KT; ++u) {
+        float y[1][8];
 #pragma unroll
-        for (int w = 0; w < RW; ++w)
-#pragma unroll
-          for (int e = 0; e < 8; ++e) x[w][e] = dp[w][8 * u + e];
-        R::template t_times<RW, false>(kt, u * 16, x, dq, lane);
+        for (int e = 0; e < 8; ++e) y[0][e] = dp[u >> 1][8 * (u & 1) + e];
+        R::template t_times<1, false>(kt, u * 16, y, dq, lane);
       }
     }
     if constexpr (WK) asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     --fly;
     slot = slot + 1 == NS ? 0 : slot + 1;
-#pragma unroll
-    for (int i = 0; i + 1 < NS; ++i) q[i] = q[i + 1];
   }
   if constexpr (WK) join_waves<NW>(dq[0], reinterpret_cast<float*>(smem), wave, lane);
+  if (mrow >= a.M) return;
+  const int64_t oi = (((int64_t)b * a.Sq + i) * a.Hq + hq) * a.D;
 #pragma unroll
-  for (int w = 0; w < RW; ++w) {
-    if (mrow[w] >= a.M) continue;
-    const int i = mrow[w] / a.G, g = mrow[w] - i * a.G;
-    const int64_t oi = (((int64_t)b * a.Sq + i) * a.Hq + hk * a.G + g) * a.D;
+  for (int dt = 0; dt < DT; ++dt) {
+    if (WK && dt % NW != wave) continue;
 #pragma unroll
-    for (int dt = 0; dt < DT; ++dt) {
-      if (WK && dt % NW != wave) continue;
+    for (int q4 = 0; q4 < 4; ++q4) {
+      const int d = dt * 32 + 8 * q4 + 4 * h;
+      if (d >= a.D) continue;
+      float x[4];
 #pragma unroll
-      for (int q4 = 0; q4 < 4; ++q4) {
-        const int d = dt * 32 + 8 * q4 + 4 * h;
-        if (d >= a.D) continue;
-        float x[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) x[e] = row[w].on ? dq[w][dt][4 * q4 + e] * a.scale : 0.f;
-        R::put4(reinterpret_cast<T*>(a.dq) + oi + d, x);
-      }
+      for (int e = 0; e < 4; ++e) x[e] = row.on ? dq[0][dt][4 * q4 + e] * a.scale : 0.f;
+      R::put4(reinterpret_cast<T*>(a.dq) + oi + d, x);
     }
   }
 }
@@ -522,11 +539,11 @@ int run_dkv(Args& a, hipStream_t st) {
   a.mtiles = (a.Sk + C::BK - 1) / C::BK;
   return launch(attn_dkv_kernel<T, DP, NW, WK>, (int64_t)a.mtiles * a.B * a.Hk, C::NT, C::LDS, a, st);
 }
-template <typename T, int DP, int NW, int RW, bool WK>
+template <typename T, int DP, int NW, bool WK>
 int run_dq(Args& a, hipStream_t st) {
-  typedef Dq<T, DP, NW, RW, WK> C;
+  typedef Dq<T, DP, NW, WK> C;
   a.mtiles = (a.M + C::BM - 1) / C::BM;
-  return launch(attn_dq_kernel<T, DP, NW, RW, WK>, (int64_t)a.mtiles * a.B * a.Hk, C::NT, C::LDS, a, st);
+  return launch(attn_dq_kernel<T, DP, NW, WK>, (int64_t)a.mtiles * a.B * a.Hk, C::NT, C::LDS, a, st);
 }
 
 template <typename T, int DP>
@@ -544,7 +561,7 @@ int bwd(Args& a, float* delta, hipStream_t st) {
   }
   if (!a.dq) return 0;
   const bool few = ((int64_t)a.M + 127) / 128 * bh < WKMAX;
-  return few ? run_dq<T, DP, WK, 1, true>(a, st) : run_dq<T, DP, 4, 1, false>(a, st);
+  return few ? run_dq<T, DP, WK, true>(a, st) : run_dq<T, DP, 4, false>(a, st);
 }
 
 }  // namespace

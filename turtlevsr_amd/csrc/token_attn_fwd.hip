@@ -117,7 +117,7 @@ __global__ __launch_bounds__(NW * 64, FWD_WAVES) void attn_fwd_kernel(Args a) {
   uint4 qf[RW][R::STEPS];
 #pragma unroll
   for (int w = 0; w < RW; ++w) {
-    const int i = mrow[w] / a.G, g = mrow[w] - i * a.G;
+    const int i = token_of(a, mrow[w]), g = mrow[w] - i * a.G;
     R::frag(row[w].on ? reinterpret_cast<const T*>(a.q) + (int64_t)b * a.qb + (int64_t)i * a.qs + (int64_t)(hk * a.G + g) * a.qh : nullptr,
             a.D, qf[w], lane);
   }
@@ -134,7 +134,7 @@ __global__ __launch_bounds__(NW * 64, FWD_WAVES) void attn_fwd_kernel(Args a) {
   // wait, in order, behind the tiles in flight
   int* win = reinterpret_cast<int*>(smem + a.lds_win) + wave * F::WIN;
   int wbase = 0, wend = 0;
-  auto page_of = [&](int key) { return a.page == 1 ? key : (int)(__umulhi((uint32_t)key, a.pmul) >> a.psh); };
+  auto page_of = [&](int key) { return quot(key, a.page, a.pmul, a.psh); };
   // starts tile t's copy into dst; returns which of its keys are seen at all (bit = key within the tile)
   auto issue = [&](int t, char* dst) -> uint64_t {
     const int k0 = t * BN;
@@ -198,40 +198,40 @@ __global__ __launch_bounds__(NW * 64, FWD_WAVES) void attn_fwd_kernel(Args a) {
     l[w] = 0.f;
   }
 
-  // the walk: tile q[0] is computed on, q[1 ..] are in flight; it ends where q[0] reaches t1
+  // The walk: tiles are started NS - 1 turns before they are computed on (q: the tiles in flight, oldest first). With a
+  // block the turn's barrier frees the slot of the tile before; a wave of its own starts the next tile at once.
   constexpr int NS = F::NS;
-  struct Tile { int t; bool mixed; uint64_t seen; } q[NS];
-  auto next = [&](int t) { return dw.template next<BN, STEP>(t, t1, 1, a.Sk, lane); };
-  int slot = 0, fly = 0;         // slot of q[0]; tiles in flight
-  auto fetch = [&](Tile& x, int t, int into) {
-    x.t = next(t);
-    x.seen = ~0ull;
+  struct Tile { int t; bool mixed; uint64_t seen; } q[NS - 1];
+  int tnew = WK ? t0 + wave : t0, fill = NS - 1, fly = 0, into = 0, slot = 0;
+  for (;;) {
+    const bool live = fill == 0;
+    if (live) {
+      if (q[0].t >= t1) break;
+      if constexpr (!WK) {
+        vm_wait_tiles<F::NLD, NS - 2>(fly - 1);
+        lds_barrier();
+      }
+    }
+    Tile x{dw.template next<BN, STEP>(tnew, t1, 1, a.Sk, lane), false, ~0ull};
     x.mixed = dw.mixed;
     if (x.t < t1) { x.seen = issue(x.t, buf + into * F::SLOT); ++fly; }
-  };
+    tnew = x.t + STEP;
+    into = into + 1 == NS ? 0 : into + 1;
+    const Tile cur = q[0];
 #pragma unroll
-  for (int i = 0; i < NS - 1; ++i) fetch(q[i], i ? q[i - 1].t + STEP : (WK ? t0 + wave : t0), i);
-  while (q[0].t < t1) {
-    const int last = slot ? slot - 1 : NS - 1;      // the slot of the tile before
-    // a wave of its own starts the newest tile first; with a block the barrier frees its slot
-    if constexpr (WK) {
-      fetch(q[NS - 1], q[NS - 2].t + STEP, last);
-      vm_wait_tiles<F::NLD, NS - 1>(fly - 1);
-    } else {
-      vm_wait_tiles<F::NLD, NS - 2>(fly - 1);
-      lds_barrier();
-      fetch(q[NS - 1], q[NS - 2].t + STEP, last);
-    }
+    for (int i = 0; i + 2 < NS; ++i) q[i] = q[i + 1];
+    q[NS - 2] = x;
+    if (!live) { --fill; continue; }
+    if constexpr (WK) vm_wait_tiles<F::NLD, NS - 1>(fly - 1);
     const char* kt = buf + slot * F::SLOT;
     const char* vt = kt + F::TILE;
-    const int k0 = q[0].t * BN;
-    const bool mixed = q[0].mixed;
-    uint64_t seen = q[0].seen;
+    const int k0 = cur.t * BN;
+    const bool mixed = cur.mixed;
+    uint64_t seen = cur.seen;
 
     if (k0 < some) {
       f32x16 s[KT][RW];
-#pragma unroll
-      for (int j = 0; j < KT; ++j) R::template times<RW>(kt, j * 32, qf, s[j], lane);
+      R::template times<KT, RW>(kt, qf, s, lane);
 
       // the rules that apply to this tile, each in a pass of its own (uniform branches)
       const bool caus = k0 + BN > whole;
@@ -329,8 +329,6 @@ __global__ __launch_bounds__(NW * 64, FWD_WAVES) void attn_fwd_kernel(Args a) {
     if constexpr (WK) asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     --fly;
     slot = slot + 1 == NS ? 0 : slot + 1;
-#pragma unroll
-    for (int i = 0; i + 1 < NS; ++i) q[i] = q[i + 1];
   }
 #pragma unroll
   for (int w = 0; w < RW; ++w) l[w] = half_sum(l[w]);
@@ -375,7 +373,7 @@ __global__ __launch_bounds__(NW * 64, FWD_WAVES) void attn_fwd_kernel(Args a) {
     if (mrow[w] >= a.M) continue;
     const float inv = (l[w] > 0.f && row[w].on) ? 1.f / l[w] : 0.f;
     const float lse = inv > 0.f ? mx[w] + log2f(l[w]) - POFF : INFINITY;
-    const int i = mrow[w] / a.G, g = mrow[w] - i * a.G;
+    const int i = token_of(a, mrow[w]), g = mrow[w] - i * a.G;
     const bool first = (!WK || wave == 0) && h == 0;
     const int64_t pi = ((int64_t)sp * a.B * a.Hk + bh) * a.M + mrow[w];
     const int64_t oi = (((int64_t)b * a.Sq + i) * a.Hq + hk * a.G + g) * a.D;
