@@ -33,6 +33,7 @@
 
 #include <algorithm>
 #include <type_traits>
+#include <utility>
 
 
 namespace turtle {
@@ -41,7 +42,7 @@ namespace {
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
-typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) char lds_char;
 
 __device__ __attribute__((aligned(64))) uint4 g_zero_ta[4];   // source of rows and channels that are not there
@@ -79,6 +80,29 @@ TURTLE_DEV float half_max(float v) { return fmaxf(v, __shfl_xor(v, 32, 64)); }
 TURTLE_DEV float half_sum(float v) { return v + __shfl_xor(v, 32, 64); }
 
 TURTLE_DEV uint32_t lds_addr(const char* p) { return (uint32_t)(uintptr_t)(const lds_char*)p; }
+// LDS reads by address: 16 bytes, a float, and 4 x 16 elements of a group of 16 lanes transposed (a lane gives the place
+// of 8 bytes and gets its column)
+TURTLE_DEV uint4 lds_ld16(uint32_t a) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  return __builtin_bit_cast(uint4, *(__attribute__((address_space(3))) const u32x4*)a);
+#else
+  return make_uint4(a, 0, 0, 0);
+#endif
+}
+TURTLE_DEV float lds_ld4(uint32_t a) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  return *(__attribute__((address_space(3))) const float*)a;
+#else
+  return (float)a;
+#endif
+}
+TURTLE_DEV uint2 lds_ld_tr(uint32_t a) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)a));
+#else
+  return make_uint2(a, 0);
+#endif
+}
 
 // 64 lanes x 16 B -> LDS (see gemm9.hip): inline asm, because the compiler would drain a builtin DMA before every
 // LDS read; waited for by vm_wait
@@ -103,6 +127,11 @@ TURTLE_DEV void vm_wait_tiles(int n) {
 // all of this wave's LDS accesses done, then the block's barrier
 TURTLE_DEV void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
+template <int N, typename F, int... I>
+TURTLE_DEV void static_for_(F f, std::integer_sequence<int, I...>) { (f(std::integral_constant<int, I>{}), ...); }
+template <int N, typename F>
+TURTLE_DEV void static_for(F f) { static_for_<N>(f, std::make_integer_sequence<int, N>{}); }
+
 // A tile of rows of DP channels (zero past D) in LDS
 template <typename T, int DP>
 struct Rows {
@@ -114,44 +143,57 @@ struct Rows {
     if constexpr (CH == 8) return (((r >> 1) & 1) << 2) | ((r >> 2) & 3);
     else return ((r & 3) << 2) | ((r >> 2) & 3);
   }
-  // row r's 16-byte chunk c
-  TURTLE_DEV static uint4 chunk(const char* t, int r, int c) { return *reinterpret_cast<const uint4*>(t + r * ROWB + ((c ^ swz(r)) << 4)); }
+  // LDS addresses. A tile starts at a multiple of ROWB and swz(r + 16) = swz(r), swz(r + 8) = swz(r) ^ 2, so all of a
+  // lane's addresses are one base with bits exchanged: no register per chunk.
+  // this lane's place in row reads: row (lane & 31), chunk (lane >> 5); chunk 2 s + (lane >> 5) is at ^ (s << 5)
+  TURTLE_DEV static uint32_t row_base(const char* t, int lane) {
+    return lds_addr(t) + (lane & 31) * ROWB + (((lane >> 5) ^ swz(lane & 31)) << 4);
+  }
+  template <int S, int J> TURTLE_DEV static uint4 chunk(uint32_t base) { return lds_ld16((base ^ (S << 5)) + J * 32 * ROWB); }
+  // ... in transposing reads of 16 rows: 4 rows from 4 (lane >> 5), 8 bytes of a chunk; channels 32 dt .. are at
+  // ^ (dt << 6), the rows 8 further at ^ 32, + 8 ROWB
+  TURTLE_DEV static uint32_t tr_base(const char* t, int lane) {
+    const int li = lane & 15, row = 4 * (lane >> 5) + (li >> 2), sub = ((lane >> 4) & 1) * 2 + ((li & 3) >> 1);
+    return lds_addr(t) + row * ROWB + ((sub ^ swz(row)) << 4) + (li & 1) * 8;
+  }
   // acc[j][w] = (rows 32 j .. 32 j + 31)(channels) x frag[w], the KT RW chains of products interleaved: frag is the B
   // operand's STEPS chunks
   template <int KT, int RW>
   TURTLE_DEV static void times(const char* t, const uint4 (&frag)[RW][STEPS], f32x16 (&acc)[KT][RW], int lane) {
+    const uint32_t base = row_base(t, lane);
 #pragma unroll
     for (int j = 0; j < KT; ++j)
 #pragma unroll
       for (int w = 0; w < RW; ++w) acc[j][w] = zero16();
+    static_for<STEPS>([&](auto s) {
+      static_for<KT>([&](auto j) {
+        const uint4 x = chunk<s(), j()>(base);
 #pragma unroll
-    for (int s = 0; s < STEPS; ++s)
-#pragma unroll
-      for (int j = 0; j < KT; ++j) {
-        const uint4 x = chunk(t, j * 32 + (lane & 31), 2 * s + (lane >> 5));
-#pragma unroll
-        for (int w = 0; w < RW; ++w) acc[j][w] = mma<T>(x, frag[w][s], acc[j][w]);
-      }
+        for (int w = 0; w < RW; ++w) acc[j()][w] = mma<T>(x, frag[w][s()], acc[j()][w]);
+      });
+    });
   }
-  // the same of two tiles with an operand each
-  template <int KT>
-  TURTLE_DEV static void times2(const char* t0, const char* t1, const uint4 (&f0)[STEPS], const uint4 (&f1)[STEPS], f32x16 (&a0)[KT],
-                                f32x16 (&a1)[KT], int lane) {
+  // the same of two tiles with an operand each; the second's is read from LDS where f1 is null
+  template <int KT, bool L1>
+  TURTLE_DEV static void times2(const char* t0, const char* t1, const uint4 (&f0)[STEPS], const uint4 (&f1)[STEPS], const char* l1,
+                                f32x16 (&a0)[KT], f32x16 (&a1)[KT], int lane) {
+    const uint32_t b0 = row_base(t0, lane), b1 = row_base(t1, lane), bl = L1 ? row_base(l1, lane) : 0;
 #pragma unroll
     for (int j = 0; j < KT; ++j) { a0[j] = zero16(); a1[j] = zero16(); }
-#pragma unroll
-    for (int s = 0; s < STEPS; ++s)
-#pragma unroll
-      for (int j = 0; j < KT; ++j) {
-        a0[j] = mma<T>(chunk(t0, j * 32 + (lane & 31), 2 * s + (lane >> 5)), f0[s], a0[j]);
-        a1[j] = mma<T>(chunk(t1, j * 32 + (lane & 31), 2 * s + (lane >> 5)), f1[s], a1[j]);
-      }
+    static_for<STEPS>([&](auto s) {
+      uint4 g;
+      if constexpr (L1) g = chunk<s(), 0>(bl);
+      else g = f1[s()];
+      static_for<KT>([&](auto j) {
+        a0[j()] = mma<T>(chunk<s(), j()>(b0), f0[s()], a0[j()]);
+        a1[j()] = mma<T>(chunk<s(), j()>(b1), g, a1[j()]);
+      });
+    });
   }
-  // acc[w][dt] += (rows r0 .. r0 + 15)^T (channels 32 dt ..) x p[w]: p = 8 accumulator registers' values of those rows.
-  // TWO: p in two terms (its rounding and the remainder), for products that keep p's fp32 value (16-bit types)
-  template <int RW, bool TWO>
-  TURTLE_DEV static void t_times(const char* t, int r0, const float (&p)[RW][8], f32x16 (&acc)[RW][DT], int lane) {
-    const int h = lane >> 5;
+  // acc[w][dt] += (rows 16 U .. 16 U + 15)^T (channels 32 dt ..) x p[w]: p = 8 accumulator registers' values of those
+  // rows. TWO: p in two terms (its rounding and the remainder), for products that keep p's fp32 value (16-bit types)
+  template <int U, int RW, bool TWO>
+  TURTLE_DEV static void t_times(const char* t, const float (&p)[RW][8], f32x16 (&acc)[RW][DT], int lane) {
     if constexpr (ES == 2) {
       uint4 hi[RW], lo[RW];
 #pragma unroll
@@ -159,32 +201,29 @@ struct Rows {
         hi[w] = pack(p[w]);
         if constexpr (TWO) lo[w] = rest(p[w], hi[w]);
       }
-      const int li = lane & 15, row = r0 + 4 * h + (li >> 2), sub = ((lane >> 4) & 1) * 2 + ((li & 3) >> 1);
-#pragma unroll
-      for (int dt = 0; dt < DT; ++dt) {
-        const char* a = t + row * ROWB + (((dt * 4 + sub) ^ swz(row)) << 4) + (li & 1) * 8;
-        const char* b = t + (row + 8) * ROWB + (((dt * 4 + sub) ^ swz(row + 8)) << 4) + (li & 1) * 8;
-        const uint2 x = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)a));
-        const uint2 y = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)b));
+      const uint32_t base = tr_base(t, lane);
+      static_for<DT>([&](auto dt) {
+        const uint32_t a = base ^ (dt() << 6);
+        const uint2 x = lds_ld_tr(a + U * 16 * ROWB), y = lds_ld_tr((a ^ 32) + (U * 16 + 8) * ROWB);
         const uint4 v = make_uint4(x.x, x.y, y.x, y.y);
 #pragma unroll
         for (int w = 0; w < RW; ++w) {
-          acc[w][dt] = mma<T>(v, hi[w], acc[w][dt]);
-          if constexpr (TWO) acc[w][dt] = mma<T>(v, lo[w], acc[w][dt]);
+          acc[w][dt()] = mma<T>(v, hi[w], acc[w][dt()]);
+          if constexpr (TWO) acc[w][dt()] = mma<T>(v, lo[w], acc[w][dt()]);
         }
-      }
+      });
     } else {
+      // row 8 (e >> 2) + (e & 3) + 4 h, channel 32 dt + (lane & 31)
+      const int h = lane >> 5;
+      static_for<8>([&](auto e) {
+        const int row = U * 16 + acc_row(e()) + 4 * h;
+        const uint32_t a = lds_addr(t) + row * ROWB + ((((lane & 31) >> 2) ^ swz(row)) << 4) + (lane & 3) * 4;
+        static_for<DT>([&](auto dt) {
+          const float v = lds_ld4(a ^ (dt() << 7));
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const int row = r0 + acc_row(e) + 4 * h;
-#pragma unroll
-        for (int dt = 0; dt < DT; ++dt) {
-          const int d = dt * 32 + (lane & 31);
-          const float v = *reinterpret_cast<const float*>(t + row * ROWB + (((d >> 2) ^ swz(row)) << 4) + (d & 3) * 4);
-#pragma unroll
-          for (int w = 0; w < RW; ++w) acc[w][dt] = __builtin_amdgcn_mfma_f32_32x32x2f32(v, p[w][e], acc[w][dt], 0, 0, 0);
-        }
-      }
+          for (int w = 0; w < RW; ++w) acc[w][dt()] = __builtin_amdgcn_mfma_f32_32x32x2f32(v, p[w][e()], acc[w][dt()], 0, 0, 0);
+        });
+      });
     }
   }
   TURTLE_DEV static uint4 rest(const float (&p)[8], uint4 hi) {

@@ -22,9 +22,6 @@
 #ifndef DKV_MT
 #define DKV_MT 2
 #endif
-#ifndef DKV_VL
-#define DKV_VL 1
-#endif
 #ifndef DQ_KT
 #define DQ_KT 2
 #endif
@@ -72,20 +69,22 @@ __global__ __launch_bounds__(256) void attn_delta_kernel(Args a, float* delta) {
 
 // WK: for small grids - the block's NW waves own the same 32 keys and take the row tiles in turn, each with its own
 // ring and no barriers, and join at the end.
-// 128 channels: the operands of S and dP and the two accumulators would take 192 registers of the 256 that let two
-// waves share a SIMD; V stays in LDS there (VL).
-template <typename T, int DP, int NW, bool WK> struct Dkv {
+// RG: row groups - RG waves share 32 keys and take a part of every row tile each, and join at the end. For 128
+// channels, where a block's grid is small and one wave a SIMD leaves its latencies bare; the operands of S and dP and
+// the two accumulators would take 192 of the 256 registers that two waves can have, so V stays in LDS there (VL).
+template <typename T, int DP, int NW, int RG, bool WK> struct Dkv {
   typedef Rows<T, DP> R;
-  static constexpr int NT = NW * 64, LT = WK ? 64 : NT;
+  static constexpr int NT = NW * RG * 64, LT = WK ? 64 : NT;
   static constexpr int BK = WK ? 32 : NW * 32;            // keys of a block
-  static constexpr int MT = (sizeof(T) == 2 && DP == 64) ? DKV_MT : 1, BM = 32 * MT;     // rows of a tile
+  static constexpr int MT = (sizeof(T) == 2 && DP == 64 && !WK) ? DKV_MT : 1, WM = 32 * MT;      // rows a wave takes of a tile
+  static constexpr int BM = WM * RG;                      // rows of a tile
   static constexpr int NS = WK ? 2 : (DP == 64 ? DKV_NS64 : DKV_NS128);
-  static constexpr bool VL = sizeof(T) == 2 && DP == 128 && !WK && DKV_VL;
+  static constexpr bool VL = RG > 1;
   static constexpr int TILE = BM * R::ROWB;
-  static constexpr int SLOT = 2 * TILE + 5 * BM * 4;      // Q, dO; softmax sum, delta, place, document, slope of a row
-  static constexpr int RING = NS * SLOT * (WK ? NW : 1), JOIN = R::DT * 16 * 64 * 4;
+  static constexpr int SLOT = (2 * TILE + 5 * BM * 4 + 511) / 512 * 512;      // Q, dO; softmax sum, delta, place, document, slope of a row
+  static constexpr int RING = NS * SLOT * (WK ? NW : 1), JOIN = R::DT * 16 * 64 * 4 * (RG > 1 ? NW : 1);
   static constexpr int LDS = (RING > JOIN ? RING : JOIN) + (VL ? BK * R::ROWB : 0);
-  static constexpr int NLD = R::template loads2<BM, LT>() + MT;
+  static constexpr int NLD = R::template loads2<BM, LT>() + BM / 32;
 };
 
 // sum of the waves' accumulators through LDS, in wave order; every wave gets it
@@ -110,15 +109,15 @@ TURTLE_DEV void join_waves(f32x16 (&acc)[DT], float* sum, int wave, int lane) {
     for (int r = 0; r < 16; ++r) acc[dt][r] = sum[(dt * 16 + r) * 64 + lane];
 }
 
-template <typename T, int DP, int NW, bool WK>
-__global__ __launch_bounds__(NW * 64, DKV_WAVES) void attn_dkv_kernel(Args a) {
-  typedef Dkv<T, DP, NW, WK> C;
+template <typename T, int DP, int NW, int RG, bool WK>
+__global__ __launch_bounds__(NW * RG * 64, DKV_WAVES) void attn_dkv_kernel(Args a) {
+  typedef Dkv<T, DP, NW, RG, WK> C;
   typedef Rows<T, DP> R;
   constexpr int BM = C::BM, MT = C::MT, DT = R::DT, NS = C::NS, STEP = WK ? NW : 1;
   // fp16: p times 2^10 as operand of dv (p of 10^4 keys would lose bits below the type's normal range)
   constexpr float POFF = std::is_same<T, f16>::value ? 10.f : 0.f, PS = std::is_same<T, f16>::value ? 1.f / 1024.f : 1.f;
-  extern __shared__ __attribute__((aligned(16))) char smem[];
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
+  extern __shared__ __attribute__((aligned(512))) char smem[];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6) % NW, rg = __builtin_amdgcn_readfirstlane(tid >> 6) / NW, h = lane >> 5;
   const int item = xcd_item(a);
   if (item >= a.total) return;
   const int kt = item % a.mtiles, bh = item / a.mtiles, b = bh / a.Hk, hk = bh - b * a.Hk;
@@ -134,7 +133,7 @@ __global__ __launch_bounds__(NW * 64, DKV_WAVES) void attn_dkv_kernel(Args a) {
   char* vlds = smem + C::LDS - C::BK * R::ROWB + wave * 32 * R::ROWB;
   if constexpr (C::VL) {
 #pragma unroll
-    for (int s = 0; s < R::STEPS; ++s)
+    for (int s = 0; s < R::STEPS; ++s)      // every row group writes the same
       *reinterpret_cast<uint4*>(vlds + (lane & 31) * R::ROWB + (((2 * s + h) ^ R::swz(lane & 31)) << 4)) = vf[s];
   }
 
@@ -199,7 +198,7 @@ __global__ __launch_bounds__(NW * 64, DKV_WAVES) void attn_dkv_kernel(Args a) {
     }
     // every wave writes the same sums and deltas, so that all count the same number of loads
 #pragma unroll
-    for (int i = 0; i < MT; ++i) {
+    for (int i = 0; i < BM / 32; ++i) {
       const int e = i * 64 + lane, m = m0 + (e & (BM - 1)), which = e / BM;
       const float* src = m < a.M ? (which ? deltas : sums) + m : g_row_pad + which;
       dma4(src, __builtin_amdgcn_readfirstlane(lds_addr(dst + 2 * C::TILE) + i * 256));
@@ -233,23 +232,17 @@ __global__ __launch_bounds__(NW * 64, DKV_WAVES) void attn_dkv_kernel(Args a) {
     q[NS - 2] = x;
     if (!live) { --fill; continue; }
     if constexpr (WK) vm_wait_tiles<C::NLD, NS - 1>(fly - 1);
-    const char* qt = ring + slot * C::SLOT;
+    const char* qt = ring + slot * C::SLOT + rg * C::WM * R::ROWB;      // this wave's rows of the tile
     const char* gt = qt + C::TILE;
-    const float* in = reinterpret_cast<const float*>(qt + 2 * C::TILE) + 4 * h;
+    const float* in = reinterpret_cast<const float*>(ring + slot * C::SLOT + 2 * C::TILE) + rg * C::WM + 4 * h;
     const int* info = reinterpret_cast<const int*>(in) + 2 * BM;
     const bool mixed = cur.mixed;
-    // causal: places of the tile's first and last row
-    const int p0 = token_of(a, cur.t * BM) + off, p1 = token_of(a, min(cur.t * BM + BM, a.M) - 1) + off;
-    if ((!a.causal || p1 >= kw || kw < pre) && kw < a.Sk) {
+    // causal: places of the first and last row
+    const int m0 = cur.t * BM + rg * C::WM, m1 = min(m0 + C::WM, a.M);
+    const int p0 = token_of(a, m0) + off, p1 = token_of(a, max(m1 - 1, 0)) + off;
+    if (m0 < m1 && (!a.causal || p1 >= kw || kw < pre) && kw < a.Sk) {
       f32x16 s[MT], dp[MT];
-      if constexpr (C::VL) {
-        uint4 vl[R::STEPS];
-#pragma unroll
-        for (int i = 0; i < R::STEPS; ++i) vl[i] = R::chunk(vlds, lane & 31, 2 * i + h);
-        R::template times2<MT>(qt, gt, kf, vl, s, dp, lane);
-      } else {
-        R::template times2<MT>(qt, gt, kf, vf, s, dp, lane);
-      }
+      R::template times2<MT, C::VL>(qt, gt, kf, vf, vlds, s, dp, lane);
       const bool caus = a.causal && p0 + 1 < kw1 && kw1 > pre;
       float mul = a.scale2;
       if (a.cap > 0.f) {
@@ -323,14 +316,13 @@ __global__ __launch_bounds__(NW * 64, DKV_WAVES) void attn_dkv_kernel(Args a) {
             dp[j][r] *= s[j][r];
           }
         }
-#pragma unroll
-      for (int u = 0; u < 2 * MT; ++u) {
+      static_for<2 * MT>([&](auto u) {
         float x[1][8], y[1][8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) { x[0][e] = s[u >> 1][8 * (u & 1) + e]; y[0][e] = dp[u >> 1][8 * (u & 1) + e]; }
-        R::template t_times<1, false>(gt, u * 16, x, dv, lane);
-        R::template t_times<1, false>(qt, u * 16, y, dk, lane);
-      }
+        for (int e = 0; e < 8; ++e) { x[0][e] = s[u() >> 1][8 * (u() & 1) + e]; y[0][e] = dp[u() >> 1][8 * (u() & 1) + e]; }
+        R::template t_times<u(), 1, false>(gt, x, dv, lane);
+        R::template t_times<u(), 1, false>(qt, y, dk, lane);
+      });
     }
     if constexpr (WK) asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     --fly;
@@ -339,6 +331,29 @@ __global__ __launch_bounds__(NW * 64, DKV_WAVES) void attn_dkv_kernel(Args a) {
   if constexpr (WK) {
     join_waves<NW>(dk[0], reinterpret_cast<float*>(smem), wave, lane);
     join_waves<NW>(dv[0], reinterpret_cast<float*>(smem), wave, lane);
+  }
+  if constexpr (RG > 1) {
+    static_assert(RG == 2, "two row groups");
+    float* sum = reinterpret_cast<float*>(smem) + wave * DT * 16 * 64 + lane;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      f32x16 (&acc)[DT] = k ? dv[0] : dk[0];
+      __syncthreads();
+      if (rg == 1) {
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) sum[(dt * 16 + r) * 64] = acc[dt][r];
+      }
+      __syncthreads();
+      if (rg == 0) {
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) acc[dt][r] += sum[(dt * 16 + r) * 64];
+      }
+    }
+    if (rg == 1) return;
   }
   if (key >= a.Sk) return;
   const int64_t oi = (((int64_t)b * a.Sk + key) * a.Hk + hk) * a.D;
@@ -378,7 +393,7 @@ __global__ __launch_bounds__(NW * 64, DQ_WAVES) void attn_dq_kernel(Args a) {
   typedef Dq<T, DP, NW, WK> C;
   typedef Rows<T, DP> R;
   constexpr int BN = C::BN, KT = C::KT, DT = R::DT, NS = C::NS, STEP = WK ? NW : 1;
-  extern __shared__ __attribute__((aligned(16))) char smem[];
+  extern __shared__ __attribute__((aligned(512))) char smem[];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
   const int item = xcd_item(a);
   if (item >= a.total) return;
@@ -400,8 +415,8 @@ __global__ __launch_bounds__(NW * 64, DQ_WAVES) void attn_dq_kernel(Args a) {
   const int mrow = mw + (lane & 31);
   const Row row = row_of(a, b, hk, mrow, off, a.Sq);
   const int i = token_of(a, mrow), g = mrow - i * a.G, hq = hk * a.G + g;
-  uint4 qf[1][R::STEPS], gf[R::STEPS];
-  R::frag(row.on ? reinterpret_cast<const T*>(a.q) + (int64_t)b * a.qb + (int64_t)i * a.qs + (int64_t)hq * a.qh : nullptr, a.D, qf[0], lane);
+  uint4 qf[R::STEPS], gf[R::STEPS];
+  R::frag(row.on ? reinterpret_cast<const T*>(a.q) + (int64_t)b * a.qb + (int64_t)i * a.qs + (int64_t)hq * a.qh : nullptr, a.D, qf, lane);
   R::frag(row.on ? reinterpret_cast<const T*>(a.dout) + (int64_t)b * a.gb + (int64_t)i * a.gs + (int64_t)hq * a.gh : nullptr, a.D, gf, lane);
   const float lse = row.on ? a.lse[(int64_t)bh * a.M + mrow] : INFINITY, delta = row.on ? a.delta[(int64_t)bh * a.M + mrow] : 0.f;
 
@@ -460,7 +475,7 @@ __global__ __launch_bounds__(NW * 64, DQ_WAVES) void attn_dq_kernel(Args a) {
     const bool mixed = cur.mixed;
     if (k0 < some) {
       f32x16 s[KT], dp[KT];
-      R::template times2<KT>(kt, vt, qf[0], gf, s, dp, lane);
+      R::template times2<KT, false>(kt, vt, qf, gf, nullptr, s, dp, lane);
       float mul = a.scale2;
       if (a.cap > 0.f) {
         tanh_all<T, KT>(s, a.icap);
@@ -503,13 +518,12 @@ __global__ __launch_bounds__(NW * 64, DQ_WAVES) void attn_dq_kernel(Args a) {
       for (int j = 0; j < KT; ++j)
 #pragma unroll
         for (int r = 0; r < 16; ++r) dp[j][r] *= __builtin_amdgcn_exp2f(fmaf(s[j][r], mul, -lse));
-#pragma unroll
-      for (int u = 0; u < 2 * KT; ++u) {
+      static_for<2 * KT>([&](auto u) {
         float y[1][8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) y[0][e] = dp[u >> 1][8 * (u & 1) + e];
-        R::template t_times<1, false>(kt, u * 16, y, dq, lane);
-      }
+        for (int e = 0; e < 8; ++e) y[0][e] = dp[u() >> 1][8 * (u() & 1) + e];
+        R::template t_times<u(), 1, false>(kt, y, dq, lane);
+      });
     }
     if constexpr (WK) asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     --fly;
@@ -533,11 +547,11 @@ __global__ __launch_bounds__(NW * 64, DQ_WAVES) void attn_dq_kernel(Args a) {
   }
 }
 
-template <typename T, int DP, int NW, bool WK>
+template <typename T, int DP, int NW, int RG, bool WK>
 int run_dkv(Args& a, hipStream_t st) {
-  typedef Dkv<T, DP, NW, WK> C;
+  typedef Dkv<T, DP, NW, RG, WK> C;
   a.mtiles = (a.Sk + C::BK - 1) / C::BK;
-  return launch(attn_dkv_kernel<T, DP, NW, WK>, (int64_t)a.mtiles * a.B * a.Hk, C::NT, C::LDS, a, st);
+  return launch(attn_dkv_kernel<T, DP, NW, RG, WK>, (int64_t)a.mtiles * a.B * a.Hk, C::NT, C::LDS, a, st);
 }
 template <typename T, int DP, int NW, bool WK>
 int run_dq(Args& a, hipStream_t st) {
@@ -556,7 +570,8 @@ int bwd(Args& a, float* delta, hipStream_t st) {
   constexpr int WK = sizeof(T) == 4 && DP == 128 ? 2 : 4;
   if (a.dk) {
     const bool few = ((int64_t)a.Sk + 127) / 128 * bh < WKMAX;
-    rc = few ? run_dkv<T, DP, WK, true>(a, st) : run_dkv<T, DP, 4, false>(a, st);
+    constexpr int RG = sizeof(T) == 2 && DP == 128 ? 2 : 1;
+    rc = few ? run_dkv<T, DP, WK, 1, true>(a, st) : run_dkv<T, DP, 4, RG, false>(a, st);
     if (rc) return rc;
   }
   if (!a.dq) return 0;

@@ -69,7 +69,7 @@ __global__ __launch_bounds__(NW * 64, FWD_WAVES) void attn_fwd_kernel(Args a) {
   // fp16: p is scaled by 2^6; with p at most 2^8 over the running maximum (below) that stays under the type's 2^16
   constexpr float POFF = std::is_same<T, f16>::value ? 6.f : 0.f;
   constexpr float SLACK = 8.f;
-  extern __shared__ __attribute__((aligned(16))) char smem[];
+  extern __shared__ __attribute__((aligned(512))) char smem[];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
 
   const int item = xcd_item(a);
@@ -312,19 +312,16 @@ __global__ __launch_bounds__(NW * 64, FWD_WAVES) void attn_fwd_kernel(Args a) {
 #pragma unroll
           for (int r = 0; r < 16; ++r) s[j][w][r] = __builtin_amdgcn_exp2f(fmaf(s[j][w][r], mul, sh));
       }
+      static_for<2 * KT>([&](auto u) {
+        float p[RW][8];
 #pragma unroll
-      for (int j = 0; j < KT; ++j)
+        for (int w = 0; w < RW; ++w) {
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          float p[RW][8];
-#pragma unroll
-          for (int w = 0; w < RW; ++w) {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) p[w][e] = s[j][w][8 * u + e];
-            l[w] = sum8(p[w], l[w]);
-          }
-          R::template t_times<RW, F::TWO>(vt, j * 32 + u * 16, p, acc, lane);
+          for (int e = 0; e < 8; ++e) p[w][e] = s[u() >> 1][w][8 * (u() & 1) + e];
+          l[w] = sum8(p[w], l[w]);
         }
+        R::template t_times<u(), RW, F::TWO>(vt, p, acc, lane);
+      });
     }
     if constexpr (WK) asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     --fly;
