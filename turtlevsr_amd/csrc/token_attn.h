@@ -41,6 +41,8 @@ namespace {
 
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef __bf16 bf16x2_ __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x2_ __attribute__((ext_vector_type(2)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) char lds_char;
@@ -173,58 +175,95 @@ struct Rows {
       });
     });
   }
-  // the same of two tiles with an operand each; the second's is read from LDS where f1 is null
-  template <int KT, bool L1>
-  TURTLE_DEV static void times2(const char* t0, const char* t1, const uint4 (&f0)[STEPS], const uint4 (&f1)[STEPS], const char* l1,
-                                f32x16 (&a0)[KT], f32x16 (&a1)[KT], int lane) {
-    const uint32_t b0 = row_base(t0, lane), b1 = row_base(t1, lane), bl = L1 ? row_base(l1, lane) : 0;
+  template <int KT>
+  TURTLE_DEV static void times(const char* t, const uint4 (&f)[STEPS], f32x16 (&acc)[KT], int lane) {
+    times<KT, 1>(t, reinterpret_cast<const uint4 (&)[1][STEPS]>(f), reinterpret_cast<f32x16 (&)[KT][1]>(acc), lane);
+  }
+  // the same of two tiles with an operand each; a1 comes with its initial values
+  template <int KT>
+  TURTLE_DEV static void times2(const char* t0, const char* t1, const uint4 (&f0)[STEPS], const uint4 (&f1)[STEPS], f32x16 (&a0)[KT],
+                                f32x16 (&a1)[KT], int lane) {
+    const uint32_t b0 = row_base(t0, lane), b1 = row_base(t1, lane);
 #pragma unroll
-    for (int j = 0; j < KT; ++j) { a0[j] = zero16(); a1[j] = zero16(); }
+    for (int j = 0; j < KT; ++j) a0[j] = zero16();
     static_for<STEPS>([&](auto s) {
-      uint4 g;
-      if constexpr (L1) g = chunk<s(), 0>(bl);
-      else g = f1[s()];
+      static_for<KT>([&](auto j) {
+        a0[j()] = mma<T>(chunk<s(), j()>(b0), f0[s()], a0[j()]);
+        a1[j()] = mma<T>(chunk<s(), j()>(b1), f1[s()], a1[j()]);
+      });
+    });
+  }
+  // ... the second operand read from LDS, from its 32 rows at l1
+  template <int KT>
+  TURTLE_DEV static void times2_lds(const char* t0, const char* t1, const uint4 (&f0)[STEPS], const char* l1, f32x16 (&a0)[KT],
+                                    f32x16 (&a1)[KT], int lane) {
+    const uint32_t b0 = row_base(t0, lane), b1 = row_base(t1, lane);
+    uint32_t bl = row_base(l1, lane);
+    asm volatile("" : "+v"(bl));      // one address, not a register for each of its chunks
+#pragma unroll
+    for (int j = 0; j < KT; ++j) a0[j] = zero16();
+    static_for<STEPS>([&](auto s) {
+      const uint4 g = chunk<s(), 0>(bl);
       static_for<KT>([&](auto j) {
         a0[j()] = mma<T>(chunk<s(), j()>(b0), f0[s()], a0[j()]);
         a1[j()] = mma<T>(chunk<s(), j()>(b1), g, a1[j()]);
       });
     });
   }
-  // acc[w][dt] += (rows 16 U .. 16 U + 15)^T (channels 32 dt ..) x p[w]: p = 8 accumulator registers' values of those
-  // rows. TWO: p in two terms (its rounding and the remainder), for products that keep p's fp32 value (16-bit types)
-  template <int U, int RW, bool TWO>
-  TURTLE_DEV static void t_times(const char* t, const float (&p)[RW][8], f32x16 (&acc)[RW][DT], int lane) {
-    if constexpr (ES == 2) {
-      uint4 hi[RW], lo[RW];
+  // acc[w][dt] += (rows 16 U .. 16 U + 15)^T (channels 32 dt ..) x p[w]: 16-bit types, p packed from 8 accumulator
+  // registers' values of those rows. LO: a second term (lo[w]) of p besides
+  template <int U, int RW, bool LO>
+  TURTLE_DEV static void t_times(const char* t, const uint4 (&hi)[RW], const uint4 (&lo)[RW], f32x16 (&acc)[RW][DT], int lane) {
+    const uint32_t base = tr_base(t, lane);
+    static_for<DT>([&](auto dt) {
+      const uint32_t a = base ^ (dt() << 6);
+      const uint2 x = lds_ld_tr(a + U * 16 * ROWB), y = lds_ld_tr((a ^ 32) + (U * 16 + 8) * ROWB);
+      const uint4 v = make_uint4(x.x, x.y, y.x, y.y);
 #pragma unroll
       for (int w = 0; w < RW; ++w) {
-        hi[w] = pack(p[w]);
-        if constexpr (TWO) lo[w] = rest(p[w], hi[w]);
+        acc[w][dt()] = mma<T>(v, hi[w], acc[w][dt()]);
+        if constexpr (LO) acc[w][dt()] = mma<T>(v, lo[w], acc[w][dt()]);
       }
-      const uint32_t base = tr_base(t, lane);
+    });
+  }
+  // the same for fp32, from register values: row 8 (e >> 2) + (e & 3) + 4 h, channel 32 dt + (lane & 31)
+  template <int U, int RW>
+  TURTLE_DEV static void t_times(const char* t, const float (&p)[RW][8], f32x16 (&acc)[RW][DT], int lane) {
+    const int h = lane >> 5;
+    static_for<8>([&](auto e) {
+      const int row = U * 16 + acc_row(e()) + 4 * h;
+      const uint32_t a = lds_addr(t) + row * ROWB + ((((lane & 31) >> 2) ^ swz(row)) << 4) + (lane & 3) * 4;
       static_for<DT>([&](auto dt) {
-        const uint32_t a = base ^ (dt() << 6);
-        const uint2 x = lds_ld_tr(a + U * 16 * ROWB), y = lds_ld_tr((a ^ 32) + (U * 16 + 8) * ROWB);
-        const uint4 v = make_uint4(x.x, x.y, y.x, y.y);
+        const float v = lds_ld4(a ^ (dt() << 7));
 #pragma unroll
-        for (int w = 0; w < RW; ++w) {
-          acc[w][dt()] = mma<T>(v, hi[w], acc[w][dt()]);
-          if constexpr (TWO) acc[w][dt()] = mma<T>(v, lo[w], acc[w][dt()]);
-        }
+        for (int w = 0; w < RW; ++w) acc[w][dt()] = __builtin_amdgcn_mfma_f32_32x32x2f32(v, p[w][e()], acc[w][dt()], 0, 0, 0);
       });
+    });
+  }
+  // one operand, rounded (16-bit) or as it is (fp32): 8 values from register 8 (U & 1) on of the tile p[U >> 1]
+  template <int U, int KT>
+  TURTLE_DEV static void t_times1(const char* t, const f32x16 (&p)[KT], f32x16 (&acc)[1][DT], int lane) {
+    float x[1][8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[0][e] = p[U >> 1][8 * (U & 1) + e];
+    if constexpr (ES == 2) {
+      const uint4 hi[1] = {pack(x[0])};
+      t_times<U, 1, false>(t, hi, hi, acc, lane);
     } else {
-      // row 8 (e >> 2) + (e & 3) + 4 h, channel 32 dt + (lane & 31)
-      const int h = lane >> 5;
-      static_for<8>([&](auto e) {
-        const int row = U * 16 + acc_row(e()) + 4 * h;
-        const uint32_t a = lds_addr(t) + row * ROWB + ((((lane & 31) >> 2) ^ swz(row)) << 4) + (lane & 3) * 4;
-        static_for<DT>([&](auto dt) {
-          const float v = lds_ld4(a ^ (dt() << 7));
-#pragma unroll
-          for (int w = 0; w < RW; ++w) acc[w][dt()] = __builtin_amdgcn_mfma_f32_32x32x2f32(v, p[w][e()], acc[w][dt()], 0, 0, 0);
-        });
-      });
+      t_times<U, 1>(t, x, acc, lane);
     }
+  }
+  // sum of the 8 packed values, added to l
+  TURTLE_DEV static float sum_packed(uint4 p, float l) {
+    const uint32_t w[4] = {p.x, p.y, p.z, p.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (std::is_same<T, bf16>::value)
+        l = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_, w[i]), bf16x2_{(bf16)1.f, (bf16)1.f}, l, false);
+      else if constexpr (ES == 2)
+        l = __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2_, w[i]), f16x2_{(f16)1.f, (f16)1.f}, l, false);
+    }
+    return l;
   }
   TURTLE_DEV static uint4 rest(const float (&p)[8], uint4 hi) {
     typedef T tx8 __attribute__((ext_vector_type(8)));

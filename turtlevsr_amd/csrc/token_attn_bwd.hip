@@ -1,30 +1,6 @@
 // Token attention, backward (token_attn.h holds the method and the shared parts): delta, then dk and dv by key tiles,
 // then dq by row tiles. No atomics: every sum has a fixed order.
 #include "token_attn.h"
-#ifndef DKV_WAVES
-#define DKV_WAVES (sizeof(T) == 2 && (DP == 64 || !WK) ? 2 : 1)
-#endif
-#ifndef DQ_WAVES
-#define DQ_WAVES (sizeof(T) == 2 ? 2 : 1)
-#endif
-#ifndef DKV_NS64
-#define DKV_NS64 3
-#endif
-#ifndef DKV_NS128
-#define DKV_NS128 2
-#endif
-#ifndef DQ_NS64
-#define DQ_NS64 3
-#endif
-#ifndef DQ_NS128
-#define DQ_NS128 3
-#endif
-#ifndef DKV_MT
-#define DKV_MT 2
-#endif
-#ifndef DQ_KT
-#define DQ_KT 2
-#endif
 #ifndef WKMAX
 #define WKMAX 128
 #endif
@@ -41,7 +17,7 @@ TURTLE_DEV void dma4(const void* gp, uint32_t lds_wave_base) {
                : "=&s"(keep) : "v"(gp), "s"(lds_wave_base) : "memory");
 }
 
-// delta [B][Hk][M] = do . (o + o_lo); 8 lanes a row, 16 bytes a lane and step
+// -delta [B][Hk][M], delta = do . (o + o_lo); 8 lanes a row, 16 bytes a lane and step
 template <typename T>
 __global__ __launch_bounds__(256) void attn_delta_kernel(Args a, float* delta) {
   constexpr int V = 16 / sizeof(T);
@@ -63,23 +39,24 @@ __global__ __launch_bounds__(256) void attn_delta_kernel(Args a, float* delta) {
       for (int e = 0; e < V; ++e) s = fmaf((float)x[e], (float)y[e] + (float)z[e], s);
     }
     s += __shfl_xor(s, 1, 64); s += __shfl_xor(s, 2, 64); s += __shfl_xor(s, 4, 64);
-    if (ln == 0) delta[((b * a.Hk + hq / a.G) * a.Sq + i) * a.G + hq % a.G] = s;
+    if (ln == 0) delta[((b * a.Hk + hq / a.G) * a.Sq + i) * a.G + hq % a.G] = -s;
   }
 }
 
 // WK: for small grids - the block's NW waves own the same 32 keys and take the row tiles in turn, each with its own
 // ring and no barriers, and join at the end.
-// RG: row groups - RG waves share 32 keys and take a part of every row tile each, and join at the end. For 128
-// channels, where a block's grid is small and one wave a SIMD leaves its latencies bare; the operands of S and dP and
-// the two accumulators would take 192 of the 256 registers that two waves can have, so V stays in LDS there (VL).
+// 128 channels: the operands of S and dP and the two accumulators take 192 registers of the 256 that two waves of a
+// SIMD can have, and one wave alone leaves its latencies bare. RG = 2: two waves share 32 keys, take half of every row
+// tile each and join at the end; V stays in LDS. SP (fp32, and the small grids): a block computes dk (S, dP, dk) or dv
+// (S, dv), 40 products for 32.
 template <typename T, int DP, int NW, int RG, bool WK> struct Dkv {
   typedef Rows<T, DP> R;
   static constexpr int NT = NW * RG * 64, LT = WK ? 64 : NT;
   static constexpr int BK = WK ? 32 : NW * 32;            // keys of a block
-  static constexpr int MT = (sizeof(T) == 2 && DP == 64 && !WK) ? DKV_MT : 1, WM = 32 * MT;      // rows a wave takes of a tile
+  static constexpr bool SP = DP == 128 && RG == 1, VL = RG > 1;
+  static constexpr int MT = (sizeof(T) == 2 && DP == 64 && !WK) ? 2 : 1, WM = 32 * MT;    // rows a wave takes of a tile
   static constexpr int BM = WM * RG;                      // rows of a tile
-  static constexpr int NS = WK ? 2 : (DP == 64 ? DKV_NS64 : DKV_NS128);
-  static constexpr bool VL = RG > 1;
+  static constexpr int NS = (WK || DP == 128) ? 2 : 3;
   static constexpr int TILE = BM * R::ROWB;
   static constexpr int SLOT = (2 * TILE + 5 * BM * 4 + 511) / 512 * 512;      // Q, dO; softmax sum, delta, place, document, slope of a row
   static constexpr int RING = NS * SLOT * (WK ? NW : 1), JOIN = R::DT * 16 * 64 * 4 * (RG > 1 ? NW : 1);
@@ -109,18 +86,27 @@ TURTLE_DEV void join_waves(f32x16 (&acc)[DT], float* sum, int wave, int lane) {
     for (int r = 0; r < 16; ++r) acc[dt][r] = sum[(dt * 16 + r) * 64 + lane];
 }
 
+// dv's accumulators: its own, or dk's where a block has only one of them
+template <bool SAME, int N, int M>
+TURTLE_DEV auto& pick(f32x16 (&x)[1][N], f32x16 (&y)[1][M]) {
+  if constexpr (SAME) return x;
+  else return y;
+}
+
 template <typename T, int DP, int NW, int RG, bool WK>
-__global__ __launch_bounds__(NW * RG * 64, DKV_WAVES) void attn_dkv_kernel(Args a) {
+__global__ __launch_bounds__(NW * RG * 64, sizeof(T) == 2 && (DP == 64 || RG == 2) ? 2 : 1) void attn_dkv_kernel(Args a) {
   typedef Dkv<T, DP, NW, RG, WK> C;
   typedef Rows<T, DP> R;
   constexpr int BM = C::BM, MT = C::MT, DT = R::DT, NS = C::NS, STEP = WK ? NW : 1;
   // fp16: p times 2^10 as operand of dv (p of 10^4 keys would lose bits below the type's normal range)
-  constexpr float POFF = std::is_same<T, f16>::value ? 10.f : 0.f, PS = std::is_same<T, f16>::value ? 1.f / 1024.f : 1.f;
+  constexpr float PUP = std::is_same<T, f16>::value ? 1024.f : 1.f;
   extern __shared__ __attribute__((aligned(512))) char smem[];
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6) % NW, rg = __builtin_amdgcn_readfirstlane(tid >> 6) / NW, h = lane >> 5;
+  const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6), wave = wv % NW, rg = wv / NW, h = lane >> 5;
   const int item = xcd_item(a);
   if (item >= a.total) return;
-  const int kt = item % a.mtiles, bh = item / a.mtiles, b = bh / a.Hk, hk = bh - b * a.Hk;
+  constexpr bool SP = C::SP;
+  const bool do_k = !SP || !(item & 1), do_v = !SP || (item & 1);
+  const int ik = SP ? item >> 1 : item, kt = ik % a.mtiles, bh = ik / a.mtiles, b = bh / a.Hk, hk = bh - b * a.Hk;
   const int k0 = kt * C::BK, k1 = min(k0 + C::BK, a.Sk), off = a.Sk - a.Sq;
   const int kw = k0 + (WK ? 0 : wave * 32), kw1 = min(kw + 32, a.Sk);
   const int pre = a.prefix ? a.prefix[b] : 0;
@@ -129,11 +115,11 @@ __global__ __launch_bounds__(NW * RG * 64, DKV_WAVES) void attn_dkv_kernel(Args 
   uint4 kf[R::STEPS], vf[R::STEPS];
   R::frag(kon ? reinterpret_cast<const T*>(a.k) + (int64_t)b * a.kb + (int64_t)key * a.ks + (int64_t)hk * a.kh : nullptr, a.D, kf, lane);
   R::frag(kon ? reinterpret_cast<const T*>(a.v) + (int64_t)b * a.vb + (int64_t)key * a.vs + (int64_t)hk * a.vh : nullptr, a.D, vf, lane);
-  // VL: each lane's own chunks, at the places `chunk` reads them from
   char* vlds = smem + C::LDS - C::BK * R::ROWB + wave * 32 * R::ROWB;
   if constexpr (C::VL) {
+    // V's chunks at the places `chunk` reads them from; every row group writes the same
 #pragma unroll
-    for (int s = 0; s < R::STEPS; ++s)      // every row group writes the same
+    for (int s = 0; s < R::STEPS; ++s)
       *reinterpret_cast<uint4*>(vlds + (lane & 31) * R::ROWB + (((2 * s + h) ^ R::swz(lane & 31)) << 4)) = vf[s];
   }
 
@@ -205,7 +191,9 @@ __global__ __launch_bounds__(NW * RG * 64, DKV_WAVES) void attn_dkv_kernel(Args 
     }
   };
 
-  f32x16 dk[1][DT], dv[1][DT];
+  // the sums of dk and dv; SP: the one or the other
+  f32x16 dk[1][DT], dv_[1][SP ? 1 : DT];
+  auto& dv = pick<SP>(dk, dv_);
 #pragma unroll
   for (int i = 0; i < DT; ++i) { dk[0][i] = zero16(); dv[0][i] = zero16(); }
 
@@ -241,8 +229,18 @@ __global__ __launch_bounds__(NW * RG * 64, DKV_WAVES) void attn_dkv_kernel(Args 
     const int m0 = cur.t * BM + rg * C::WM, m1 = min(m0 + C::WM, a.M);
     const int p0 = token_of(a, m0) + off, p1 = token_of(a, max(m1 - 1, 0)) + off;
     if (m0 < m1 && (!a.causal || p1 >= kw || kw < pre) && kw < a.Sk) {
+      // dP starts from -delta (stored negated)
       f32x16 s[MT], dp[MT];
-      R::template times2<MT, C::VL>(qt, gt, kf, vf, vlds, s, dp, lane);
+#pragma unroll
+      for (int j = 0; j < MT; ++j)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const float4 del = *reinterpret_cast<const float4*>(in + BM + j * 32 + 8 * c);
+          dp[j][4 * c] = del.x; dp[j][4 * c + 1] = del.y; dp[j][4 * c + 2] = del.z; dp[j][4 * c + 3] = del.w;
+        }
+      if constexpr (C::VL) R::template times2_lds<MT>(qt, gt, kf, vlds, s, dp, lane);
+      else if (do_k) R::template times2<MT>(qt, gt, kf, vf, s, dp, lane);
+      else R::template times<MT>(qt, kf, s, lane);
       const bool caus = a.causal && p0 + 1 < kw1 && kw1 > pre;
       float mul = a.scale2;
       if (a.cap > 0.f) {
@@ -251,25 +249,7 @@ __global__ __launch_bounds__(NW * RG * 64, DKV_WAVES) void attn_dkv_kernel(Args 
 #pragma unroll
         for (int j = 0; j < MT; ++j)
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            const float4 del = *reinterpret_cast<const float4*>(in + BM + j * 32 + 8 * c);
-            const float de[4] = {del.x, del.y, del.z, del.w};
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const int r = 4 * c + e;
-              dp[j][r] = (dp[j][r] - de[e]) * fmaf(-s[j][r] * PS, s[j][r], PS);      // times the cap's slope
-            }
-          }
-      } else {
-#pragma unroll
-        for (int j = 0; j < MT; ++j)
-#pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            const float4 del = *reinterpret_cast<const float4*>(in + BM + j * 32 + 8 * c);
-            const float de[4] = {del.x, del.y, del.z, del.w};
-#pragma unroll
-            for (int e = 0; e < 4; ++e) dp[j][4 * c + e] = (dp[j][4 * c + e] - de[e]) * PS;
-          }
+          for (int r = 0; r < 16; ++r) dp[j][r] *= fmaf(-s[j][r], s[j][r], 1.f);      // times the cap's slope
       }
       if (a.slopes) {
 #pragma unroll
@@ -312,16 +292,14 @@ __global__ __launch_bounds__(NW * RG * 64, DKV_WAVES) void attn_dkv_kernel(Args 
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const int r = 4 * c + e;
-            s[j][r] = __builtin_amdgcn_exp2f(fmaf(s[j][r], mul, POFF - ls[e]));
+            s[j][r] = __builtin_amdgcn_exp2f(fmaf(s[j][r], mul, -ls[e]));
             dp[j][r] *= s[j][r];
+            if constexpr (PUP != 1.f) s[j][r] *= PUP;
           }
         }
       static_for<2 * MT>([&](auto u) {
-        float x[1][8], y[1][8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) { x[0][e] = s[u() >> 1][8 * (u() & 1) + e]; y[0][e] = dp[u() >> 1][8 * (u() & 1) + e]; }
-        R::template t_times<u(), 1, false>(gt, x, dv, lane);
-        R::template t_times<u(), 1, false>(qt, y, dk, lane);
+        if (do_v) R::template t_times1<u()>(gt, s, dv, lane);
+        if (do_k) R::template t_times1<u()>(qt, dp, dk, lane);
       });
     }
     if constexpr (WK) asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
@@ -330,10 +308,10 @@ __global__ __launch_bounds__(NW * RG * 64, DKV_WAVES) void attn_dkv_kernel(Args 
   }
   if constexpr (WK) {
     join_waves<NW>(dk[0], reinterpret_cast<float*>(smem), wave, lane);
-    join_waves<NW>(dv[0], reinterpret_cast<float*>(smem), wave, lane);
+    if constexpr (!SP) join_waves<NW>(dv[0], reinterpret_cast<float*>(smem), wave, lane);
   }
   if constexpr (RG > 1) {
-    static_assert(RG == 2, "two row groups");
+    // the row groups' sums, in order, through LDS
     float* sum = reinterpret_cast<float*>(smem) + wave * DT * 16 * 64 + lane;
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
@@ -353,7 +331,7 @@ __global__ __launch_bounds__(NW * RG * 64, DKV_WAVES) void attn_dkv_kernel(Args 
           for (int r = 0; r < 16; ++r) acc[dt][r] += sum[(dt * 16 + r) * 64];
       }
     }
-    if (rg == 1) return;
+    if (rg > 0) return;
   }
   if (key >= a.Sk) return;
   const int64_t oi = (((int64_t)b * a.Sk + key) * a.Hk + hk) * a.D;
@@ -368,10 +346,10 @@ __global__ __launch_bounds__(NW * RG * 64, DKV_WAVES) void attn_dkv_kernel(Args 
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         x[e] = kon ? dk[0][dt][4 * q4 + e] * a.scale : 0.f;
-        y[e] = kon ? dv[0][dt][4 * q4 + e] * PS : 0.f;
+        y[e] = kon ? dv[0][dt][4 * q4 + e] * (1.f / PUP) : 0.f;
       }
-      R::put4(reinterpret_cast<T*>(a.dk) + oi + d, x);
-      R::put4(reinterpret_cast<T*>(a.dv) + oi + d, y);
+      if (do_k) R::put4(reinterpret_cast<T*>(a.dk) + oi + d, x);
+      if (do_v) R::put4(reinterpret_cast<T*>(a.dv) + oi + d, y);
     }
   }
 }
@@ -380,8 +358,8 @@ template <typename T, int DP, int NW, bool WK> struct Dq {
   typedef Rows<T, DP> R;
   static constexpr int NT = NW * 64, LT = WK ? 64 : NT;
   static constexpr int BM = WK ? 32 : NW * 32;            // rows of a block
-  static constexpr int KT = (sizeof(T) == 2 && DP == 64) ? DQ_KT : 1, BN = 32 * KT;      // keys of a tile
-  static constexpr int NS = WK ? 2 : (DP == 64 ? DQ_NS64 : DQ_NS128);
+  static constexpr int KT = (sizeof(T) == 2 && DP == 64) ? 2 : 1, BN = 32 * KT;      // keys of a tile
+  static constexpr int NS = WK ? 2 : 3;
   static constexpr int TILE = BN * R::ROWB, SLOT = 2 * TILE;
   static constexpr int RING = NS * SLOT * (WK ? NW : 1), JOIN = R::DT * 16 * 64 * 4;
   static constexpr int LDS = RING > JOIN ? RING : JOIN;
@@ -389,7 +367,7 @@ template <typename T, int DP, int NW, bool WK> struct Dq {
 };
 
 template <typename T, int DP, int NW, bool WK>
-__global__ __launch_bounds__(NW * 64, DQ_WAVES) void attn_dq_kernel(Args a) {
+__global__ __launch_bounds__(NW * 64, sizeof(T) == 2 ? 2 : 1) void attn_dq_kernel(Args a) {
   typedef Dq<T, DP, NW, WK> C;
   typedef Rows<T, DP> R;
   constexpr int BN = C::BN, KT = C::KT, DT = R::DT, NS = C::NS, STEP = WK ? NW : 1;
@@ -419,6 +397,9 @@ __global__ __launch_bounds__(NW * 64, DQ_WAVES) void attn_dq_kernel(Args a) {
   R::frag(row.on ? reinterpret_cast<const T*>(a.q) + (int64_t)b * a.qb + (int64_t)i * a.qs + (int64_t)hq * a.qh : nullptr, a.D, qf, lane);
   R::frag(row.on ? reinterpret_cast<const T*>(a.dout) + (int64_t)b * a.gb + (int64_t)i * a.gs + (int64_t)hq * a.gh : nullptr, a.D, gf, lane);
   const float lse = row.on ? a.lse[(int64_t)bh * a.M + mrow] : INFINITY, delta = row.on ? a.delta[(int64_t)bh * a.M + mrow] : 0.f;
+  f32x16 ndelta;      // dP starts from -delta (stored negated)
+#pragma unroll
+  for (int r = 0; r < 16; ++r) ndelta[r] = delta;
 
   const char* kbase = reinterpret_cast<const char*>(a.k) + ((int64_t)b * a.kb + (int64_t)hk * a.kh) * R::ES;
   const char* vbase = reinterpret_cast<const char*>(a.v) + ((int64_t)b * a.vb + (int64_t)hk * a.vh) * R::ES;
@@ -475,7 +456,9 @@ __global__ __launch_bounds__(NW * 64, DQ_WAVES) void attn_dq_kernel(Args a) {
     const bool mixed = cur.mixed;
     if (k0 < some) {
       f32x16 s[KT], dp[KT];
-      R::template times2<KT, false>(kt, vt, qf, gf, nullptr, s, dp, lane);
+#pragma unroll
+      for (int j = 0; j < KT; ++j) dp[j] = ndelta;
+      R::template times2<KT>(kt, vt, qf, gf, s, dp, lane);
       float mul = a.scale2;
       if (a.cap > 0.f) {
         tanh_all<T, KT>(s, a.icap);
@@ -483,12 +466,7 @@ __global__ __launch_bounds__(NW * 64, DQ_WAVES) void attn_dq_kernel(Args a) {
 #pragma unroll
         for (int j = 0; j < KT; ++j)
 #pragma unroll
-          for (int r = 0; r < 16; ++r) dp[j][r] = (dp[j][r] - delta) * fmaf(-s[j][r], s[j][r], 1.f);      // times the cap's slope
-      } else {
-#pragma unroll
-        for (int j = 0; j < KT; ++j)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) dp[j][r] -= delta;
+          for (int r = 0; r < 16; ++r) dp[j][r] *= fmaf(-s[j][r], s[j][r], 1.f);      // times the cap's slope
       }
       if (a.slopes) {
 #pragma unroll
@@ -518,12 +496,7 @@ __global__ __launch_bounds__(NW * 64, DQ_WAVES) void attn_dq_kernel(Args a) {
       for (int j = 0; j < KT; ++j)
 #pragma unroll
         for (int r = 0; r < 16; ++r) dp[j][r] *= __builtin_amdgcn_exp2f(fmaf(s[j][r], mul, -lse));
-      static_for<2 * KT>([&](auto u) {
-        float y[1][8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) y[0][e] = dp[u() >> 1][8 * (u() & 1) + e];
-        R::template t_times<u(), 1, false>(kt, y, dq, lane);
-      });
+      static_for<2 * KT>([&](auto u) { R::template t_times1<u()>(kt, dp, dq, lane); });
     }
     if constexpr (WK) asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     --fly;
@@ -551,7 +524,7 @@ template <typename T, int DP, int NW, int RG, bool WK>
 int run_dkv(Args& a, hipStream_t st) {
   typedef Dkv<T, DP, NW, RG, WK> C;
   a.mtiles = (a.Sk + C::BK - 1) / C::BK;
-  return launch(attn_dkv_kernel<T, DP, NW, RG, WK>, (int64_t)a.mtiles * a.B * a.Hk, C::NT, C::LDS, a, st);
+  return launch(attn_dkv_kernel<T, DP, NW, RG, WK>, (int64_t)a.mtiles * a.B * a.Hk * (C::SP ? 2 : 1), C::NT, C::LDS, a, st);
 }
 template <typename T, int DP, int NW, bool WK>
 int run_dq(Args& a, hipStream_t st) {
@@ -570,8 +543,7 @@ int bwd(Args& a, float* delta, hipStream_t st) {
   constexpr int WK = sizeof(T) == 4 && DP == 128 ? 2 : 4;
   if (a.dk) {
     const bool few = ((int64_t)a.Sk + 127) / 128 * bh < WKMAX;
-    constexpr int RG = sizeof(T) == 2 && DP == 128 ? 2 : 1;
-    rc = few ? run_dkv<T, DP, WK, 1, true>(a, st) : run_dkv<T, DP, 4, RG, false>(a, st);
+    rc = few ? run_dkv<T, DP, WK, 1, true>(a, st) : run_dkv<T, DP, 4, sizeof(T) == 2 && DP == 128 ? 2 : 1, false>(a, st);
     if (rc) return rc;
   }
   if (!a.dq) return 0;

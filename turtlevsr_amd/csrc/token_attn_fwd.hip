@@ -1,49 +1,57 @@
 // Token attention, forward: dense and paged (token_attn.h holds the method and the shared parts).
 //
-// Four shapes of one kernel, chosen by the number of rows M = Sq G of a (sequence, key head):
-//   M <= 32 (new tokens)        the block's waves take the key tiles in turn, each with its own LDS buffers and no
-//                               block barrier, and join at the end: the call is bound by reading K and V once
+// Three shapes of one kernel, chosen by the number of rows M = Sq G of a (sequence, key head):
+//   M <= 32, or a small grid    the block's waves take the key tiles of 32 rows in turn, each with its own LDS ring and
+//                               no block barrier, and join at the end
 //   M <= 64, or <= 256 keys     2 waves x 32 rows
-//   otherwise                   4 waves x 32 or x 64 rows: 64 rows read every K and V tile from LDS once for two
-//                               row groups, which halves the LDS traffic that bounds the 32-row form; it is taken
-//                               when its blocks still fill the chip
+//   otherwise                   4 waves x 32 rows
 // The first two have matrix instructions to spare and multiply p in two terms (TWO): with few keys, p's rounding
 // would be as large an error as the result's own.
 #include "token_attn.h"
 #ifndef LMIN
 #define LMIN 512
 #endif
-#ifndef FWD_WAVES
-#define FWD_WAVES (DP == 128 && (RW == 2 || sizeof(T)==4) ? 1 : 2)
-#endif
 
 namespace turtle {
 namespace {
 
-#ifndef NS64
-#define NS64 3
-#endif
-#ifndef BN128
-#define BN128 64
-#endif
-#ifndef NS128
-#define NS128 2
-#endif
-#ifndef NSWK
-#define NSWK 2
-#endif
-template <typename T, int DP, int NW, int RW, bool WK> struct Fwd {
+template <typename T, int DP, int NW, bool WK> struct Fwd {
   typedef Rows<T, DP> R;
+  static constexpr int RW = 1;                        // row groups of 32 a wave
   static constexpr int NT = NW * 64;
   static constexpr int WROWS = 32 * RW;               // rows of a wave
   static constexpr int BM = WK ? WROWS : NW * WROWS;  // rows of a block
-  static constexpr int BN = (WK || sizeof(T) == 4) ? 32 : (DP == 64 ? 64 : BN128);
-  static constexpr int NS = WK ? NSWK : (DP == 64 ? NS64 : NS128);     // slots of the ring
+  static constexpr int BN = (WK || sizeof(T) == 4) ? 32 : 64;
+  static constexpr int NS = 2;                        // slots of the ring
   static constexpr int TILE = BN * R::ROWB, SLOT = 2 * TILE;
   static constexpr int LT = WK ? 64 : NT;             // threads that load a tile
   static constexpr int NLD = R::template loads2<BN, LT>();
   static constexpr int WIN = 256;                     // page numbers a wave keeps at hand
   static constexpr bool TWO = sizeof(T) == 2 && (WK || NW == 2);
+  // the tile's probabilities as operands of the second product
+  struct P {
+    uint4 hi[2 * BN / 32][RW], lo[TWO ? 2 * BN / 32 : 1][RW];
+    float x[sizeof(T) == 4 ? 2 * BN / 32 : 1][RW][8];
+    // 8 values of row group w; returns l + their sum (16-bit types: of what the product takes)
+    TURTLE_DEV float put(int u, int w, const float (&v)[8], float l) {
+      if constexpr (sizeof(T) == 2) {
+        hi[u][w] = R::pack(v);
+        if constexpr (!TWO) return R::sum_packed(hi[u][w], l);
+        else lo[u][w] = R::rest(v, hi[u][w]);
+      }
+      float a = 0.f, b = 0.f;
+#pragma unroll
+      for (int e = 0; e < 8; e += 2) {
+        a += v[e]; b += v[e + 1];
+        if constexpr (sizeof(T) == 4) { x[u][w][e] = v[e]; x[u][w][e + 1] = v[e + 1]; }
+      }
+      return l + (a + b);
+    }
+    template <int U> TURTLE_DEV void times(const char* vt, f32x16 (&acc)[RW][R::DT], int lane) const {
+      if constexpr (sizeof(T) == 2) R::template t_times<U, RW, TWO>(vt, hi[U], lo[TWO ? U : 0], acc, lane);
+      else R::template t_times<U, RW>(vt, x[U], acc, lane);
+    }
+  };
   // LDS without the page numbers; a call with fewer tiles than slots takes only those
   static int lds(int64_t keys) {
     const int64_t tiles = (keys + BN - 1) / BN;
@@ -53,20 +61,12 @@ template <typename T, int DP, int NW, int RW, bool WK> struct Fwd {
   }
 };
 
-// l + the sum of 8 probabilities
-TURTLE_DEV float sum8(const float (&p)[8], float l) {
-  float a = 0.f, b = 0.f;
-#pragma unroll
-  for (int e = 0; e < 8; e += 2) { a += p[e]; b += p[e + 1]; }
-  return l + (a + b);
-}
-
-template <typename T, int DP, int NW, int RW, bool WK, bool PAGED>
-__global__ __launch_bounds__(NW * 64, FWD_WAVES) void attn_fwd_kernel(Args a) {
-  typedef Fwd<T, DP, NW, RW, WK> F;
+template <typename T, int DP, int NW, bool WK, bool PAGED>
+__global__ __launch_bounds__(NW * 64, DP == 128 && sizeof(T) == 4 ? 1 : 2) void attn_fwd_kernel(Args a) {
+  typedef Fwd<T, DP, NW, WK> F;
   typedef Rows<T, DP> R;
-  constexpr int BN = F::BN, KT = BN / 32, DT = R::DT, STEP = WK ? NW : 1;
-  // fp16: p is scaled by 2^6; with p at most 2^8 over the running maximum (below) that stays under the type's 2^16
+  constexpr int BN = F::BN, KT = BN / 32, RW = F::RW, DT = R::DT, STEP = WK ? NW : 1;
+  // fp16: p is scaled by 2^6 (p of many keys would lose bits below the type's normal range) and stays under its 2^16
   constexpr float POFF = std::is_same<T, f16>::value ? 6.f : 0.f;
   constexpr float SLACK = 8.f;
   extern __shared__ __attribute__((aligned(512))) char smem[];
@@ -232,7 +232,6 @@ __global__ __launch_bounds__(NW * 64, FWD_WAVES) void attn_fwd_kernel(Args a) {
     if (k0 < some) {
       f32x16 s[KT][RW];
       R::template times<KT, RW>(kt, qf, s, lane);
-
       // the rules that apply to this tile, each in a pass of its own (uniform branches)
       const bool caus = k0 + BN > whole;
       bool gaps = k0 + BN > kn;
@@ -288,7 +287,8 @@ __global__ __launch_bounds__(NW * 64, FWD_WAVES) void attn_fwd_kernel(Args a) {
           }
       }
 
-      // running maximum; the accumulators are only rescaled when it grew by more than 2^SLACK in some row
+      // p = 2^(s - mx) against the running reference mx, a maximum of earlier tiles: it serves as long as no score of a
+      // lane is over it by more than SLACK. Only else are the row's halves compared and the accumulators rescaled.
 #pragma unroll
       for (int w = 0; w < RW; ++w) {
         float tm = -INFINITY;
@@ -296,8 +296,8 @@ __global__ __launch_bounds__(NW * 64, FWD_WAVES) void attn_fwd_kernel(Args a) {
         for (int j = 0; j < KT; ++j)
 #pragma unroll
           for (int r = 0; r < 16; ++r) tm = fmaxf(tm, s[j][w][r]);
-        const float mn = fmaxf(mx[w], half_max(tm) * mul);
-        if (__any(mn > mx[w] + SLACK)) {
+        if (__any(!(tm * mul <= mx[w] + SLACK))) {
+          const float mn = fmaxf(mx[w], half_max(tm) * mul);
           const float al = __builtin_amdgcn_exp2f(mx[w] - (mn == -INFINITY ? 0.f : mn));
           mx[w] = mn;
           l[w] *= al;
@@ -306,22 +306,20 @@ __global__ __launch_bounds__(NW * 64, FWD_WAVES) void attn_fwd_kernel(Args a) {
 #pragma unroll
             for (int r = 0; r < 16; ++r) acc[w][i][r] *= al;
         }
+      }
+      typename F::P p;
+#pragma unroll
+      for (int w = 0; w < RW; ++w) {
         const float sh = POFF - (mx[w] == -INFINITY ? 0.f : mx[w]);
 #pragma unroll
-        for (int j = 0; j < KT; ++j)
+        for (int u = 0; u < 2 * KT; ++u) {
+          float x[8];
 #pragma unroll
-          for (int r = 0; r < 16; ++r) s[j][w][r] = __builtin_amdgcn_exp2f(fmaf(s[j][w][r], mul, sh));
-      }
-      static_for<2 * KT>([&](auto u) {
-        float p[RW][8];
-#pragma unroll
-        for (int w = 0; w < RW; ++w) {
-#pragma unroll
-          for (int e = 0; e < 8; ++e) p[w][e] = s[u() >> 1][w][8 * (u() & 1) + e];
-          l[w] = sum8(p[w], l[w]);
+          for (int e = 0; e < 8; ++e) x[e] = __builtin_amdgcn_exp2f(fmaf(s[u >> 1][w][8 * (u & 1) + e], mul, sh));
+          l[w] = p.put(u, w, x, l[w]);
         }
-        R::template t_times<u(), RW, F::TWO>(vt, p, acc, lane);
-      });
+      }
+      static_for<2 * KT>([&](auto u) { p.template times<u()>(vt, acc, lane); });
     }
     if constexpr (WK) asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     --fly;
@@ -446,7 +444,7 @@ __global__ __launch_bounds__(256) void attn_join_kernel(Args a) {
   if (a.lse && d == 0) a.lse[r] = l > 0.f ? mx + log2f(l) : INFINITY;
 }
 
-struct Plan { int kind, nsplit; int64_t mtiles; };      // kind: 0 new tokens, 1 two waves, 2 four waves, 3 four waves x 64 rows
+struct Plan { int kind, nsplit; int64_t mtiles; };      // kind: 0 waves split the keys, 1 two waves, 2 four waves
 
 Plan plan_of(const In* x, int dtype) {
   const int64_t M = (int64_t)x->Sq * (x->Hq / x->Hk), bh = (int64_t)x->B * x->Hk, room = key_room(x);
@@ -455,7 +453,6 @@ Plan plan_of(const In* x, int dtype) {
   const int64_t b64 = (M + 63) / 64 * bh;
   if (M <= 32 || b64 < 256) { p.kind = 0; bm = 32; }
   else if (dtype != 0 && (M <= 64 || room <= 256)) { p.kind = 1; bm = 64; }
-  else if (dtype != 0 && x->D <= 64 && (M + 255) / 256 * bh >= LMIN) { p.kind = 3; bm = 256; }
   else { p.kind = 2; bm = 128; }
   p.mtiles = (M + bm - 1) / bm;
   // too few blocks to fill the 256 CUs: the keys are split over blocks too, 512 at least each, and joined by a second
@@ -475,12 +472,12 @@ size_t ws_bytes(const In* x, int dtype) {
   return (size_t)p.nsplit * x->B * x->Sq * x->Hq * (x->D + 1) * sizeof(float);
 }
 
-template <typename T, int DP, int NW, int RW, bool WK, bool PAGED>
+template <typename T, int DP, int NW, bool WK, bool PAGED>
 int run(Args& a, const Plan& p, int64_t keys, hipStream_t st) {
-  typedef Fwd<T, DP, NW, RW, WK> F;
+  typedef Fwd<T, DP, NW, WK> F;
   a.lds_win = F::lds(keys);
   const int lds = a.lds_win + (PAGED ? NW * F::WIN * 4 : 0);
-  return launch(attn_fwd_kernel<T, DP, NW, RW, WK, PAGED>, p.mtiles * a.B * a.Hk * p.nsplit, F::NT, lds, a, st);
+  return launch(attn_fwd_kernel<T, DP, NW, WK, PAGED>, p.mtiles * a.B * a.Hk * p.nsplit, F::NT, lds, a, st);
 }
 
 template <typename T, int DP, bool PAGED>
@@ -489,10 +486,9 @@ int fwd(Args& a, const Plan& p, int64_t keys, hipStream_t st) {
   a.mtiles = (int)p.mtiles;
   a.nsplit = p.nsplit;
   int rc;
-  if (p.kind == 0) rc = run<T, DP, WK, 1, true, PAGED>(a, p, keys, st);
-  else if (sizeof(T) == 4 || p.kind == 2) rc = run<T, DP, 4, 1, false, PAGED>(a, p, keys, st);
-  else if (p.kind == 1) rc = run<T, DP, sizeof(T) == 4 ? 4 : 2, 1, false, PAGED>(a, p, keys, st);
-  else rc = run<T, DP, 4, sizeof(T) == 4 ? 1 : 2, false, PAGED>(a, p, keys, st);
+  if (p.kind == 0) rc = run<T, DP, WK, true, PAGED>(a, p, keys, st);
+  else if (sizeof(T) == 2 && p.kind == 1) rc = run<T, DP, sizeof(T) == 4 ? 4 : 2, false, PAGED>(a, p, keys, st);
+  else rc = run<T, DP, 4, false, PAGED>(a, p, keys, st);
   if (rc || p.nsplit <= 1) return rc;
   const int64_t n = (int64_t)a.B * a.Hk * a.M * (a.D / 4);
   attn_join_kernel<T><<<(unsigned)((n + 255) / 256), 256, 0, st>>>(a);
