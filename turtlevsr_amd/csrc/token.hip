@@ -91,11 +91,19 @@ TURTLE_DEV float row_sum(float v) {
   return v;
 }
 
+// 1 / sqrt(x): the hardware's (one ulp or so); fp32 with a Newton step
+template <typename T>
+TURTLE_DEV float rsqrt_of(float x) {
+  const float r = __builtin_amdgcn_rsqf(x);
+  if constexpr (sizeof(T) == 2) return r;
+  else return r * fmaf(-0.5f * x * r, r, 1.5f);
+}
+
 struct RopeArgs {
   Side s[2];
   Axes ax;
   const void* pos;
-  int64_t pos_b, S, N;       // N = B * S tokens
+  int64_t pos_b, S, B;
   int D, hs;                 // hs: threads (a power of two) that share a token's heads
   int pos64;
   float eps, sign;
@@ -134,9 +142,8 @@ struct Turn {
     }
   }
   template <typename T>
-  TURTLE_DEV void at(const RopeArgs& a, int64_t n) {
-    const int64_t b = a.pos_b ? n / a.S : 0;
-    const int64_t o = a.pos_b ? b * a.pos_b + (n - b * a.S) * a.ax.naxis : (n % a.S) * a.ax.naxis;
+  TURTLE_DEV void at(const RopeArgs& a, int64_t b, int64_t t) {
+    const int64_t o = b * a.pos_b + t * a.ax.naxis;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int64_t p = a.pos64 ? reinterpret_cast<const int64_t*>(a.pos)[o + ax[i]] : (int64_t)reinterpret_cast<const int32_t*>(a.pos)[o + ax[i]];
@@ -168,9 +175,10 @@ __global__ __launch_bounds__(NTHR) void rope_kernel(RopeArgs a) {
       for (int e = 0; e < 8; ++e) w[i][e] = (p.on && a.s[i].w) ? a.s[i].w[p.c + e] : 1.f;
   }
   const float invD = 1.f / (float)a.D;
-  for (int64_t n = (int64_t)blockIdx.x * p.step + p.tok; n < a.N; n += (int64_t)gridDim.x * p.step) {
-    const int64_t b = n / a.S, t = n - b * a.S;
-    tn.at<T>(a, n);
+  for (int64_t b = blockIdx.y; b < a.B; b += gridDim.y)
+  for (int64_t t = (int64_t)blockIdx.x * p.step + p.tok; t < a.S; t += (int64_t)gridDim.x * p.step) {
+    const int64_t n = b * a.S + t;
+    tn.at<T>(a, b, t);
     for (int h0 = p.h0; h0 < HT; h0 += UF * a.hs) {
       float v[UF][8];
 #pragma unroll
@@ -191,7 +199,7 @@ __global__ __launch_bounds__(NTHR) void rope_kernel(RopeArgs a) {
           float ss = 0.f;
 #pragma unroll
           for (int e = 0; e < 8; ++e) ss = fmaf(v[u][e], v[u][e], ss);
-          const float r = 1.f / sqrtf(fmaf(row_sum<LB>(ss), invD, a.eps));
+          const float r = rsqrt_of<T>(fmaf(row_sum<LB>(ss), invD, a.eps));
 #pragma unroll
           for (int e = 0; e < 8; ++e) v[u][e] *= r * (k ? w[1][e] : w[0][e]);
         }
@@ -214,9 +222,10 @@ __global__ __launch_bounds__(NTHR) void norm_rope_bwd_kernel(RopeArgs a) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) { w[i][e] = (p.on && a.s[i].w) ? a.s[i].w[p.c + e] : 1.f; dw[i][e] = 0.f; }
   const float invD = 1.f / (float)a.D;
-  for (int64_t n = (int64_t)blockIdx.x * p.step + p.tok; n < a.N; n += (int64_t)gridDim.x * p.step) {
-    const int64_t b = n / a.S, t = n - b * a.S;
-    tn.at<T>(a, n);
+  for (int64_t b = blockIdx.y; b < a.B; b += gridDim.y)
+  for (int64_t t = (int64_t)blockIdx.x * p.step + p.tok; t < a.S; t += (int64_t)gridDim.x * p.step) {
+    const int64_t n = b * a.S + t;
+    tn.at<T>(a, b, t);
     for (int h0 = p.h0; h0 < HT; h0 += UB * a.hs) {
       float x[UB][8], g[UB][8];
 #pragma unroll
@@ -240,7 +249,7 @@ __global__ __launch_bounds__(NTHR) void norm_rope_bwd_kernel(RopeArgs a) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) ss = fmaf(x[u][e], x[u][e], ss);
         const float sum = row_sum<LB>(ss);
-        const float r = h < HT ? 1.f / sqrtf(fmaf(sum, invD, a.eps)) : 0.f;
+        const float r = h < HT ? rsqrt_of<T>(fmaf(sum, invD, a.eps)) : 0.f;
         float dot = 0.f;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
@@ -269,23 +278,27 @@ __global__ __launch_bounds__(NTHR) void norm_rope_bwd_kernel(RopeArgs a) {
     if ((int)threadIdx.x < a.D) {
       float s = 0.f;
       for (int i = 0; i < (NTHR >> LB); ++i) s += red[(i << LB) * 8 + threadIdx.x];
-      a.part[((int64_t)blockIdx.x * 2 + k) * a.D + threadIdx.x] = s;
+      a.part[(((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * 2 + k) * a.D + threadIdx.x] = s;
     }
   }
 }
 
-// dw[c] = sum over the blocks' partials: 8 columns of 2 D a block, 32 threads a column
+// dw[c] = sum over the blocks' partials: 16 of the 2 D columns a block, 4 a thread, 64 threads a column group
 __global__ __launch_bounds__(NTHR) void dw_sum_kernel(const float* __restrict__ part, float* __restrict__ dw, int nblk, int cols) {
-  __shared__ float red[NTHR];
-  const int col = blockIdx.x * 8 + (threadIdx.x & 7), r0 = threadIdx.x >> 3;
-  float s = 0.f;
-  for (int r = r0; r < nblk; r += 32) s += part[(int64_t)r * cols + col];
+  __shared__ float4 red[NTHR];
+  const int col = blockIdx.x * 16 + (threadIdx.x & 3) * 4, r0 = threadIdx.x >> 2;
+  float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+  for (int r = r0; r < nblk; r += 64) {
+    const float4 x = *reinterpret_cast<const float4*>(part + (int64_t)r * cols + col);
+    s.x += x.x; s.y += x.y; s.z += x.z; s.w += x.w;
+  }
   red[threadIdx.x] = s;
   __syncthreads();
-  if (threadIdx.x < 8) {
+  if (threadIdx.x < 16) {
     float t = 0.f;
-    for (int i = 0; i < 32; ++i) t += red[i * 8 + threadIdx.x];
-    dw[col] = t;
+    for (int i = 0; i < 64; ++i) t += reinterpret_cast<const float*>(&red[i * 4])[threadIdx.x];
+    dw[blockIdx.x * 16 + threadIdx.x] = t;
   }
 }
 
@@ -311,7 +324,7 @@ bool fill(RopeArgs& r, const Side* a, const Side* b, const Axes* axes, const voi
   if (b && b->x) r.s[1] = *b;
   r.ax = *axes;
   r.pos = pos; r.pos_b = pos_b; r.pos64 = pos64;
-  r.S = S; r.N = B * S; r.D = D;
+  r.S = S; r.B = B; r.D = D;
   // heads dealt so that a thread has about `unroll` rows: they share its angles and are in flight together
   const int slots = NTHR >> lane_bits(D), HT = r.s[0].H + r.s[1].H;
   int hs = 1;
@@ -320,14 +333,15 @@ bool fill(RopeArgs& r, const Side* a, const Side* b, const Axes* axes, const voi
   return true;
 }
 
-unsigned blocks_for(const RopeArgs& r) {
-  const int64_t step = (NTHR >> lane_bits(r.D)) / r.hs;
-  return (unsigned)std::min<int64_t>((r.N + step - 1) / step, 1 << 16);
+// blocks (x: tokens, y: sequences), at most `most` of them
+dim3 blocks_for(const RopeArgs& r, int64_t most) {
+  const int64_t step = (NTHR >> lane_bits(r.D)) / r.hs, y = std::min<int64_t>({r.B, most, 1 << 15});
+  return dim3((unsigned)std::min<int64_t>((r.S + step - 1) / step, std::max<int64_t>(1, most / y)), (unsigned)y);
 }
 
 template <typename T, bool NORM>
 void launch_rope(const RopeArgs& r, hipStream_t st) {
-  const unsigned g = blocks_for(r);
+  const dim3 g = blocks_for(r, 1 << 20);
   switch (lane_bits(r.D)) {
     case 0: rope_kernel<T, NORM, 0><<<g, NTHR, 0, st>>>(r); break;
     case 1: rope_kernel<T, NORM, 1><<<g, NTHR, 0, st>>>(r); break;
@@ -337,7 +351,7 @@ void launch_rope(const RopeArgs& r, hipStream_t st) {
   }
 }
 template <typename T>
-void launch_bwd(const RopeArgs& r, unsigned g, hipStream_t st) {
+void launch_bwd(const RopeArgs& r, dim3 g, hipStream_t st) {
   switch (lane_bits(r.D)) {
     case 0: norm_rope_bwd_kernel<T, 0><<<g, NTHR, 0, st>>>(r); break;
     case 1: norm_rope_bwd_kernel<T, 1><<<g, NTHR, 0, st>>>(r); break;
@@ -390,15 +404,16 @@ int turtle_token_norm_rope_bwd(const turtle_token_side* a, const turtle_token_si
                                void* ws, size_t ws_bytes, int dtype, void* stream) {
   RopeArgs r;
   if (!fill(r, a, b, axes, pos, pos_b, pos64, B, S, D, dtype, true, UB)) return -1;
-  const unsigned g = std::min<unsigned>(blocks_for(r), MAXB);
-  if (dw && (!ws || ws_bytes < (size_t)g * 2 * D * sizeof(float))) return -1;
+  const dim3 g = blocks_for(r, dw ? MAXB : 1 << 20);
+  const int nblk = (int)(g.x * g.y);
+  if (dw && (!ws || (uintptr_t)ws % 16 || ws_bytes < (size_t)nblk * 2 * D * sizeof(float))) return -1;
   r.eps = eps;
   r.part = dw ? (float*)ws : nullptr;
   hipStream_t st = (hipStream_t)stream;
   if (dtype == 0) launch_bwd<float>(r, g, st);
   else if (dtype == 1) launch_bwd<bf16>(r, g, st);
   else launch_bwd<f16>(r, g, st);
-  if (dw) dw_sum_kernel<<<2 * D / 8, NTHR, 0, st>>>((const float*)ws, dw, (int)g, 2 * D);
+  if (dw) dw_sum_kernel<<<2 * D / 16, NTHR, 0, st>>>((const float*)ws, dw, nblk, 2 * D);
   return (int)hipGetLastError();
 }
 

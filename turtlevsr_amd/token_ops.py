@@ -317,8 +317,8 @@ def qk_norm_rope(q, k, pos, q_weight, k_weight, axes, base: float = 10000.0, eps
             raise ValueError(f"{n}: shape {tuple(w.shape)}, expected {(D,)}")
         _same(q, w, n)
     eps = float(eps)
-    if not 0.0 <= eps < float("inf"):
-        raise ValueError(f"eps = {eps}, must be finite and not negative")
+    if not 1e-30 <= eps < float("inf"):
+        raise ValueError(f"eps = {eps}, must be finite and at least 1e-30")
     tab, naxis = _axes(axes, base, D)
     rest = (*_pos(pos, B, S, naxis, q), tab, eps)
     _device(q)
