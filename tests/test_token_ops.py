@@ -860,3 +860,18 @@ def test_op_set_takes_the_autocast_type():
     assert all(torch.equal(a, c) for a, c in zip(y, T.qk_norm_rope(b[0], b[1], pos, None, None, ax)))
     assert torch.equal(z, T.attention(*b, causal=True)) and torch.equal(p, T.paged_attention(b[0], b[1], b[2], table, lens))
     assert HipOps.attention(q, k, v).dtype == torch.float32
+
+
+def test_workspace_sizes_from_python_are_the_library_s():
+    """The cached sizes: what the C entry says for the same call, dense and paged."""
+    L = T.lib()
+    for B, Sq, Sk, Hq, Hk, D in ((1, 1, 9000, 8, 2, 64), (2, 700, 2100, 4, 4, 128), (16, 64, 64, 2, 1, 40)):
+        q = torch.zeros(B, Sq, Hq, D, dtype=torch.bfloat16)
+        k = torch.zeros(B, Sk, Hk, D, dtype=torch.bfloat16)
+        blk = T._attn_block(q, k, k, (1.0, 0.0, 0), (None,) * 4, q, Sk)
+        assert T._workspace_bytes(q.shape, Hk, Sk, (0, 0, 0), 1) == L.turtle_token_attn_workspace(blk, 1)
+        table = torch.zeros(B, 40, dtype=torch.int32)
+        blk = T._attn_block(q, k, k, (1.0, 0.0, 1), (None,) * 4, q, 0, (256, 9, 40), (table, table, None))
+        assert T._workspace_bytes(q.shape, Hk, 0, (256, 9, 40), 1) == L.turtle_token_attn_workspace(blk, 1)
+    assert T._workspace_bytes(torch.Size((1, 1, 8, 64)), 2, 9000, (0, 0, 0), 1) > 0
+    assert T._norm_workspace(5000, 64) == L.turtle_token_norm_rope_workspace(5000, 64)

@@ -88,10 +88,6 @@ def _strides(t):
     return (st[0] if n[0] > 1 else 0, st[1] if n[1] > 1 else 0, st[2] if n[2] > 1 else 0)
 
 
-def _stream(t) -> int:
-    return torch._C._cuda_getCurrentRawStream(t.device.index)
-
-
 def _check_tokens(t, name: str, D=None):
     if not isinstance(t, torch.Tensor) or t.dim() != 4:
         raise ValueError(f"{name}: expected a [B, S, heads, D] tensor")
@@ -150,13 +146,19 @@ def _scale(scale, D: int) -> float:
     return s
 
 
+_device_now, _raw_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
+
+
 def _run(t, what: str, entry, *args):
     """One library call on ``t``'s device (made the current one where it is not) and its current stream."""
-    if torch.cuda.current_device() == t.device.index:
-        _check(entry(*args, _stream(t)), what)
+    i = t.device.index
+    if _device_now() == i:
+        rc = entry(*args, _raw_stream(i))
     else:
-        with torch.cuda.device(t.device):
-            _check(entry(*args, _stream(t)), what)
+        with torch.cuda.device(i):
+            rc = entry(*args, _raw_stream(i))
+    if rc:
+        _check(rc, what)
 
 
 def _wants_grad(*ts) -> bool:
@@ -279,19 +281,25 @@ class _QkNormRope(torch.autograd.Function):
         B, S, _, D = q.shape
         dyq, dyk = _tokens(dyq), _tokens(dyk)
         dq, dk = _dense(q), _dense(k)
-        need = [w is not None and n for w, n in zip((wq, wk), ctx.needs_input_grad[2:4])]
-        L, buf, dw, ws, n = lib(), None, 0, 0, 0
-        if need[0] or need[1]:                    # the two gains' gradients, then the kernel's partial sums
-            n = L.turtle_token_norm_rope_workspace(B * S, D) if B and S else 0
+        need = ctx.needs_input_grad
+        nq, nk = need[2] and wq is not None, need[3] and wk is not None
+        buf, dw, ws, n = None, 0, 0, 0
+        if nq or nk:                              # the two gains' gradients, then the kernel's partial sums
+            n = _norm_workspace(B * S, D)
             buf = torch.empty(2 * D + n // 4, dtype=torch.float32, device=q.device)
             dw = buf.data_ptr()
             ws = dw + 8 * D
         if B and S:
-            _run(q, "token_norm_rope_bwd", L.turtle_token_norm_rope_bwd, _side(q, dq, wq, dyq), _side(k, dk, wk, dyk), tab, pos.data_ptr(),
-                 pos_b, pos64, B, S, D, eps, dw, ws, n, _dt(q))
+            _run(q, "token_norm_rope_bwd", lib().turtle_token_norm_rope_bwd, _side(q, dq, wq, dyq), _side(k, dk, wk, dyk), tab,
+                 pos.data_ptr(), pos_b, pos64, B, S, D, eps, dw, ws, n, _dt(q))
         elif buf is not None:
             buf.zero_()
-        return (dq, dk) + tuple(buf[i * D:(i + 1) * D].to(ctx.w_dt[i]) if need[i] else None for i in range(2)) + (None,) * 5
+        return (dq, dk, buf[:D].to(ctx.w_dt[0]) if nq else None, buf[D:2 * D].to(ctx.w_dt[1]) if nk else None, None, None, None, None, None)
+
+
+@functools.lru_cache(maxsize=256)
+def _norm_workspace(tokens: int, D: int) -> int:
+    return lib().turtle_token_norm_rope_workspace(tokens, D)
 
 
 def qk_norm_rope(q, k, pos, q_weight, k_weight, axes, base: float = 10000.0, eps: float = 1e-6):
@@ -355,7 +363,7 @@ def _attn_forward(q, k, v, rules, masks, grad):
         ranges = p + parts[3] if docs else 0
         if grad:
             lo, lse = (p if dt else 0), p + parts[1]
-    ws, nws = _attn_workspace(_attn_block(q, k, v, rules, masks, o, Sk), dt, q)
+    ws, nws = _attn_workspace(q.shape, k.shape[2], Sk, (0, 0, 0), dt, q.device)
     blk = _attn_block(q, k, v, rules, masks, o, Sk, lo=lo, lse=lse, ranges=ranges, ws=_ptr(ws), ws_bytes=nws)
     _run(q, "token_attn_fwd", lib().turtle_token_attn_fwd, blk, dt)
     return o, aux
@@ -369,9 +377,18 @@ def _aux_parts(n: int, D: int, dt: int, nr: int):
     return 0, a, b, c, c + nr
 
 
-def _attn_workspace(blk, dt: int, like):
-    n = lib().turtle_token_attn_workspace(blk, dt)
-    return (torch.empty(n, dtype=torch.uint8, device=like.device), n) if n else (None, 0)
+@functools.lru_cache(maxsize=256)
+def _workspace_bytes(q_shape, Hk: int, Sk: int, pages, dt: int) -> int:
+    """The library's answer for these sizes (it goes by nothing else)."""
+    B, Sq, Hq, D = q_shape
+    a = [0] * 37
+    a[12:18], a[25:28], a[28] = (B, Sq, Sk, Hq, Hk, D), pages, 1 if pages[0] else 0
+    return lib().turtle_token_attn_workspace(_ATTN.pack(*a), dt)
+
+
+def _attn_workspace(q_shape, Hk: int, Sk: int, pages, dt: int, device):
+    n = _workspace_bytes(q_shape, Hk, Sk, pages, dt)
+    return (torch.empty(n, dtype=torch.uint8, device=device), n) if n else (None, 0)
 
 
 class _NoKeys(torch.autograd.Function):
@@ -501,6 +518,6 @@ def paged_attention(q, k_pages, v_pages, block_table, kv_lens, *, q_lens=None, s
     cache = (block_table.contiguous(), kv_lens.contiguous(), None if q_lens is None else q_lens.contiguous())
     rules, masks, pages = (scale, softcap, 1 if causal else 0), (slopes, None, None, None), (kp.shape[1], kp.shape[0], block_table.shape[1])
     o, dt = _dense(q), _dt(q)
-    ws, nws = _attn_workspace(_attn_block(q, kp, vp, rules, masks, o, 0, pages, cache), dt, q)
+    ws, nws = _attn_workspace(q.shape, kp.shape[2], 0, pages, dt, q.device)
     _run(q, "token_attn_fwd", lib().turtle_token_attn_fwd, _attn_block(q, kp, vp, rules, masks, o, 0, pages, cache, ws=_ptr(ws), ws_bytes=nws), dt)
     return o
