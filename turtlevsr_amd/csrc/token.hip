@@ -16,6 +16,7 @@
 #include "../../include/turtle_token.h"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace turtle {
 namespace {
@@ -24,26 +25,35 @@ typedef turtle_token_side Side;
 typedef turtle_token_axes Axes;
 
 constexpr int NTHR = 256;
-constexpr int UF = 4;             // rows a thread has in flight, forward
-constexpr int UB = 2;             // ... backward (two inputs each)
+constexpr int U = 2;              // rows of each tensor a thread has in flight
 constexpr int MAXB = 1024;        // blocks of the backward: its dw partials are one row of 2 D floats a block
 
-TURTLE_DEV void ld8(const float* p, float (&v)[8]) {
-  const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
-  v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-}
-TURTLE_DEV void ld8(const bf16* p, float (&v)[8]) {
-  const uint4 q = *reinterpret_cast<const uint4*>(p);
-  const uint32_t w[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) { v[2 * i] = __uint_as_float(w[i] << 16); v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u); }
-}
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
-TURTLE_DEV void ld8(const f16* p, float (&v)[8]) {
-  const f16x8 q = *reinterpret_cast<const f16x8*>(p);
+// 8 elements as loaded: unpacked when they are used, so that rows in flight take few registers
+template <typename T> struct Raw {
+  uint4 q;
+  TURTLE_DEV void load(const T* p) { q = *reinterpret_cast<const uint4*>(p); }
+  TURTLE_DEV void zero() { q = make_uint4(0, 0, 0, 0); }
+  TURTLE_DEV void get(float (&v)[8]) const {
+    if constexpr (std::is_same<T, bf16>::value) {
+      const uint32_t w[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = (float)q[i];
-}
+      for (int i = 0; i < 4; ++i) { v[2 * i] = __uint_as_float(w[i] << 16); v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u); }
+    } else {
+      const f16x8 x = __builtin_bit_cast(f16x8, q);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = (float)x[i];
+    }
+  }
+};
+template <> struct Raw<float> {
+  float4 a, b;
+  TURTLE_DEV void load(const float* p) { a = *reinterpret_cast<const float4*>(p); b = *reinterpret_cast<const float4*>(p + 4); }
+  TURTLE_DEV void zero() { a = b = make_float4(0.f, 0.f, 0.f, 0.f); }
+  TURTLE_DEV void get(float (&v)[8]) const {
+    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+  }
+};
 TURTLE_DEV void st8(float* p, const float (&v)[8]) {
   *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
   *reinterpret_cast<float4*>(p + 4) = make_float4(v[4], v[5], v[6], v[7]);
@@ -105,8 +115,8 @@ struct RopeArgs {
   const void* pos;
   int64_t pos_b, S, B;
   int D, hs;                 // hs: threads (a power of two) that share a token's heads
-  int pos64;
-  float eps, sign;
+  int pos64, whole;          // whole: every channel is rotated
+  float eps;
   float* part;               // backward: [gridDim.x][2][D] or NULL
 };
 
@@ -150,21 +160,24 @@ struct Turn {
       sincos_rev<T>((uint32_t)(((uint64_t)p * f[i]) >> 32), s[i], c[i]);
     }
   }
-  // channels that are not rotated pass unchanged, whatever they hold
-  TURTLE_DEV void apply(float (&v)[8], float sign) const {
+  // channels that are not rotated pass unchanged, whatever they hold. INV: by the angle's negative
+  template <bool INV>
+  TURTLE_DEV void apply(float (&v)[8], bool whole) const {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const float x0 = v[2 * i], x1 = v[2 * i + 1], sn = s[i] * sign;
-      v[2 * i] = rot[i] ? x0 * c[i] - x1 * sn : x0;
-      v[2 * i + 1] = rot[i] ? x0 * sn + x1 * c[i] : x1;
+      const float x0 = v[2 * i], x1 = v[2 * i + 1], sn = INV ? -s[i] : s[i];
+      const float y0 = fmaf(x0, c[i], -x1 * sn), y1 = fmaf(x0, sn, x1 * c[i]);
+      v[2 * i] = whole || rot[i] ? y0 : x0;
+      v[2 * i + 1] = whole || rot[i] ? y1 : x1;
     }
   }
 };
 
-template <typename T, bool NORM, int LB>
+template <typename T, bool NORM, bool INV, int LB>
 __global__ __launch_bounds__(NTHR) void rope_kernel(RopeArgs a) {
   const Place p = Place::of<LB>(a);
-  const int HT = a.s[0].H + a.s[1].H;
+  const int H = max(a.s[0].H, a.s[1].H);
+  const bool whole = a.whole;
   Turn tn;
   tn.init(a.ax, p.c);
   float w[2][8];
@@ -177,35 +190,35 @@ __global__ __launch_bounds__(NTHR) void rope_kernel(RopeArgs a) {
   const float invD = 1.f / (float)a.D;
   for (int64_t b = blockIdx.y; b < a.B; b += gridDim.y)
   for (int64_t t = (int64_t)blockIdx.x * p.step + p.tok; t < a.S; t += (int64_t)gridDim.x * p.step) {
-    const int64_t n = b * a.S + t;
-    tn.at<T>(a, b, t);
-    for (int h0 = p.h0; h0 < HT; h0 += UF * a.hs) {
-      float v[UF][8];
+    for (int h0 = p.h0; h0 < H; h0 += U * a.hs) {
+      Raw<T> x[2][U];
 #pragma unroll
-      for (int u = 0; u < UF; ++u) {
-        const int h = h0 + u * a.hs, k = h >= a.s[0].H ? 1 : 0;
-        if (h < HT && p.on) {
-          const Side& sd = a.s[k];
-          ld8(reinterpret_cast<const T*>(sd.x) + b * sd.sb + t * sd.ss + (int64_t)(h - (k ? a.s[0].H : 0)) * sd.sh + p.c, v[u]);
-        } else {
+      for (int k = 0; k < 2; ++k)
 #pragma unroll
-          for (int e = 0; e < 8; ++e) v[u][e] = 0.f;
+        for (int u = 0; u < U; ++u) {
+          const int h = h0 + u * a.hs;
+          x[k][u].zero();
+          if (h < a.s[k].H && p.on) x[k][u].load(reinterpret_cast<const T*>(a.s[k].x) + b * a.s[k].sb + t * a.s[k].ss + h * a.s[k].sh + p.c);
         }
-      }
+      if (h0 == p.h0) tn.at<T>(a, b, t);      // the angles while the first rows are on their way
 #pragma unroll
-      for (int u = 0; u < UF; ++u) {
-        const int h = h0 + u * a.hs, k = h >= a.s[0].H ? 1 : 0;
-        if constexpr (NORM) {
-          float ss = 0.f;
+      for (int k = 0; k < 2; ++k)
 #pragma unroll
-          for (int e = 0; e < 8; ++e) ss = fmaf(v[u][e], v[u][e], ss);
-          const float r = rsqrt_of<T>(fmaf(row_sum<LB>(ss), invD, a.eps));
+        for (int u = 0; u < U; ++u) {
+          const int h = h0 + u * a.hs;
+          float v[8];
+          x[k][u].get(v);
+          if constexpr (NORM) {
+            float ss = 0.f;
 #pragma unroll
-          for (int e = 0; e < 8; ++e) v[u][e] *= r * (k ? w[1][e] : w[0][e]);
+            for (int e = 0; e < 8; ++e) ss = fmaf(v[e], v[e], ss);
+            const float r = rsqrt_of<T>(fmaf(row_sum<LB>(ss), invD, a.eps));
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] *= r * w[k][e];
+          }
+          tn.apply<INV>(v, whole);
+          if (h < a.s[k].H && p.on) st8(reinterpret_cast<T*>(a.s[k].y) + ((b * a.S + t) * a.s[k].H + h) * a.D + p.c, v);
         }
-        tn.apply(v[u], a.sign);
-        if (h < HT && p.on) st8(reinterpret_cast<T*>(a.s[k].y) + (n * a.s[k].H + (h - (k ? a.s[0].H : 0))) * a.D + p.c, v[u]);
-      }
     }
   }
 }
@@ -213,7 +226,8 @@ __global__ __launch_bounds__(NTHR) void rope_kernel(RopeArgs a) {
 template <typename T, int LB>
 __global__ __launch_bounds__(NTHR) void norm_rope_bwd_kernel(RopeArgs a) {
   const Place p = Place::of<LB>(a);
-  const int HT = a.s[0].H + a.s[1].H;
+  const int H = max(a.s[0].H, a.s[1].H);
+  const bool whole = a.whole;
   Turn tn;
   tn.init(a.ax, p.c);
   float w[2][8], dw[2][8];
@@ -224,47 +238,47 @@ __global__ __launch_bounds__(NTHR) void norm_rope_bwd_kernel(RopeArgs a) {
   const float invD = 1.f / (float)a.D;
   for (int64_t b = blockIdx.y; b < a.B; b += gridDim.y)
   for (int64_t t = (int64_t)blockIdx.x * p.step + p.tok; t < a.S; t += (int64_t)gridDim.x * p.step) {
-    const int64_t n = b * a.S + t;
-    tn.at<T>(a, b, t);
-    for (int h0 = p.h0; h0 < HT; h0 += UB * a.hs) {
-      float x[UB][8], g[UB][8];
+    for (int h0 = p.h0; h0 < H; h0 += U * a.hs) {
+      Raw<T> rx[2][U], rg[2][U];
 #pragma unroll
-      for (int u = 0; u < UB; ++u) {
-        const int h = h0 + u * a.hs, k = h >= a.s[0].H ? 1 : 0;
-        if (h < HT && p.on) {
-          const Side& sd = a.s[k];
-          const int64_t hl = h - (k ? a.s[0].H : 0);
-          ld8(reinterpret_cast<const T*>(sd.x) + b * sd.sb + t * sd.ss + hl * sd.sh + p.c, x[u]);
-          ld8(reinterpret_cast<const T*>(sd.dy) + b * sd.gb + t * sd.gs + hl * sd.gh + p.c, g[u]);
-        } else {
+      for (int k = 0; k < 2; ++k)
 #pragma unroll
-          for (int e = 0; e < 8; ++e) x[u][e] = g[u][e] = 0.f;
+        for (int u = 0; u < U; ++u) {
+          const int h = h0 + u * a.hs;
+          rx[k][u].zero();
+          rg[k][u].zero();
+          if (h < a.s[k].H && p.on) {
+            rx[k][u].load(reinterpret_cast<const T*>(a.s[k].x) + b * a.s[k].sb + t * a.s[k].ss + h * a.s[k].sh + p.c);
+            rg[k][u].load(reinterpret_cast<const T*>(a.s[k].dy) + b * a.s[k].gb + t * a.s[k].gs + h * a.s[k].gh + p.c);
+          }
         }
-      }
+      if (h0 == p.h0) tn.at<T>(a, b, t);
 #pragma unroll
-      for (int u = 0; u < UB; ++u) {
-        const int h = h0 + u * a.hs, k = h >= a.s[0].H ? 1 : 0;
-        tn.apply(g[u], -1.f);
-        float ss = 0.f;
+      for (int k = 0; k < 2; ++k)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) ss = fmaf(x[u][e], x[u][e], ss);
-        const float sum = row_sum<LB>(ss);
-        const float r = h < HT ? rsqrt_of<T>(fmaf(sum, invD, a.eps)) : 0.f;
-        float dot = 0.f;
+        for (int u = 0; u < U; ++u) {
+          const int h = h0 + u * a.hs;
+          float x[8], g[8];
+          rx[k][u].get(x);
+          rg[k][u].get(g);
+          tn.apply<true>(g, whole);
+          float ss = 0.f;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          x[u][e] *= r;
-          const float d = g[u][e] * x[u][e];
-          dw[0][e] += k ? 0.f : d;
-          dw[1][e] += k ? d : 0.f;
-          g[u][e] *= k ? w[1][e] : w[0][e];
-          dot = fmaf(g[u][e], x[u][e], dot);
+          for (int e = 0; e < 8; ++e) ss = fmaf(x[e], x[e], ss);
+          const float r = rsqrt_of<T>(fmaf(row_sum<LB>(ss), invD, a.eps));
+          float dot = 0.f;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            x[e] *= r;
+            dw[k][e] = fmaf(g[e], x[e], dw[k][e]);      // rows that are not there are zero
+            g[e] *= w[k][e];
+            dot = fmaf(g[e], x[e], dot);
+          }
+          const float m = row_sum<LB>(dot) * invD;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) g[e] = r * fmaf(-x[e], m, g[e]);
+          if (h < a.s[k].H && p.on) st8(reinterpret_cast<T*>(a.s[k].y) + ((b * a.S + t) * a.s[k].H + h) * a.D + p.c, g);
         }
-        const float m = row_sum<LB>(dot) * invD;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) g[u][e] = r * (g[u][e] - x[u][e] * m);
-        if (h < HT && p.on) st8(reinterpret_cast<T*>(a.s[k].y) + (n * a.s[k].H + (h - (k ? a.s[0].H : 0))) * a.D + p.c, g[u]);
-      }
     }
   }
   if (!a.part) return;
@@ -312,7 +326,7 @@ bool side_ok(const Side* s, int D, int es, bool bwd) {
 int lane_bits(int D) { int lb = 0; while ((8 << lb) < D) ++lb; return lb; }
 
 bool fill(RopeArgs& r, const Side* a, const Side* b, const Axes* axes, const void* pos, int64_t pos_b, int pos64, int64_t B, int64_t S,
-          int D, int dtype, bool bwd, int unroll) {
+          int D, int dtype, bool bwd) {
   if (!a || !axes || !pos || B <= 0 || S <= 0 || D <= 0 || D % 8 || D > 128 || dtype < 0 || dtype > 2) return false;
   const int es = dtype == 0 ? 4 : 2;
   if (!side_ok(a, D, es, bwd) || (b && b->x && !side_ok(b, D, es, bwd))) return false;
@@ -325,10 +339,11 @@ bool fill(RopeArgs& r, const Side* a, const Side* b, const Axes* axes, const voi
   r.ax = *axes;
   r.pos = pos; r.pos_b = pos_b; r.pos64 = pos64;
   r.S = S; r.B = B; r.D = D;
-  // heads dealt so that a thread has about `unroll` rows: they share its angles and are in flight together
-  const int slots = NTHR >> lane_bits(D), HT = r.s[0].H + r.s[1].H;
+  r.whole = 2 * axes->npair == D;
+  // heads dealt so that a thread has about U rows of each tensor: they share its angles and are in flight together
+  const int slots = NTHR >> lane_bits(D), H = std::max(r.s[0].H, r.s[1].H);
   int hs = 1;
-  while (hs < slots && hs * unroll < HT) hs *= 2;
+  while (hs < slots && hs * U < H) hs *= 2;
   r.hs = hs;
   return true;
 }
@@ -339,16 +354,21 @@ dim3 blocks_for(const RopeArgs& r, int64_t most) {
   return dim3((unsigned)std::min<int64_t>((r.S + step - 1) / step, std::max<int64_t>(1, most / y)), (unsigned)y);
 }
 
-template <typename T, bool NORM>
+template <typename T, bool NORM, bool INV>
 void launch_rope(const RopeArgs& r, hipStream_t st) {
   const dim3 g = blocks_for(r, 1 << 20);
   switch (lane_bits(r.D)) {
-    case 0: rope_kernel<T, NORM, 0><<<g, NTHR, 0, st>>>(r); break;
-    case 1: rope_kernel<T, NORM, 1><<<g, NTHR, 0, st>>>(r); break;
-    case 2: rope_kernel<T, NORM, 2><<<g, NTHR, 0, st>>>(r); break;
-    case 3: rope_kernel<T, NORM, 3><<<g, NTHR, 0, st>>>(r); break;
-    default: rope_kernel<T, NORM, 4><<<g, NTHR, 0, st>>>(r); break;
+    case 0: rope_kernel<T, NORM, INV, 0><<<g, NTHR, 0, st>>>(r); break;
+    case 1: rope_kernel<T, NORM, INV, 1><<<g, NTHR, 0, st>>>(r); break;
+    case 2: rope_kernel<T, NORM, INV, 2><<<g, NTHR, 0, st>>>(r); break;
+    case 3: rope_kernel<T, NORM, INV, 3><<<g, NTHR, 0, st>>>(r); break;
+    default: rope_kernel<T, NORM, INV, 4><<<g, NTHR, 0, st>>>(r); break;
   }
+}
+template <typename T>
+void launch_turn(const RopeArgs& r, bool inverse, hipStream_t st) {
+  if (inverse) launch_rope<T, false, true>(r, st);
+  else launch_rope<T, false, false>(r, st);
 }
 template <typename T>
 void launch_bwd(const RopeArgs& r, dim3 g, hipStream_t st) {
@@ -371,12 +391,11 @@ extern "C" {
 int turtle_token_rope(const turtle_token_side* a, const turtle_token_side* b, const turtle_token_axes* axes, const void* pos,
                       int64_t pos_b, int pos64, int64_t B, int64_t S, int D, int inverse, int dtype, void* stream) {
   RopeArgs r;
-  if (!fill(r, a, b, axes, pos, pos_b, pos64, B, S, D, dtype, false, UF)) return -1;
-  r.sign = inverse ? -1.f : 1.f;
+  if (!fill(r, a, b, axes, pos, pos_b, pos64, B, S, D, dtype, false)) return -1;
   hipStream_t st = (hipStream_t)stream;
-  if (dtype == 0) launch_rope<float, false>(r, st);
-  else if (dtype == 1) launch_rope<bf16, false>(r, st);
-  else launch_rope<f16, false>(r, st);
+  if (dtype == 0) launch_turn<float>(r, inverse, st);
+  else if (dtype == 1) launch_turn<bf16>(r, inverse, st);
+  else launch_turn<f16>(r, inverse, st);
   return (int)hipGetLastError();
 }
 
@@ -384,13 +403,12 @@ int turtle_token_norm_rope_fwd(const turtle_token_side* a, const turtle_token_si
                                const void* pos, int64_t pos_b, int pos64, int64_t B, int64_t S, int D, float eps, int dtype,
                                void* stream) {
   RopeArgs r;
-  if (!fill(r, a, b, axes, pos, pos_b, pos64, B, S, D, dtype, false, UF)) return -1;
-  r.sign = 1.f;
+  if (!fill(r, a, b, axes, pos, pos_b, pos64, B, S, D, dtype, false)) return -1;
   r.eps = eps;
   hipStream_t st = (hipStream_t)stream;
-  if (dtype == 0) launch_rope<float, true>(r, st);
-  else if (dtype == 1) launch_rope<bf16, true>(r, st);
-  else launch_rope<f16, true>(r, st);
+  if (dtype == 0) launch_rope<float, true, false>(r, st);
+  else if (dtype == 1) launch_rope<bf16, true, false>(r, st);
+  else launch_rope<f16, true, false>(r, st);
   return (int)hipGetLastError();
 }
 
@@ -403,7 +421,7 @@ int turtle_token_norm_rope_bwd(const turtle_token_side* a, const turtle_token_si
                                const void* pos, int64_t pos_b, int pos64, int64_t B, int64_t S, int D, float eps, float* dw,
                                void* ws, size_t ws_bytes, int dtype, void* stream) {
   RopeArgs r;
-  if (!fill(r, a, b, axes, pos, pos_b, pos64, B, S, D, dtype, true, UB)) return -1;
+  if (!fill(r, a, b, axes, pos, pos_b, pos64, B, S, D, dtype, true)) return -1;
   const dim3 g = blocks_for(r, dw ? MAXB : 1 << 20);
   const int nblk = (int)(g.x * g.y);
   if (dw && (!ws || (uintptr_t)ws % 16 || ws_bytes < (size_t)nblk * 2 * D * sizeof(float))) return -1;
