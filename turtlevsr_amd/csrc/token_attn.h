@@ -14,9 +14,9 @@
 // two 4-key pieces. Nothing is exchanged through memory between the two products.
 //
 // Tiles of BN keys of K and V go HBM -> LDS by LDS-DMA into a ring of NS slots, NS - 1 tiles in flight behind the
-// current one's products; one barrier a tile (it frees the slot of the tile before). LDS rows are not padded (the DMA writes lane-linear): 16-byte chunk c of row r sits at chunk
-// c ^ swz(r), applied on the DMA's source address, so that both the row reads (K: 32 rows, one chunk) and the
-// transposing reads (V: 4 rows, 4 chunks) touch distinct banks.
+// current one's products; one barrier a tile (it frees the slot of the tile before). LDS rows are not padded (the DMA
+// writes lane-linear): 16-byte chunk c of row r sits at chunk c ^ swz(r), applied on the DMA's source address, so that
+// both the row reads (K: 32 rows, one chunk) and the transposing reads (V: 4 rows, 4 chunks) touch distinct banks.
 //
 // Backward, two kernels and no atomics, so results do not depend on the launch's order:
 //   dk, dv: a wave owns 32 keys and walks over the rows: S = Q K^T, dP = dO V^T (rows x keys, lane = key), then
@@ -158,26 +158,16 @@ struct Rows {
     const int li = lane & 15, row = 4 * (lane >> 5) + (li >> 2), sub = ((lane >> 4) & 1) * 2 + ((li & 3) >> 1);
     return lds_addr(t) + row * ROWB + ((sub ^ swz(row)) << 4) + (li & 1) * 8;
   }
-  // acc[j][w] = (rows 32 j .. 32 j + 31)(channels) x frag[w], the KT RW chains of products interleaved: frag is the B
-  // operand's STEPS chunks
-  template <int KT, int RW>
-  TURTLE_DEV static void times(const char* t, const uint4 (&frag)[RW][STEPS], f32x16 (&acc)[KT][RW], int lane) {
+  // acc[j] = (rows 32 j .. 32 j + 31)(channels) x frag, the KT chains of products interleaved: frag is the B operand's
+  // STEPS chunks
+  template <int KT>
+  TURTLE_DEV static void times(const char* t, const uint4 (&frag)[STEPS], f32x16 (&acc)[KT], int lane) {
     const uint32_t base = row_base(t, lane);
 #pragma unroll
-    for (int j = 0; j < KT; ++j)
-#pragma unroll
-      for (int w = 0; w < RW; ++w) acc[j][w] = zero16();
+    for (int j = 0; j < KT; ++j) acc[j] = zero16();
     static_for<STEPS>([&](auto s) {
-      static_for<KT>([&](auto j) {
-        const uint4 x = chunk<s(), j()>(base);
-#pragma unroll
-        for (int w = 0; w < RW; ++w) acc[j()][w] = mma<T>(x, frag[w][s()], acc[j()][w]);
-      });
+      static_for<KT>([&](auto j) { acc[j()] = mma<T>(chunk<s(), j()>(base), frag[s()], acc[j()]); });
     });
-  }
-  template <int KT>
-  TURTLE_DEV static void times(const char* t, const uint4 (&f)[STEPS], f32x16 (&acc)[KT], int lane) {
-    times<KT, 1>(t, reinterpret_cast<const uint4 (&)[1][STEPS]>(f), reinterpret_cast<f32x16 (&)[KT][1]>(acc), lane);
   }
   // the same of two tiles with an operand each; a1 comes with its initial values
   template <int KT>
@@ -210,48 +200,39 @@ struct Rows {
       });
     });
   }
-  // acc[w][dt] += (rows 16 U .. 16 U + 15)^T (channels 32 dt ..) x p[w]: 16-bit types, p packed from 8 accumulator
-  // registers' values of those rows. LO: a second term (lo[w]) of p besides
-  template <int U, int RW, bool LO>
-  TURTLE_DEV static void t_times(const char* t, const uint4 (&hi)[RW], const uint4 (&lo)[RW], f32x16 (&acc)[RW][DT], int lane) {
+  // acc[dt] += (rows 16 U .. 16 U + 15)^T (channels 32 dt ..) x p: 16-bit types, p packed from 8 accumulator registers'
+  // values of those rows. LO: a second term of p besides
+  template <int U, bool LO>
+  TURTLE_DEV static void t_times(const char* t, uint4 hi, uint4 lo, f32x16 (&acc)[DT], int lane) {
     const uint32_t base = tr_base(t, lane);
     static_for<DT>([&](auto dt) {
       const uint32_t a = base ^ (dt() << 6);
       const uint2 x = lds_ld_tr(a + U * 16 * ROWB), y = lds_ld_tr((a ^ 32) + (U * 16 + 8) * ROWB);
       const uint4 v = make_uint4(x.x, x.y, y.x, y.y);
-#pragma unroll
-      for (int w = 0; w < RW; ++w) {
-        acc[w][dt()] = mma<T>(v, hi[w], acc[w][dt()]);
-        if constexpr (LO) acc[w][dt()] = mma<T>(v, lo[w], acc[w][dt()]);
-      }
+      acc[dt()] = mma<T>(v, hi, acc[dt()]);
+      if constexpr (LO) acc[dt()] = mma<T>(v, lo, acc[dt()]);
     });
   }
   // the same for fp32, from register values: row 8 (e >> 2) + (e & 3) + 4 h, channel 32 dt + (lane & 31)
-  template <int U, int RW>
-  TURTLE_DEV static void t_times(const char* t, const float (&p)[RW][8], f32x16 (&acc)[RW][DT], int lane) {
+  template <int U>
+  TURTLE_DEV static void t_times(const char* t, const float (&p)[8], f32x16 (&acc)[DT], int lane) {
     const int h = lane >> 5;
     static_for<8>([&](auto e) {
       const int row = U * 16 + acc_row(e()) + 4 * h;
       const uint32_t a = lds_addr(t) + row * ROWB + ((((lane & 31) >> 2) ^ swz(row)) << 4) + (lane & 3) * 4;
       static_for<DT>([&](auto dt) {
-        const float v = lds_ld4(a ^ (dt() << 7));
-#pragma unroll
-        for (int w = 0; w < RW; ++w) acc[w][dt()] = __builtin_amdgcn_mfma_f32_32x32x2f32(v, p[w][e()], acc[w][dt()], 0, 0, 0);
+        acc[dt()] = __builtin_amdgcn_mfma_f32_32x32x2f32(lds_ld4(a ^ (dt() << 7)), p[e()], acc[dt()], 0, 0, 0);
       });
     });
   }
   // one operand, rounded (16-bit) or as it is (fp32): 8 values from register 8 (U & 1) on of the tile p[U >> 1]
   template <int U, int KT>
-  TURTLE_DEV static void t_times1(const char* t, const f32x16 (&p)[KT], f32x16 (&acc)[1][DT], int lane) {
-    float x[1][8];
+  TURTLE_DEV static void t_times1(const char* t, const f32x16 (&p)[KT], f32x16 (&acc)[DT], int lane) {
+    float x[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) x[0][e] = p[U >> 1][8 * (U & 1) + e];
-    if constexpr (ES == 2) {
-      const uint4 hi[1] = {pack(x[0])};
-      t_times<U, 1, false>(t, hi, hi, acc, lane);
-    } else {
-      t_times<U, 1>(t, x, acc, lane);
-    }
+    for (int e = 0; e < 8; ++e) x[e] = p[U >> 1][8 * (U & 1) + e];
+    if constexpr (ES == 2) t_times<U, false>(t, pack(x), make_uint4(0, 0, 0, 0), acc, lane);
+    else t_times<U>(t, x, acc, lane);
   }
   // sum of the 8 packed values, added to l
   TURTLE_DEV static float sum_packed(uint4 p, float l) {

@@ -1,9 +1,6 @@
 // Token attention, backward (token_attn.h holds the method and the shared parts): delta, then dk and dv by key tiles,
 // then dq by row tiles. No atomics: every sum has a fixed order.
 #include "token_attn.h"
-#ifndef WKMAX
-#define WKMAX 128
-#endif
 
 namespace turtle {
 namespace {
@@ -88,7 +85,7 @@ TURTLE_DEV void join_waves(f32x16 (&acc)[DT], float* sum, int wave, int lane) {
 
 // dv's accumulators: its own, or dk's where a block has only one of them
 template <bool SAME, int N, int M>
-TURTLE_DEV auto& pick(f32x16 (&x)[1][N], f32x16 (&y)[1][M]) {
+TURTLE_DEV auto& pick(f32x16 (&x)[N], f32x16 (&y)[M]) {
   if constexpr (SAME) return x;
   else return y;
 }
@@ -192,10 +189,10 @@ __global__ __launch_bounds__(NW * RG * 64, sizeof(T) == 2 && (DP == 64 || RG == 
   };
 
   // the sums of dk and dv; SP: the one or the other
-  f32x16 dk[1][DT], dv_[1][SP ? 1 : DT];
+  f32x16 dk[DT], dv_[SP ? 1 : DT];
   auto& dv = pick<SP>(dk, dv_);
 #pragma unroll
-  for (int i = 0; i < DT; ++i) { dk[0][i] = zero16(); dv[0][i] = zero16(); }
+  for (int i = 0; i < DT; ++i) { dk[i] = zero16(); dv[i] = zero16(); }
 
   // the walk over row tiles: as the forward's over key tiles
   struct Tile { int t; bool mixed; } q[NS - 1];
@@ -307,15 +304,15 @@ __global__ __launch_bounds__(NW * RG * 64, sizeof(T) == 2 && (DP == 64 || RG == 
     slot = slot + 1 == NS ? 0 : slot + 1;
   }
   if constexpr (WK) {
-    join_waves<NW>(dk[0], reinterpret_cast<float*>(smem), wave, lane);
-    if constexpr (!SP) join_waves<NW>(dv[0], reinterpret_cast<float*>(smem), wave, lane);
+    join_waves<NW>(dk, reinterpret_cast<float*>(smem), wave, lane);
+    if constexpr (!SP) join_waves<NW>(dv, reinterpret_cast<float*>(smem), wave, lane);
   }
   if constexpr (RG > 1) {
     // the row groups' sums, in order, through LDS
     float* sum = reinterpret_cast<float*>(smem) + wave * DT * 16 * 64 + lane;
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
-      f32x16 (&acc)[DT] = k ? dv[0] : dk[0];
+      f32x16 (&acc)[DT] = k ? dv : dk;
       __syncthreads();
       if (rg == 1) {
 #pragma unroll
@@ -345,8 +342,8 @@ __global__ __launch_bounds__(NW * RG * 64, sizeof(T) == 2 && (DP == 64 || RG == 
       float x[4], y[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        x[e] = kon ? dk[0][dt][4 * q4 + e] * a.scale : 0.f;
-        y[e] = kon ? dv[0][dt][4 * q4 + e] * (1.f / PUP) : 0.f;
+        x[e] = kon ? dk[dt][4 * q4 + e] * a.scale : 0.f;
+        y[e] = kon ? dv[dt][4 * q4 + e] * (1.f / PUP) : 0.f;
       }
       if (do_k) R::put4(reinterpret_cast<T*>(a.dk) + oi + d, x);
       if (do_v) R::put4(reinterpret_cast<T*>(a.dv) + oi + d, y);
@@ -424,9 +421,9 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 ? 2 : 1) void attn_dq_kerne
       p1 = vbase + key * vst;
     });
   };
-  f32x16 dq[1][DT];
+  f32x16 dq[DT];
 #pragma unroll
-  for (int j = 0; j < DT; ++j) dq[0][j] = zero16();
+  for (int j = 0; j < DT; ++j) dq[j] = zero16();
 
   struct Tile { int t; bool mixed; } q[NS - 1];
   int tnew = WK ? wave : 0, fill = NS - 1, fly = 0, into = 0, slot = 0;
@@ -502,7 +499,7 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 ? 2 : 1) void attn_dq_kerne
     --fly;
     slot = slot + 1 == NS ? 0 : slot + 1;
   }
-  if constexpr (WK) join_waves<NW>(dq[0], reinterpret_cast<float*>(smem), wave, lane);
+  if constexpr (WK) join_waves<NW>(dq, reinterpret_cast<float*>(smem), wave, lane);
   if (mrow >= a.M) return;
   const int64_t oi = (((int64_t)b * a.Sq + i) * a.Hq + hq) * a.D;
 #pragma unroll
@@ -514,7 +511,7 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 ? 2 : 1) void attn_dq_kerne
       if (d >= a.D) continue;
       float x[4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) x[e] = row.on ? dq[0][dt][4 * q4 + e] * a.scale : 0.f;
+      for (int e = 0; e < 4; ++e) x[e] = row.on ? dq[dt][4 * q4 + e] * a.scale : 0.f;
       R::put4(reinterpret_cast<T*>(a.dq) + oi + d, x);
     }
   }
@@ -541,13 +538,20 @@ int bwd(Args& a, float* delta, hipStream_t st) {
   if (rc) return rc;
   a.delta = delta;
   constexpr int WK = sizeof(T) == 4 && DP == 128 ? 2 : 4;
+  // WK gives four times the blocks of 32 keys (rows) instead of 128: taken up to a number of 128-blocks. Measured at 1024
+  // tokens and 8, 16, 24 and 32 heads (64 .. 256 blocks), us with / without WK:
+  //   dk, dv  bf16, 64 channels 21 / 40, 24 / 40, 39 / 42, 43 / 43; 128 channels 46 / 48, 91 / 51, 132 / 53, 176 / 56
+  //           fp32, 64 channels 58 / 181, 112 / 184, 165 / 187, 222 / 190; 128 channels 268 / 258 (32 blocks 135 / 255), 536 / 265
+  //   dq      bf16, 64 channels 11 / 22, 20 / 22, 28 / 23, 37 / 24; 128 channels 18 / 40, 36 / 41, 52 / 42, 69 / 44
+  //           fp32, 64 channels 40 / 128, 77 / 131, 115 / 135, 156 / 137; 128 channels 129 / 242, 261 / 247
+  constexpr int64_t FEWK = DP == 64 ? 255 : 64, FEWQ = sizeof(T) == 2 ? 128 : DP == 64 ? 255 : 64;
   if (a.dk) {
-    const bool few = ((int64_t)a.Sk + 127) / 128 * bh < WKMAX;
+    const bool few = ((int64_t)a.Sk + 127) / 128 * bh <= FEWK;
     rc = few ? run_dkv<T, DP, WK, 1, true>(a, st) : run_dkv<T, DP, 4, sizeof(T) == 2 && DP == 128 ? 2 : 1, false>(a, st);
     if (rc) return rc;
   }
   if (!a.dq) return 0;
-  const bool few = ((int64_t)a.M + 127) / 128 * bh < WKMAX;
+  const bool few = ((int64_t)a.M + 127) / 128 * bh <= FEWQ;
   return few ? run_dq<T, DP, WK, true>(a, st) : run_dq<T, DP, 4, false>(a, st);
 }
 

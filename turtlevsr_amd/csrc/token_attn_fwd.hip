@@ -1,26 +1,21 @@
 // Token attention, forward: dense and paged (token_attn.h holds the method and the shared parts).
 //
-// Three shapes of one kernel, chosen by the number of rows M = Sq G of a (sequence, key head):
-//   M <= 32, or a small grid    the block's waves take the key tiles of 32 rows in turn, each with its own LDS ring and
-//                               no block barrier, and join at the end
-//   M <= 64, or <= 256 keys     2 waves x 32 rows
-//   otherwise                   4 waves x 32 rows
+// Three shapes of one kernel, chosen in plan_of by the rows M = Sq G of a (sequence, key head) and the keys:
+//   kind 0   the block's waves take the key tiles of 32 rows in turn, each with its own LDS ring and no block barrier, and
+//            join at the end
+//   kind 1   2 waves x 32 rows
+//   kind 2   4 waves x 32 rows
 // The first two have matrix instructions to spare and multiply p in two terms (TWO): with few keys, p's rounding
 // would be as large an error as the result's own.
 #include "token_attn.h"
-#ifndef LMIN
-#define LMIN 512
-#endif
 
 namespace turtle {
 namespace {
 
 template <typename T, int DP, int NW, bool WK> struct Fwd {
   typedef Rows<T, DP> R;
-  static constexpr int RW = 1;                        // row groups of 32 a wave
   static constexpr int NT = NW * 64;
-  static constexpr int WROWS = 32 * RW;               // rows of a wave
-  static constexpr int BM = WK ? WROWS : NW * WROWS;  // rows of a block
+  static constexpr int BM = WK ? 32 : NW * 32;        // rows of a block, 32 a wave
   static constexpr int BN = (WK || sizeof(T) == 4) ? 32 : 64;
   static constexpr int NS = 2;                        // slots of the ring
   static constexpr int TILE = BN * R::ROWB, SLOT = 2 * TILE;
@@ -30,26 +25,26 @@ template <typename T, int DP, int NW, bool WK> struct Fwd {
   static constexpr bool TWO = sizeof(T) == 2 && (WK || NW == 2);
   // the tile's probabilities as operands of the second product
   struct P {
-    uint4 hi[2 * BN / 32][RW], lo[TWO ? 2 * BN / 32 : 1][RW];
-    float x[sizeof(T) == 4 ? 2 * BN / 32 : 1][RW][8];
-    // 8 values of row group w; returns l + their sum (16-bit types: of what the product takes)
-    TURTLE_DEV float put(int u, int w, const float (&v)[8], float l) {
+    uint4 hi[2 * BN / 32], lo[TWO ? 2 * BN / 32 : 1];
+    float x[sizeof(T) == 4 ? 2 * BN / 32 : 1][8];
+    // 8 values; returns l + their sum (16-bit types: of what the product takes)
+    TURTLE_DEV float put(int u, const float (&v)[8], float l) {
       if constexpr (sizeof(T) == 2) {
-        hi[u][w] = R::pack(v);
-        if constexpr (!TWO) return R::sum_packed(hi[u][w], l);
-        else lo[u][w] = R::rest(v, hi[u][w]);
+        hi[u] = R::pack(v);
+        if constexpr (!TWO) return R::sum_packed(hi[u], l);
+        else lo[u] = R::rest(v, hi[u]);
       }
       float a = 0.f, b = 0.f;
 #pragma unroll
       for (int e = 0; e < 8; e += 2) {
         a += v[e]; b += v[e + 1];
-        if constexpr (sizeof(T) == 4) { x[u][w][e] = v[e]; x[u][w][e + 1] = v[e + 1]; }
+        if constexpr (sizeof(T) == 4) { x[u][e] = v[e]; x[u][e + 1] = v[e + 1]; }
       }
       return l + (a + b);
     }
-    template <int U> TURTLE_DEV void times(const char* vt, f32x16 (&acc)[RW][R::DT], int lane) const {
-      if constexpr (sizeof(T) == 2) R::template t_times<U, RW, TWO>(vt, hi[U], lo[TWO ? U : 0], acc, lane);
-      else R::template t_times<U, RW>(vt, x[U], acc, lane);
+    template <int U> TURTLE_DEV void times(const char* vt, f32x16 (&acc)[R::DT], int lane) const {
+      if constexpr (sizeof(T) == 2) R::template t_times<U, TWO>(vt, hi[U], lo[TWO ? U : 0], acc, lane);
+      else R::template t_times<U>(vt, x[U], acc, lane);
     }
   };
   // LDS without the page numbers; a call with fewer tiles than slots takes only those
@@ -65,7 +60,7 @@ template <typename T, int DP, int NW, bool WK, bool PAGED>
 __global__ __launch_bounds__(NW * 64, DP == 128 && sizeof(T) == 4 ? 1 : 2) void attn_fwd_kernel(Args a) {
   typedef Fwd<T, DP, NW, WK> F;
   typedef Rows<T, DP> R;
-  constexpr int BN = F::BN, KT = BN / 32, RW = F::RW, DT = R::DT, STEP = WK ? NW : 1;
+  constexpr int BN = F::BN, KT = BN / 32, DT = R::DT, STEP = WK ? NW : 1;
   // fp16: p is scaled by 2^6 (p of many keys would lose bits below the type's normal range) and stays under its 2^16
   constexpr float POFF = std::is_same<T, f16>::value ? 6.f : 0.f;
   constexpr float SLACK = 8.f;
@@ -87,14 +82,9 @@ __global__ __launch_bounds__(NW * 64, DP == 128 && sizeof(T) == 4 ? 1 : 2) void 
   }
   const int m0 = mt * F::BM, mend = min(a.M, nq * a.G), m1 = min(m0 + F::BM, mend);   // rows of this block that exist: [m0, m1)
   const int pre = (!PAGED && a.prefix) ? a.prefix[b] : 0;
-  const int mw = m0 + (WK ? 0 : wave * F::WROWS), mw1 = min(mw + F::WROWS, mend);     // ... of this wave
-  int mrow[RW];
-  Row row[RW];
-#pragma unroll
-  for (int w = 0; w < RW; ++w) {
-    mrow[w] = mw + w * 32 + (lane & 31);
-    row[w] = row_of(a, b, hk, mrow[w], off, nq);
-  }
+  const int mw = m0 + (WK ? 0 : wave * 32), mw1 = min(mw + 32, mend);     // ... of this wave
+  const int mrow = mw + (lane & 31);
+  const Row row = row_of(a, b, hk, mrow, off, nq);
 
   // key tiles this block walks over
   int kend = kn;
@@ -114,13 +104,10 @@ __global__ __launch_bounds__(NW * 64, DP == 128 && sizeof(T) == 4 ? 1 : 2) void 
   const int whole = a.causal ? max(mw / a.G + off + 1, pre) : 0x7fffffff;
   const int some = mw1 <= mw ? 0 : (a.causal ? max((mw1 - 1) / a.G + off + 1, pre) : 0x7fffffff);
 
-  uint4 qf[RW][R::STEPS];
-#pragma unroll
-  for (int w = 0; w < RW; ++w) {
-    const int i = token_of(a, mrow[w]), g = mrow[w] - i * a.G;
-    R::frag(row[w].on ? reinterpret_cast<const T*>(a.q) + (int64_t)b * a.qb + (int64_t)i * a.qs + (int64_t)(hk * a.G + g) * a.qh : nullptr,
-            a.D, qf[w], lane);
-  }
+  uint4 qf[R::STEPS];
+  const int qi = token_of(a, mrow), qg = mrow - qi * a.G;
+  R::frag(row.on ? reinterpret_cast<const T*>(a.q) + (int64_t)b * a.qb + (int64_t)qi * a.qs + (int64_t)(hk * a.G + qg) * a.qh : nullptr, a.D,
+          qf, lane);
 
   char* buf = smem + (WK ? wave * F::NS * F::SLOT : 0);
   const char* kbase = reinterpret_cast<const char*>(a.k) + ((PAGED ? 0 : (int64_t)b * a.kb) + (int64_t)hk * a.kh) * R::ES;
@@ -188,15 +175,10 @@ __global__ __launch_bounds__(NW * 64, DP == 128 && sizeof(T) == 4 ? 1 : 2) void 
     }
   };
 
-  f32x16 acc[RW][DT];
-  float mx[RW], l[RW];
+  f32x16 acc[DT];
+  float mx = -INFINITY, l = 0.f;
 #pragma unroll
-  for (int w = 0; w < RW; ++w) {
-#pragma unroll
-    for (int i = 0; i < DT; ++i) acc[w][i] = zero16();
-    mx[w] = -INFINITY;
-    l[w] = 0.f;
-  }
+  for (int i = 0; i < DT; ++i) acc[i] = zero16();
 
   // The walk: tiles are started NS - 1 turns before they are computed on (q: the tiles in flight, oldest first). With a
   // block the turn's barrier frees the slot of the tile before; a wave of its own starts the next tile at once.
@@ -230,38 +212,33 @@ __global__ __launch_bounds__(NW * 64, DP == 128 && sizeof(T) == 4 ? 1 : 2) void 
     uint64_t seen = cur.seen;
 
     if (k0 < some) {
-      f32x16 s[KT][RW];
-      R::template times<KT, RW>(kt, qf, s, lane);
+      f32x16 s[KT];
+      R::template times<KT>(kt, qf, s, lane);
       // the rules that apply to this tile, each in a pass of its own (uniform branches)
       const bool caus = k0 + BN > whole;
       bool gaps = k0 + BN > kn;
       if constexpr (PAGED) gaps = BN == 32 ? (uint32_t)seen != ~0u : seen != ~0ull;
       float mul = a.scale2;
       if (a.cap > 0.f) {
-#pragma unroll
-        for (int j = 0; j < KT; ++j) tanh_all<T, RW>(s[j], a.icap);
+        tanh_all<T, KT>(s, a.icap);
         mul = a.cap2;
       }
       if (a.slopes || mul <= 0.f) {
 #pragma unroll
-        for (int j = 0; j < KT; ++j)
+        for (int j = 0; j < KT; ++j) {
+          const int at = row.pos - k0 - j * 32 - 4 * h;
 #pragma unroll
-          for (int w = 0; w < RW; ++w) {
-            const int at = row[w].pos - k0 - j * 32 - 4 * h;
-#pragma unroll
-            for (int r = 0; r < 16; ++r) s[j][w][r] = fmaf(-row[w].slope2, fabsf((float)(at - acc_row(r))), s[j][w][r] * mul);
-          }
+          for (int r = 0; r < 16; ++r) s[j][r] = fmaf(-row.slope2, fabsf((float)(at - acc_row(r))), s[j][r] * mul);
+        }
         mul = 1.f;
       }
       if (caus) {
 #pragma unroll
-        for (int j = 0; j < KT; ++j)
+        for (int j = 0; j < KT; ++j) {
+          const int last = max(row.pos, pre - 1) - k0 - j * 32 - 4 * h;      // the last key in sight
 #pragma unroll
-          for (int w = 0; w < RW; ++w) {
-            const int last = max(row[w].pos, pre - 1) - k0 - j * 32 - 4 * h;      // the last key in sight
-#pragma unroll
-            for (int r = 0; r < 16; ++r) s[j][w][r] = acc_row(r) <= last ? s[j][w][r] : -INFINITY;
-          }
+          for (int r = 0; r < 16; ++r) s[j][r] = acc_row(r) <= last ? s[j][r] : -INFINITY;
+        }
       }
       if (gaps) {
         if constexpr (!PAGED) seen = kn - k0 >= 64 ? ~0ull : (1ull << (kn - k0)) - 1;
@@ -269,9 +246,7 @@ __global__ __launch_bounds__(NW * 64, DP == 128 && sizeof(T) == 4 ? 1 : 2) void 
         for (int j = 0; j < KT; ++j) {
           const uint32_t bits = (uint32_t)(seen >> (j * 32)) >> (4 * h);
 #pragma unroll
-          for (int w = 0; w < RW; ++w)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) s[j][w][r] = (bits >> acc_row(r)) & 1 ? s[j][w][r] : -INFINITY;
+          for (int r = 0; r < 16; ++r) s[j][r] = (bits >> acc_row(r)) & 1 ? s[j][r] : -INFINITY;
         }
       }
       if (mixed) {
@@ -282,42 +257,35 @@ __global__ __launch_bounds__(NW * 64, DP == 128 && sizeof(T) == 4 ? 1 : 2) void 
 #pragma unroll
           for (int r = 0; r < 16; ++r) {
             const int d = __shfl(kd, j * 32 + acc_row(r) + 4 * h, 64);
-#pragma unroll
-            for (int w = 0; w < RW; ++w) s[j][w][r] = d == row[w].doc ? s[j][w][r] : -INFINITY;
+            s[j][r] = d == row.doc ? s[j][r] : -INFINITY;
           }
       }
 
       // p = 2^(s - mx) against the running reference mx, a maximum of earlier tiles: it serves as long as no score of a
       // lane is over it by more than SLACK. Only else are the row's halves compared and the accumulators rescaled.
+      float tm = -INFINITY;
 #pragma unroll
-      for (int w = 0; w < RW; ++w) {
-        float tm = -INFINITY;
+      for (int j = 0; j < KT; ++j)
 #pragma unroll
-        for (int j = 0; j < KT; ++j)
+        for (int r = 0; r < 16; ++r) tm = fmaxf(tm, s[j][r]);
+      if (__any(!(tm * mul <= mx + SLACK))) {
+        const float mn = fmaxf(mx, half_max(tm) * mul);
+        const float al = __builtin_amdgcn_exp2f(mx - (mn == -INFINITY ? 0.f : mn));
+        mx = mn;
+        l *= al;
 #pragma unroll
-          for (int r = 0; r < 16; ++r) tm = fmaxf(tm, s[j][w][r]);
-        if (__any(!(tm * mul <= mx[w] + SLACK))) {
-          const float mn = fmaxf(mx[w], half_max(tm) * mul);
-          const float al = __builtin_amdgcn_exp2f(mx[w] - (mn == -INFINITY ? 0.f : mn));
-          mx[w] = mn;
-          l[w] *= al;
+        for (int i = 0; i < DT; ++i)
 #pragma unroll
-          for (int i = 0; i < DT; ++i)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) acc[w][i][r] *= al;
-        }
+          for (int r = 0; r < 16; ++r) acc[i][r] *= al;
       }
       typename F::P p;
+      const float sh = POFF - (mx == -INFINITY ? 0.f : mx);
 #pragma unroll
-      for (int w = 0; w < RW; ++w) {
-        const float sh = POFF - (mx[w] == -INFINITY ? 0.f : mx[w]);
+      for (int u = 0; u < 2 * KT; ++u) {
+        float x[8];
 #pragma unroll
-        for (int u = 0; u < 2 * KT; ++u) {
-          float x[8];
-#pragma unroll
-          for (int e = 0; e < 8; ++e) x[e] = __builtin_amdgcn_exp2f(fmaf(s[u >> 1][w][8 * (u & 1) + e], mul, sh));
-          l[w] = p.put(u, w, x, l[w]);
-        }
+        for (int e = 0; e < 8; ++e) x[e] = __builtin_amdgcn_exp2f(fmaf(s[u >> 1][8 * (u & 1) + e], mul, sh));
+        l = p.put(u, x, l);
       }
       static_for<2 * KT>([&](auto u) { p.template times<u()>(vt, acc, lane); });
     }
@@ -325,25 +293,24 @@ __global__ __launch_bounds__(NW * 64, DP == 128 && sizeof(T) == 4 ? 1 : 2) void 
     --fly;
     slot = slot + 1 == NS ? 0 : slot + 1;
   }
-#pragma unroll
-  for (int w = 0; w < RW; ++w) l[w] = half_sum(l[w]);
+  l = half_sum(l);
 
   if constexpr (WK) {
     // join the waves: their (max, sum), then the rescaled accumulators summed through LDS in wave order
     float* ml = reinterpret_cast<float*>(smem);
     float* sum = ml + 2 * NW * 32;
     __syncthreads();
-    if (h == 0) { ml[wave * 32 + lane] = mx[0]; ml[(NW + wave) * 32 + lane] = l[0]; }
+    if (h == 0) { ml[wave * 32 + lane] = mx; ml[(NW + wave) * 32 + lane] = l; }
     __syncthreads();
     float mall = -INFINITY;
 #pragma unroll
     for (int w = 0; w < NW; ++w) mall = fmaxf(mall, ml[w * 32 + (lane & 31)]);
     const float mb = mall == -INFINITY ? 0.f : mall;
-    l[0] = 0.f;
+    l = 0.f;
 #pragma unroll
-    for (int w = 0; w < NW; ++w) l[0] += ml[(NW + w) * 32 + (lane & 31)] * __builtin_amdgcn_exp2f(ml[w * 32 + (lane & 31)] - mb);
-    const float f = __builtin_amdgcn_exp2f(mx[0] - mb);
-    mx[0] = mall;
+    for (int w = 0; w < NW; ++w) l += ml[(NW + w) * 32 + (lane & 31)] * __builtin_amdgcn_exp2f(ml[w * 32 + (lane & 31)] - mb);
+    const float f = __builtin_amdgcn_exp2f(mx - mb);
+    mx = mall;
     for (int w = 0; w < NW; ++w) {
       if (wave == w) {
 #pragma unroll
@@ -351,7 +318,7 @@ __global__ __launch_bounds__(NW * 64, DP == 128 && sizeof(T) == 4 ? 1 : 2) void 
 #pragma unroll
           for (int r = 0; r < 16; ++r) {
             float* p = sum + (dt * 16 + r) * 64 + lane;
-            *p = (w ? *p : 0.f) + acc[0][dt][r] * f;
+            *p = (w ? *p : 0.f) + acc[dt][r] * f;
           }
       }
       __syncthreads();
@@ -360,36 +327,32 @@ __global__ __launch_bounds__(NW * 64, DP == 128 && sizeof(T) == 4 ? 1 : 2) void 
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) acc[0][dt][r] = sum[(dt * 16 + r) * 64 + lane];
+      for (int r = 0; r < 16; ++r) acc[dt][r] = sum[(dt * 16 + r) * 64 + lane];
   }
 
+  if (mrow >= a.M) return;
+  const float inv = (l > 0.f && row.on) ? 1.f / l : 0.f;
+  const float lse = inv > 0.f ? mx + log2f(l) - POFF : INFINITY;
+  const bool first = (!WK || wave == 0) && h == 0;
+  const int64_t pi = ((int64_t)sp * a.B * a.Hk + bh) * a.M + mrow;
+  const int64_t oi = (((int64_t)b * a.Sq + qi) * a.Hq + hk * a.G + qg) * a.D;
+  if (first && a.nsplit > 1) a.plse[pi] = lse;
+  if (first && a.nsplit <= 1 && a.lse) a.lse[(int64_t)bh * a.M + mrow] = lse;
 #pragma unroll
-  for (int w = 0; w < RW; ++w) {
-    if (mrow[w] >= a.M) continue;
-    const float inv = (l[w] > 0.f && row[w].on) ? 1.f / l[w] : 0.f;
-    const float lse = inv > 0.f ? mx[w] + log2f(l[w]) - POFF : INFINITY;
-    const int i = token_of(a, mrow[w]), g = mrow[w] - i * a.G;
-    const bool first = (!WK || wave == 0) && h == 0;
-    const int64_t pi = ((int64_t)sp * a.B * a.Hk + bh) * a.M + mrow[w];
-    const int64_t oi = (((int64_t)b * a.Sq + i) * a.Hq + hk * a.G + g) * a.D;
-    if (first && a.nsplit > 1) a.plse[pi] = lse;
-    if (first && a.nsplit <= 1 && a.lse) a.lse[(int64_t)bh * a.M + mrow[w]] = lse;
+  for (int dt = 0; dt < DT; ++dt) {
+    if (WK && dt % NW != wave) continue;
 #pragma unroll
-    for (int dt = 0; dt < DT; ++dt) {
-      if (WK && dt % NW != wave) continue;
+    for (int q4 = 0; q4 < 4; ++q4) {
+      const int d = dt * 32 + 8 * q4 + 4 * h;
+      if (d >= a.D) continue;
+      float v[4], lo[4];
 #pragma unroll
-      for (int q4 = 0; q4 < 4; ++q4) {
-        const int d = dt * 32 + 8 * q4 + 4 * h;
-        if (d >= a.D) continue;
-        float v[4], lo[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) { v[e] = acc[w][dt][4 * q4 + e] * inv; lo[e] = v[e] - to_f((T)v[e]); }
-        if (a.nsplit > 1) {
-          *reinterpret_cast<float4*>(a.part + pi * a.D + d) = make_float4(v[0], v[1], v[2], v[3]);
-        } else {
-          R::put4(reinterpret_cast<T*>(a.o) + oi + d, v);
-          if (a.olo) R::put4(reinterpret_cast<T*>(a.olo) + oi + d, lo);
-        }
+      for (int e = 0; e < 4; ++e) { v[e] = acc[dt][4 * q4 + e] * inv; lo[e] = v[e] - to_f((T)v[e]); }
+      if (a.nsplit > 1) {
+        *reinterpret_cast<float4*>(a.part + pi * a.D + d) = make_float4(v[0], v[1], v[2], v[3]);
+      } else {
+        R::put4(reinterpret_cast<T*>(a.o) + oi + d, v);
+        if (a.olo) R::put4(reinterpret_cast<T*>(a.olo) + oi + d, lo);
       }
     }
   }
@@ -420,18 +383,21 @@ __global__ __launch_bounds__(256) void attn_join_kernel(Args a) {
   const int64_t r = u / c4;
   const int d = (int)(u - r * c4) * 4;
   float mx = -INFINITY;
+#pragma unroll 8
   for (int s = 0; s < a.nsplit; ++s) {
     const float x = a.plse[s * stride + r];
-    if (x != INFINITY) mx = fmaxf(mx, x);
+    mx = fmaxf(mx, x == INFINITY ? -INFINITY : x);
   }
   float v[4] = {0.f, 0.f, 0.f, 0.f}, l = 0.f;
-  for (int s = 0; s < a.nsplit; ++s) {
+#pragma unroll 8
+  for (int s = 0; s < a.nsplit; ++s) {                    // unrolled, no branch: the loads of 8 splits are in flight
     const float x = a.plse[s * stride + r];
-    if (x == INFINITY) continue;
-    const float w = __builtin_amdgcn_exp2f(x - mx);
     const float4 p = *reinterpret_cast<const float4*>(a.part + (s * stride + r) * a.D + d);
+    const bool none = x == INFINITY;
+    const float w = none ? 0.f : __builtin_amdgcn_exp2f(x - mx);
     l += w;
-    v[0] = fmaf(w, p.x, v[0]); v[1] = fmaf(w, p.y, v[1]); v[2] = fmaf(w, p.z, v[2]); v[3] = fmaf(w, p.w, v[3]);
+    v[0] = fmaf(w, none ? 0.f : p.x, v[0]); v[1] = fmaf(w, none ? 0.f : p.y, v[1]);
+    v[2] = fmaf(w, none ? 0.f : p.z, v[2]); v[3] = fmaf(w, none ? 0.f : p.w, v[3]);
   }
   const float inv = l > 0.f ? 1.f / l : 0.f;
   float lo[4];
@@ -446,18 +412,30 @@ __global__ __launch_bounds__(256) void attn_join_kernel(Args a) {
 
 struct Plan { int kind, nsplit; int64_t mtiles; };      // kind: 0 waves split the keys, 1 two waves, 2 four waves
 
+// The shape of the grid. All times are of bf16 and 64 / 128 channels, fp32 where its choice differs.
+//   kind 0 gives four times the blocks of kind 2 and no barriers, but each block re-reads its keys for 32 rows only:
+//   taken for up to 32 rows (24 rows x 1024 keys, 256 heads: 18 / 28 us for 24 / 32), and for small grids (1024 x 1024, 8
+//   heads: 14 / 20 for 19 / 25; 32 heads: 32 / 67 for 23 / 32). A small grid with long keys has work enough when they
+//   are split (256 rows x 4096 keys, 16 heads: 25 / 39 for 23 / 32; 2048 keys: 19 / 26 for 20 / 27). And with a tile or
+//   less for each of the four waves there is nothing to split (24 x 24, 512 heads: 8 / 17 for 7 / 9; fp32, where only
+//   kind 2 has no split and its blocks are large: 18 / 27 for 9 / 23 at 24 keys, but 25 for 34 at 64).
+//   kind 1 is kind 2 with p in two terms, for few keys (256 x 256, 512 heads: 33 / 60 us, kind 2 25 / 39).
 Plan plan_of(const In* x, int dtype) {
   const int64_t M = (int64_t)x->Sq * (x->Hq / x->Hk), bh = (int64_t)x->B * x->Hk, room = key_room(x);
+  const bool half = dtype != 0;
   Plan p;
   int bm;
-  const int64_t b64 = (M + 63) / 64 * bh;
-  if (M <= 32 || b64 < 256) { p.kind = 0; bm = 32; }
-  else if (dtype != 0 && (M <= 64 || room <= 256)) { p.kind = 1; bm = 64; }
+  const int64_t b64 = (M + 63) / 64 * bh, b128 = (M + 127) / 128 * bh;
+  const bool small = b64 < 256 && (M <= 64 || b128 * room < (1 << 17));
+  if ((M <= 32 || small) && room > (half ? 128 : 32)) { p.kind = 0; bm = 32; }
+  else if (half && room <= 256) { p.kind = 1; bm = 64; }
   else { p.kind = 2; bm = 128; }
   p.mtiles = (M + bm - 1) / bm;
-  // too few blocks to fill the 256 CUs: the keys are split over blocks too, 512 at least each, and joined by a second
-  // kernel
-  const int64_t want = std::max<int64_t>(1, (p.kind == 0 && dtype != 0 && x->D <= 64 ? 512 : 256) / (p.mtiles * bh)), most = std::max<int64_t>(1, room / 512);
+  // Too few blocks to fill the 256 CUs: the keys are split over blocks too, 512 at least each, and joined by a second
+  // kernel. 16-bit types of up to 64 channels: two blocks a CU have room (256 rows x 8192 keys, 16 heads: 30 us, with one
+  // 34); else one (one token, 16384 keys, 16 sequences x 4 key heads x 4, 128 channels: 92 us, with two 100).
+  const int64_t full = half && x->D <= 64 ? 512 : 256;
+  const int64_t blocks = p.mtiles * bh, want = blocks >= 256 ? 1 : full / blocks, most = std::max<int64_t>(1, room / 512);
   p.nsplit = (int)std::min<int64_t>({want, most, 64});
   return p;
 }
