@@ -862,6 +862,84 @@ def test_op_set_takes_the_autocast_type():
     assert HipOps.attention(q, k, v).dtype == torch.float32
 
 
+def _masked(kind, B, Sq, Sk, Hq):
+    if kind == "causal_prefix":
+        return dict(causal=True, prefix=torch.tensor([(Sk * b) // (2 * B) for b in range(B)], device=DEV))
+    if kind == "bias_cap":
+        return dict(softcap=2.0, slopes=torch.linspace(0.0, 0.3, Hq, device=DEV))
+    if kind == "docs":
+        d = _docs(B, max(Sq, Sk), B, 0)
+        d[:, Sk - 21:] = -1
+        d[B // 2] = -1                         # a sequence of padding alone
+        return dict(q_doc=d[:, :Sq], k_doc=d[:, :Sk], causal=Sq == Sk, softcap=3.0)
+    return {}
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("D", [40, 64, 104, 128])
+@pytest.mark.parametrize("kind", ["full", "causal_prefix", "bias_cap", "docs"])
+def test_attention_large_grids(dt, D, kind):
+    """Enough sequences that blocks of 128 rows (keys) fill the card: forward, dk and dv, dq with a block's waves side by
+    side, ragged last tiles, three query heads a key head; queries and keys of one length and of two."""
+    for Sq, Sk in ((300, 300), (261, 300)):
+        B, Hq, Hk = 45, 6, 2
+        q, k, v = (randn(B, s, h, D, dtype=dt, seed=i) for i, (s, h) in enumerate(((Sq, Hq), (Sk, Hk), (Sk, Hk))))
+        check_attention(q, k, v, randn(B, Sq, Hq, D, dtype=dt, seed=9), **_masked(kind, B, Sq, Sk, Hq))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("Sq,Sk,B", [(130, 8200, 8), (70, 100, 3), (60, 200, 140), (9, 30, 300)])
+def test_attention_middle_shapes(dt, D, Sq, Sk, B):
+    """Many rows whose long keys are split, few keys in small and large grids."""
+    for kind in ("full", "bias_cap"):
+        q, k, v = (randn(B, s, h, D, dtype=dt, seed=i) for i, (s, h) in enumerate(((Sq, 2), (Sk, 2), (Sk, 2))))
+        check_attention(q, k, v, randn(B, Sq, 2, D, dtype=dt, seed=9), **_masked(kind, B, Sq, Sk, 2))
+    q, k, v = (randn(B, s, h, D, dtype=dt, seed=i) for i, (s, h) in enumerate(((Sq, 2), (Sk, 1), (Sk, 1))))
+    check_attention(q, k, v, randn(B, Sq, 2, D, dtype=dt, seed=9), **_masked("docs", B, Sq, Sk, 2))
+    check_attention(q, k, v, randn(B, Sq, 2, D, dtype=dt, seed=9), causal=True)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16])
+def test_attention_many_heads_share_a_key(dt):
+    """80 query heads on one key head: more rows of one query than a tile has, 27 of them: a share that divides nothing."""
+    for Hq, Hk, S in ((80, 1, 7), (54, 2, 33)):
+        q, k, v = randn(2, S, Hq, 64, dtype=dt, seed=1), randn(2, S + 3, Hk, 64, dtype=dt, seed=2), randn(2, S + 3, Hk, 64, dtype=dt, seed=3)
+        check_attention(q, k, v, randn(2, S, Hq, 64, dtype=dt, seed=4), causal=True, slopes=torch.linspace(0, 0.5, Hq, device=DEV))
+
+
+@pytest.mark.gpu
+def test_more_sequences_than_a_grid_axis_has_blocks():
+    B = 70000
+    q, k = randn(B, 1, 3, 8, dtype=torch.bfloat16, seed=1).requires_grad_(True), randn(B, 1, 1, 8, dtype=torch.bfloat16, seed=2)
+    pos, w = torch.arange(B, device=DEV).view(B, 1, 1), torch.linspace(0.5, 2, 8, device=DEV)
+    flat = lambda t: t.reshape(1, B, *t.shape[2:])
+    assert torch.equal(flat(T.axial_rope(q, pos, (8,))), T.axial_rope(flat(q), flat(pos), (8,)))
+    dy = randn(B, 1, 3, 8, dtype=torch.bfloat16, seed=3)
+    a, b = T.qk_norm_rope(q, k, pos, w, w, (8,)), T.qk_norm_rope(flat(q), flat(k), flat(pos), w, w, (8,))
+    assert torch.equal(flat(a[0]), b[0]) and torch.equal(flat(a[1]), b[1])
+    (da,), (db,) = torch.autograd.grad(a[0], q, dy), torch.autograd.grad(b[0], q, flat(dy))
+    assert torch.equal(da, db)
+    kv = randn(B, 2, 1, 8, dtype=torch.bfloat16, seed=4)
+    check_attention(q.detach(), kv[..., :1, :], kv[..., :1, :], dy)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("D,Sq,n,B", [(64, 200, 4300, 8), (128, 200, 4300, 8), (64, 65, 300, 130), (104, 130, 340, 70), (64, 70, 120, 4)])
+def test_paged_large_grids(dt, D, Sq, n, B):
+    """Blocks of 128 rows over a cache, with its keys split and whole; caches of few keys; ragged lengths."""
+    lens = [max(0, n - 37 * (b % 9)) if b % 5 else min(n, 3 + b) for b in range(B)]
+    ql = [min(Sq, lens[b]) - (b % 3 if lens[b] > 3 else 0) for b in range(B)]
+    kp, vp, table, k, v = _pages(B, lens, 50, 2, D, dt, seed=Sq)
+    q = randn(B, Sq, 4, D, dtype=dt, seed=6)
+    check_paged(q, kp, vp, table, lens, k, v, ql)
+    check_paged(q, kp, vp, table, lens, k, v, ql, causal=False, softcap=2.0, slopes=torch.linspace(0, 0.3, 4, device=DEV))
+
+
 def test_workspace_sizes_from_python_are_the_library_s():
     """The cached sizes: what the C entry says for the same call, dense and paged."""
     L = T.lib()
