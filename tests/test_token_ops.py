@@ -940,6 +940,128 @@ def test_paged_large_grids(dt, D, Sq, n, B):
     check_paged(q, kp, vp, table, lens, k, v, ql, causal=False, softcap=2.0, slopes=torch.linspace(0, 0.3, 4, device=DEV))
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("G,D", [(33, 64), (40, 128), (64, 64)])
+def test_attention_bias_of_half_a_wave_and_more_sharing_heads(dt, G, D):
+    """Gradients of every sharing head under its own slope, where more heads share a key than a tile has rows."""
+    q, k, v = randn(2, 9, G, D, dtype=dt, seed=1), randn(2, 50, 1, D, dtype=dt, seed=2), randn(2, 50, 1, D, dtype=dt, seed=3)
+    check_attention(q, k, v, randn(2, 9, G, D, dtype=dt, seed=4), slopes=torch.linspace(0.01, 0.7, G, device=DEV))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("Sq,Sk,B", [(3, 9000, 1), (70, 100, 2), (200, 300, 70), (130, 8200, 8)])
+def test_attention_not_a_number_stays_in_its_row(Sq, Sk, B):
+    """A query that is not a number gives such a row - its keys split over blocks or not - and no other."""
+    q, k, v = (randn(B, s, 2, 64, dtype=torch.bfloat16, seed=i) for i, s in enumerate((Sq, Sk, Sk)))
+    want = T.attention(q, k, v)
+    q[0, 1, 1] = float("nan")
+    got = T.attention(q, k, v)
+    assert got[0, 1, 1].isnan().all()
+    got[0, 1, 1] = want[0, 1, 1]
+    assert torch.equal(got, want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", [torch.float32, torch.float16])
+@pytest.mark.parametrize("Sq,B", [(5, 2), (200, 2), (200, 70)])
+def test_rows_that_see_nothing_are_zero_beside_infinite_values(dt, Sq, B):
+    """The rows that do see the infinite value are not finite; infinity or not a number is left open: p may be multiplied as
+    hi + lo, and hi inf + lo inf with lo < 0 or lo = 0 is not a number."""
+    q, k, v = (randn(B, s, 2, 64, dtype=dt, seed=i) for i, s in enumerate((Sq, 300, 300)))
+    v[:, 7] = float("inf")
+    doc = torch.zeros(B, 300, dtype=torch.int64, device=DEV)
+    qd = doc[:, :Sq].clone()
+    qd[:, 2], qd[:, 3] = 5, -1
+    o = T.attention(q, k, v, q_doc=qd, k_doc=doc)
+    assert not o[:, 2:4].any() and not o[:, 4].isfinite().any()
+    lens = torch.full((B,), 300, dtype=torch.int32, device=DEV)
+    table = torch.arange(B * 3, dtype=torch.int32, device=DEV).view(B, 3)
+    ql = torch.full((B,), Sq - 2, dtype=torch.int32, device=DEV)
+    o = T.paged_attention(q, k.view(B * 3, 100, 2, 64), v.view(B * 3, 100, 2, 64), table, lens, q_lens=ql, causal=False)
+    assert not o[:, Sq - 2:].any() and not o[:, :Sq - 2].isfinite().any()
+
+
+@pytest.mark.gpu
+def test_attention_rules_at_the_ends_of_their_range():
+    """Prefixes below zero and past every key, 64-bit ones past 32 bits; document numbers at the top of 32 bits; padding
+    numbers below them."""
+    q, k, v = (randn(2, s, 2, 64, seed=i) for i, s in enumerate((40, 70, 70)))
+    do = randn(2, 40, 2, 64, seed=5)
+    ints = lambda *x: torch.tensor(x, device=DEV)
+    for got, same in ((ints(-2 ** 31, 2 ** 31 - 1).int(), ints(0, 70)), (ints(-2 ** 40, 2 ** 40), ints(0, 70)), (-7, 0), (10 ** 12, 70)):
+        leaves = [t.detach().requires_grad_(True) for t in (q, k, v)]
+        a, b = T.attention(*leaves, causal=True, prefix=got), T.attention(*leaves, causal=True, prefix=same)
+        assert torch.equal(a, b)
+        assert all(torch.equal(x, y) for x, y in zip(torch.autograd.grad(a, leaves, do), torch.autograd.grad(b, leaves, do)))
+    qd, kd = torch.zeros(2, 40, dtype=torch.int64, device=DEV), torch.zeros(2, 70, dtype=torch.int64, device=DEV)
+    qd[:, ::2], kd[:, ::3], kd[:, 1::3] = 2 ** 31 - 1, 2 ** 31 - 1, 2 ** 31 - 2
+    check_attention(q, k, v, do, q_doc=qd, k_doc=kd)
+    low = kd.clone()
+    low[:, 5:60], kd[:, 5:60] = -2 ** 40, -1
+    assert torch.equal(T.attention(q, k, v, q_doc=qd, k_doc=low), T.attention(q, k, v, q_doc=qd, k_doc=kd))
+
+
+@pytest.mark.gpu
+def test_one_forward_walked_backward_by_two_graphs():
+    """Two captured backward passes of one forward, replayed on two streams at once."""
+    side = torch.cuda.Stream()
+    leaves = [randn(2, 500, 4, 64, dtype=torch.bfloat16, seed=i).requires_grad_(True) for i in range(3)]
+    dos = [randn(2, 500, 4, 64, dtype=torch.bfloat16, seed=5 + i) for i in range(2)]
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        o = T.attention(*leaves, causal=True)
+        want = [torch.autograd.grad(o, leaves, do, retain_graph=True) for do in dos]
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for do in dos:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=side):
+            outs.append(torch.autograd.grad(o, leaves, do, retain_graph=True))
+        graphs.append(g)
+    streams = [torch.cuda.Stream() for _ in dos]
+    for _ in range(4):
+        for out in outs:
+            for t in out:
+                t.zero_()
+        torch.cuda.synchronize()
+        for s, g in zip(streams, graphs):
+            with torch.cuda.stream(s):
+                g.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(outs, want):
+            assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+@pytest.mark.gpu
+def test_rope_rows_past_32_bit_offsets():
+    """Tokens 5 GB apart, and a dense result of 5 GB."""
+    S, D, stride = 40001, 64, 65536
+    big = torch.empty(S * stride, dtype=torch.bfloat16, device=DEV)
+    x = big.as_strided((1, S, 2, D), (0, stride, D, 1))
+    x.copy_(randn(1, S, 2, D, dtype=torch.bfloat16, seed=1))
+    pos, w = _grid(S, 3), torch.linspace(0.5, 2, D, device=DEV)
+    assert torch.equal(T.axial_rope(x, pos, (16, 24, 24)), T.axial_rope(x.contiguous(), pos, (16, 24, 24)))
+    ends = [T.qk_norm_rope(t, t[:, :, :1], pos, w, w, (16, 24, 24)) for t in (x, x.contiguous())]
+    assert all(torch.equal(a, b) for a, b in zip(*ends))
+    del big, x
+    x = torch.empty(1, 300000, 64, 128, dtype=torch.bfloat16, device=DEV).normal_()
+    pos = _grid(300000, 3)
+    y = T.axial_rope(x, pos, (32, 48, 48))
+    for at in (0, 131071, 262140, 299990):
+        assert torch.equal(y[:, at:at + 10], T.axial_rope(x[:, at:at + 10], pos[at:at + 10], (32, 48, 48)))
+
+
+def test_refusals_of_scales_and_caps():
+    q = _cpu(1, 4, 2, 64)
+    for c in (1e-9, 1e31, float("inf")):
+        with pytest.raises(ValueError, match="softcap"):
+            T.attention(q, q, q, softcap=c)
+    for s in (1e31, float("nan")):
+        with pytest.raises(ValueError, match="scale"):
+            T.attention(q, q, q, scale=s)
+
+
 def test_workspace_sizes_from_python_are_the_library_s():
     """The cached sizes: what the C entry says for the same call, dense and paged."""
     L = T.lib()

@@ -32,6 +32,7 @@
 #include "../../include/turtle_token.h"
 
 #include <algorithm>
+#include <cmath>
 #include <type_traits>
 #include <utility>
 
@@ -507,6 +508,7 @@ bool fill(Args& a, const In* x, int dtype) {
   a.B = x->B; a.Sq = x->Sq; a.Sk = x->table ? 0 : x->Sk; a.Hq = x->Hq; a.Hk = x->Hk; a.G = x->Hq / x->Hk; a.D = x->D; a.M = x->Sq * a.G;
   a.scale = x->scale; a.scale2 = x->scale * LOG2E; a.cap = x->softcap;
   if (x->softcap > 0.f) { a.icap = x->scale / x->softcap; a.cap2 = x->softcap * LOG2E; }
+  if (!std::isfinite(a.scale2) || !(x->softcap >= 0.f) || !std::isfinite(a.icap) || !std::isfinite(a.cap2)) return false;
   a.slopes = x->slopes; a.prefix = x->prefix; a.qdoc = x->qdoc; a.kdoc = x->kdoc; a.causal = x->causal;
   a.nqr = (x->Sq + RT - 1) / RT; a.nkr = x->table ? 0 : (x->Sk + RT - 1) / RT;
   a.qr = (const int4*)x->ranges; a.kr = a.qr ? a.qr + (int64_t)x->B * a.nqr : nullptr;

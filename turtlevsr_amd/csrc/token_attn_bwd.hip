@@ -106,7 +106,7 @@ __global__ __launch_bounds__(NW * RG * 64, sizeof(T) == 2 && (DP == 64 || RG == 
   const int ik = SP ? item >> 1 : item, kt = ik % a.mtiles, bh = ik / a.mtiles, b = bh / a.Hk, hk = bh - b * a.Hk;
   const int k0 = kt * C::BK, k1 = min(k0 + C::BK, a.Sk), off = a.Sk - a.Sq;
   const int kw = k0 + (WK ? 0 : wave * 32), kw1 = min(kw + 32, a.Sk);
-  const int pre = a.prefix ? a.prefix[b] : 0;
+  const int pre = a.prefix ? max(a.prefix[b], 0) : 0;
   const int key = kw + (lane & 31), kdoc = (a.kdoc && key < a.Sk) ? a.kdoc[(int64_t)b * a.Sk + key] : 0;
   const bool kon = key < a.Sk && kdoc >= 0;
   uint4 kf[R::STEPS], vf[R::STEPS];
@@ -149,10 +149,10 @@ __global__ __launch_bounds__(NW * RG * 64, sizeof(T) == 2 && (DP == 64 || RG == 
   const float* deltas = a.delta + (int64_t)bh * a.M;
   char* ring = smem + (WK ? wave * NS * C::SLOT : 0);
   auto issue = [&](int t, char* dst) {
+    const int m = t * BM + ltid, i = token_of(a, m), g = m - i * a.G;
+    float s = 0.f;
+    if (a.slopes) s = a.G <= 64 ? __shfl(sl, g & 63, 64) : a.slopes[hk * a.G + g] * LOG2E;      // by all lanes: each gives one
     if (rules && ltid < BM) {
-      const int m = t * BM + ltid, i = token_of(a, m), g = m - i * a.G;
-      float s = 0.f;
-      if (a.slopes) s = a.G <= 64 ? __shfl(sl, g, 64) : a.slopes[hk * a.G + g] * LOG2E;
       int d = 0;
       if (dw.mixed) d = m < a.M ? a.qdoc[(int64_t)b * a.Sq + i] : -1;
       int* info = reinterpret_cast<int*>(dst + 2 * C::TILE) + 2 * BM + ltid;
@@ -181,10 +181,10 @@ __global__ __launch_bounds__(NW * RG * 64, sizeof(T) == 2 && (DP == 64 || RG == 
     }
     // every wave writes the same sums and deltas, so that all count the same number of loads
 #pragma unroll
-    for (int i = 0; i < BM / 32; ++i) {
-      const int e = i * 64 + lane, m = m0 + (e & (BM - 1)), which = e / BM;
-      const float* src = m < a.M ? (which ? deltas : sums) + m : g_row_pad + which;
-      dma4(src, __builtin_amdgcn_readfirstlane(lds_addr(dst + 2 * C::TILE) + i * 256));
+    for (int j = 0; j < BM / 32; ++j) {
+      const int e = j * 64 + lane, mr = m0 + (e & (BM - 1)), which = e / BM;
+      const float* src = mr < a.M ? (which ? deltas : sums) + mr : g_row_pad + which;
+      dma4(src, __builtin_amdgcn_readfirstlane(lds_addr(dst + 2 * C::TILE) + j * 256));
     }
   };
 
@@ -375,7 +375,7 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 ? 2 : 1) void attn_dq_kerne
   const int mt = a.mtiles - 1 - item % a.mtiles, bh = item / a.mtiles, b = bh / a.Hk, hk = bh - b * a.Hk;
   const int off = a.Sk - a.Sq, m0 = mt * C::BM, m1 = min(m0 + C::BM, a.M);
   const int mw = m0 + (WK ? 0 : wave * 32), mw1 = min(mw + 32, a.M);
-  const int pre = a.prefix ? a.prefix[b] : 0;
+  const int pre = a.prefix ? max(a.prefix[b], 0) : 0;
   int kend = a.Sk;
   if (a.causal) kend = min(a.Sk, max(token_of(a, m1 - 1) + off + 1, pre));
   const int t1 = (max(kend, 0) + BN - 1) / BN;

@@ -81,7 +81,7 @@ __global__ __launch_bounds__(NW * 64, DP == 128 && sizeof(T) == 4 ? 1 : 2) void 
     kn = max(0, (int)min((int64_t)kl, room));
   }
   const int m0 = mt * F::BM, mend = min(a.M, nq * a.G), m1 = min(m0 + F::BM, mend);   // rows of this block that exist: [m0, m1)
-  const int pre = (!PAGED && a.prefix) ? a.prefix[b] : 0;
+  const int pre = (!PAGED && a.prefix) ? max(a.prefix[b], 0) : 0;
   const int mw = m0 + (WK ? 0 : wave * 32), mw1 = min(mw + 32, mend);     // ... of this wave
   const int mrow = mw + (lane & 31);
   const Row row = row_of(a, b, hk, mrow, off, nq);
@@ -331,13 +331,14 @@ __global__ __launch_bounds__(NW * 64, DP == 128 && sizeof(T) == 4 ? 1 : 2) void 
   }
 
   if (mrow >= a.M) return;
-  const float inv = (l > 0.f && row.on) ? 1.f / l : 0.f;
-  const float lse = inv > 0.f ? mx + log2f(l) - POFF : INFINITY;
+  // a row that sees nothing: zeros, whatever the tile's values were; a sum that is not a number stays one
+  const bool none = l == 0.f || !row.on;
+  const float inv = none ? 0.f : 1.f / l, lse = none ? INFINITY : mx + log2f(l) - POFF;
   const bool first = (!WK || wave == 0) && h == 0;
   const int64_t pi = ((int64_t)sp * a.B * a.Hk + bh) * a.M + mrow;
   const int64_t oi = (((int64_t)b * a.Sq + qi) * a.Hq + hk * a.G + qg) * a.D;
   if (first && a.nsplit > 1) a.plse[pi] = lse;
-  if (first && a.nsplit <= 1 && a.lse) a.lse[(int64_t)bh * a.M + mrow] = lse;
+  if (first && a.nsplit <= 1 && a.lse) a.lse[(int64_t)bh * a.M + mrow] = l > 0.f ? lse : INFINITY;
 #pragma unroll
   for (int dt = 0; dt < DT; ++dt) {
     if (WK && dt % NW != wave) continue;
@@ -347,7 +348,7 @@ __global__ __launch_bounds__(NW * 64, DP == 128 && sizeof(T) == 4 ? 1 : 2) void 
       if (d >= a.D) continue;
       float v[4], lo[4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) { v[e] = acc[dt][4 * q4 + e] * inv; lo[e] = v[e] - to_f((T)v[e]); }
+      for (int e = 0; e < 4; ++e) { v[e] = none ? 0.f : acc[dt][4 * q4 + e] * inv; lo[e] = v[e] - to_f((T)v[e]); }
       if (a.nsplit > 1) {
         *reinterpret_cast<float4*>(a.part + pi * a.D + d) = make_float4(v[0], v[1], v[2], v[3]);
       } else {
@@ -399,7 +400,7 @@ __global__ __launch_bounds__(256) void attn_join_kernel(Args a) {
     v[0] = fmaf(w, none ? 0.f : p.x, v[0]); v[1] = fmaf(w, none ? 0.f : p.y, v[1]);
     v[2] = fmaf(w, none ? 0.f : p.z, v[2]); v[3] = fmaf(w, none ? 0.f : p.w, v[3]);
   }
-  const float inv = l > 0.f ? 1.f / l : 0.f;
+  const float inv = l == 0.f ? 0.f : 1.f / l;
   float lo[4];
 #pragma unroll
   for (int e = 0; e < 4; ++e) { v[e] *= inv; lo[e] = v[e] - to_f((T)v[e]); }
@@ -487,7 +488,7 @@ using namespace turtle;
 
 extern "C" {
 
-size_t turtle_token_attn_ranges(const turtle_token_attn_args* a) { return a ? ranges_bytes(a) : 0; }
+size_t turtle_token_attn_ranges(const turtle_token_attn_args* a) { return sizes_ok(a, 0) ? ranges_bytes(a) : 0; }
 size_t turtle_token_attn_workspace(const turtle_token_attn_args* a, int dtype) { return sizes_ok(a, dtype) ? ws_bytes(a, dtype) : 0; }
 
 int turtle_token_attn_fwd(const turtle_token_attn_args* x, int dtype, void* stream) {

@@ -110,13 +110,13 @@ def _same(a, b, name: str):
 
 
 def _ints(t, shape, name: str, like):
-    """An int32 tensor of ``shape`` on ``like``'s device from an integer tensor."""
+    """An int32 tensor of ``shape`` on ``like``'s device from an integer tensor (64-bit values are cut to the range)."""
     if not isinstance(t, torch.Tensor) or t.dtype not in (torch.int32, torch.int64):
         raise TypeError(f"{name}: expected an int32 or int64 tensor")
     if tuple(t.shape) != tuple(shape):
         raise ValueError(f"{name}: shape {tuple(t.shape)}, expected {tuple(shape)}")
     _same(like, t, name)
-    return t.to(torch.int32).contiguous()
+    return (t if t.dtype == torch.int32 else t.clamp(-2 ** 31, 2 ** 31 - 1).to(torch.int32)).contiguous()
 
 
 def _slopes(t, H: int, like):
@@ -134,15 +134,15 @@ def _slopes(t, H: int, like):
 
 def _cap(softcap) -> float:
     c = float(softcap)
-    if not 0.0 <= c < float("inf"):
-        raise ValueError(f"softcap = {softcap}, must be finite and not negative (0: none)")
+    if not (c == 0.0 or 1e-6 <= c <= 1e30):
+        raise ValueError(f"softcap = {softcap}, must be 0 (none) or of 1e-6 to 1e30")
     return c
 
 
 def _scale(scale, D: int) -> float:
     s = D ** -0.5 if scale is None else float(scale)
-    if not abs(s) < float("inf"):
-        raise ValueError(f"scale = {scale}, must be finite")
+    if not abs(s) <= 1e30:
+        raise ValueError(f"scale = {scale}, must be finite and at most 1e30")
     return s
 
 
@@ -283,18 +283,17 @@ class _QkNormRope(torch.autograd.Function):
         dq, dk = _dense(q), _dense(k)
         need = ctx.needs_input_grad
         nq, nk = need[2] and wq is not None, need[3] and wk is not None
-        buf, dw, ws, n = None, 0, 0, 0
-        if nq or nk:                              # the two gains' gradients, then the kernel's partial sums
+        dw, ws, n = None, None, 0
+        if nq or nk:
             n = _norm_workspace(B * S, D)
-            buf = torch.empty(2 * D + n // 4, dtype=torch.float32, device=q.device)
-            dw = buf.data_ptr()
-            ws = dw + 8 * D
+            dw = torch.empty(2 * D, dtype=torch.float32, device=q.device)
+            ws = torch.empty(n, dtype=torch.uint8, device=q.device)
         if B and S:
             _run(q, "token_norm_rope_bwd", lib().turtle_token_norm_rope_bwd, _side(q, dq, wq, dyq), _side(k, dk, wk, dyk), tab,
-                 pos.data_ptr(), pos_b, pos64, B, S, D, eps, dw, ws, n, _dt(q))
-        elif buf is not None:
-            buf.zero_()
-        return (dq, dk, buf[:D].to(ctx.w_dt[0]) if nq else None, buf[D:2 * D].to(ctx.w_dt[1]) if nk else None, None, None, None, None, None)
+                 pos.data_ptr(), pos_b, pos64, B, S, D, eps, _ptr(dw), _ptr(ws), n, _dt(q))
+        elif dw is not None:
+            dw.zero_()
+        return (dq, dk, dw[:D].to(ctx.w_dt[0]) if nq else None, dw[D:].to(ctx.w_dt[1]) if nk else None, None, None, None, None, None)
 
 
 @functools.lru_cache(maxsize=256)
@@ -349,7 +348,7 @@ def _attn_block(q, k, v, rules, masks, o, Sk, pages=(0, 0, 0), cache=(None, None
 
 def _attn_forward(q, k, v, rules, masks, grad):
     """(o, aux) of readable, non-empty q, k, v; aux (or None): what the backward needs besides - o's rounding remainder
-    (16-bit types), the rows' softmax sums, room for their deltas, the document ranges - in one buffer."""
+    (16-bit types), the rows' softmax sums, the document ranges - in one buffer."""
     o = _dense(q)
     n, Sk, dt = q.shape[0] * q.shape[1] * q.shape[2], k.shape[1], _dt(q)
     lo = lse = ranges = 0
@@ -357,12 +356,12 @@ def _attn_forward(q, k, v, rules, masks, grad):
     docs = masks[2] is not None
     if grad or docs:
         nr = lib().turtle_token_attn_ranges(_attn_block(q, k, v, rules, masks, o, Sk)) if docs else 0
-        parts = _aux_parts(n, q.shape[3], dt, nr) if grad else (0, 0, 0, 0, nr)
-        aux = torch.empty(parts[4], dtype=torch.uint8, device=q.device)
+        parts = _aux_parts(n, q.shape[3], dt, nr) if grad else (0, 0, nr)
+        aux = torch.empty(parts[2], dtype=torch.uint8, device=q.device)
         p = aux.data_ptr()
-        ranges = p + parts[3] if docs else 0
+        ranges = p + parts[1] if docs else 0
         if grad:
-            lo, lse = (p if dt else 0), p + parts[1]
+            lo, lse = (p if dt else 0), p + parts[0]
     ws, nws = _attn_workspace(q.shape, k.shape[2], Sk, (0, 0, 0), dt, q.device)
     blk = _attn_block(q, k, v, rules, masks, o, Sk, lo=lo, lse=lse, ranges=ranges, ws=_ptr(ws), ws_bytes=nws)
     _run(q, "token_attn_fwd", lib().turtle_token_attn_fwd, blk, dt)
@@ -370,11 +369,10 @@ def _attn_forward(q, k, v, rules, masks, grad):
 
 
 def _aux_parts(n: int, D: int, dt: int, nr: int):
-    """Byte offsets of (remainder, sums, deltas, ranges, end) for n rows."""
+    """Byte offsets of (sums, ranges, end) for n rows, behind the remainder."""
     a = 2 * n * D if dt else 0
-    b = a + 4 * n
-    c = (b + 4 * n + 15) // 16 * 16
-    return 0, a, b, c, c + nr
+    b = (a + 4 * n + 15) // 16 * 16
+    return a, b, b + nr
 
 
 @functools.lru_cache(maxsize=256)
@@ -421,11 +419,12 @@ class _Attention(torch.autograd.Function):
         need = ctx.needs_input_grad
         do = _tokens(do)
         n, dt, p = q.shape[0] * q.shape[1] * q.shape[2], _dt(q), aux.data_ptr()
-        _, lse, delta, ranges, _ = _aux_parts(n, q.shape[3], dt, 0)
+        lse, ranges, _ = _aux_parts(n, q.shape[3], dt, 0)
+        delta = torch.empty(n, dtype=torch.float32, device=q.device)      # this run's own: a graph may be walked twice at once
         dq = _dense(q) if need[0] else None
         dk, dv = (_dense(k), _dense(v)) if need[1] or need[2] else (None, None)
         blk = _attn_block(q, k, v, ctx.rules, masks, o, k.shape[1], lo=p if dt else 0, lse=p + lse, ranges=p + ranges if masks[2] is not None else 0)
-        blk += _GRADS.pack(do.data_ptr(), *_strides(do), _ptr(dq), _ptr(dk), _ptr(dv), p + delta)
+        blk += _GRADS.pack(do.data_ptr(), *_strides(do), _ptr(dq), _ptr(dk), _ptr(dv), delta.data_ptr())
         _run(q, "token_attn_bwd", lib().turtle_token_attn_bwd, blk, dt)
         return (dq, dk if need[1] else None, dv if need[2] else None) + (None,) * 5
 
@@ -454,11 +453,12 @@ def attention(q, k, v, *, scale=None, softcap: float = 0.0, slopes=None, causal:
     * slopes (fp32 [Hq]): z -= slopes[head] * |distance of the places|;
     * causal: a query sees the keys up to its own place, and the first ``prefix`` keys (int, or [B] integers) of its
       sequence in any case;
-    * q_doc [B, Sq], k_doc [B, Sk] (k_doc None: q_doc, with Sq == Sk): integers; a query sees only keys of its own
-      document. Negative: padding, which sees nothing and is seen by nobody - its rows may hold anything.
+    * q_doc [B, Sq], k_doc [B, Sk] (k_doc None: q_doc, with Sq == Sk): integers below 2^31; a query sees only keys
+      of its own document. Negative: padding, which sees nothing and is seen by nobody - its rows may hold anything.
 
-    A query that sees nothing gives zeros and passes no gradient. A value that is not finite in a key or value
-    that ANY query may see can reach every query of its tile. Returns a dense [B, Sq, Hq, D] of q's type."""
+    A query that sees nothing gives zeros and passes no gradient. A query, key or value that is not finite makes the
+    results that depend on it infinite or not a number; in a key or value that ANY query may see it can reach every
+    query of its tile. Returns a dense [B, Sq, Hq, D] of q's type."""
     _check_qkv(q, k, v)
     B, Sq, Hq, D = q.shape
     Sk = k.shape[1]
@@ -467,7 +467,7 @@ def attention(q, k, v, *, scale=None, softcap: float = 0.0, slopes=None, causal:
     if prefix is not None:
         if not causal:
             raise ValueError("prefix: only with causal (without, every key is visible)")
-        prefix = torch.full((B,), prefix, dtype=torch.int32, device=q.device) if isinstance(prefix, int) else _ints(prefix, (B,), "prefix", q)
+        prefix = torch.full((B,), max(0, min(prefix, 2 ** 31 - 1)), dtype=torch.int32, device=q.device) if isinstance(prefix, int) else _ints(prefix, (B,), "prefix", q)
     if q_doc is None and k_doc is not None:
         raise ValueError("k_doc without q_doc")
     if q_doc is not None:
