@@ -114,6 +114,12 @@ TURTLE_DEV void dma16(const void* gp, uint32_t lds_wave_base) {
   asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off\n\ts_mov_b32 m0, %0"
                : "=&s"(keep) : "v"(gp), "s"(lds_wave_base) : "memory");
 }
+// 64 lanes x 4 B -> LDS
+TURTLE_DEV void dma4(const void* gp, uint32_t lds_wave_base) {
+  unsigned keep;
+  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %1, off\n\ts_mov_b32 m0, %0"
+               : "=&s"(keep) : "v"(gp), "s"(lds_wave_base) : "memory");
+}
 // at most N vector-memory operations of this wave still in flight
 template <int N>
 TURTLE_DEV void vm_wait() {
@@ -134,6 +140,33 @@ template <int N, typename F, int... I>
 TURTLE_DEV void static_for_(F f, std::integer_sequence<int, I...>) { (f(std::integral_constant<int, I>{}), ...); }
 template <int N, typename F>
 TURTLE_DEV void static_for(F f) { static_for_<N>(f, std::make_integer_sequence<int, N>{}); }
+
+// Values loaded before a loop are waited for here: left to their first use inside it, the wait would stand in the loop and
+// drain the copies in flight at every turn
+TURTLE_DEV void arrived(uint4& x) { asm volatile("" : "+v"(x.x), "+v"(x.y), "+v"(x.z), "+v"(x.w)); }
+TURTLE_DEV void arrived(float& x) { asm volatile("" : "+v"(x)); }
+TURTLE_DEV void arrived(int& x) { asm volatile("" : "+v"(x)); }
+template <typename X, int N>
+TURTLE_DEV void arrived(X (&x)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) arrived(x[i]);
+}
+
+// N steps of an LDS read and a product: read n + AHEAD is started before product n, by the order that an empty statement
+// with memory effects keeps. Left alone the compiler reads an operand right before its product and waits the read out
+// each time (a wave alone on its SIMD has nothing else to do then).
+template <int N, int AHEAD, typename Read, typename Use>
+TURTLE_DEV void in_steps(Read read, Use use) {
+  typedef decltype(read(std::integral_constant<int, 0>{})) V;
+  V v[AHEAD + 1];
+  static_for<(AHEAD < N ? AHEAD : N)>([&](auto n) { v[n()] = read(n); });
+  static_for<N>([&](auto n) {
+    if constexpr (n() + AHEAD < N) v[(n() + AHEAD) % (AHEAD + 1)] = read(std::integral_constant<int, n() + AHEAD>{});
+    u32x4 x = __builtin_bit_cast(u32x4, v[n() % (AHEAD + 1)]);
+    asm volatile("" : "+v"(x) : : "memory");
+    use(n, __builtin_bit_cast(V, x));
+  });
+}
 
 // A tile of rows of DP channels (zero past D) in LDS
 template <typename T, int DP>
@@ -166,9 +199,8 @@ struct Rows {
     const uint32_t base = row_base(t, lane);
 #pragma unroll
     for (int j = 0; j < KT; ++j) acc[j] = zero16();
-    static_for<STEPS>([&](auto s) {
-      static_for<KT>([&](auto j) { acc[j()] = mma<T>(chunk<s(), j()>(base), frag[s()], acc[j()]); });
-    });
+    in_steps<KT * STEPS, 3>([&](auto n) { return chunk<n() / KT, n() % KT>(base); },
+                                 [&](auto n, uint4 x) { acc[n() % KT] = mma<T>(x, frag[n() / KT], acc[n() % KT]); });
   }
   // the same of two tiles with an operand each; a1 comes with its initial values
   template <int KT>
@@ -177,29 +209,26 @@ struct Rows {
     const uint32_t b0 = row_base(t0, lane), b1 = row_base(t1, lane);
 #pragma unroll
     for (int j = 0; j < KT; ++j) a0[j] = zero16();
-    static_for<STEPS>([&](auto s) {
-      static_for<KT>([&](auto j) {
-        a0[j()] = mma<T>(chunk<s(), j()>(b0), f0[s()], a0[j()]);
-        a1[j()] = mma<T>(chunk<s(), j()>(b1), f1[s()], a1[j()]);
-      });
-    });
+    in_steps<2 * KT * STEPS, 2>([&](auto n) { return chunk<n() / (2 * KT), n() / 2 % KT>(n() & 1 ? b1 : b0); },
+                                     [&](auto n, uint4 x) {
+                                       f32x16& a = n() & 1 ? a1[n() / 2 % KT] : a0[n() / 2 % KT];
+                                       a = mma<T>(x, n() & 1 ? f1[n() / (2 * KT)] : f0[n() / (2 * KT)], a);
+                                     });
   }
-  // ... the second operand read from LDS, from its 32 rows at l1
-  template <int KT>
-  TURTLE_DEV static void times2_lds(const char* t0, const char* t1, const uint4 (&f0)[STEPS], const char* l1, f32x16 (&a0)[KT],
-                                    f32x16 (&a1)[KT], int lane) {
+  // ... one row group; the second operand read from LDS, from its 32 rows at l1
+  TURTLE_DEV static void times2_lds(const char* t0, const char* t1, const uint4 (&f0)[STEPS], const char* l1, f32x16& a0, f32x16& a1,
+                                    int lane) {
     const uint32_t b0 = row_base(t0, lane), b1 = row_base(t1, lane);
     uint32_t bl = row_base(l1, lane);
     asm volatile("" : "+v"(bl));      // one address, not a register for each of its chunks
-#pragma unroll
-    for (int j = 0; j < KT; ++j) a0[j] = zero16();
-    static_for<STEPS>([&](auto s) {
-      const uint4 g = chunk<s(), 0>(bl);
-      static_for<KT>([&](auto j) {
-        a0[j()] = mma<T>(chunk<s(), j()>(b0), f0[s()], a0[j()]);
-        a1[j()] = mma<T>(chunk<s(), j()>(b1), g, a1[j()]);
-      });
-    });
+    a0 = zero16();
+    uint4 g;
+    in_steps<3 * STEPS, 3>([&](auto n) { return chunk<n() / 3, 0>(n() % 3 == 0 ? b0 : n() % 3 == 1 ? bl : b1); },
+                           [&](auto n, uint4 x) {
+                             if constexpr (n() % 3 == 0) a0 = mma<T>(x, f0[n() / 3], a0);
+                             else if constexpr (n() % 3 == 1) g = x;
+                             else a1 = mma<T>(x, g, a1);
+                           });
   }
   // acc[dt] += (rows 16 U .. 16 U + 15)^T (channels 32 dt ..) x p: 16-bit types, p packed from 8 accumulator registers'
   // values of those rows. LO: a second term of p besides
@@ -226,14 +255,36 @@ struct Rows {
       });
     });
   }
-  // one operand, rounded (16-bit) or as it is (fp32): 8 values from register 8 (U & 1) on of the tile p[U >> 1]
-  template <int U, int KT>
-  TURTLE_DEV static void t_times1(const char* t, const f32x16 (&p)[KT], f32x16 (&acc)[DT], int lane) {
+  // V^T operand of rows 16 U .. 16 U + 15, channels 32 dt .. (16-bit types)
+  template <int U, int I> TURTLE_DEV static uint4 tr_frag(uint32_t base) {
+    const uint32_t a = base ^ (I << 6);
+    const uint2 x = lds_ld_tr(a + U * 16 * ROWB), y = lds_ld_tr((a ^ 32) + (U * 16 + 8) * ROWB);
+    return make_uint4(x.x, x.y, y.x, y.y);
+  }
+  // acc += (the tile's 32 KT rows)^T x p, p rounded (16-bit) or as it is (fp32)
+  template <int KT>
+  TURTLE_DEV static void t_times_all(const char* t, const f32x16 (&p)[KT], f32x16 (&acc)[DT], int lane) {
+    if constexpr (ES == 2) {
+      uint4 hi[2 * KT];
+#pragma unroll
+      for (int u = 0; u < 2 * KT; ++u) hi[u] = pack_of(p[u >> 1], 8 * (u & 1));
+      const uint32_t base = tr_base(t, lane);
+      in_steps<2 * KT * DT, 2>([&](auto n) { return tr_frag<n() / DT, n() % DT>(base); },
+                               [&](auto n, uint4 v) { acc[n() % DT] = mma<T>(v, hi[n() / DT], acc[n() % DT]); });
+    } else {
+      static_for<2 * KT>([&](auto u) {
+        float x[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = p[u() >> 1][8 * (u() & 1) + e];
+        t_times<u()>(t, x, acc, lane);
+      });
+    }
+  }
+  TURTLE_DEV static uint4 pack_of(const f32x16& p, int at) {
     float x[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = p[U >> 1][8 * (U & 1) + e];
-    if constexpr (ES == 2) t_times<U, false>(t, pack(x), make_uint4(0, 0, 0, 0), acc, lane);
-    else t_times<U>(t, x, acc, lane);
+    for (int e = 0; e < 8; ++e) x[e] = p[at + e];
+    return pack(x);
   }
   // sum of the 8 packed values, added to l
   TURTLE_DEV static float sum_packed(uint4 p, float l) {
@@ -343,12 +394,18 @@ struct Args {
 };
 
 // work item of a block. Blocks are dealt to the 8 XCDs in turn, each with an L2 of its own: with enough key heads, runs
-// of consecutive items go to one XCD, so that the tiles of a key head share its L2; with few, items are dealt as they
-// come - a run would be a piece of one sequence, and pieces cost unequally (causal, documents)
+// of consecutive items go to one XCD (runs = 1), so that the tiles of a key head share its L2; with few, items are dealt as
+// they come (0) - a run would be a piece of one sequence, and pieces cost unequally (causal, documents). Causal items
+// of a few rounds of blocks go out longest first over all of an XCD's key heads (2): 5120 tokens, prefix 2048, 16
+// heads of 64 channels, dk and dv 210 us for 228, dq 122 for 132, forward 117 for 123.
 TURTLE_DEV int xcd_item(const Args& a) {
   if (!a.runs) return (int)blockIdx.x;
-  const int chunk = (a.total + 7) >> 3;
-  return (int)(blockIdx.x & 7) * chunk + (int)(blockIdx.x >> 3);
+  const int x = (int)(blockIdx.x & 7), j = (int)(blockIdx.x >> 3);
+  if (a.runs == 2) {
+    const int heads = a.B * a.Hk >> 3, n = a.total / (a.B * a.Hk);
+    return (x * heads + j % heads) * n + j / heads;
+  }
+  return x * ((a.total + 7) >> 3) + j;
 }
 
 TURTLE_DEV int quot(int n, int d, uint32_t mul, uint32_t sh) { return d == 1 ? n : (int)(__umulhi((uint32_t)n, mul) >> sh); }
@@ -421,16 +478,26 @@ TURTLE_DEV int4 doc_range(const int4* ranges, int nr, int t0, int t1) {
 
 // A walk over tiles of UNIT tokens that may hold a document of [lo, hi]: 64 tiles are looked up at a time, a lane each.
 // Of the tile it stops at: mixed = not every pair of it with a pure tile of document `pure` (-1: none) is visible;
-// holes = it has tokens without a document.
+// holes = it has tokens without a document; mine = it may hold one of this wave's own documents (own_docs): a block over
+// the border of documents walks over all of theirs (forward, 8192 tokens in 7 of 1170, 16 heads on 4, 128 channels: 196 us
+// with the waves keeping to their own, 208 without; dk and dv 468 and 464, so there they do not).
 struct DocWalk {
   const int4* ranges;     // of this sequence; null: every tile, all visible
-  int nr, lo, hi, pure;
-  uint64_t act, mix, hole;
+  int nr, lo, hi, pure, wlo, whi;
+  uint64_t act, mix, hole, own;
   int base;
-  bool mixed, holes;
-  TURTLE_DEV void init(const int4* r, int n, int4 mine) {
-    ranges = r; nr = n; lo = mine.x; hi = mine.y; pure = mine.z ? mine.x : -1;
-    base = -1; act = mix = hole = 0; mixed = holes = false;
+  bool mixed, holes, mine;
+  TURTLE_DEV void none() { ranges = nullptr; nr = 0; lo = hi = pure = wlo = whi = 0; base = -1; act = mix = hole = own = 0; mixed = holes = false; mine = true; }
+  // block: the range of the block's tokens
+  TURTLE_DEV void init(const int4* r, int n, int4 block) {
+    none();
+    ranges = r; nr = n; lo = wlo = block.x; hi = whi = block.y; pure = block.z ? block.x : -1;
+  }
+  // doc: the document of this lane's token, or negative
+  TURTLE_DEV void own_docs(int doc) {
+    wlo = doc < 0 ? 0x7fffffff : doc; whi = doc;
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) { wlo = min(wlo, __shfl_xor(wlo, o, 64)); whi = max(whi, __shfl_xor(whi, o, 64)); }
   }
   // the first tile >= t (in steps of STRIDE), or `end`; G rows share a token, there are ntok tokens
   template <int UNIT, int STRIDE>
@@ -445,6 +512,7 @@ struct DocWalk {
         act = __ballot(x.x <= hi && x.y >= lo);
         mix = __ballot(!(x.z && x.x == pure));
         hole = __ballot(x.w != 0);
+        own = __ballot(x.x <= whi && x.y >= wlo);
       }
       const int at = (t - base) / STRIDE;
       const uint64_t left = act >> at;
@@ -452,6 +520,7 @@ struct DocWalk {
         const int k = at + __builtin_ctzll(left);
         mixed = (mix >> k) & 1;
         holes = (hole >> k) & 1;
+        mine = (own >> k) & 1;
         return base + k * STRIDE;
       }
       t = base + 64 * STRIDE;
@@ -459,6 +528,17 @@ struct DocWalk {
     return end;
   }
 };
+
+__device__ const int g_no_doc = -1;
+
+// documents of a tile's N keys -> 256 bytes of LDS, by every wave before the tile's own copy: a register load would be
+// waited for in order, behind the tiles in flight. (Waits count the tile's own operations, so with this one more in
+// flight they wait for it too: never for less.)
+template <int N>
+TURTLE_DEV void key_docs(const Args& a, int b, int k0, char* dst, int lane) {
+  const int key = k0 + (lane & (N - 1));
+  dma4(key < a.Sk ? a.kdoc + (int64_t)b * a.Sk + key : &g_no_doc, __builtin_amdgcn_readfirstlane(lds_addr(dst)));
+}
 
 // -------------------------------------------------------------------------------------------------
 // host
@@ -525,6 +605,7 @@ int launch(K kernel, int64_t total, int threads, int lds, Args& a, hipStream_t s
   const int bh = a.B * a.Hk;
   a.total = (int)total;
   a.runs = bh % 8 == 0 || bh >= 64;
+  if (a.causal && bh % 8 == 0 && total <= 8 * 256) a.runs = 2;
   if (lds > 64 * 1024) {
     const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
     if (e != hipSuccess) return (int)e;

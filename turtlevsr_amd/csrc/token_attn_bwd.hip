@@ -7,13 +7,6 @@ namespace {
 
 __device__ const float g_row_pad[2] = {INFINITY, 0.f};   // softmax sum and delta of a row that is not there
 
-// 64 lanes x 4 B -> LDS
-TURTLE_DEV void dma4(const void* gp, uint32_t lds_wave_base) {
-  unsigned keep;
-  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %1, off\n\ts_mov_b32 m0, %0"
-               : "=&s"(keep) : "v"(gp), "s"(lds_wave_base) : "memory");
-}
-
 // -delta [B][Hk][M], delta = do . (o + o_lo); 8 lanes a row, 16 bytes a lane and step
 template <typename T>
 __global__ __launch_bounds__(256) void attn_delta_kernel(Args a, float* delta) {
@@ -55,7 +48,7 @@ template <typename T, int DP, int NW, int RG, bool WK> struct Dkv {
   static constexpr int BM = WM * RG;                      // rows of a tile
   static constexpr int NS = (WK || DP == 128) ? 2 : 3;
   static constexpr int TILE = BM * R::ROWB;
-  static constexpr int SLOT = (2 * TILE + 5 * BM * 4 + 511) / 512 * 512;      // Q, dO; softmax sum, delta, place, document, slope of a row
+  static constexpr int SLOT = (2 * TILE + 4 * BM * 4 + 256 + 511) / 512 * 512;      // Q, dO; softmax sum, delta, place, slope, document of a row
   static constexpr int RING = NS * SLOT * (WK ? NW : 1), JOIN = R::DT * 16 * 64 * 4 * (RG > 1 ? NW : 1);
   static constexpr int LDS = (RING > JOIN ? RING : JOIN) + (VL ? BK * R::ROWB : 0);
   static constexpr int NLD = R::template loads2<BM, LT>() + BM / 32;
@@ -107,11 +100,13 @@ __global__ __launch_bounds__(NW * RG * 64, sizeof(T) == 2 && (DP == 64 || RG == 
   const int k0 = kt * C::BK, k1 = min(k0 + C::BK, a.Sk), off = a.Sk - a.Sq;
   const int kw = k0 + (WK ? 0 : wave * 32), kw1 = min(kw + 32, a.Sk);
   const int pre = a.prefix ? max(a.prefix[b], 0) : 0;
-  const int key = kw + (lane & 31), kdoc = (a.kdoc && key < a.Sk) ? a.kdoc[(int64_t)b * a.Sk + key] : 0;
+  const int key = kw + (lane & 31);
+  int kdoc = (a.kdoc && key < a.Sk) ? a.kdoc[(int64_t)b * a.Sk + key] : 0;
   const bool kon = key < a.Sk && kdoc >= 0;
   uint4 kf[R::STEPS], vf[R::STEPS];
   R::frag(kon ? reinterpret_cast<const T*>(a.k) + (int64_t)b * a.kb + (int64_t)key * a.ks + (int64_t)hk * a.kh : nullptr, a.D, kf, lane);
   R::frag(kon ? reinterpret_cast<const T*>(a.v) + (int64_t)b * a.vb + (int64_t)key * a.vs + (int64_t)hk * a.vh : nullptr, a.D, vf, lane);
+  arrived(kdoc);
   char* vlds = smem + C::LDS - C::BK * R::ROWB + wave * 32 * R::ROWB;
   if constexpr (C::VL) {
     // V's chunks at the places `chunk` reads them from; every row group writes the same
@@ -125,9 +120,10 @@ __global__ __launch_bounds__(NW * RG * 64, sizeof(T) == 2 && (DP == 64 || RG == 
   if (a.causal && k0 >= pre) mfirst = max(0, k0 - off) * a.G;
   const int t1 = (a.M + BM - 1) / BM, t0 = min(t1, mfirst / BM);
   DocWalk dw;
-  dw.init(nullptr, 0, make_int4(0, 0, 0, 0));
+  dw.none();
   if (a.qdoc) dw.init(a.qr + (int64_t)b * a.nqr, a.nqr, doc_range(a.kr + (int64_t)b * a.nkr, a.nkr, k0, k1));
-  const float sl = (a.slopes && lane < a.G) ? a.slopes[hk * a.G + lane] * LOG2E : 0.f;
+  float sl = (a.slopes && lane < a.G) ? a.slopes[hk * a.G + lane] * LOG2E : 0.f;
+  arrived(sl);
   const bool rules = a.causal || a.slopes || a.qdoc;
 
   const char* qbase = reinterpret_cast<const char*>(a.q) + ((int64_t)b * a.qb + (int64_t)hk * a.G * a.qh) * R::ES;
@@ -148,17 +144,18 @@ __global__ __launch_bounds__(NW * RG * 64, sizeof(T) == 2 && (DP == 64 || RG == 
   const float* sums = a.lse + (int64_t)bh * a.M;
   const float* deltas = a.delta + (int64_t)bh * a.M;
   char* ring = smem + (WK ? wave * NS * C::SLOT : 0);
-  auto issue = [&](int t, char* dst) {
+  auto issue = [&](int t, char* dst) __attribute__((always_inline)) {
+    if (dw.mixed) {
+      const int m = t * BM + (lane & (BM - 1));
+      dma4(m < a.M ? a.qdoc + (int64_t)b * a.Sq + token_of(a, m) : &g_no_doc, __builtin_amdgcn_readfirstlane(lds_addr(dst + 2 * C::TILE + 16 * BM)));
+    }
     const int m = t * BM + ltid, i = token_of(a, m), g = m - i * a.G;
     float s = 0.f;
     if (a.slopes) s = a.G <= 64 ? __shfl(sl, g & 63, 64) : a.slopes[hk * a.G + g] * LOG2E;      // by all lanes: each gives one
     if (rules && ltid < BM) {
-      int d = 0;
-      if (dw.mixed) d = m < a.M ? a.qdoc[(int64_t)b * a.Sq + i] : -1;
       int* info = reinterpret_cast<int*>(dst + 2 * C::TILE) + 2 * BM + ltid;
       info[0] = i + off;
-      info[BM] = d;
-      info[2 * BM] = __float_as_int(s);
+      info[BM] = __float_as_int(s);
     }
     const int m0 = t * BM;
     if (plain && !dw.holes && m0 + BM <= a.M && (!a.causal || t * per + off >= 0 || pre > 0)) {
@@ -196,26 +193,29 @@ __global__ __launch_bounds__(NW * RG * 64, sizeof(T) == 2 && (DP == 64 || RG == 
 
   // the walk over row tiles: as the forward's over key tiles
   struct Tile { int t; bool mixed; } q[NS - 1];
-  int tnew = WK ? t0 + wave : t0, fill = NS - 1, fly = 0, into = 0, slot = 0;
-  for (;;) {
-    const bool live = fill == 0;
-    if (live) {
-      if (q[0].t >= t1) break;
-      if constexpr (!WK) {
-        vm_wait_tiles<C::NLD, NS - 2>(fly - 1);
-        lds_barrier();
-      }
-    }
+  int tnew = WK ? t0 + wave : t0, fly = 0, into = 0, slot = 0;
+  auto start = [&]() __attribute__((always_inline)) {
     Tile x{dw.template next<BM, STEP>(tnew, t1, a.G, a.Sq, lane), false};
     x.mixed = dw.mixed;
     if (x.t < t1) { issue(x.t, ring + into * C::SLOT); ++fly; }
     tnew = x.t + STEP;
     into = into + 1 == NS ? 0 : into + 1;
-    const Tile cur = q[0];
 #pragma unroll
     for (int i = 0; i + 2 < NS; ++i) q[i] = q[i + 1];
     q[NS - 2] = x;
-    if (!live) { --fill; continue; }
+  };
+#pragma unroll 1
+  for (int i = 0; i < NS - 1; ++i) start();
+  arrived(kf);
+  if constexpr (!C::VL) arrived(vf);
+  for (;;) {
+    const Tile cur = q[0];
+    if (cur.t >= t1) break;
+    if constexpr (!WK) {
+      vm_wait_tiles<C::NLD, NS - 2>(fly - 1);
+      lds_barrier();
+    }
+    start();
     if constexpr (WK) vm_wait_tiles<C::NLD, NS - 1>(fly - 1);
     const char* qt = ring + slot * C::SLOT + rg * C::WM * R::ROWB;      // this wave's rows of the tile
     const char* gt = qt + C::TILE;
@@ -235,7 +235,7 @@ __global__ __launch_bounds__(NW * RG * 64, sizeof(T) == 2 && (DP == 64 || RG == 
           const float4 del = *reinterpret_cast<const float4*>(in + BM + j * 32 + 8 * c);
           dp[j][4 * c] = del.x; dp[j][4 * c + 1] = del.y; dp[j][4 * c + 2] = del.z; dp[j][4 * c + 3] = del.w;
         }
-      if constexpr (C::VL) R::template times2_lds<MT>(qt, gt, kf, vlds, s, dp, lane);
+      if constexpr (C::VL) R::times2_lds(qt, gt, kf, vlds, s[0], dp[0], lane);
       else if (do_k) R::template times2<MT>(qt, gt, kf, vf, s, dp, lane);
       else R::template times<MT>(qt, kf, s, lane);
       const bool caus = a.causal && p0 + 1 < kw1 && kw1 > pre;
@@ -254,7 +254,7 @@ __global__ __launch_bounds__(NW * RG * 64, sizeof(T) == 2 && (DP == 64 || RG == 
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
             const int4 pos = *reinterpret_cast<const int4*>(info + j * 32 + 8 * c);
-            const float4 slp = *reinterpret_cast<const float4*>(info + 2 * BM + j * 32 + 8 * c);
+            const float4 slp = *reinterpret_cast<const float4*>(info + BM + j * 32 + 8 * c);
             const int po[4] = {pos.x, pos.y, pos.z, pos.w};
             const float sp[4] = {slp.x, slp.y, slp.z, slp.w};
 #pragma unroll
@@ -262,24 +262,34 @@ __global__ __launch_bounds__(NW * RG * 64, sizeof(T) == 2 && (DP == 64 || RG == 
           }
         mul = 1.f;
       }
+      // the pairs that do not see each other: p = 0, whatever dP holds there (a pass for each rule, free of branches)
       if (caus || mixed) {
-        // the pairs that do not see each other: p = 0, whatever dP holds there
+#pragma unroll
+        for (int j = 0; j < MT; ++j)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) s[j][r] *= mul;
+        mul = 1.f;
+      }
+      auto hide = [&](const int* at, auto sees) {
 #pragma unroll
         for (int j = 0; j < MT; ++j)
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
-            const int4 pos = *reinterpret_cast<const int4*>(info + j * 32 + 8 * c), doc = *reinterpret_cast<const int4*>(info + BM + j * 32 + 8 * c);
-            const int po[4] = {pos.x, pos.y, pos.z, pos.w}, dc[4] = {doc.x, doc.y, doc.z, doc.w};
+            const int4 x = *reinterpret_cast<const int4*>(at + j * 32 + 8 * c);
+            const int y[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              const int r = 4 * c + e;
-              const bool vis = (!caus || max(po[e], pre - 1) >= key) && (!mixed || dc[e] == kdoc);
-              s[j][r] = vis ? s[j][r] * mul : -INFINITY;
-              dp[j][r] = vis ? dp[j][r] : 0.f;
+              const bool vis = sees(y[e]);
+              s[j][4 * c + e] = vis ? s[j][4 * c + e] : -INFINITY;
+              dp[j][4 * c + e] = vis ? dp[j][4 * c + e] : 0.f;
             }
           }
-        mul = 1.f;
+      };
+      if (caus) {
+        const int from = key < pre ? -0x7fffffff - 1 : key;      // the first place that sees the key
+        hide(info, [&](int place) { return place >= from; });
       }
+      if (mixed) hide(info + 2 * BM, [&](int doc) { return doc == kdoc; });
 #pragma unroll
       for (int j = 0; j < MT; ++j)
 #pragma unroll
@@ -294,10 +304,8 @@ __global__ __launch_bounds__(NW * RG * 64, sizeof(T) == 2 && (DP == 64 || RG == 
             if constexpr (PUP != 1.f) s[j][r] *= PUP;
           }
         }
-      static_for<2 * MT>([&](auto u) {
-        if (do_v) R::template t_times1<u()>(gt, s, dv, lane);
-        if (do_k) R::template t_times1<u()>(qt, dp, dk, lane);
-      });
+      if (do_v) R::template t_times_all<MT>(gt, s, dv, lane);
+      if (do_k) R::template t_times_all<MT>(qt, dp, dk, lane);
     }
     if constexpr (WK) asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     --fly;
@@ -357,7 +365,7 @@ template <typename T, int DP, int NW, bool WK> struct Dq {
   static constexpr int BM = WK ? 32 : NW * 32;            // rows of a block
   static constexpr int KT = (sizeof(T) == 2 && DP == 64) ? 2 : 1, BN = 32 * KT;      // keys of a tile
   static constexpr int NS = WK ? 2 : 3;
-  static constexpr int TILE = BN * R::ROWB, SLOT = 2 * TILE;
+  static constexpr int TILE = BN * R::ROWB, SLOT = 2 * TILE + 512;      // K, V; document of a key
   static constexpr int RING = NS * SLOT * (WK ? NW : 1), JOIN = R::DT * 16 * 64 * 4;
   static constexpr int LDS = RING > JOIN ? RING : JOIN;
   static constexpr int NLD = R::template loads2<BN, LT>();
@@ -379,24 +387,21 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 ? 2 : 1) void attn_dq_kerne
   int kend = a.Sk;
   if (a.causal) kend = min(a.Sk, max(token_of(a, m1 - 1) + off + 1, pre));
   const int t1 = (max(kend, 0) + BN - 1) / BN;
-  DocWalk dw;
-  dw.init(nullptr, 0, make_int4(0, 0, 0, 0));
-  if (a.qdoc)
-    dw.init(a.kr + (int64_t)b * a.nkr, a.nkr, doc_range(a.qr + (int64_t)b * a.nqr, a.nqr, token_of(a, m0), token_of(a, m1 - 1) + 1));
   // what this wave's rows see whole: keys before `whole`; and at all: keys before `some`
   const int whole = a.causal ? max(token_of(a, mw) + off + 1, pre) : 0x7fffffff;
   const int some = mw1 <= mw ? 0 : (a.causal ? max(token_of(a, mw1 - 1) + off + 1, pre) : 0x7fffffff);
 
   const int mrow = mw + (lane & 31);
-  const Row row = row_of(a, b, hk, mrow, off, a.Sq);
+  Row row = row_of(a, b, hk, mrow, off, a.Sq);
+  DocWalk dw;
+  dw.none();
+  if (a.qdoc)
+    dw.init(a.kr + (int64_t)b * a.nkr, a.nkr, doc_range(a.qr + (int64_t)b * a.nqr, a.nqr, token_of(a, m0), token_of(a, m1 - 1) + 1));
   const int i = token_of(a, mrow), g = mrow - i * a.G, hq = hk * a.G + g;
   uint4 qf[R::STEPS], gf[R::STEPS];
   R::frag(row.on ? reinterpret_cast<const T*>(a.q) + (int64_t)b * a.qb + (int64_t)i * a.qs + (int64_t)hq * a.qh : nullptr, a.D, qf, lane);
   R::frag(row.on ? reinterpret_cast<const T*>(a.dout) + (int64_t)b * a.gb + (int64_t)i * a.gs + (int64_t)hq * a.gh : nullptr, a.D, gf, lane);
-  const float lse = row.on ? a.lse[(int64_t)bh * a.M + mrow] : INFINITY, delta = row.on ? a.delta[(int64_t)bh * a.M + mrow] : 0.f;
-  f32x16 ndelta;      // dP starts from -delta (stored negated)
-#pragma unroll
-  for (int r = 0; r < 16; ++r) ndelta[r] = delta;
+  float lse = row.on ? a.lse[(int64_t)bh * a.M + mrow] : INFINITY, delta = row.on ? a.delta[(int64_t)bh * a.M + mrow] : 0.f;
 
   const char* kbase = reinterpret_cast<const char*>(a.k) + ((int64_t)b * a.kb + (int64_t)hk * a.kh) * R::ES;
   const char* vbase = reinterpret_cast<const char*>(a.v) + ((int64_t)b * a.vb + (int64_t)hk * a.vh) * R::ES;
@@ -406,8 +411,9 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 ? 2 : 1) void attn_dq_kerne
   klin.init(ltid, kst);
   vlin.init(ltid, vst);
   char* ring = smem + (WK ? wave * NS * C::SLOT : 0);
-  auto issue = [&](int t, char* dst) {
+  auto issue = [&](int t, char* dst) __attribute__((always_inline)) {
     const int k0 = t * BN;
+    if (dw.mixed) key_docs<BN>(a, b, k0, dst + 2 * C::TILE, lane);
     if (!dw.holes && k0 + BN <= a.Sk && a.D == DP) {
       klin.template load<BN>(dst, ltid, kbase + k0 * kst, kst);
       vlin.template load<BN>(dst + C::TILE, ltid, vbase + k0 * vst, vst);
@@ -426,26 +432,36 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 ? 2 : 1) void attn_dq_kerne
   for (int j = 0; j < DT; ++j) dq[j] = zero16();
 
   struct Tile { int t; bool mixed; } q[NS - 1];
-  int tnew = WK ? wave : 0, fill = NS - 1, fly = 0, into = 0, slot = 0;
-  for (;;) {
-    const bool live = fill == 0;
-    if (live) {
-      if (q[0].t >= t1) break;
-      if constexpr (!WK) {
-        vm_wait_tiles<C::NLD, NS - 2>(fly - 1);
-        lds_barrier();
-      }
-    }
+  int tnew = WK ? wave : 0, fly = 0, into = 0, slot = 0;
+  auto start = [&]() __attribute__((always_inline)) {
     Tile x{dw.template next<BN, STEP>(tnew, t1, 1, a.Sk, lane), false};
     x.mixed = dw.mixed;
     if (x.t < t1) { issue(x.t, ring + into * C::SLOT); ++fly; }
     tnew = x.t + STEP;
     into = into + 1 == NS ? 0 : into + 1;
-    const Tile cur = q[0];
 #pragma unroll
     for (int j = 0; j + 2 < NS; ++j) q[j] = q[j + 1];
     q[NS - 2] = x;
-    if (!live) { --fill; continue; }
+  };
+#pragma unroll 1
+  for (int j = 0; j < NS - 1; ++j) start();
+  arrived(qf);
+  arrived(gf);
+  arrived(lse);
+  arrived(delta);
+  arrived(row.doc);
+  arrived(row.slope2);
+  f32x16 ndelta;      // dP starts from -delta (stored negated)
+#pragma unroll
+  for (int r = 0; r < 16; ++r) ndelta[r] = delta;
+  for (;;) {
+    const Tile cur = q[0];
+    if (cur.t >= t1) break;
+    if constexpr (!WK) {
+      vm_wait_tiles<C::NLD, NS - 2>(fly - 1);
+      lds_barrier();
+    }
+    start();
     if constexpr (WK) vm_wait_tiles<C::NLD, NS - 1>(fly - 1);
     const char* kt = ring + slot * C::SLOT;
     const char* vt = kt + C::TILE;
@@ -477,15 +493,21 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 ? 2 : 1) void attn_dq_kerne
       if (k0 + BN > whole || mixed || k0 + BN > a.Sk) {
         // the last key in sight; the pairs that do not see each other: p = 0, whatever dP holds there
         const int last = min(a.causal ? max(row.pos, pre - 1) : a.Sk, a.Sk - 1) - k0 - 4 * h;
-        const int key = k0 + (lane & (BN - 1)), kd = mixed && key < a.Sk ? a.kdoc[(int64_t)b * a.Sk + key] : -1;
+        const int* kd = reinterpret_cast<const int*>(kt + 2 * C::TILE) + 4 * h;
 #pragma unroll
         for (int j = 0; j < KT; ++j)
 #pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            bool vis = j * 32 + acc_row(r) <= last;
-            if (mixed) { const int d = __shfl(kd, j * 32 + acc_row(r) + 4 * h, 64); vis = vis && d == row.doc; }   // every lane gives its number
-            s[j][r] = vis ? s[j][r] * mul : -INFINITY;
-            dp[j][r] = vis ? dp[j][r] : 0.f;
+          for (int c = 0; c < 4; ++c) {
+            int4 doc = make_int4(row.doc, row.doc, row.doc, row.doc);
+            if (mixed) doc = *reinterpret_cast<const int4*>(kd + j * 32 + 8 * c);
+            const int dc[4] = {doc.x, doc.y, doc.z, doc.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int r = 4 * c + e;
+              const bool vis = j * 32 + acc_row(r) <= last && dc[e] == row.doc;
+              s[j][r] = vis ? s[j][r] * mul : -INFINITY;
+              dp[j][r] = vis ? dp[j][r] : 0.f;
+            }
           }
         mul = 1.f;
       }
@@ -493,7 +515,7 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 ? 2 : 1) void attn_dq_kerne
       for (int j = 0; j < KT; ++j)
 #pragma unroll
         for (int r = 0; r < 16; ++r) dp[j][r] *= __builtin_amdgcn_exp2f(fmaf(s[j][r], mul, -lse));
-      static_for<2 * KT>([&](auto u) { R::template t_times1<u()>(kt, dp, dq, lane); });
+      R::template t_times_all<KT>(kt, dp, dq, lane);
     }
     if constexpr (WK) asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     --fly;

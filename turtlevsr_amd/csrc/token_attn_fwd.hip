@@ -18,7 +18,7 @@ template <typename T, int DP, int NW, bool WK> struct Fwd {
   static constexpr int BM = WK ? 32 : NW * 32;        // rows of a block, 32 a wave
   static constexpr int BN = (WK || sizeof(T) == 4) ? 32 : 64;
   static constexpr int NS = 2;                        // slots of the ring
-  static constexpr int TILE = BN * R::ROWB, SLOT = 2 * TILE;
+  static constexpr int TILE = BN * R::ROWB, SLOT = 2 * TILE + 512;      // K, V; document of a key
   static constexpr int LT = WK ? 64 : NT;             // threads that load a tile
   static constexpr int NLD = R::template loads2<BN, LT>();
   static constexpr int WIN = 256;                     // page numbers a wave keeps at hand
@@ -84,7 +84,7 @@ __global__ __launch_bounds__(NW * 64, DP == 128 && sizeof(T) == 4 ? 1 : 2) void 
   const int pre = (!PAGED && a.prefix) ? max(a.prefix[b], 0) : 0;
   const int mw = m0 + (WK ? 0 : wave * 32), mw1 = min(mw + 32, mend);     // ... of this wave
   const int mrow = mw + (lane & 31);
-  const Row row = row_of(a, b, hk, mrow, off, nq);
+  Row row = row_of(a, b, hk, mrow, off, nq);
 
   // key tiles this block walks over
   int kend = kn;
@@ -97,9 +97,11 @@ __global__ __launch_bounds__(NW * 64, DP == 128 && sizeof(T) == 4 ? 1 : 2) void 
     t1 = min(t1, t0 + per);
   }
   DocWalk dw;
-  dw.init(nullptr, 0, make_int4(0, 0, 0, 0));
-  if (!PAGED && a.qdoc && m1 > m0)
+  dw.none();
+  if (!PAGED && a.qdoc && m1 > m0) {
     dw.init(a.kr + (int64_t)b * a.nkr, a.nkr, doc_range(a.qr + (int64_t)b * a.nqr, a.nqr, m0 / a.G, (m1 - 1) / a.G + 1));
+    dw.own_docs(row.on ? row.doc : -1);
+  }
   // what this wave's rows see whole: keys before `whole`; and at all: keys before `some`
   const int whole = a.causal ? max(mw / a.G + off + 1, pre) : 0x7fffffff;
   const int some = mw1 <= mw ? 0 : (a.causal ? max((mw1 - 1) / a.G + off + 1, pre) : 0x7fffffff);
@@ -123,7 +125,7 @@ __global__ __launch_bounds__(NW * 64, DP == 128 && sizeof(T) == 4 ? 1 : 2) void 
   int wbase = 0, wend = 0;
   auto page_of = [&](int key) { return quot(key, a.page, a.pmul, a.psh); };
   // starts tile t's copy into dst; returns which of its keys are seen at all (bit = key within the tile)
-  auto issue = [&](int t, char* dst) -> uint64_t {
+  auto issue = [&](int t, char* dst) __attribute__((always_inline)) -> uint64_t {
     const int k0 = t * BN;
     if constexpr (PAGED) {
       const int p0 = page_of(k0), p1 = page_of(min(k0 + BN, kn) - 1);
@@ -160,6 +162,7 @@ __global__ __launch_bounds__(NW * 64, DP == 128 && sizeof(T) == 4 ? 1 : 2) void 
       return __ballot(ok);
     } else {
       const bool holes = dw.holes;
+      if (dw.mixed) key_docs<BN>(a, b, k0, dst + 2 * F::TILE, lane);
       if (!holes && k0 + BN <= kn && a.D == DP) {
         klin.template load<BN>(dst, ltid, kbase + k0 * kst, kst);
         vlin.template load<BN>(dst + F::TILE, ltid, vbase + k0 * vst, vst);
@@ -183,27 +186,32 @@ __global__ __launch_bounds__(NW * 64, DP == 128 && sizeof(T) == 4 ? 1 : 2) void 
   // The walk: tiles are started NS - 1 turns before they are computed on (q: the tiles in flight, oldest first). With a
   // block the turn's barrier frees the slot of the tile before; a wave of its own starts the next tile at once.
   constexpr int NS = F::NS;
-  struct Tile { int t; bool mixed; uint64_t seen; } q[NS - 1];
-  int tnew = WK ? t0 + wave : t0, fill = NS - 1, fly = 0, into = 0, slot = 0;
-  for (;;) {
-    const bool live = fill == 0;
-    if (live) {
-      if (q[0].t >= t1) break;
-      if constexpr (!WK) {
-        vm_wait_tiles<F::NLD, NS - 2>(fly - 1);
-        lds_barrier();
-      }
-    }
-    Tile x{dw.template next<BN, STEP>(tnew, t1, 1, a.Sk, lane), false, ~0ull};
+  struct Tile { int t; bool mixed, mine; uint64_t seen; } q[NS - 1];
+  int tnew = WK ? t0 + wave : t0, fly = 0, into = 0, slot = 0;
+  auto start = [&]() __attribute__((always_inline)) {
+    Tile x{dw.template next<BN, STEP>(tnew, t1, 1, a.Sk, lane), false, true, ~0ull};
     x.mixed = dw.mixed;
+    x.mine = dw.mine;
     if (x.t < t1) { x.seen = issue(x.t, buf + into * F::SLOT); ++fly; }
     tnew = x.t + STEP;
     into = into + 1 == NS ? 0 : into + 1;
-    const Tile cur = q[0];
 #pragma unroll
     for (int i = 0; i + 2 < NS; ++i) q[i] = q[i + 1];
     q[NS - 2] = x;
-    if (!live) { --fill; continue; }
+  };
+#pragma unroll 1
+  for (int i = 0; i < NS - 1; ++i) start();
+  arrived(qf);
+  arrived(row.doc);
+  arrived(row.slope2);
+  for (;;) {
+    const Tile cur = q[0];
+    if (cur.t >= t1) break;
+    if constexpr (!WK) {
+      vm_wait_tiles<F::NLD, NS - 2>(fly - 1);
+      lds_barrier();
+    }
+    start();
     if constexpr (WK) vm_wait_tiles<F::NLD, NS - 1>(fly - 1);
     const char* kt = buf + slot * F::SLOT;
     const char* vt = kt + F::TILE;
@@ -211,7 +219,7 @@ __global__ __launch_bounds__(NW * 64, DP == 128 && sizeof(T) == 4 ? 1 : 2) void 
     const bool mixed = cur.mixed;
     uint64_t seen = cur.seen;
 
-    if (k0 < some) {
+    if (k0 < some && cur.mine) {
       f32x16 s[KT];
       R::template times<KT>(kt, qf, s, lane);
       // the rules that apply to this tile, each in a pass of its own (uniform branches)
@@ -250,14 +258,15 @@ __global__ __launch_bounds__(NW * 64, DP == 128 && sizeof(T) == 4 ? 1 : 2) void 
         }
       }
       if (mixed) {
-        const int key = k0 + (lane & (BN - 1));
-        const int kd = key < kn ? a.kdoc[(int64_t)b * a.Sk + key] : -1;
+        const int* kd = reinterpret_cast<const int*>(kt + 2 * F::TILE) + 4 * h;
 #pragma unroll
         for (int j = 0; j < KT; ++j)
 #pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            const int d = __shfl(kd, j * 32 + acc_row(r) + 4 * h, 64);
-            s[j][r] = d == row.doc ? s[j][r] : -INFINITY;
+          for (int c = 0; c < 4; ++c) {
+            const int4 doc = *reinterpret_cast<const int4*>(kd + j * 32 + 8 * c);
+            const int dc[4] = {doc.x, doc.y, doc.z, doc.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[j][4 * c + e] = dc[e] == row.doc ? s[j][4 * c + e] : -INFINITY;
           }
       }
 
