@@ -1,4 +1,5 @@
-/* libturtle_hip token-attention kernels (turtlevsr_amd/csrc/token.hip, token_attn.hip), bound by
+/* libturtle_hip token-attention kernels (turtlevsr_amd/csrc/token.hip, token_attn_fwd.hip,
+ * token_attn_bwd.hip), bound by
  * turtlevsr_amd/token_ops.py.
  *
  * Tokens are rows of heads: element (b, s, h, d) of a tensor at base[b * sb + s * ss + h * sh + d], strides in
@@ -52,7 +53,7 @@ int turtle_token_norm_rope_bwd(const turtle_token_side* a, const turtle_token_si
                                void* ws, size_t ws_bytes, int dtype, void* stream);
 
 /* Attention. Query i of sequence b stands at i + Sk - Sq, key j at j. z = scale q.k; softcap > 0:
- * z = softcap tanh(z / softcap); slopes [Hq] or NULL: z -= slope |distance|. Visible pairs: causal = 0, or key place
+ * z = softcap tanh(z / softcap) (scale, softcap, scale / softcap and both times log2 e finite in fp32); slopes [Hq] or NULL: z -= slope |distance|. Visible pairs: causal = 0, or key place
  * <= query place, or key place < prefix[b] (prefix NULL: 0); and, with documents (qdoc [B][Sq], kdoc [B][Sk]), equal
  * numbers >= 0. Query head h reads key head h / (Hq / Hk). A query that sees nothing gives zeros and no gradient.
  * Paged (table != NULL): key j of sequence b is row j % page of page table[b][j / page] of the pools k / v

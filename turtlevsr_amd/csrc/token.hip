@@ -10,6 +10,9 @@
 // thread keeps ONE token and channel chunk and walks over the heads of q and k: the angles (4 pairs a lane) are
 // computed once for all of them.
 //
+// Measured: 32640 tokens, 8 + 8 heads of 64 channels, bf16: 34 us (3.9 TB/s; a large copy reaches 4.9); 40960 tokens,
+// forward 42 us, backward with both gains' gradients 57 + 4 us (4.4 TB/s).
+//
 // Angles: f_i is a 64-bit fixed-point number of revolutions per position, so pos * f_i wraps exactly and
 // position 10^6 is as precise as position 0 (fp32 products would be off by 0.06 rad there).
 #include "common.h"

@@ -1,5 +1,14 @@
 // Token attention, backward (token_attn.h holds the method and the shared parts): delta, then dk and dv by key tiles,
 // then dq by row tiles. No atomics: every sum has a fixed order.
+//
+// Two kernels compute S and dP twice (14 products of a tile pair for 10) and in exchange neither dk, dv nor dq is ever
+// summed through memory. A wave's step is a chain - S and dP, the rules, the exponential, two products with the results -
+// so with two waves on a SIMD what counts is the chain's waits: LDS reads started ahead of their products (dq at 128
+// channels 400 -> 365 us, dk and dv at 64 channels 212 -> 188), masks without branches (packed documents 850 -> 690).
+// Measured, bf16: 2 x 5120 tokens causal with prefix 2048, 8 heads of 64 channels: dk, dv 181 us (4 products a pair, 690
+// TF/s), dq 119 us (3 products, 785 TF/s), delta 8 us; 7 documents in 8192 tokens, 16 heads on 4 of 128 channels: dk, dv
+// 639 us, dq 361 us, delta 16 us - there the block over the border of the longest documents is the call's time, 2.5 times
+// the mean block's.
 #include "token_attn.h"
 
 namespace turtle {
