@@ -82,7 +82,8 @@ size_t turtle_token_attn_ranges(const turtle_token_attn_args* a);
 size_t turtle_token_attn_workspace(const turtle_token_attn_args* a, int dtype);
 int turtle_token_attn_fwd(const turtle_token_attn_args* a, int dtype, void* stream);
 
-/* backward (not paged): q, k, v, o, o_lo, lse, ranges as the forward left them; dout strided (gb, gs, gh); dq, dk, dv
+/* backward (not paged): q, k, v, o, o_lo, lse, ranges as the forward left them, ws scratch of
+ * turtle_token_attn_bwd_workspace(&f, dtype) bytes (qdoc set where documents are used); dout strided (gb, gs, gh); dq, dk, dv
  * dense, dq or (dk and dv) NULL when not wanted; delta: scratch, B * Sq * Hq floats. Fixed summation order. */
 typedef struct {
   turtle_token_attn_args f;
@@ -91,6 +92,7 @@ typedef struct {
   void *dq, *dk, *dv;
   float* delta;
 } turtle_token_attn_grads;
+size_t turtle_token_attn_bwd_workspace(const turtle_token_attn_args* a, int dtype);
 int turtle_token_attn_bwd(const turtle_token_attn_grads* g, int dtype, void* stream);
 
 #ifdef __cplusplus

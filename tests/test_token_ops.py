@@ -146,7 +146,7 @@ def check_attention(q, k, v, do=None, **kw):
 def test_token_exports_match_header():
     hdr = open(os.path.join(REPO, "include", "turtle_token.h")).read()
     declared = set(re.findall(r"\b(turtle_token_[a-z0-9_]+)\s*\(", hdr))
-    assert len(declared) == 8
+    assert len(declared) == 9
     L = _lib.lib()
     for s in declared:
         assert hasattr(L, s), s
@@ -903,6 +903,31 @@ def test_attention_middle_shapes(dt, D, Sq, Sk, B):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("B,Hk,Sq,Sk", [(4, 4, 260, 260), (8, 2, 700, 700), (48, 2, 300, 300), (8, 1, 100, 900), (2, 4, 3, 4000)])
+def test_attention_causal_key_heads_in_eights(dt, D, B, Hk, Sq, Sk):
+    """Key heads a multiple of eight, few blocks each: the order in which causal blocks go out."""
+    q, k, v = randn(B, Sq, 2 * Hk, D, dtype=dt, seed=1), randn(B, Sk, Hk, D, dtype=dt, seed=2), randn(B, Sk, Hk, D, dtype=dt, seed=3)
+    check_attention(q, k, v, randn(B, Sq, 2 * Hk, D, dtype=dt, seed=4), causal=True)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("D", [64, 104])
+@pytest.mark.parametrize("Sq,Sk", [(3000, 40), (2500, 1), (6, 2000), (900, 900)])
+def test_attention_gradients_of_long_walks(dt, D, Sq, Sk):
+    """Few keys under many queries and the reverse, one pair of heads: the walks split over blocks and added up."""
+    q, k, v = (randn(1, s, h, D, dtype=dt, seed=i) for i, (s, h) in enumerate(((Sq, 2), (Sk, 1), (Sk, 1))))
+    do = randn(1, Sq, 2, D, dtype=dt, seed=9)
+    check_attention(q, k, v, do, softcap=2.0, slopes=torch.tensor([0.3, 0.0], device=DEV))
+    check_attention(q, k, v, do, causal=True, prefix=torch.tensor([Sk // 2], device=DEV))
+    g = torch.Generator().manual_seed(Sq)
+    docs = [(torch.arange(s) * 5 // s - (torch.rand(s, generator=g) < 0.1).int() * 9)[None].to(DEV) for s in (Sq, Sk)]
+    check_attention(q, k, v, do, q_doc=docs[0], k_doc=docs[1])
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16])
 def test_attention_many_heads_share_a_key(dt):
     """80 query heads on one key head: more rows of one query than a tile has, 27 of them: a share that divides nothing."""
@@ -1060,6 +1085,24 @@ def test_refusals_of_scales_and_caps():
     for s in (1e31, float("nan")):
         with pytest.raises(ValueError, match="scale"):
             T.attention(q, q, q, scale=s)
+
+
+def test_backward_workspace_sizes_and_their_check():
+    """The cached sizes are the C entry's, and a call without the scratch is refused before anything runs."""
+    L, some = T.lib(), 0
+    for B, Sq, Sk, Hq, Hk, D in ((1, 3, 9000, 8, 2, 64), (1, 8192, 64, 2, 1, 128), (8, 2048, 2048, 8, 8, 64), (1, 8192, 8192, 16, 4, 128)):
+        for docs in (False, True):
+            q, k = torch.zeros(B, Sq, Hq, D, dtype=torch.bfloat16), torch.zeros(B, Sk, Hk, D, dtype=torch.bfloat16)
+            m = torch.zeros(B * max(Sq, Sk), dtype=torch.int32)
+            room = torch.zeros(64, dtype=torch.float32)
+            blk = T._attn_block(q, k, k, (1.0, 0.0, 0), (None, None, m, m) if docs else (None,) * 4, q, Sk, lse=room.data_ptr(), ranges=m.data_ptr())
+            n = T._bwd_workspace_bytes(q.shape, Hk, Sk, docs, 1)
+            assert n == L.turtle_token_attn_bwd_workspace(blk, 1)
+            some += n > 0
+            if n:
+                blk += T._GRADS.pack(q.data_ptr(), *T._strides(q), q.data_ptr(), k.data_ptr(), k.data_ptr(), room.data_ptr())
+                assert L.turtle_token_attn_bwd(blk, 1, None) == -1
+    assert some > 3
 
 
 def test_workspace_sizes_from_python_are_the_library_s():

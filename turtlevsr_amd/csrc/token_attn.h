@@ -506,14 +506,14 @@ struct DocWalk {
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) { wlo = min(wlo, __shfl_xor(wlo, o, 64)); whi = max(whi, __shfl_xor(whi, o, 64)); }
   }
-  // the first tile >= t (in steps of STRIDE), or `end`; G rows share a token, there are ntok tokens
-  template <int UNIT, int STRIDE>
-  TURTLE_DEV int next(int t, int end, int G, int ntok, int lane) {
+  // the first tile >= t (in steps of `stride`), or `end`; G rows share a token, there are ntok tokens
+  template <int UNIT>
+  TURTLE_DEV int next(int t, int end, int stride, int G, int ntok, int lane) {
     if (!ranges) return min(t, end);
     while (t < end) {
-      if (base < 0 || t >= base + 64 * STRIDE) {
+      if (base < 0 || t >= base + 64 * stride) {
         base = t;
-        const int tt = t + lane * STRIDE;
+        const int tt = t + lane * stride;
         int4 x = make_int4(0x7fffffff, -1, 0, 0);
         if (tt < end) x = doc_range(ranges, nr, tt * UNIT / G, min((tt * UNIT + UNIT - 1) / G + 1, ntok));
         act = __ballot(x.x <= hi && x.y >= lo);
@@ -521,16 +521,16 @@ struct DocWalk {
         hole = __ballot(x.w != 0);
         own = __ballot(x.x <= whi && x.y >= wlo);
       }
-      const int at = (t - base) / STRIDE;
+      const int at = (t - base) / stride;
       const uint64_t left = act >> at;
       if (left) {
         const int k = at + __builtin_ctzll(left);
         mixed = (mix >> k) & 1;
         holes = (hole >> k) & 1;
         mine = (own >> k) & 1;
-        return base + k * STRIDE;
+        return base + k * stride;
       }
-      t = base + 64 * STRIDE;
+      t = base + 64 * stride;
     }
     return end;
   }

@@ -92,7 +92,7 @@ TURTLE_DEV auto& pick(f32x16 (&x)[N], f32x16 (&y)[M]) {
   else return y;
 }
 
-template <typename T, int DP, int NW, int RG, bool WK>
+template <typename T, int DP, int NW, int RG, bool WK, bool SPLIT>
 __global__ __launch_bounds__(NW * RG * 64, sizeof(T) == 2 && (DP == 64 || RG == 2) ? 2 : 1) void attn_dkv_kernel(Args a) {
   typedef Dkv<T, DP, NW, RG, WK> C;
   typedef Rows<T, DP> R;
@@ -105,7 +105,8 @@ __global__ __launch_bounds__(NW * RG * 64, sizeof(T) == 2 && (DP == 64 || RG == 
   if (item >= a.total) return;
   constexpr bool SP = C::SP;
   const bool do_k = !SP || !(item & 1), do_v = !SP || (item & 1);
-  const int ik = SP ? item >> 1 : item, kt = ik % a.mtiles, bh = ik / a.mtiles, b = bh / a.Hk, hk = bh - b * a.Hk;
+  const int nsplit = SPLIT ? a.nsplit : 1, ik = SP ? item >> 1 : item, is = ik / nsplit, sp = ik - is * nsplit, step = STEP * nsplit;
+  const int kt = is % a.mtiles, bh = is / a.mtiles, b = bh / a.Hk, hk = bh - b * a.Hk;
   const int k0 = kt * C::BK, k1 = min(k0 + C::BK, a.Sk), off = a.Sk - a.Sq;
   const int kw = k0 + (WK ? 0 : wave * 32), kw1 = min(kw + 32, a.Sk);
   const int pre = a.prefix ? max(a.prefix[b], 0) : 0;
@@ -202,12 +203,12 @@ __global__ __launch_bounds__(NW * RG * 64, sizeof(T) == 2 && (DP == 64 || RG == 
 
   // the walk over row tiles: as the forward's over key tiles
   struct Tile { int t; bool mixed; } q[NS - 1];
-  int tnew = WK ? t0 + wave : t0, fly = 0, into = 0, slot = 0;
+  int tnew = t0 + sp * STEP + (WK ? wave : 0), fly = 0, into = 0, slot = 0;
   auto start = [&]() __attribute__((always_inline)) {
-    Tile x{dw.template next<BM, STEP>(tnew, t1, a.G, a.Sq, lane), false};
+    Tile x{dw.template next<BM>(tnew, t1, step, a.G, a.Sq, lane), false};
     x.mixed = dw.mixed;
     if (x.t < t1) { issue(x.t, ring + into * C::SLOT); ++fly; }
-    tnew = x.t + STEP;
+    tnew = x.t + step;
     into = into + 1 == NS ? 0 : into + 1;
 #pragma unroll
     for (int i = 0; i + 2 < NS; ++i) q[i] = q[i + 1];
@@ -362,8 +363,14 @@ __global__ __launch_bounds__(NW * RG * 64, sizeof(T) == 2 && (DP == 64 || RG == 
         x[e] = kon ? dk[dt][4 * q4 + e] * a.scale : 0.f;
         y[e] = kon ? dv[dt][4 * q4 + e] * (1.f / PUP) : 0.f;
       }
-      if (do_k) R::put4(reinterpret_cast<T*>(a.dk) + oi + d, x);
-      if (do_v) R::put4(reinterpret_cast<T*>(a.dv) + oi + d, y);
+      if constexpr (SPLIT) {
+        float* part = a.part + (int64_t)sp * 2 * a.B * a.Sk * a.Hk * a.D + oi + d;
+        if (do_k) *reinterpret_cast<float4*>(part) = make_float4(x[0], x[1], x[2], x[3]);
+        if (do_v) *reinterpret_cast<float4*>(part + (int64_t)a.B * a.Sk * a.Hk * a.D) = make_float4(y[0], y[1], y[2], y[3]);
+      } else {
+        if (do_k) R::put4(reinterpret_cast<T*>(a.dk) + oi + d, x);
+        if (do_v) R::put4(reinterpret_cast<T*>(a.dv) + oi + d, y);
+      }
     }
   }
 }
@@ -380,7 +387,7 @@ template <typename T, int DP, int NW, bool WK> struct Dq {
   static constexpr int NLD = R::template loads2<BN, LT>();
 };
 
-template <typename T, int DP, int NW, bool WK>
+template <typename T, int DP, int NW, bool WK, bool SPLIT>
 __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 ? 2 : 1) void attn_dq_kernel(Args a) {
   typedef Dq<T, DP, NW, WK> C;
   typedef Rows<T, DP> R;
@@ -389,7 +396,8 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 ? 2 : 1) void attn_dq_kerne
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
   const int item = xcd_item(a);
   if (item >= a.total) return;
-  const int mt = a.mtiles - 1 - item % a.mtiles, bh = item / a.mtiles, b = bh / a.Hk, hk = bh - b * a.Hk;
+  const int nsplit = SPLIT ? a.nsplit : 1, is = item / nsplit, sp = item - is * nsplit, step = STEP * nsplit;
+  const int mt = a.mtiles - 1 - is % a.mtiles, bh = is / a.mtiles, b = bh / a.Hk, hk = bh - b * a.Hk;
   const int off = a.Sk - a.Sq, m0 = mt * C::BM, m1 = min(m0 + C::BM, a.M);
   const int mw = m0 + (WK ? 0 : wave * 32), mw1 = min(mw + 32, a.M);
   const int pre = a.prefix ? max(a.prefix[b], 0) : 0;
@@ -441,12 +449,12 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 ? 2 : 1) void attn_dq_kerne
   for (int j = 0; j < DT; ++j) dq[j] = zero16();
 
   struct Tile { int t; bool mixed; } q[NS - 1];
-  int tnew = WK ? wave : 0, fly = 0, into = 0, slot = 0;
+  int tnew = sp * STEP + (WK ? wave : 0), fly = 0, into = 0, slot = 0;
   auto start = [&]() __attribute__((always_inline)) {
-    Tile x{dw.template next<BN, STEP>(tnew, t1, 1, a.Sk, lane), false};
+    Tile x{dw.template next<BN>(tnew, t1, step, 1, a.Sk, lane), false};
     x.mixed = dw.mixed;
     if (x.t < t1) { issue(x.t, ring + into * C::SLOT); ++fly; }
-    tnew = x.t + STEP;
+    tnew = x.t + step;
     into = into + 1 == NS ? 0 : into + 1;
 #pragma unroll
     for (int j = 0; j + 2 < NS; ++j) q[j] = q[j + 1];
@@ -543,47 +551,95 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 ? 2 : 1) void attn_dq_kerne
       float x[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) x[e] = row.on ? dq[dt][4 * q4 + e] * a.scale : 0.f;
-      R::put4(reinterpret_cast<T*>(a.dq) + oi + d, x);
+      if constexpr (SPLIT) *reinterpret_cast<float4*>(a.part + (int64_t)sp * a.B * a.Sq * a.Hq * a.D + oi + d) = make_float4(x[0], x[1], x[2], x[3]);
+      else R::put4(reinterpret_cast<T*>(a.dq) + oi + d, x);
     }
   }
 }
+
+// the splits' sums -> o0 (first half of a split's values) and o1, 4 of n values a thread
+template <typename T>
+__global__ __launch_bounds__(256) void attn_sum_kernel(const float* __restrict__ part, T* o0, T* o1, int64_t n, int nsplit) {
+  const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4, all = o1 ? 2 * n : n;
+  if (i >= all) return;
+  float v[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (int s = 0; s < nsplit; ++s) {
+    const float4 x = *reinterpret_cast<const float4*>(part + s * all + i);
+    v[0] += x.x; v[1] += x.y; v[2] += x.z; v[3] += x.w;
+  }
+  Rows<T, 64>::put4(i < n ? o0 + i : o1 + (i - n), v);
+}
+
+// The shape of a backward kernel. few: a block's waves own 32 keys (rows) together (WK) instead of 32 each: four times the
+// blocks. Measured at 1024 tokens and 8, 16, 24 and 32 heads (64 .. 256 blocks of 128), us with / without:
+//   dk, dv  bf16, 64 channels 21 / 40, 24 / 40, 39 / 42, 43 / 43; 128 channels 46 / 48, 91 / 51, 132 / 53, 176 / 56
+//           fp32, 64 channels 58 / 181, 112 / 184, 165 / 187, 222 / 190; 128 channels 268 / 258 (32 blocks 135 / 255), 536 / 265
+//   dq      bf16, 64 channels 11 / 22, 20 / 22, 28 / 23, 37 / 24; 128 channels 18 / 40, 36 / 41, 52 / 42, 69 / 44
+//           fp32, 64 channels 40 / 128, 77 / 131, 115 / 135, 156 / 137; 128 channels 129 / 242, 261 / 247
+// split: blocks take every split-th tile of the walk, 2 at least for each wave, and a second kernel adds up their fp32
+// sums: where the blocks are fewer than the CUs (bf16 of 128 channels, 3 rows on 9000 keys, 2 heads, dq 84 us without, 14 + 4
+// with; 8192 rows on 64 keys, dk and dv 120, 19 + 5; 1024 tokens, 1 head, dk and dv 24, 15 + 4), and with documents, where
+// walks differ in length, up to four times as many (8192 tokens in 7 documents of 29 to 2535, 16 heads on 4, dk and
+// dv 674 us without, 576 + 13 split in two, 504 + 23 in four; in 4 of 2048, 403, 405 + 13, 417 + 22). Full grids
+// without documents gain nothing (1024 tokens, 8 heads to twice the CUs: dq 18 us, 28 + 4).
+struct Shape { bool few; int split; };
+Shape shape_of(const In* x, int dtype, bool dq) {
+  const bool half = dtype != 0, wide = x->D > 64;
+  const int64_t M = (int64_t)x->Sq * (x->Hq / x->Hk), own = dq ? M : x->Sk, walk = dq ? x->Sk : M, bh = (int64_t)x->B * x->Hk;
+  Shape p;
+  p.few = (own + 127) / 128 * bh <= (dq && half ? 128 : wide ? 64 : 255);
+  const int64_t blocks = (own + (p.few ? 31 : 127)) / (p.few ? 32 : 128) * bh * (!dq && wide && (p.few || !half) ? 2 : 1);
+  const int64_t tiles = (walk + 31) / 32 / (p.few ? (half || !wide ? 4 : 2) : 1);      // of a wave, about
+  p.split = (int)std::max<int64_t>(1, std::min<int64_t>({(x->qdoc ? 1024 : 256) / blocks, tiles / 2, 16}));
+  return p;
+}
+
+// bytes of a split's sums
+size_t part_bytes(const In* x, bool dq) { return (size_t)x->B * (dq ? (size_t)x->Sq * x->Hq : (size_t)2 * x->Sk * x->Hk) * x->D * sizeof(float); }
 
 template <typename T, int DP, int NW, int RG, bool WK>
 int run_dkv(Args& a, hipStream_t st) {
   typedef Dkv<T, DP, NW, RG, WK> C;
   a.mtiles = (a.Sk + C::BK - 1) / C::BK;
-  return launch(attn_dkv_kernel<T, DP, NW, RG, WK>, (int64_t)a.mtiles * a.B * a.Hk * (C::SP ? 2 : 1), C::NT, C::LDS, a, st);
+  const int64_t total = (int64_t)a.mtiles * a.nsplit * a.B * a.Hk * (C::SP ? 2 : 1);
+  return a.nsplit > 1 ? launch(attn_dkv_kernel<T, DP, NW, RG, WK, true>, total, C::NT, C::LDS, a, st)
+                      : launch(attn_dkv_kernel<T, DP, NW, RG, WK, false>, total, C::NT, C::LDS, a, st);
 }
 template <typename T, int DP, int NW, bool WK>
 int run_dq(Args& a, hipStream_t st) {
   typedef Dq<T, DP, NW, WK> C;
   a.mtiles = (a.M + C::BM - 1) / C::BM;
-  return launch(attn_dq_kernel<T, DP, NW, WK>, (int64_t)a.mtiles * a.B * a.Hk, C::NT, C::LDS, a, st);
+  const int64_t total = (int64_t)a.mtiles * a.nsplit * a.B * a.Hk;
+  return a.nsplit > 1 ? launch(attn_dq_kernel<T, DP, NW, WK, true>, total, C::NT, C::LDS, a, st)
+                      : launch(attn_dq_kernel<T, DP, NW, WK, false>, total, C::NT, C::LDS, a, st);
+}
+template <typename T>
+int sum_splits(const Args& a, void* o0, void* o1, int64_t n, hipStream_t st) {
+  if (a.nsplit <= 1) return 0;
+  const int64_t blocks = ((o1 ? 2 * n : n) / 4 + 255) / 256;
+  attn_sum_kernel<T><<<(unsigned)blocks, 256, 0, st>>>(a.part, (T*)o0, (T*)o1, n, a.nsplit);
+  return (int)hipGetLastError();
 }
 
 template <typename T, int DP>
-int bwd(Args& a, float* delta, hipStream_t st) {
-  const int64_t rows = (int64_t)a.B * a.Sq * a.Hq, bh = (int64_t)a.B * a.Hk;
+int bwd(Args& a, Shape kv, Shape q, float* delta, hipStream_t st) {
+  const int64_t rows = (int64_t)a.B * a.Sq * a.Hq;
   attn_delta_kernel<T><<<(unsigned)((rows + 31) / 32), 256, 0, st>>>(a, delta);
   int rc = (int)hipGetLastError();
   if (rc) return rc;
   a.delta = delta;
   constexpr int WK = sizeof(T) == 4 && DP == 128 ? 2 : 4;
-  // WK gives four times the blocks of 32 keys (rows) instead of 128: taken up to a number of 128-blocks. Measured at 1024
-  // tokens and 8, 16, 24 and 32 heads (64 .. 256 blocks), us with / without WK:
-  //   dk, dv  bf16, 64 channels 21 / 40, 24 / 40, 39 / 42, 43 / 43; 128 channels 46 / 48, 91 / 51, 132 / 53, 176 / 56
-  //           fp32, 64 channels 58 / 181, 112 / 184, 165 / 187, 222 / 190; 128 channels 268 / 258 (32 blocks 135 / 255), 536 / 265
-  //   dq      bf16, 64 channels 11 / 22, 20 / 22, 28 / 23, 37 / 24; 128 channels 18 / 40, 36 / 41, 52 / 42, 69 / 44
-  //           fp32, 64 channels 40 / 128, 77 / 131, 115 / 135, 156 / 137; 128 channels 129 / 242, 261 / 247
-  constexpr int64_t FEWK = DP == 64 ? 255 : 64, FEWQ = sizeof(T) == 2 ? 128 : DP == 64 ? 255 : 64;
   if (a.dk) {
-    const bool few = ((int64_t)a.Sk + 127) / 128 * bh <= FEWK;
-    rc = few ? run_dkv<T, DP, WK, 1, true>(a, st) : run_dkv<T, DP, 4, sizeof(T) == 2 && DP == 128 ? 2 : 1, false>(a, st);
+    a.nsplit = kv.split;
+    rc = kv.few ? run_dkv<T, DP, WK, 1, true>(a, st) : run_dkv<T, DP, 4, sizeof(T) == 2 && DP == 128 ? 2 : 1, false>(a, st);
+    if (!rc) rc = sum_splits<T>(a, a.dk, a.dv, (int64_t)a.B * a.Sk * a.Hk * a.D, st);
     if (rc) return rc;
   }
   if (!a.dq) return 0;
-  const bool few = ((int64_t)a.M + 127) / 128 * bh <= FEWQ;
-  return few ? run_dq<T, DP, WK, true>(a, st) : run_dq<T, DP, 4, false>(a, st);
+  a.nsplit = q.split;
+  rc = q.few ? run_dq<T, DP, WK, true>(a, st) : run_dq<T, DP, 4, false>(a, st);
+  return rc ? rc : sum_splits<T>(a, a.dq, nullptr, rows * a.D, st);
 }
 
 }  // namespace
@@ -591,16 +647,34 @@ int bwd(Args& a, float* delta, hipStream_t st) {
 
 using namespace turtle;
 
-extern "C" int turtle_token_attn_bwd(const turtle_token_attn_grads* g, int dtype, void* stream) {
+extern "C" {
+
+size_t turtle_token_attn_bwd_workspace(const turtle_token_attn_args* x, int dtype) {
+  if (!sizes_ok(x, dtype) || x->table) return 0;
+  size_t n = 0;
+  for (int dq = 0; dq < 2; ++dq) {
+    const int split = shape_of(x, dtype, dq).split;
+    if (split > 1) n = std::max(n, split * part_bytes(x, dq));
+  }
+  return n;
+}
+
+int turtle_token_attn_bwd(const turtle_token_attn_grads* g, int dtype, void* stream) {
   Args a;
   if (!g || g->f.table || !fill(a, &g->f, dtype)) return -1;
   const int es = dtype == 0 ? 4 : 2;
   if (!rows16(g->dout, g->gb, g->gs, g->gh, es) || !a.lse || (!g->dk) != (!g->dv) || !g->delta) return -1;
+  const size_t n = turtle_token_attn_bwd_workspace(&g->f, dtype);
+  if (n && (!g->f.ws || g->f.ws_bytes < n || (uintptr_t)g->f.ws % 16)) return -1;
+  const Shape kv = shape_of(&g->f, dtype, false), q = shape_of(&g->f, dtype, true);
+  a.part = (float*)g->f.ws;
   a.dout = g->dout; a.gb = g->gb; a.gs = g->gs; a.gh = g->gh;
   a.dq = g->dq; a.dk = g->dk; a.dv = g->dv;
   hipStream_t st = (hipStream_t)stream;
   const bool small = a.D <= 64;
-  if (dtype == 0) return small ? bwd<float, 64>(a, g->delta, st) : bwd<float, 128>(a, g->delta, st);
-  if (dtype == 1) return small ? bwd<bf16, 64>(a, g->delta, st) : bwd<bf16, 128>(a, g->delta, st);
-  return small ? bwd<f16, 64>(a, g->delta, st) : bwd<f16, 128>(a, g->delta, st);
+  if (dtype == 0) return small ? bwd<float, 64>(a, kv, q, g->delta, st) : bwd<float, 128>(a, kv, q, g->delta, st);
+  if (dtype == 1) return small ? bwd<bf16, 64>(a, kv, q, g->delta, st) : bwd<bf16, 128>(a, kv, q, g->delta, st);
+  return small ? bwd<f16, 64>(a, kv, q, g->delta, st) : bwd<f16, 128>(a, kv, q, g->delta, st);
 }
+
+}  // extern "C"

@@ -195,7 +195,7 @@ __global__ __launch_bounds__(NW * 64, DP == 128 && sizeof(T) == 4 ? 1 : 2) void 
   struct Tile { int t; bool mixed, mine; uint64_t seen; } q[NS - 1];
   int tnew = WK ? t0 + wave : t0, fly = 0, into = 0, slot = 0;
   auto start = [&]() __attribute__((always_inline)) {
-    Tile x{dw.template next<BN, STEP>(tnew, t1, 1, a.Sk, lane), false, true, ~0ull};
+    Tile x{dw.template next<BN>(tnew, t1, STEP, 1, a.Sk, lane), false, true, ~0ull};
     x.mixed = dw.mixed;
     x.mine = dw.mine;
     if (x.t < t1) { x.seen = issue(x.t, buf + into * F::SLOT); ++fly; }

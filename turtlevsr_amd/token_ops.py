@@ -57,6 +57,8 @@ def lib():
     L.turtle_token_attn_ranges.restype = sz
     L.turtle_token_attn_workspace.argtypes = [blk, ci]
     L.turtle_token_attn_workspace.restype = sz
+    L.turtle_token_attn_bwd_workspace.argtypes = [blk, ci]
+    L.turtle_token_attn_bwd_workspace.restype = sz
     L.turtle_token_attn_fwd.argtypes = [blk, ci, vp]
     L.turtle_token_attn_bwd.argtypes = [blk, ci, vp]
     _bound = L
@@ -389,6 +391,14 @@ def _attn_workspace(q_shape, Hk: int, Sk: int, pages, dt: int, device):
     return (torch.empty(n, dtype=torch.uint8, device=device), n) if n else (None, 0)
 
 
+@functools.lru_cache(maxsize=256)
+def _bwd_workspace_bytes(q_shape, Hk: int, Sk: int, docs: bool, dt: int) -> int:
+    B, Sq, Hq, D = q_shape
+    a = [0] * 37
+    a[12:18], a[22] = (B, Sq, Sk, Hq, Hk, D), 1 if docs else 0
+    return lib().turtle_token_attn_bwd_workspace(_ATTN.pack(*a), dt)
+
+
 class _NoKeys(torch.autograd.Function):
     """Attention where there are no keys, or no queries: zeros, and zero gradients."""
 
@@ -423,7 +433,11 @@ class _Attention(torch.autograd.Function):
         delta = torch.empty(n, dtype=torch.float32, device=q.device)      # this run's own: a graph may be walked twice at once
         dq = _dense(q) if need[0] else None
         dk, dv = (_dense(k), _dense(v)) if need[1] or need[2] else (None, None)
-        blk = _attn_block(q, k, v, ctx.rules, masks, o, k.shape[1], lo=p if dt else 0, lse=p + lse, ranges=p + ranges if masks[2] is not None else 0)
+        docs = masks[2] is not None
+        nws = _bwd_workspace_bytes(q.shape, k.shape[2], k.shape[1], docs, dt)
+        ws = torch.empty(nws, dtype=torch.uint8, device=q.device) if nws else None
+        blk = _attn_block(q, k, v, ctx.rules, masks, o, k.shape[1], lo=p if dt else 0, lse=p + lse, ranges=p + ranges if docs else 0, ws=_ptr(ws),
+                          ws_bytes=nws)
         blk += _GRADS.pack(do.data_ptr(), *_strides(do), _ptr(dq), _ptr(dk), _ptr(dv), delta.data_ptr())
         _run(q, "token_attn_bwd", lib().turtle_token_attn_bwd, blk, dt)
         return (dq, dk if need[1] else None, dv if need[2] else None) + (None,) * 5
