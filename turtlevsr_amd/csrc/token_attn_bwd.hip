@@ -1,14 +1,14 @@
 // Token attention, backward (token_attn.h holds the method and the shared parts): delta, then dk and dv by key tiles,
-// then dq by row tiles. No atomics: every sum has a fixed order.
+// then dq by row tiles, then the sums of split walks. No atomics: every sum has a fixed order.
 //
 // Two kernels compute S and dP twice (14 products of a tile pair for 10) and in exchange neither dk, dv nor dq is ever
 // summed through memory. A wave's step is a chain - S and dP, the rules, the exponential, two products with the results -
 // so with two waves on a SIMD what counts is the chain's waits: LDS reads started ahead of their products (dq at 128
 // channels 400 -> 365 us, dk and dv at 64 channels 212 -> 188), masks without branches (packed documents 850 -> 690).
-// Measured, bf16: 2 x 5120 tokens causal with prefix 2048, 8 heads of 64 channels: dk, dv 181 us (4 products a pair, 690
-// TF/s), dq 119 us (3 products, 785 TF/s), delta 8 us; 7 documents in 8192 tokens, 16 heads on 4 of 128 channels: dk, dv
-// 639 us, dq 361 us, delta 16 us - there the block over the border of the longest documents is the call's time, 2.5 times
-// the mean block's.
+// Measured, bf16: 2 x 5120 tokens causal with prefix 2048, 8 heads of 64 channels: dk, dv 180 us (4 products a pair, 690
+// TF/s), dq 118 us (3 products, 790 TF/s), delta 8 us; 7 documents in 8192 tokens, 16 heads on 4 of 128 channels: dk, dv
+// 534 us and 25 for their sums, dq 354 us, delta 17 us - unsplit, dk and dv took 639: the block over the border of the longest
+// documents walks 2.5 times the mean block's way. fp32, 2 x 333 on 517 tokens, 6 heads on 3 of 48 channels: 34, 22, 4 us.
 #include "token_attn.h"
 
 namespace turtle {
@@ -557,18 +557,27 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 ? 2 : 1) void attn_dq_kerne
   }
 }
 
-// the splits' sums -> o0 (first half of a split's values) and o1, 4 of n values a thread
+// the splits' sums of one kernel -> o0 (first half of a split's values) and, if there, o1, of n values each
+struct Sum {
+  const float* part;
+  void *o0, *o1;
+  int64_t n;
+  int nsplit;
+};
+
+// both kernels' (blockIdx.y), 4 values a thread
 template <typename T>
-__global__ __launch_bounds__(256) void attn_sum_kernel(const float* __restrict__ part, T* o0, T* o1, int64_t n, int nsplit) {
-  const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4, all = o1 ? 2 * n : n;
+__global__ __launch_bounds__(256) void attn_sum_kernel(Sum kv, Sum q) {
+  const Sum a = blockIdx.y ? q : kv;
+  const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4, all = a.o1 ? 2 * a.n : a.n;
   if (i >= all) return;
   float v[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
-  for (int s = 0; s < nsplit; ++s) {
-    const float4 x = *reinterpret_cast<const float4*>(part + s * all + i);
+  for (int s = 0; s < a.nsplit; ++s) {
+    const float4 x = *reinterpret_cast<const float4*>(a.part + s * all + i);
     v[0] += x.x; v[1] += x.y; v[2] += x.z; v[3] += x.w;
   }
-  Rows<T, 64>::put4(i < n ? o0 + i : o1 + (i - n), v);
+  Rows<T, 64>::put4(i < a.n ? reinterpret_cast<T*>(a.o0) + i : reinterpret_cast<T*>(a.o1) + (i - a.n), v);
 }
 
 // The shape of a backward kernel. few: a block's waves own 32 keys (rows) together (WK) instead of 32 each: four times the
@@ -595,8 +604,11 @@ Shape shape_of(const In* x, int dtype, bool dq) {
   return p;
 }
 
-// bytes of a split's sums
-size_t part_bytes(const In* x, bool dq) { return (size_t)x->B * (dq ? (size_t)x->Sq * x->Hq : (size_t)2 * x->Sk * x->Hk) * x->D * sizeof(float); }
+// bytes of a kernel's sums, 0 where it is not split
+size_t part_bytes(const In* x, int dtype, bool dq) {
+  const int split = shape_of(x, dtype, dq).split;
+  return split > 1 ? (size_t)split * x->B * (dq ? (size_t)x->Sq * x->Hq : (size_t)2 * x->Sk * x->Hk) * x->D * sizeof(float) : 0;
+}
 
 template <typename T, int DP, int NW, int RG, bool WK>
 int run_dkv(Args& a, hipStream_t st) {
@@ -614,32 +626,33 @@ int run_dq(Args& a, hipStream_t st) {
   return a.nsplit > 1 ? launch(attn_dq_kernel<T, DP, NW, WK, true>, total, C::NT, C::LDS, a, st)
                       : launch(attn_dq_kernel<T, DP, NW, WK, false>, total, C::NT, C::LDS, a, st);
 }
-template <typename T>
-int sum_splits(const Args& a, void* o0, void* o1, int64_t n, hipStream_t st) {
-  if (a.nsplit <= 1) return 0;
-  const int64_t blocks = ((o1 ? 2 * n : n) / 4 + 255) / 256;
-  attn_sum_kernel<T><<<(unsigned)blocks, 256, 0, st>>>(a.part, (T*)o0, (T*)o1, n, a.nsplit);
-  return (int)hipGetLastError();
-}
-
 template <typename T, int DP>
-int bwd(Args& a, Shape kv, Shape q, float* delta, hipStream_t st) {
+int bwd(Args& a, Shape kv, Shape q, float* part_kv, float* part_q, float* delta, hipStream_t st) {
   const int64_t rows = (int64_t)a.B * a.Sq * a.Hq;
   attn_delta_kernel<T><<<(unsigned)((rows + 31) / 32), 256, 0, st>>>(a, delta);
   int rc = (int)hipGetLastError();
   if (rc) return rc;
   a.delta = delta;
   constexpr int WK = sizeof(T) == 4 && DP == 128 ? 2 : 4;
+  Sum sums[2] = {};
   if (a.dk) {
     a.nsplit = kv.split;
+    a.part = part_kv;
     rc = kv.few ? run_dkv<T, DP, WK, 1, true>(a, st) : run_dkv<T, DP, 4, sizeof(T) == 2 && DP == 128 ? 2 : 1, false>(a, st);
-    if (!rc) rc = sum_splits<T>(a, a.dk, a.dv, (int64_t)a.B * a.Sk * a.Hk * a.D, st);
     if (rc) return rc;
+    if (kv.split > 1) sums[0] = Sum{part_kv, a.dk, a.dv, (int64_t)a.B * a.Sk * a.Hk * a.D, kv.split};
   }
-  if (!a.dq) return 0;
-  a.nsplit = q.split;
-  rc = q.few ? run_dq<T, DP, WK, true>(a, st) : run_dq<T, DP, 4, false>(a, st);
-  return rc ? rc : sum_splits<T>(a, a.dq, nullptr, rows * a.D, st);
+  if (a.dq) {
+    a.nsplit = q.split;
+    a.part = part_q;
+    rc = q.few ? run_dq<T, DP, WK, true>(a, st) : run_dq<T, DP, 4, false>(a, st);
+    if (rc) return rc;
+    if (q.split > 1) sums[1] = Sum{part_q, a.dq, nullptr, rows * a.D, q.split};
+  }
+  const int64_t most = std::max(2 * sums[0].n, sums[1].n);
+  if (!most) return 0;
+  attn_sum_kernel<T><<<dim3((unsigned)((most / 4 + 255) / 256), 2), 256, 0, st>>>(sums[0], sums[1]);
+  return (int)hipGetLastError();
 }
 
 }  // namespace
@@ -651,12 +664,7 @@ extern "C" {
 
 size_t turtle_token_attn_bwd_workspace(const turtle_token_attn_args* x, int dtype) {
   if (!sizes_ok(x, dtype) || x->table) return 0;
-  size_t n = 0;
-  for (int dq = 0; dq < 2; ++dq) {
-    const int split = shape_of(x, dtype, dq).split;
-    if (split > 1) n = std::max(n, split * part_bytes(x, dq));
-  }
-  return n;
+  return part_bytes(x, dtype, false) + part_bytes(x, dtype, true);
 }
 
 int turtle_token_attn_bwd(const turtle_token_attn_grads* g, int dtype, void* stream) {
@@ -667,14 +675,14 @@ int turtle_token_attn_bwd(const turtle_token_attn_grads* g, int dtype, void* str
   const size_t n = turtle_token_attn_bwd_workspace(&g->f, dtype);
   if (n && (!g->f.ws || g->f.ws_bytes < n || (uintptr_t)g->f.ws % 16)) return -1;
   const Shape kv = shape_of(&g->f, dtype, false), q = shape_of(&g->f, dtype, true);
-  a.part = (float*)g->f.ws;
+  float *pkv = (float*)g->f.ws, *pq = pkv + part_bytes(&g->f, dtype, false) / sizeof(float);
   a.dout = g->dout; a.gb = g->gb; a.gs = g->gs; a.gh = g->gh;
   a.dq = g->dq; a.dk = g->dk; a.dv = g->dv;
   hipStream_t st = (hipStream_t)stream;
   const bool small = a.D <= 64;
-  if (dtype == 0) return small ? bwd<float, 64>(a, kv, q, g->delta, st) : bwd<float, 128>(a, kv, q, g->delta, st);
-  if (dtype == 1) return small ? bwd<bf16, 64>(a, kv, q, g->delta, st) : bwd<bf16, 128>(a, kv, q, g->delta, st);
-  return small ? bwd<f16, 64>(a, kv, q, g->delta, st) : bwd<f16, 128>(a, kv, q, g->delta, st);
+  if (dtype == 0) return small ? bwd<float, 64>(a, kv, q, pkv, pq, g->delta, st) : bwd<float, 128>(a, kv, q, pkv, pq, g->delta, st);
+  if (dtype == 1) return small ? bwd<bf16, 64>(a, kv, q, pkv, pq, g->delta, st) : bwd<bf16, 128>(a, kv, q, pkv, pq, g->delta, st);
+  return small ? bwd<f16, 64>(a, kv, q, pkv, pq, g->delta, st) : bwd<f16, 128>(a, kv, q, pkv, pq, g->delta, st);
 }
 
 }  // extern "C"

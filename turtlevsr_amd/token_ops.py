@@ -430,15 +430,16 @@ class _Attention(torch.autograd.Function):
         do = _tokens(do)
         n, dt, p = q.shape[0] * q.shape[1] * q.shape[2], _dt(q), aux.data_ptr()
         lse, ranges, _ = _aux_parts(n, q.shape[3], dt, 0)
-        delta = torch.empty(n, dtype=torch.float32, device=q.device)      # this run's own: a graph may be walked twice at once
         dq = _dense(q) if need[0] else None
         dk, dv = (_dense(k), _dense(v)) if need[1] or need[2] else (None, None)
         docs = masks[2] is not None
         nws = _bwd_workspace_bytes(q.shape, k.shape[2], k.shape[1], docs, dt)
-        ws = torch.empty(nws, dtype=torch.uint8, device=q.device) if nws else None
-        blk = _attn_block(q, k, v, ctx.rules, masks, o, k.shape[1], lo=p if dt else 0, lse=p + lse, ranges=p + ranges if docs else 0, ws=_ptr(ws),
+        # the split sums, then the rows' deltas: this run's own, a graph may be walked twice at once
+        ws = torch.empty(nws + 4 * n, dtype=torch.uint8, device=q.device)
+        pws = ws.data_ptr()
+        blk = _attn_block(q, k, v, ctx.rules, masks, o, k.shape[1], lo=p if dt else 0, lse=p + lse, ranges=p + ranges if docs else 0, ws=pws,
                           ws_bytes=nws)
-        blk += _GRADS.pack(do.data_ptr(), *_strides(do), _ptr(dq), _ptr(dk), _ptr(dv), delta.data_ptr())
+        blk += _GRADS.pack(do.data_ptr(), *_strides(do), _ptr(dq), _ptr(dk), _ptr(dv), pws + nws)
         _run(q, "token_attn_bwd", lib().turtle_token_attn_bwd, blk, dt)
         return (dq, dk if need[1] else None, dv if need[2] else None) + (None,) * 5
 
