@@ -8,9 +8,9 @@
 // The first two have matrix instructions to spare and multiply p in two terms (TWO): with few keys, p's rounding
 // would be as large an error as the result's own.
 //
-// Measured: 32640 x 32640 tokens, 8 heads of 64 channels, bf16, 2490 us (875 TF/s; at 64 rows a wave instead of 32, no
-// faster: 2 x 16 more registers hold off one of three waves of a SIMD); causal with prefix 2048, 2 x 5120 tokens, 112 us
-// (556 TF/s); 510 windows of 64 tokens, 4 heads, 20 us (3.3 TB/s; the start of its one-tile blocks); one token on 16
+// Measured: 32640 x 32640 tokens, 8 heads of 64 channels, bf16, 2490 - 2600 us (840 - 875 TF/s; at 64 rows a wave instead of 32, no
+// faster: 2 x 16 more registers hold off one of three waves of a SIMD); causal with prefix 2048, 2 x 5120 tokens, 110 us
+// (566 TF/s); 510 windows of 64 tokens, 4 heads, 20 us (3.3 TB/s; the start of its one-tile blocks); one token on 16
 // histories of up to 16384 keys, 16 heads on 4 of 128 channels, 80 + 5 us for the join (4.5 TB/s while it reads); 256
 // tokens on 4 histories of 5040, fp16, 8 heads, 32 + 6 us.
 #include "token_attn.h"
@@ -192,6 +192,7 @@ __global__ __launch_bounds__(NW * 64, DP == 128 && sizeof(T) == 4 ? 1 : 2) void 
   // The walk: tiles are started NS - 1 turns before they are computed on (q: the tiles in flight, oldest first). With a
   // block the turn's barrier frees the slot of the tile before; a wave of its own starts the next tile at once.
   constexpr int NS = F::NS;
+  static_assert(NS == 2, "one tile in flight: the last one ends the walk");
   struct Tile { int t; bool mixed, mine; uint64_t seen; } q[NS - 1];
   int tnew = WK ? t0 + wave : t0, fly = 0, into = 0, slot = 0;
   auto start = [&]() __attribute__((always_inline)) {
@@ -207,9 +208,11 @@ __global__ __launch_bounds__(NW * 64, DP == 128 && sizeof(T) == 4 ? 1 : 2) void 
   };
 #pragma unroll 1
   for (int i = 0; i < NS - 1; ++i) start();
-  arrived(qf);
-  arrived(row.doc);
-  arrived(row.slope2);
+  if constexpr (WK || NW > 2) {      // kind 1 has a few tiles, nothing worth keeping in flight
+    arrived(qf);
+    arrived(row.doc);
+    arrived(row.slope2);
+  }
   for (;;) {
     const Tile cur = q[0];
     if (cur.t >= t1) break;
@@ -217,7 +220,8 @@ __global__ __launch_bounds__(NW * 64, DP == 128 && sizeof(T) == 4 ? 1 : 2) void 
       vm_wait_tiles<F::NLD, NS - 2>(fly - 1);
       lds_barrier();
     }
-    start();
+    if (tnew < t1) start();
+    else q[0].t = t1;
     if constexpr (WK) vm_wait_tiles<F::NLD, NS - 1>(fly - 1);
     const char* kt = buf + slot * F::SLOT;
     const char* vt = kt + F::TILE;
