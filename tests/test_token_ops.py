@@ -1118,3 +1118,45 @@ def test_workspace_sizes_from_python_are_the_library_s():
         assert T._workspace_bytes(q.shape, Hk, 0, (256, 9, 40), 1) == L.turtle_token_attn_workspace(blk, 1)
     assert T._workspace_bytes(torch.Size((1, 1, 8, 64)), 2, 9000, (0, 0, 0), 1) > 0
     assert T._norm_workspace(5000, 64) == L.turtle_token_norm_rope_workspace(5000, 64)
+
+
+# -------------------------------------------------------------------------------------------------
+# forward mode
+# -------------------------------------------------------------------------------------------------
+
+def test_forward_mode_derivatives_are_refused(monkeypatch):
+    """A tensor that carries a tangent (with or without requires_grad) is refused by every operator, wherever it
+    enters: a result without a tangent would be a wrong derivative. Tensors without one pass at the same level."""
+    import torch.autograd.forward_ad as fw
+    monkeypatch.setattr(T, "_device", lambda t: None)
+    monkeypatch.setattr(T, "_run", lambda *a: None)             # no launch: what the calls would enqueue is not of interest
+    x, w = torch.zeros(2, 5, 4, 64), torch.ones(64)
+    pos, ax = torch.zeros(5, 3, dtype=torch.int32), (16, 24, 24)
+    tab, kl = torch.zeros(2, 3, dtype=torch.int32), torch.zeros(2, dtype=torch.int32)
+    calls = {
+        "rope x": (T.axial_rope, (x, pos, ax), {}, [0]),
+        "norm q, k, gains": (T.qk_norm_rope, (x, x.clone(), pos, w, w.clone(), ax), {}, [0, 1, 3, 4]),
+        "attention q, k, v": (T.attention, (x, x.clone(), x.clone()), {}, [0, 1, 2]),
+        "attention slopes": (T.attention, (x, x, x), {"slopes": torch.ones(4)}, ["slopes"]),
+        "attention without keys": (T.attention, (x, x[:, :0], x[:, :0]), {}, [0]),
+        "paged q, pools": (T.paged_attention, (x, torch.zeros(6, 16, 2, 64), torch.zeros(6, 16, 2, 64), tab, kl), {}, [0, 1, 2]),
+        "paged slopes": (T.paged_attention, (x, torch.zeros(6, 16, 2, 64), torch.zeros(6, 16, 2, 64), tab, kl), {"slopes": torch.ones(4)}, ["slopes"]),
+    }
+    for name, (f, args, kw, at) in calls.items():
+        with torch.no_grad():
+            f(*args, **kw)
+        for i in at:
+            for rg in (False, True):
+                if rg and (i == "slopes" or f is T.paged_attention):
+                    continue                                     # refused for its gradient already
+                a, k = list(args), dict(kw)
+                with fw.dual_level():
+                    plain = (a if i != "slopes" else k)[i]
+                    dual = fw.make_dual(plain.clone().requires_grad_(rg), torch.ones_like(plain))
+                    if i == "slopes":
+                        k[i] = dual
+                    else:
+                        a[i] = dual
+                    with pytest.raises(RuntimeError, match="forward-mode"):
+                        f(*a, **k)
+                    f(*args, **kw)

@@ -15,7 +15,8 @@ device and can be captured into a graph. There is no CPU path: a CPU tensor or a
   and document masks;
 * ``paged_attention(q, k_pages, v_pages, block_table, kv_lens, ...)``: the serving form, no gradient.
 
-The first three are differentiable (first order); sums run in a fixed order, so results repeat bit for bit.
+The first three are differentiable (first order, reverse mode; a tensor with a forward-mode tangent is refused); sums run
+in a fixed order, so results repeat bit for bit.
 """
 from __future__ import annotations
 
@@ -24,6 +25,7 @@ import functools
 import struct
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib
@@ -163,6 +165,14 @@ def _run(t, what: str, entry, *args):
         _check(rc, what)
 
 
+def _no_tangents(*ts):
+    """Refuses tensors with a tangent: whether they require a gradient or not, the result would have none."""
+    if forward_ad._current_level >= 0 and torch._C._is_fwd_grad_enabled():
+        for t in ts:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise RuntimeError("turtle token operators have no forward-mode derivative")
+
+
 def _wants_grad(*ts) -> bool:
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)
 
@@ -248,6 +258,7 @@ def axial_rope(x, pos, axes, base: float = 10000.0):
     tab, naxis = _axes(axes, base, D)
     p, pos_b, pos64 = _pos(pos, B, S, naxis, x)
     _device(x)
+    _no_tangents(x)
     return _Rope.apply(x, p, pos_b, pos64, tab) if _wants_grad(x) else _turn(x, p, pos_b, pos64, tab, 0)
 
 
@@ -331,6 +342,7 @@ def qk_norm_rope(q, k, pos, q_weight, k_weight, axes, base: float = 10000.0, eps
     tab, naxis = _axes(axes, base, D)
     rest = (*_pos(pos, B, S, naxis, q), tab, eps)
     _device(q)
+    _no_tangents(q, k, q_weight, k_weight)
     if _wants_grad(q, k, q_weight, k_weight):
         return _QkNormRope.apply(q, k, q_weight, k_weight, *rest)
     return _norm_turn(_tokens(q), _tokens(k), _gain(q_weight), _gain(k_weight), *rest)
@@ -490,6 +502,7 @@ def attention(q, k, v, *, scale=None, softcap: float = 0.0, slopes=None, causal:
             raise ValueError(f"q_doc alone needs Sq == Sk ({Sq}, {Sk}): pass k_doc")
         q_doc = _ints(q_doc, (B, Sq), "q_doc", q)
         k_doc = q_doc if k_doc is None else _ints(k_doc, (B, Sk), "k_doc", q)
+    _no_tangents(q, k, v, slopes)
     scale, softcap, slopes = _scale(scale, D), _cap(softcap), _slopes(slopes, Hq, q)
     _device(q)
     rules, masks = (scale, softcap, 1 if causal else 0), (slopes, prefix, q_doc, k_doc)
@@ -525,6 +538,7 @@ def paged_attention(q, k_pages, v_pages, block_table, kv_lens, *, q_lens=None, s
         if n != "block_table" and tuple(t.shape) != (B,):
             raise ValueError(f"{n}: shape {tuple(t.shape)}, expected {(B,)}")
         _same(q, t, n)
+    _no_tangents(q, k_pages, v_pages, slopes)
     scale, softcap, slopes = _scale(scale, D), _cap(softcap), _slopes(slopes, Hq, q)
     _device(q)
     if q.numel() == 0 or k_pages.numel() == 0 or block_table.numel() == 0:
