@@ -1160,3 +1160,83 @@ def test_forward_mode_derivatives_are_refused(monkeypatch):
                     with pytest.raises(RuntimeError, match="forward-mode"):
                         f(*a, **k)
                     f(*args, **kw)
+
+
+# -------------------------------------------------------------------------------------------------
+# sizes of gradients
+# -------------------------------------------------------------------------------------------------
+
+def _fp16_grads(q, k, v, do, scale):
+    """dq and dk of one head in fp64 and bounds on the sums of squared errors by element. dS = p (dP - delta) is rounded
+    once, p carries the scores' error E, so a dS is off by at most s = sqrt(u^2 + E^2) of itself, independently of the
+    others; delta by the same roundings of p: s^2 sum (p (|dP| + |delta|))^2, and dP by fp32 arithmetic. Errors of
+    independent roundings add in squares, and a rounding's variance is a third of its bound's square; results are rounded
+    once more, by u or half of fp16's smallest step."""
+    u = unit(torch.float16)
+    Q, K, V, g = (t.double() for t in (q, k, v, do))
+    D = Q.shape[-1]
+    raw = Q @ K.transpose(-1, -2) * scale
+    p = torch.softmax(raw, -1)
+    e32 = (D / 2 + 8) * 2.0 ** -23
+    E = e32 * float((Q.abs() @ K.abs().transpose(-1, -2)).max()) * abs(scale) + 2.0 ** -20
+    dp = g @ V.transpose(-1, -2)
+    delta = (p * dp).sum(-1, keepdim=True)
+    ds = p * (dp - delta)
+    s2 = u * u + E * E
+    edl2 = s2 * (p * (dp.abs() + delta.abs())).square().sum(-1, keepdim=True) + ((e32 + 2 * u * u) * (g.abs() * (p @ V.abs())).sum(-1, keepdim=True)).square()
+    eds2 = s2 * ds.square() + (p * e32 * (g.abs() @ V.abs().transpose(-1, -2))).square()
+    last = lambda r: (u * r).square() + 2.0 ** -50
+    dq, dk = ds @ K * scale, ds.transpose(-1, -2) @ Q * scale
+    dq2 = (eds2 @ K.square() + edl2 * (p @ K).square()) * scale ** 2 + last(dq)
+    dk2 = (eds2 + edl2 * p.square()).transpose(-1, -2) @ Q.square() * scale ** 2 + last(dk)
+    return (dq, dq2), (dk, dk2)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D", [64, 128, 40])
+@pytest.mark.parametrize("n,Sq,Sk", [(1, 96, 4096), (1, 4096, 96), (2, 700, 3000), (24, 1200, 1100)])
+@pytest.mark.parametrize("kind", ["1e-3", "1e-4", "rows", "keys"])
+def test_attention_fp16_gradients_of_any_size(D, n, Sq, Sk, kind):
+    """Gradients far from one: small ones over many keys, rows of 2^-12 to 2^9 in one call, growing along the walks, and
+    values that grow along the keys. The norm of the error of all values, of the small rows and of the first keys is at
+    most twice the bounds' (which are themselves 1.7 times what independent roundings give)."""
+    q, k = randn(n, Sq, 1, D, seed=1).mul(2.0 ** -8).half(), randn(n, Sk, 1, D, seed=2).mul(2.0 ** -8).half()
+    v, do = randn(n, Sk, 1, D, seed=3), randn(n, Sq, 1, D, seed=4)
+    ramp = lambda s, lo, hi: torch.linspace(lo, hi, s, device=DEV).exp2().view(1, s, 1, 1)
+    if kind == "rows":
+        do = do * ramp(Sq, -12, 9) * 1e-2
+    elif kind == "keys":
+        v, do = v * ramp(Sk, -6, 6), do * 1e-3
+    else:
+        do = do * float(kind)
+    v, do, scale = v.half(), do.half(), 2.0 ** 16 * D ** -0.5
+    leaves = [t.requires_grad_(True) for t in (q, k, v)]
+    dq, dk, _ = torch.autograd.grad(T.attention(*leaves, scale=scale), leaves, do)
+    ref = _fp16_grads(*(t.detach()[:, :, 0] for t in (q, k, v, do)), scale)
+    for name, got, (want, e2), part in (("dq", dq, ref[0], Sq // 4), ("dk", dk, ref[1], Sk // 4)):
+        err = got[:, :, 0].double() - want
+        assert torch.isfinite(err).all(), name
+        for what, x in (("all", slice(None)), ("first quarter", slice(0, part))):
+            a, b = float(err[:, x].norm()), 2 * float(e2[:, x].sum().sqrt())
+            assert a <= b, (name, what, a, b, float(want[:, x].norm()))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("n", [1, 300])
+def test_attention_fp16_gradients_past_the_type_s_range_inside(D, n):
+    """dO of 2e4 on three keys: dS passes 65504, the gradients do not."""
+    q, k, v = (randn(n, s, 1, D, dtype=torch.float16, seed=i) for i, s in enumerate((4, 3, 3)))
+    do = (randn(n, 4, 1, D, seed=4) * 2e4).clamp(-5e4, 5e4).half()
+    scale = 2.0 ** -8
+    leaves = [t.requires_grad_(True) for t in (q, k, v)]
+    grads = torch.autograd.grad(T.attention(*leaves, scale=scale), leaves, do)
+    ref = _fp16_grads(*(t.detach()[:, :, 0] for t in (q, k, v, do)), scale)
+    p = torch.softmax(q.detach()[:, :, 0].double() @ k.detach()[:, :, 0].double().transpose(1, 2) * scale, -1)
+    ds = p * (do[:, :, 0].double() @ v.detach()[:, :, 0].double().transpose(1, 2))
+    assert float(ds.abs().max()) > 65504
+    for name, got, (want, e2) in (("dq", grads[0], ref[0]), ("dk", grads[1], ref[1])):
+        assert float(want.abs().max()) < 60000
+        err = got[:, :, 0].double() - want
+        assert torch.isfinite(err).all(), name
+        assert float(err.norm()) <= 2 * float(e2.sum().sqrt()), name

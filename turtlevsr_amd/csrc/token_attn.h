@@ -26,10 +26,10 @@
 //   would otherwise get 16-bit noise as its gradient.
 //
 // What is rounded: p and dS to the inputs' type as operands of the second products (fp16: p times 2^6 in the forward,
-// which leaves room for the 2^8 it may stand over the running maximum, 2^10 in dk's and dv's kernel, so that p of 10^4
-// keys keep their bits), results at the end; scores, maxima, sums and accumulators are fp32. The 16-bit rounding of p
-// and dS is what separates the 16-bit results from the rounded exact ones: relative error of all values 2.4e-3 in bf16
-// and 3.0e-4 in fp16, the rounding of the result alone being 1.7e-3 and 2.1e-4.
+// which leaves room for the 2^8 it may stand over the running maximum, 2^10 for dv, so that p of 10^4 keys keep their
+// bits; dS times a power of two of the row's or key's own), results at the end; scores, maxima, sums and accumulators are
+// fp32. The 16-bit rounding of p and dS is what separates the 16-bit results from the rounded exact ones: relative error of
+// all values 2.4e-3 in bf16 and 3.0e-4 in fp16, the rounding of the result alone being 1.7e-3 and 2.1e-4.
 //
 // Bound: the matrix products where rows are many (a large bf16 product reaches 1188 TF/s on the card, fp32 153), HBM
 // where they are few (a large copy reaches 4.9 TB/s). Beside the products every score costs an exponential (10 clocks of

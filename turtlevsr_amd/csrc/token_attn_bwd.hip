@@ -85,6 +85,52 @@ TURTLE_DEV void join_waves(f32x16 (&acc)[DT], float* sum, int wave, int lane) {
     for (int r = 0; r < 16; ++r) acc[dt][r] = sum[(dt * 16 + r) * 64 + lane];
 }
 
+// dS as an fp16 operand of dk (dq) is taken times 2^e: unscaled, a pair among 4096 keys under a dO of 1e-3 is near the type's
+// smallest numbers (dq off by 0.5 %, by 5 % at 1e-4), and one of a large dO past 65504. e belongs to the key (row) that a
+// lane and lane ^ 32 own, one column of the accumulators. It starts at 60, falls when a |dS| 2^e passes 2^15 - to where the
+// largest one is under 2^8 - and never rises, so what is lost lies 2^-32 below the column's largest dS. Powers of two:
+// the sums are scaled over without an error, and no lane's result depends on another column's.
+template <typename T> struct Lift {
+  static constexpr bool on = std::is_same<T, f16>::value;
+  int e;
+  TURTLE_DEV static float pow2(int n) { return __int_as_float((127 + n) << 23); }
+  // ds of a tile, times 2^e; acc: the sums of the tiles before
+  template <int N, int DT>
+  TURTLE_DEV void fit(f32x16 (&ds)[N], f32x16 (&acc)[DT]) {
+    if constexpr (!on) return;
+    float big = 0.f;
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) big = fmaxf(big, fabsf(ds[j][r]));
+    if (__any(big * pow2(e) > 32768.f)) {
+      big = half_max(big);
+      const int to = big * pow2(e) > 32768.f ? min(e, 8 - __builtin_amdgcn_frexp_expf(big)) : e;      // -120 at least
+      const float f = ldexpf(1.f, to - e);
+#pragma unroll
+      for (int i = 0; i < DT; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[i][r] *= f;
+      e = to;
+    }
+    const float up = pow2(e);
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) ds[j][r] *= up;
+  }
+  // the sums as they are
+  template <int DT>
+  TURTLE_DEV void drop(f32x16 (&acc)[DT]) const {
+    if constexpr (!on) return;
+    const float down = pow2(-e);
+#pragma unroll
+    for (int i = 0; i < DT; ++i)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[i][r] *= down;
+  }
+};
+
 // dv's accumulators: its own, or dk's where a block has only one of them
 template <bool SAME, int N, int M>
 TURTLE_DEV auto& pick(f32x16 (&x)[N], f32x16 (&y)[M]) {
@@ -200,6 +246,7 @@ __global__ __launch_bounds__(NW * RG * 64, sizeof(T) == 2 && (DP == 64 || RG == 
   auto& dv = pick<SP>(dk, dv_);
 #pragma unroll
   for (int i = 0; i < DT; ++i) { dk[i] = zero16(); dv[i] = zero16(); }
+  Lift<T> lift{60};
 
   // the walk over row tiles: as the forward's over key tiles
   struct Tile { int t; bool mixed; } q[NS - 1];
@@ -315,12 +362,16 @@ __global__ __launch_bounds__(NW * RG * 64, sizeof(T) == 2 && (DP == 64 || RG == 
           }
         }
       if (do_v) R::template t_times_all<MT>(gt, s, dv, lane);
-      if (do_k) R::template t_times_all<MT>(qt, dp, dk, lane);
+      if (do_k) {
+        lift.fit(dp, dk);
+        R::template t_times_all<MT>(qt, dp, dk, lane);
+      }
     }
     if constexpr (WK) asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     --fly;
     slot = slot + 1 == NS ? 0 : slot + 1;
   }
+  if (do_k) lift.drop(dk);
   if constexpr (WK) {
     join_waves<NW>(dk, reinterpret_cast<float*>(smem), wave, lane);
     if constexpr (!SP) join_waves<NW>(dv, reinterpret_cast<float*>(smem), wave, lane);
@@ -447,6 +498,7 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 ? 2 : 1) void attn_dq_kerne
   f32x16 dq[DT];
 #pragma unroll
   for (int j = 0; j < DT; ++j) dq[j] = zero16();
+  Lift<T> lift{60};
 
   struct Tile { int t; bool mixed; } q[NS - 1];
   int tnew = sp * STEP + (WK ? wave : 0), fly = 0, into = 0, slot = 0;
@@ -532,12 +584,14 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 ? 2 : 1) void attn_dq_kerne
       for (int j = 0; j < KT; ++j)
 #pragma unroll
         for (int r = 0; r < 16; ++r) dp[j][r] *= __builtin_amdgcn_exp2f(fmaf(s[j][r], mul, -lse));
+      lift.fit(dp, dq);
       R::template t_times_all<KT>(kt, dp, dq, lane);
     }
     if constexpr (WK) asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     --fly;
     slot = slot + 1 == NS ? 0 : slot + 1;
   }
+  lift.drop(dq);
   if constexpr (WK) join_waves<NW>(dq, reinterpret_cast<float*>(smem), wave, lane);
   if (mrow >= a.M) return;
   const int64_t oi = (((int64_t)b * a.Sq + i) * a.Hq + hq) * a.D;
