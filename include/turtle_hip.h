@@ -172,7 +172,7 @@ int turtle_set_option(TurtleHandle* h, const char* name, int value);
 
 const char* turtle_last_error(void);
 
-/* Hash of the kernel sources (turtlevsr_amd/csrc + build.py, turtlevsr_amd/build.py source_hash) the
+/* Hash of the kernel sources (turtlevsr_amd/csrc, build.py and include/; turtlevsr_amd/build.py source_hash) the
  * library was built from: the Python binding refuses a library whose hash is not the tree's. */
 const char* turtle_source_hash(void);
 

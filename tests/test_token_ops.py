@@ -1240,3 +1240,64 @@ def test_attention_fp16_gradients_past_the_type_s_range_inside(D, n):
         err = got[:, :, 0].double() - want
         assert torch.isfinite(err).all(), name
         assert float(err.norm()) <= 2 * float(e2.sum().sqrt()), name
+
+
+# -------------------------------------------------------------------------------------------------
+# the library and its header
+# -------------------------------------------------------------------------------------------------
+
+def test_a_changed_header_makes_the_built_library_stale(tmp_path, monkeypatch):
+    """The argument blocks' layout stands in include/: a library built from another header is another library."""
+    import shutil
+    from turtlevsr_amd import build as B
+    (tmp_path / "turtlevsr_amd").mkdir()
+    for d, src in (("turtlevsr_amd/csrc", B.CSRC), ("include", os.path.join(REPO, "include"))):
+        shutil.copytree(src, tmp_path / d)
+    shutil.copy(os.path.join(REPO, "turtlevsr_amd", "build.py"), tmp_path / "turtlevsr_amd")
+    monkeypatch.setattr(B, "REPO", str(tmp_path))
+    monkeypatch.setattr(B, "CSRC", str(tmp_path / "turtlevsr_amd" / "csrc"))
+    seen = {B.source_hash()}
+    for h in sorted(os.listdir(tmp_path / "include")):
+        with open(tmp_path / "include" / h, "a") as f:
+            f.write("/* */\n")
+        seen.add(B.source_hash())
+    assert len(seen) == 1 + len(os.listdir(tmp_path / "include"))
+
+
+def test_packed_blocks_have_the_header_s_layout(tmp_path):
+    """Every field of include/turtle_token.h's structs against the formats the calls are packed with, by the C compiler."""
+    import shutil
+    import struct
+    import subprocess
+    cc = shutil.which("gcc") or shutil.which("cc") or shutil.which("clang")
+    assert cc, "no C compiler"
+    hdr = re.sub(r"/\*.*?\*/", "", open(os.path.join(REPO, "include", "turtle_token.h")).read(), flags=re.S)
+    body = {}
+    for m in re.finditer(r"typedef struct \{([^{}]*)\} (turtle_token_\w+);", hdr):
+        names = []
+        for decl in filter(None, (d.strip() for d in m.group(1).split(";"))):
+            names += [re.search(r"(\w+)(?:\[\d+\])?\s*$", part).group(1) for part in decl.split(",")]
+        body[m.group(2)] = names
+    assert set(body) == {"turtle_token_axes", "turtle_token_side", "turtle_token_attn_args", "turtle_token_attn_grads"}
+    src = '#include <stdio.h>\n#include "turtle_token.h"\nint main(void) {\n'
+    for s, names in body.items():
+        src += f'printf("{s} %zu", sizeof({s}));\n' + "".join(f'printf(" %zu", offsetof({s}, {n}));\n' for n in names) + 'puts("");\n'
+    (tmp_path / "a.c").write_text(src + "return 0; }\n")
+    subprocess.run([cc, "-I", os.path.join(REPO, "include"), str(tmp_path / "a.c"), "-o", str(tmp_path / "a")], check=True)
+    c = {x.split()[0]: [int(n) for n in x.split()[1:]] for x in subprocess.run([str(tmp_path / "a")], check=True, capture_output=True, text=True).stdout.splitlines()}
+
+    def offsets(fmt):
+        at, out = 0, []
+        for n, t in re.findall(r"(\d*)([A-Za-z])", fmt):
+            size = struct.calcsize("@" + t)
+            at = -(-at // size) * size
+            out += [at + size * i for i in range(int(n or 1))]
+            at += size * int(n or 1)
+        return out
+    side, attn = offsets(T._SIDE.format), offsets(T._ATTN.format)
+    assert c["turtle_token_side"] == [T._SIDE.size] + side
+    assert c["turtle_token_axes"][0] == T._AXES.size
+    q, b, i = re.findall(r"\d*[A-Za-z]", T._AXES.format)
+    assert (q, b, i) == ("64Q", "64B", "2i") and c["turtle_token_axes"][1:] == [0, 512, 576, 580]
+    assert c["turtle_token_attn_args"] == [T._ATTN.size] + attn
+    assert c["turtle_token_attn_grads"] == [T._ATTN.size + T._GRADS.size, 0] + [T._ATTN.size + o for o in offsets(T._GRADS.format)]

@@ -16,6 +16,7 @@ import sys
 PKG = os.path.dirname(os.path.abspath(__file__))
 REPO = os.path.dirname(PKG)
 CSRC = os.path.join(PKG, "csrc")
+HEADERS = ("turtle_hip.h", "turtle_train.h", "turtle_token.h")       # include/: the C surface and its argument blocks
 OBJ = os.path.join(PKG, "build")
 LIB = os.path.join(PKG, "lib", "libturtle_hip.so")
 SOURCES = ["gemm.hip", "gemm2.hip", "gemm3.hip", "gemm5.hip", "spatial.hip", "attn.hip", "sab.hip", "fused.hip", "fused2.hip", "dwgemm.hip", "tilepd.hip", "gffn.hip", "gemm8.hip", "gemm9.hip", "gemm_f32.hip", "gemm_sk.hip", "ffn.hip", "t0.hip", "train_ops.hip", "token.hip", "token_attn_fwd.hip", "token_attn_bwd.hip", "turtle.cpp"]
@@ -39,7 +40,7 @@ def _compile(src: str, force: bool) -> str:
     obj = os.path.join(OBJ, src + ".o")
     path = os.path.join(CSRC, src)
     deps = [path] + [os.path.join(CSRC, h) for h in os.listdir(CSRC) if h.endswith(".h")]
-    deps += [os.path.join(REPO, "include", h) for h in ("turtle_hip.h", "turtle_train.h", "turtle_token.h")]
+    deps += [os.path.join(REPO, "include", h) for h in HEADERS]
     if not force and os.path.exists(obj) and os.path.getmtime(obj) >= max(os.path.getmtime(d) for d in deps):
         return obj
     cmd = [hipcc()] + _flags() + ["-x", "hip", "-c", path, "-o", obj]
@@ -50,11 +51,11 @@ def _compile(src: str, force: bool) -> str:
 
 
 def source_hash() -> str:
-    """Hash of the HIP kernel sources + this build script: ties committed PMC counters
-    (profiles/pmc_traffic.json) to the kernels they were measured on."""
+    """Hash of the HIP kernel sources, the C headers and this build script: ties a built library to the tree's sources and
+    argument layouts, and committed PMC counters (profiles/pmc_traffic.json) to the kernels they were measured on."""
     import hashlib
     hs = hashlib.sha256()
-    for rel in sorted(os.listdir(CSRC)) + ["../build.py"]:
+    for rel in sorted(os.listdir(CSRC)) + ["../build.py"] + ["../../include/" + h for h in HEADERS]:
         path = os.path.join(CSRC, rel)
         if os.path.isfile(path):
             hs.update(rel.encode())
