@@ -1301,3 +1301,55 @@ def test_packed_blocks_have_the_header_s_layout(tmp_path):
     assert (q, b, i) == ("64Q", "64B", "2i") and c["turtle_token_axes"][1:] == [0, 512, 576, 580]
     assert c["turtle_token_attn_args"] == [T._ATTN.size] + attn
     assert c["turtle_token_attn_grads"] == [T._ATTN.size + T._GRADS.size, 0] + [T._ATTN.size + o for o in offsets(T._GRADS.format)]
+
+
+# -------------------------------------------------------------------------------------------------
+# far positions
+# -------------------------------------------------------------------------------------------------
+
+def _turns(pos, j, d, base):
+    """pos base^(-j / d) / 2 pi mod 1 (nearest to zero), in 60 digits; pi from Machin's formula."""
+    from decimal import Decimal, getcontext, localcontext
+    with localcontext() as c:
+        c.prec = 60
+
+        def arctan_inverse(n):
+            x, s, k = Decimal(1) / n, Decimal(0), 0
+            while abs(x) > Decimal(10) ** -58:
+                s += x / (2 * k + 1) * (-1) ** k
+                x, k = x / (n * n), k + 1
+            return s
+        pi = 16 * arctan_inverse(5) - 4 * arctan_inverse(239)
+        r = Decimal(pos) * (-Decimal(j) / d * Decimal(base).ln()).exp() / (2 * pi)
+        return float(r - r.to_integral_value())
+
+
+FAR = [0, 1, -1, 10 ** 6, 2 ** 31 - 1, -2 ** 31, 10 ** 9 + 7, 10 ** 12, -10 ** 12 - 1, 2 ** 45 + 3, 2 ** 50, -2 ** 50 + 1]
+
+
+@pytest.mark.parametrize("base,d", [(10000.0, 24), (10000.0, 64), (100.5, 16), (1.0, 8), (1e30, 128)])
+def test_frequencies_hold_for_far_positions(base, d):
+    """Revolutions of every pair from the table, pos * freq mod 2^64: off by at most |pos| / 2 of the 2^-64 that freq is
+    rounded to, besides the comparison's own 2^-50."""
+    tab = T._AXES.unpack(T._axes((d,), base, 128)[0])
+    for i in range(d // 2):
+        for pos in FAR:
+            got = (pos * tab[i] % 2 ** 64) / 2 ** 64
+            off = abs(got - _turns(pos, 2 * i, d, base)) % 1.0
+            assert min(off, 1 - off) <= abs(pos) * 2.0 ** -65 + 2.0 ** -50, (i, pos)
+
+
+@pytest.mark.gpu
+def test_axial_rope_turns_far_64_bit_positions_rightly():
+    """fp32: the functions' error of the other fp32 test (2^-22 of the pair), the angle's 2^-32 revolutions and the table's
+    |pos| 2^-65."""
+    d = 24
+    pos = torch.tensor(FAR, dtype=torch.int64, device=DEV)[:, None]
+    x = randn(1, len(FAR), 2, d, seed=1)
+    turns = torch.tensor([[_turns(p, 2 * i, d, 10000.0) for i in range(d // 2)] for p in FAR], dtype=torch.float64, device=DEV)
+    th = (turns * 2 * math.pi)[:, None]
+    x0, x1 = x.double()[..., ::2], x.double()[..., 1::2]
+    ref = torch.stack((x0 * th.cos() - x1 * th.sin(), x0 * th.sin() + x1 * th.cos()), -1).flatten(-2)
+    pair = (x0.abs() + x1.abs()).repeat_interleave(2, -1)
+    far = pos.double().abs()[:, None] * 2.0 ** -65 * 2 * math.pi
+    within(T.axial_rope(x, pos, (d,)), ref, (2.0 ** -22 + 2.0 ** -29 + far) * pair, "y")

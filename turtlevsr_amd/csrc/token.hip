@@ -13,8 +13,9 @@
 // Measured: 32640 tokens, 8 + 8 heads of 64 channels, bf16: 34 us (3.9 TB/s; a large copy reaches 4.9); 40960 tokens,
 // forward 42 us, backward with both gains' gradients 57 + 4 us (4.4 TB/s).
 //
-// Angles: f_i is a 64-bit fixed-point number of revolutions per position, so pos * f_i wraps exactly and
-// position 10^6 is as precise as position 0 (fp32 products would be off by 0.06 rad there).
+// Angles: f_i is a 64-bit fixed-point number of revolutions per position, so pos * f_i wraps exactly: what is lost is
+// |pos| 2^-65 revolutions of f_i's rounding, and position 10^6 is as precise as position 0 (fp32 products would be off by
+// 0.06 rad there).
 #include "common.h"
 #include "../../include/turtle_token.h"
 

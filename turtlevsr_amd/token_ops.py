@@ -21,6 +21,7 @@ in a fixed order, so results repeat bit for bit.
 from __future__ import annotations
 
 import ctypes as C
+import decimal
 import functools
 import struct
 
@@ -181,16 +182,22 @@ def _wants_grad(*ts) -> bool:
 # rotation
 # -------------------------------------------------------------------------------------------------
 
+_TWO_PI = 2 * decimal.Decimal("3.14159265358979323846264338327950288419716939937510582097494459")
+
+
 @functools.lru_cache(maxsize=64)
 def _axes_table(axes, base: float):
-    """Every rotated pair's axis and its revolutions per unit of position in 64-bit fixed point: with it
-    pos * freq mod 2^64 is the exact angle, however far the position."""
+    """Every rotated pair's axis and its revolutions per unit of position in 64-bit fixed point, rounded once: pos * freq
+    mod 2^64 is the angle but for |pos| 2^-65 revolutions (a double has 53 bits: at 2^50 it would be arbitrary to 0.03)."""
     freq, axis = [0] * 64, [0] * 64
     i = 0
-    for a, d in enumerate(axes):
-        for j in range(0, d, 2):
-            freq[i], axis[i] = int(base ** (-j / d) / 6.283185307179586476925 * 2.0 ** 64), a
-            i += 1
+    with decimal.localcontext() as c:
+        c.prec = 50
+        ln = decimal.Decimal(base).ln()
+        for a, d in enumerate(axes):
+            for j in range(0, d, 2):
+                freq[i], axis[i] = int((2 ** 64 * (-ln * j / d).exp() / _TWO_PI).to_integral_value()), a
+                i += 1
     return _AXES.pack(*freq, *axis, i, len(axes))
 
 
@@ -251,8 +258,8 @@ def axial_rope(x, pos, axes, base: float = 10000.0):
     unchanged. Within an axis of d channels, pair i - channels (2 i, 2 i + 1) - turns by the angle
     ``pos[axis] * base ** (-2 i / d)``.
 
-    x [B, S, heads, D]; pos int32 or int64 [S, len(axes)] or [B, S, len(axes)] (any sign, exact at any
-    distance); axes one to four even numbers. Returns a dense tensor of x's type."""
+    x [B, S, heads, D]; pos int32 or int64 [S, len(axes)] or [B, S, len(axes)] (any sign; an angle is off by at most
+    2^-23 and ``|pos| 2^-62`` rad, the latter 6e-5 at 2^48); axes one to four even numbers. Returns a dense tensor of x's type."""
     _check_tokens(x, "x")
     B, S, _, D = x.shape
     tab, naxis = _axes(axes, base, D)
