@@ -1353,3 +1353,35 @@ def test_axial_rope_turns_far_64_bit_positions_rightly():
     pair = (x0.abs() + x1.abs()).repeat_interleave(2, -1)
     far = pos.double().abs()[:, None] * 2.0 ** -65 * 2 * math.pi
     within(T.axial_rope(x, pos, (d,)), ref, (2.0 ** -22 + 2.0 ** -29 + far) * pair, "y")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16])
+def test_qk_norm_of_rows_past_the_range_of_squares(dt):
+    """A head whose squares pass fp32's range has a norm of infinity: zeros, zero gradients and nothing in the gain's, as from
+    x * rsqrt(mean(x^2) + eps) in fp32; the other heads are as without it. Values whose squares just fit are normed."""
+    q, k = randn(2, 9, 3, 64, dtype=dt, seed=1), randn(2, 9, 1, 64, dtype=dt, seed=2)
+    pos, w = _grid(9, 3), torch.linspace(0.5, 2, 64, device=DEV)
+    g = randn(2, 9, 3, 64, dtype=dt, seed=3), randn(2, 9, 1, 64, dtype=dt, seed=4)
+
+    def call(q, k):
+        leaves = [t.detach().requires_grad_(True) for t in (q, k, w, w)]
+        y = T.qk_norm_rope(leaves[0], leaves[1], pos, leaves[2], leaves[3], (16, 24, 24))
+        return [t.detach() for t in y] + list(torch.autograd.grad(y, leaves, g))
+    small = q.clone()
+    small[0, 4, 1] = 0
+    want = call(small, k)
+    for big in (1e20, 3e38):
+        huge = q.clone()
+        huge[0, 4, 1] = big
+        got = call(huge, k)
+        assert not got[0][0, 4, 1].any() and not got[2][0, 4, 1].any()
+        for a, b in zip(got, want):
+            assert torch.isfinite(a).all()
+        got[2][0, 4, 1] = want[2][0, 4, 1] = 0
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    edge = q.clone()
+    edge[0, 4, 1] = 2e18                                       # 64 squares of 4e36 add up to 2.6e38
+    y = call(edge, k)[0][0, 4, 1].double()
+    ref = rope_ref(w.double().expand(1, 1, 1, 64).clone(), pos[4:5], (16, 24, 24))[0, 0, 0]
+    within(y, ref, (unit(dt) + 2.0 ** -18) * 4 + 0 * ref, "edge")

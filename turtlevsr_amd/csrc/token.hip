@@ -105,12 +105,12 @@ TURTLE_DEV float row_sum(float v) {
   return v;
 }
 
-// 1 / sqrt(x): the hardware's (one ulp or so); fp32 with a Newton step
+// 1 / sqrt(x): the hardware's (one ulp or so); fp32 with a Newton step, but 0 of infinity (a row whose squares pass fp32)
 template <typename T>
 TURTLE_DEV float rsqrt_of(float x) {
   const float r = __builtin_amdgcn_rsqf(x);
   if constexpr (sizeof(T) == 2) return r;
-  else return r * fmaf(-0.5f * x * r, r, 1.5f);
+  else return x < INFINITY ? r * fmaf(-0.5f * x * r, r, 1.5f) : r;
 }
 
 struct RopeArgs {

@@ -326,7 +326,8 @@ def qk_norm_rope(q, k, pos, q_weight, k_weight, axes, base: float = 10000.0, eps
     / ``k_weight`` [D], or None), then ``axial_rope``, in one pass over q and k.
 
     q [B, S, Hq, D], k [B, S, Hk, D] of one type at the same tokens; pos, axes and base as in ``axial_rope``.
-    Gradients go to q, k and the gains."""
+    Gradients go to q, k and the gains. Squares are fp32: a head whose mean square passes that range gives zeros and
+    passes no gradient."""
     _check_tokens(q, "q")
     _check_tokens(k, "k")
     B, S, _, D = q.shape
