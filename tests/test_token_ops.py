@@ -1385,3 +1385,33 @@ def test_qk_norm_of_rows_past_the_range_of_squares(dt):
     y = call(edge, k)[0][0, 4, 1].double()
     ref = rope_ref(w.double().expand(1, 1, 1, 64).clone(), pos[4:5], (16, 24, 24))[0, 0, 0]
     within(y, ref, (unit(dt) + 2.0 ** -18) * 4 + 0 * ref, "edge")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("Sq,Sk,n", [(20, 300, 1), (100, 200, 3), (200, 300, 70)])
+def test_attention_cap_keeps_small_scores_beside_large_ones(dt, Sq, Sk, n):
+    """A cap of 10^6 that one query reaches: the scores of the other rows, which it leaves as they are (tanh x = x to
+    (s / 10^6)^2 / 3), keep fp32's relative accuracy. tanh's part of their error is 2^-20 of the largest, a fifth of the
+    bound on the fp32 sums. The one query has no gradient, so those of the keys are of the other rows too. fp16 results under
+    2^-14 are rounded to multiples of 2^-24, by 2^-25 at most however small they are: added to the relative bounds."""
+    q, k, v = (randn(n, s, 2, 64, dtype=dt, seed=i) for i, s in enumerate((Sq, Sk, Sk)))
+    do = randn(n, Sq, 2, 64, dtype=dt, seed=5)
+    q[:, 3], do[:, 3] = 6e4 * q[:, 3].sign(), 0
+    assert float((q[:, 3].double()[:, None] * k.double()).sum(-1).abs().max()) > 5e5
+    rest = [i for i in range(Sq) if i != 3]
+    ref = attn_ref(q[:, rest], k, v, torch.ones(n, Sq - 1, Sk, dtype=torch.bool, device=DEV), scale=1.0, do=do[:, rest])
+    leaves = [t.requires_grad_(True) for t in (q, k, v)]
+    o = T.attention(*leaves, scale=1.0, softcap=1e6)
+    dq, dk, dv = torch.autograd.grad(o, leaves, do)
+    for name, got in (("o", o[:, rest]), ("dq", dq[:, rest]), ("dk", dk), ("dv", dv)):
+        within(got, ref[name][0], 1.2 * ref[name][1] + (2.0 ** -25 if dt == torch.float16 else 0.0), name)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("cap", [0.5, 64.0, 64.5])
+def test_attention_caps_that_scores_reach(dt, cap):
+    """Scores of up to a few caps, under the cap where a 16-bit tanh changes its form and over it."""
+    q, k, v = (randn(2, s, 2, 64, dtype=dt, seed=i) for i, s in enumerate((70, 150, 150)))
+    check_attention(q, k, v, randn(2, 70, 2, 64, dtype=dt, seed=5), scale=cap / 8, softcap=cap)

@@ -439,36 +439,38 @@ TURTLE_DEV Row row_of(const Args& a, int b, int hk, int m, int off, int nq) {
 }
 
 // tanh of the scores in place, for the cap. While every |x| of the wave is at most 1/2 - scores within half the cap -
-// an odd polynomial (least-maximum fit of tanh(x) / x in x^2: relative error 5.5e-7 for 16-bit inputs, 3.2e-10 for
-// fp32): 5 instructions where the exponential form takes two of the slow ones besides. Beyond: 16-bit inputs
-// 1 - 2 / (e^2x + 1), absolute error ~1e-7, under the scores' own rounding there; fp32 the library's.
+// an odd polynomial (least-maximum fit of tanh(x) / x in x^2: relative error 5.5e-7 for 16-bit inputs, 3.3e-9 for
+// fp32, to which fp32 arithmetic adds 9e-8): 5 instructions where the exponential form takes two of the slow ones besides.
+// Beyond: 16-bit inputs 1 - 2 / (e^2x + 1), off by 1e-7: of a cap up to 64 that is 2^-17, nothing to a 16-bit p; over
+// it the wave's values up to 1/2 keep the polynomial (for every cap that would cost 16 % of packed documents at cap 2,
+// 25 % of a paged chunk). fp32 the library's.
+template <typename T>
+TURTLE_DEV float tanh_small(float x) {
+  const float u = x * x;
+  if constexpr (sizeof(T) == 2) return x * fmaf(u, fmaf(u, fmaf(u, -0.0444022265f, 0.131902966f), -0.333263179f), 0.999999456f);
+  else return x * fmaf(u, fmaf(u, fmaf(u, fmaf(u, fmaf(u, -0.0066134277f, 0.0212747076f), -0.0538934189f), 0.13332902f), -0.333333242f), 1.f);
+}
 template <typename T, int N>
-TURTLE_DEV void tanh_all(f32x16 (&s)[N], float icap) {
+TURTLE_DEV void tanh_all(f32x16 (&s)[N], float icap, float cap) {
   float big = 0.f;
 #pragma unroll
   for (int w = 0; w < N; ++w)
 #pragma unroll
     for (int r = 0; r < 16; ++r) { s[w][r] *= icap; big = fmaxf(big, fabsf(s[w][r])); }
+  auto all = [&](auto f) __attribute__((always_inline)) {
+#pragma unroll
+    for (int w = 0; w < N; ++w)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[w][r] = f(s[w][r]);
+  };
   if (!__any(!(big <= 0.5f))) {
-#pragma unroll
-    for (int w = 0; w < N; ++w)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const float x = s[w][r], u = x * x;
-        float p;
-        if constexpr (sizeof(T) == 2) p = fmaf(u, fmaf(u, fmaf(u, -0.0444022265f, 0.131902966f), -0.333263179f), 0.999999456f);
-        else p = fmaf(u, fmaf(u, fmaf(u, fmaf(u, fmaf(u, -0.0066134277f, 0.0212747076f), -0.0538934189f), 0.13332902f), -0.333333242f), 1.f);
-        s[w][r] = x * p;
-      }
+    all([](float x) { return tanh_small<T>(x); });
+  } else if constexpr (sizeof(T) == 4) {
+    all([](float x) { return tanhf(x); });
   } else {
-#pragma unroll
-    for (int w = 0; w < N; ++w)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const float x = s[w][r];
-        if constexpr (sizeof(T) == 4) s[w][r] = tanhf(x);
-        else s[w][r] = 1.f - 2.f * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(2.f * LOG2E * x));
-      }
+    auto far = [](float x) { return 1.f - 2.f * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(2.f * LOG2E * x)); };
+    if (cap <= 64.f) all(far);
+    else all([&](float x) { return fabsf(x) <= 0.5f ? tanh_small<T>(x) : far(x); });
   }
 }
 

@@ -298,7 +298,7 @@ __global__ __launch_bounds__(NW * RG * 64, sizeof(T) == 2 && (DP == 64 || RG == 
       const bool caus = a.causal && p0 + 1 < kw1 && kw1 > pre;
       float mul = a.scale2;
       if (a.cap > 0.f) {
-        tanh_all<T, MT>(s, a.icap);
+        tanh_all<T, MT>(s, a.icap, a.cap);
         mul = a.cap2;
 #pragma unroll
         for (int j = 0; j < MT; ++j)
@@ -543,7 +543,7 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 ? 2 : 1) void attn_dq_kerne
       R::template times2<KT>(kt, vt, qf, gf, s, dp, lane);
       float mul = a.scale2;
       if (a.cap > 0.f) {
-        tanh_all<T, KT>(s, a.icap);
+        tanh_all<T, KT>(s, a.icap, a.cap);
         mul = a.cap2;
 #pragma unroll
         for (int j = 0; j < KT; ++j)

@@ -238,7 +238,7 @@ __global__ __launch_bounds__(NW * 64, DP == 128 && sizeof(T) == 4 ? 1 : 2) void 
       if constexpr (PAGED) gaps = BN == 32 ? (uint32_t)seen != ~0u : seen != ~0ull;
       float mul = a.scale2;
       if (a.cap > 0.f) {
-        tanh_all<T, KT>(s, a.icap);
+        tanh_all<T, KT>(s, a.icap, a.cap);
         mul = a.cap2;
       }
       if (a.slopes || mul <= 0.f) {
