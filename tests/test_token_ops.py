@@ -1415,3 +1415,29 @@ def test_attention_caps_that_scores_reach(dt, cap):
     """Scores of up to a few caps, under the cap where a 16-bit tanh changes its form and over it."""
     q, k, v = (randn(2, s, 2, 64, dtype=dt, seed=i) for i, s in enumerate((70, 150, 150)))
     check_attention(q, k, v, randn(2, 70, 2, 64, dtype=dt, seed=5), scale=cap / 8, softcap=cap)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("B,Sq,Sk,D", [(1, 3, 9000, 64), (2, 70, 100, 64), (2, 70, 100, 128), (70, 200, 300, 64), (40, 300, 300, 104)])
+@pytest.mark.parametrize("what", ["key", "query"])
+def test_gradients_that_depend_on_a_number_that_is_none_are_none(dt, B, Sq, Sk, D, what):
+    """A key that is not a number makes the softmax of every query of its sequence so: no gradient of them comes out finite.
+    A query: no gradient of its sequence's keys; its neighbours' stay as they are."""
+    q, k, v = (randn(B, s, 2, D, dtype=dt, seed=i) for i, s in enumerate((Sq, Sk, Sk)))
+    do = randn(B, Sq, 2, D, dtype=dt, seed=5)
+    def grads():
+        leaves = [t.detach().requires_grad_(True) for t in (q, k, v)]
+        return torch.autograd.grad(T.attention(*leaves), leaves, do)
+    want = grads()
+    (k if what == "key" else q)[0, 1, 1, 3] = float("nan")
+    got = grads()
+    for n, a, b in zip(("dq", "dk", "dv"), got, want):
+        if n == "dq" and what == "query":
+            assert not a[0, 1, 1].isfinite().any()
+            a, b = a.clone(), b.clone()
+            a[0, 1, 1] = b[0, 1, 1] = 0
+            assert torch.equal(a, b)
+        else:
+            assert not a[0, :, 1].isfinite().any(), n
+            assert torch.equal(a[:, :, 0], b[:, :, 0]) and torch.equal(a[1:], b[1:]), n

@@ -438,6 +438,11 @@ TURTLE_DEV Row row_of(const Args& a, int b, int hk, int m, int off, int nq) {
   return r;
 }
 
+// A row's softmax sum (log2) as the backward takes it, where p = 2^(s - sum): infinity for a row that sees nothing, so all
+// its p are 0; where the sum is not a number the least value, so the p of keys it sees are infinite or not a number as
+// all that depends on them has to be, and those of hidden ones (s = -infinity) still 0.
+TURTLE_DEV float kept_sum(float lse) { return lse == lse ? lse : -3.402823466e38f; }
+
 // tanh of the scores in place, for the cap. While every |x| of the wave is at most 1/2 - scores within half the cap -
 // an odd polynomial (least-maximum fit of tanh(x) / x in x^2: relative error 5.5e-7 for 16-bit inputs, 3.3e-9 for
 // fp32, to which fp32 arithmetic adds 9e-8): 5 instructions where the exponential form takes two of the slow ones besides.

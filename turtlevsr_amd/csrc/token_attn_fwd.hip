@@ -357,7 +357,7 @@ __global__ __launch_bounds__(NW * 64, DP == 128 && sizeof(T) == 4 ? 1 : 2) void 
   const int64_t pi = ((int64_t)sp * a.B * a.Hk + bh) * a.M + mrow;
   const int64_t oi = (((int64_t)b * a.Sq + qi) * a.Hq + hk * a.G + qg) * a.D;
   if (first && a.nsplit > 1) a.plse[pi] = lse;
-  if (first && a.nsplit <= 1 && a.lse) a.lse[(int64_t)bh * a.M + mrow] = l > 0.f ? lse : INFINITY;
+  if (first && a.nsplit <= 1 && a.lse) a.lse[(int64_t)bh * a.M + mrow] = kept_sum(lse);
 #pragma unroll
   for (int dt = 0; dt < DT; ++dt) {
     if (WK && dt % NW != wave) continue;
@@ -427,7 +427,7 @@ __global__ __launch_bounds__(256) void attn_join_kernel(Args a) {
   const int64_t oi = ((b * a.Sq + i) * a.Hq + hk * a.G + g) * a.D + d;
   Rows<T, 64>::put4(reinterpret_cast<T*>(a.o) + oi, v);
   if (a.olo) Rows<T, 64>::put4(reinterpret_cast<T*>(a.olo) + oi, lo);
-  if (a.lse && d == 0) a.lse[r] = l > 0.f ? mx + log2f(l) : INFINITY;
+  if (a.lse && d == 0) a.lse[r] = kept_sum(l == 0.f ? INFINITY : mx + log2f(l));
 }
 
 struct Plan { int kind, nsplit; int64_t mtiles; };      // kind: 0 waves split the keys, 1 two waves, 2 four waves
