@@ -73,7 +73,7 @@ typedef struct {
   void* o;            /* dense [B][Sq][Hq][D] */
   void* o_lo;         /* training: o's rounding remainder, as o (fp32: NULL), or NULL */
   float* lse;         /* training: [B][Hk][Sq * Hq / Hk] in log2 units, or NULL */
-  void* ranges;       /* documents: scratch of turtle_token_attn_ranges bytes, kept for the backward */
+  void* ranges;       /* documents: scratch of turtle_token_attn_ranges bytes, kept for the backward (which writes marks there) */
   void* ws;           /* scratch of turtle_token_attn_workspace bytes (NULL when that is 0) */
   size_t ws_bytes;
 } turtle_token_attn_args;

@@ -1441,3 +1441,26 @@ def test_gradients_that_depend_on_a_number_that_is_none_are_none(dt, B, Sq, Sk, 
         else:
             assert not a[0, :, 1].isfinite().any(), n
             assert torch.equal(a[:, :, 0], b[:, :, 0]) and torch.equal(a[1:], b[1:]), n
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("B,Sq,Sk,Hq,Hk,D", [(2, 150, 333, 4, 2, 64), (1, 60, 90, 2, 1, 128), (40, 300, 300, 6, 2, 64), (24, 261, 300, 6, 2, 104), (1, 3000, 40, 2, 1, 40)])
+@pytest.mark.parametrize("causal", [False, True])
+def test_queries_that_see_nothing_pass_no_gradient_whatever_they_hold(dt, B, Sq, Sk, Hq, Hk, D, causal):
+    """Queries of documents that no key has, or (causal, documents out of order) has later only: their rows and the gradients
+    that arrive there hold not-a-numbers and infinities, and nothing of them comes out."""
+    q, k, v = (randn(B, s, h, D, dtype=dt, seed=i) for i, (s, h) in enumerate(((Sq, Hq), (Sk, Hk), (Sk, Hk))))
+    do = randn(B, Sq, Hq, D, dtype=dt, seed=9)
+    g = torch.Generator().manual_seed(Sq)
+    qd = (torch.arange(Sq)[None] * -(-Sk // 40) // Sq).repeat(B, 1)
+    qd[torch.rand(B, Sq, generator=g) < 0.1] = 1000            # single ones, a whole tile, a last piece
+    qd[:, 64:130], qd[:, -5:] = 1001, 1002
+    kd = (torch.arange(Sk)[None] // 40).repeat(B, 1)
+    if causal:
+        kd = kd.flip(1)
+    qd, kd = qd.to(DEV), kd.to(DEV)
+    blind = ~visible_ref(B, Sq, Sk, causal, None, qd, kd).any(2)
+    assert blind.any() and not blind.all()
+    q[blind], do[blind] = float("nan"), float("inf")
+    check_attention(q, k, v, do, q_doc=qd, k_doc=kd, causal=causal)

@@ -479,7 +479,8 @@ TURTLE_DEV void tanh_all(f32x16 (&s)[N], float icap, float cap) {
   }
 }
 
-// document range of tokens [t0, t1): {lo, hi, 1 if all are the same valid number, 1 if any is invalid}
+// document range of tokens [t0, t1): {lo, hi, 1 if all are the same valid number, 1 if any is invalid (backward: or any
+// query sees nothing)}
 TURTLE_DEV int4 doc_range(const int4* ranges, int nr, int t0, int t1) {
   int4 x = make_int4(0x7fffffff, -1, 1, 0);
   for (int r = t0 / RT; r <= (t1 - 1) / RT && r < nr; ++r) {

@@ -16,7 +16,9 @@ namespace {
 
 __device__ const float g_row_pad[2] = {INFINITY, 0.f};   // softmax sum and delta of a row that is not there
 
-// -delta [B][Hk][M], delta = do . (o + o_lo); 8 lanes a row, 16 bytes a lane and step
+// -delta [B][Hk][M], delta = do . (o + o_lo); 8 lanes a row, 16 bytes a lane and step. A row that sees nothing may hold
+// anything, in q and in do: its delta is 0, and with documents its tile is marked as one with holes, so that dk's and dv's
+// kernel asks for each row (every backward writes the same mark).
 template <typename T>
 __global__ __launch_bounds__(256) void attn_delta_kernel(Args a, float* delta) {
   constexpr int V = 16 / sizeof(T);
@@ -26,9 +28,11 @@ __global__ __launch_bounds__(256) void attn_delta_kernel(Args a, float* delta) {
   float s = 0.f;
   if (u < n) {
     const int64_t b = u / ((int64_t)a.Sq * a.Hq), j = u - b * a.Sq * a.Hq, i = j / a.Hq, hq = j - i * a.Hq;
+    const int64_t at = ((b * a.Hk + hq / a.G) * a.Sq + i) * a.G + hq % a.G;
     const T* g = reinterpret_cast<const T*>(a.dout) + b * a.gb + i * a.gs + hq * a.gh;
     const T* o = reinterpret_cast<const T*>(a.o) + u * a.D;
     const T* lo = a.olo ? reinterpret_cast<const T*>(a.olo) + u * a.D : nullptr;
+    const bool blind = a.lse[at] == INFINITY;
     typedef T tv __attribute__((ext_vector_type(V)));
     for (int d = ln * V; d < a.D; d += 8 * V) {
       const tv x = *reinterpret_cast<const tv*>(g + d), y = *reinterpret_cast<const tv*>(o + d);
@@ -38,7 +42,10 @@ __global__ __launch_bounds__(256) void attn_delta_kernel(Args a, float* delta) {
       for (int e = 0; e < V; ++e) s = fmaf((float)x[e], (float)y[e] + (float)z[e], s);
     }
     s += __shfl_xor(s, 1, 64); s += __shfl_xor(s, 2, 64); s += __shfl_xor(s, 4, 64);
-    if (ln == 0) delta[((b * a.Hk + hq / a.G) * a.Sq + i) * a.G + hq % a.G] = -s;
+    if (ln == 0) {
+      delta[at] = blind ? 0.f : -s;
+      if (blind && a.qdoc) const_cast<int4*>(a.qr)[b * a.nqr + i / RT].w = 1;
+    }
   }
 }
 
@@ -227,7 +234,7 @@ __global__ __launch_bounds__(NW * RG * 64, sizeof(T) == 2 && (DP == 64 || RG == 
       R::template load2<BM, C::LT>(dst, dst + C::TILE, ltid, a.D, [&](int r, const char*& p0, const char*& p1) {
         const int m = m0 + r, i = token_of(a, m), g = m - i * a.G;
         // rows that see nothing may hold anything: they are not read
-        if (m >= a.M || (a.causal && i + off < 0 && pre <= 0) || (holes && a.qdoc[(int64_t)b * a.Sq + i] < 0)) return;
+        if (m >= a.M || (a.causal && i + off < 0 && pre <= 0) || (holes && sums[m] == INFINITY)) return;
         p0 = qbase + ((int64_t)i * a.qs + (int64_t)g * a.qh) * R::ES;
         p1 = gbase + ((int64_t)i * a.gs + (int64_t)g * a.gh) * R::ES;
       });
