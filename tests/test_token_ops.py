@@ -1464,3 +1464,14 @@ def test_queries_that_see_nothing_pass_no_gradient_whatever_they_hold(dt, B, Sq,
     assert blind.any() and not blind.all()
     q[blind], do[blind] = float("nan"), float("inf")
     check_attention(q, k, v, do, q_doc=qd, k_doc=kd, causal=causal)
+
+
+def test_the_caller_s_decimal_context_does_not_matter():
+    import decimal
+    T._axes_table.cache_clear()
+    want = T._axes_table((16, 24), 10000.0)
+    T._axes_table.cache_clear()
+    with decimal.localcontext() as c:
+        c.prec, c.rounding = 3, decimal.ROUND_UP
+        c.traps[decimal.Inexact] = c.traps[decimal.FloatOperation] = True
+        assert T._axes_table((16, 24), 10000.0) == want

@@ -191,8 +191,7 @@ def _axes_table(axes, base: float):
     mod 2^64 is the angle but for |pos| 2^-65 revolutions (a double has 53 bits: at 2^50 it would be arbitrary to 0.03)."""
     freq, axis = [0] * 64, [0] * 64
     i = 0
-    with decimal.localcontext() as c:
-        c.prec = 50
+    with decimal.localcontext(decimal.Context(prec=50)):
         ln = decimal.Decimal(base).ln()
         for a, d in enumerate(axes):
             for j in range(0, d, 2):
