@@ -1194,7 +1194,7 @@ def _fp16_grads(q, k, v, do, scale):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("D", [64, 128, 40])
-@pytest.mark.parametrize("n,Sq,Sk", [(1, 96, 4096), (1, 4096, 96), (2, 700, 3000), (24, 1200, 1100)])
+@pytest.mark.parametrize("n,Sq,Sk", [(1, 96, 4096), (1, 4096, 96), (2, 700, 3000), (24, 1200, 1100), (32, 900, 1000)])
 @pytest.mark.parametrize("kind", ["1e-3", "1e-4", "rows", "keys"])
 def test_attention_fp16_gradients_of_any_size(D, n, Sq, Sk, kind):
     """Gradients far from one: small ones over many keys, rows of 2^-12 to 2^9 in one call, growing along the walks, and
