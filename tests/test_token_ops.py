@@ -1475,3 +1475,60 @@ def test_the_caller_s_decimal_context_does_not_matter():
         c.prec, c.rounding = 3, decimal.ROUND_UP
         c.traps[decimal.Inexact] = c.traps[decimal.FloatOperation] = True
         assert T._axes_table((16, 24), 10000.0) == want
+
+
+# -------------------------------------------------------------------------------------------------
+# combinations
+# -------------------------------------------------------------------------------------------------
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("B,Sq,Sk,Hq,Hk,D", [(2, 90, 130, 4, 2, 64), (1, 300, 200, 3, 1, 128), (45, 300, 290, 6, 2, 40), (1, 5, 2500, 8, 2, 96), (1, 2500, 70, 2, 2, 64)])
+def test_attention_all_rules_at_once(dt, B, Sq, Sk, Hq, Hk, D):
+    """Documents in any order, causal, a prefix for each sequence, a bias and a cap, a scale below zero."""
+    q, k, v = (randn(B, s, h, D, dtype=dt, seed=i) for i, (s, h) in enumerate(((Sq, Hq), (Sk, Hk), (Sk, Hk))))
+    g = torch.Generator().manual_seed(Sq)
+    n = max(Sq, Sk)
+    doc = torch.randint(0, 4, (B, n // 20 + 1), generator=g).repeat_interleave(20, 1)[:, :n]
+    doc[torch.rand(B, n, generator=g) < 0.05] = -3
+    check_attention(q, k, v, randn(B, Sq, Hq, D, dtype=dt, seed=9), causal=True, prefix=torch.tensor([(7 * b) % Sk for b in range(B)], device=DEV),
+                    q_doc=doc[:, :Sq].to(DEV), k_doc=doc[:, -Sk:].to(DEV), slopes=torch.linspace(-0.02, 0.2, Hq, device=DEV), softcap=4.0, scale=-0.2)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("G,Sq,D", [(40, 1, 64), (96, 1, 128), (33, 7, 40), (64, 3, 64)])
+def test_paged_many_heads_share_a_key(dt, G, Sq, D):
+    lens = [700, 33, Sq]
+    kp, vp, table, k, v = _pages(3, lens, 24, 1, D, dt, seed=G)
+    check_paged(randn(3, Sq, G, D, dtype=dt, seed=6), kp, vp, table, lens, k, v, slopes=torch.linspace(0, 0.3, G, device=DEV))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("Sq", [1, 70])
+@pytest.mark.parametrize("causal", [True, False])
+def test_paged_lengths_at_the_ends_of_their_range(Sq, causal):
+    """More keys than 32 bits count past the table's room, fewer than none, more queries than the chunk has or than keys,
+    fewer than none: keys are cut to [0, room], queries to [0, Sq], a query's place is kv_lens - queries + i."""
+    most, least = 2 ** 31 - 1, -2 ** 31
+    lens, ql = [most, least, 64, 5, 64, -1, most], [Sq, Sq, most, Sq, least, most, least]
+    page = 16
+    kp, vp, table, k, v = _pages(7, [64] * 7, page, 2, 64, torch.bfloat16, seed=1)
+    q = randn(7, Sq, 4, 64, dtype=torch.bfloat16, seed=2)
+    check_paged(q, kp, vp, table, lens, k, v, ql, causal=causal)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", DTYPES)
+def test_qk_norm_rope_with_more_key_heads(dt):
+    """Heads of k past q's: as k's own call gives them; gradients too."""
+    q, k = randn(2, 31, 1, 40, dtype=dt, seed=1), randn(2, 31, 5, 40, dtype=dt, seed=2)
+    pos, w = _grid(31, 2), torch.linspace(0.5, 2, 40, device=DEV)
+    g = randn(2, 31, 5, 40, dtype=dt, seed=3)
+    a, b = k.detach().requires_grad_(True), k.detach().requires_grad_(True)
+    wa, wb = w.clone().requires_grad_(True), w.clone().requires_grad_(True)
+    x, y = T.qk_norm_rope(q, a, pos, None, wa, (16, 8))[1], T.qk_norm_rope(b, k, pos, wb, None, (16, 8))[0]
+    assert torch.equal(x, y)
+    da, dwa = torch.autograd.grad(x, (a, wa), g)
+    db, dwb = torch.autograd.grad(y, (b, wb), g)
+    assert torch.equal(da, db) and torch.equal(dwa, dwb)

@@ -530,9 +530,10 @@ def paged_attention(q, k_pages, v_pages, block_table, kv_lens, *, q_lens=None, s
     int32 [B, max pages]: key j of sequence b is row j % page of page block_table[b, j // page]; kv_lens int32 [B]:
     keys of every sequence, the chunk's own - written to the cache before the call - included; q_lens int32 [B] or
     None (all Sq): queries of every sequence. Query i stands at place kv_lens - q_lens + i; rows past q_lens give
-    zeros. scale, softcap, slopes and causal as in ``attention``. Lengths past the table's room are cut to it; keys
-    of a page number outside the pools are seen by nobody; what the pools hold past a sequence's length is never
-    read. Lengths and tables stay on the device, so a captured call follows their contents. No gradient."""
+    zeros. scale, softcap, slopes and causal as in ``attention``. Lengths past the table's room are cut to it (a
+    query's place goes by kv_lens as it is), those below zero count as zero; keys of a page number outside the pools are
+    seen by nobody; what the pools hold past a sequence's length is never read. Lengths and
+    tables stay on the device, so a captured call follows their contents. No gradient."""
     _check_qkv(q, k_pages, v_pages)
     if torch.is_grad_enabled() and (q.requires_grad or k_pages.requires_grad or v_pages.requires_grad):
         raise RuntimeError("paged_attention has no gradient: call it under torch.no_grad()")
