@@ -5,10 +5,11 @@
 // summed through memory. A wave's step is a chain - S and dP, the rules, the exponential, two products with the results -
 // so with two waves on a SIMD what counts is the chain's waits: LDS reads started ahead of their products (dq at 128
 // channels 400 -> 365 us, dk and dv at 64 channels 212 -> 188), masks without branches (packed documents 850 -> 690).
-// Measured, bf16: 2 x 5120 tokens causal with prefix 2048, 8 heads of 64 channels: dk, dv 180 us (4 products a pair, 690
-// TF/s), dq 118 us (3 products, 790 TF/s), delta 8 us; 7 documents in 8192 tokens, 16 heads on 4 of 128 channels: dk, dv
-// 534 us and 25 for their sums, dq 354 us, delta 17 us - unsplit, dk and dv took 639: the block over the border of the longest
-// documents walks 2.5 times the mean block's way. fp32, 2 x 333 on 517 tokens, 6 heads on 3 of 48 channels: 34, 22, 4 us.
+// Measured, bf16: 2 x 5120 tokens causal with prefix 2048, 8 heads of 64 channels: dk, dv 182 us (4 products a pair, 686
+// TF/s), dq 125 us (3 products, 750 TF/s), delta 9 us; 7 documents in 8192 tokens, 16 heads on 4 of 128 channels: dk, dv
+// 495 us and 25 for their sums, dq 359 us, delta 17 us (whole walks instead of split ones take 20 % more: the block over the
+// border of the longest documents walks 2.5 times the mean block's way). fp32, 2 x 333 on 517 tokens, 6 heads on 3 of 48
+// channels: 33, 22, 5 us.
 #include "token_attn.h"
 
 namespace turtle {

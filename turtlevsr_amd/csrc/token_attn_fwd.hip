@@ -8,9 +8,9 @@
 // The first two have matrix instructions to spare and multiply p in two terms (TWO): with few keys, p's rounding
 // would be as large an error as the result's own.
 //
-// Measured: 32640 x 32640 tokens, 8 heads of 64 channels, bf16, 2490 - 2600 us (840 - 875 TF/s; at 64 rows a wave instead of 32, no
-// faster: 2 x 16 more registers hold off one of three waves of a SIMD); causal with prefix 2048, 2 x 5120 tokens, 110 us
-// (566 TF/s); 510 windows of 64 tokens, 4 heads, 20 us (3.3 TB/s; the start of its one-tile blocks); one token on 16
+// Measured: 32640 x 32640 tokens, 8 heads of 64 channels, bf16, 2450 - 2700 us (810 - 890 TF/s; at 64 rows a wave instead of 32, no
+// faster: 2 x 16 more registers hold off one of three waves of a SIMD); causal with prefix 2048, 2 x 5120 tokens, 108 us
+// (575 TF/s); 510 windows of 64 tokens, 4 heads, 19 us (3.5 TB/s; the start of its one-tile blocks); one token on 16
 // histories of up to 16384 keys, 16 heads on 4 of 128 channels, 80 + 5 us for the join (4.5 TB/s while it reads); 256
 // tokens on 4 histories of 5040, fp16, 8 heads, 32 + 6 us.
 #include "token_attn.h"
