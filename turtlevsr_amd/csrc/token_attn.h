@@ -30,6 +30,8 @@
 // bits; dS times a power of two of the row's or key's own), results at the end; scores, maxima, sums and accumulators are
 // fp32. The 16-bit rounding of p and dS is what separates the 16-bit results from the rounded exact ones: relative error of
 // all values 2.4e-3 in bf16 and 3.0e-4 in fp16, the rounding of the result alone being 1.7e-3 and 2.1e-4.
+// Where p has one term, the row's sum (in fp32) is of the rounded p, so that o's weights add up to one; the backward's p
+// takes it too and is off, all of a row alike, by half a step at most (bf16: 1.5e-3 in rows of a few keys, 3e-4 at 1500).
 //
 // Bound: the matrix products where rows are many (a large bf16 product reaches 1188 TF/s on the card, fp32 153), HBM
 // where they are few (a large copy reaches 4.9 TB/s). Beside the products every score costs an exponential (10 clocks of

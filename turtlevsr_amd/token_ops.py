@@ -490,10 +490,11 @@ def attention(q, k, v, *, scale=None, softcap: float = 0.0, slopes=None, causal:
     * q_doc [B, Sq], k_doc [B, Sk] (k_doc None: q_doc, with Sq == Sk): integers below 2^31; a query sees only keys
       of its own document. Negative: padding, which sees nothing and is seen by nobody - its rows may hold anything.
 
-    A query that sees nothing gives zeros and passes no gradient, whatever it and its gradient hold. Elsewhere what is
-    not finite makes the results that depend on it infinite or not a number, and can reach further within its tile (32 to
-    64 tokens, those it is hidden from included): a key or value - of any document but padding - the results of
-    queries and their dq, a query or its gradient the dk and dv of keys; a query's own result stays in its row. Returns a dense
+    A query that sees nothing gives zeros and passes no gradient, whatever it and its gradient hold (so does one whose
+    every visible score is minus infinity). Elsewhere what is not finite makes the results that depend on it infinite or
+    not a number, and can reach further within its tile (32 to 64 tokens, those it is hidden from included): a key or
+    value - of any document but padding - the results of queries and their dq, a query or its gradient the dk and dv of
+    keys; a query's own result stays in its row. Returns a dense
     [B, Sq, Hq, D] of q's type."""
     _check_qkv(q, k, v)
     B, Sq, Hq, D = q.shape
