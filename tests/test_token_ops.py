@@ -1532,3 +1532,42 @@ def test_qk_norm_rope_with_more_key_heads(dt):
     da, dwa = torch.autograd.grad(x, (a, wa), g)
     db, dwb = torch.autograd.grad(y, (b, wb), g)
     assert torch.equal(da, db) and torch.equal(dwa, dwb)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D", [64, 128])
+def test_training_step_with_documents_in_a_graph(D):
+    """Forward and backward captured, replayed with other documents: queries that see nothing in one replay (and hold
+    not-a-numbers there) are ordinary ones in the next."""
+    leaves = [randn(2, 333, h, D, dtype=torch.float16, seed=i).requires_grad_(True) for i, h in enumerate((4, 2, 2))]
+    do = randn(2, 333, 4, D, dtype=torch.float16, seed=5)
+    qd, kd = torch.zeros(2, 333, dtype=torch.int32, device=DEV), torch.zeros(2, 333, dtype=torch.int32, device=DEV)
+
+    def step():
+        o = T.attention(*leaves, q_doc=qd, k_doc=kd, causal=True)
+        return (o.detach(),) + torch.autograd.grad(o, leaves, do)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = step()
+    for n in range(5):
+        with torch.no_grad():
+            for i, t in enumerate(leaves):
+                t.copy_(randn(*t.shape, dtype=t.dtype, seed=100 + 10 * n + i))
+            do.copy_(randn(*do.shape, dtype=do.dtype, seed=100 + 10 * n + 7))
+            kd.copy_((torch.arange(333, device=DEV) // (20 + 30 * n))[None].expand(2, -1))
+            qd.copy_(kd)
+            qd[:, 40 * n:40 * n + 70] = 500
+            if n % 2:
+                leaves[0][:, 40 * n:40 * n + 70], do[:, 40 * n:40 * n + 70] = float("nan"), float("inf")
+        g.replay()
+        got = [t.clone() for t in out]
+        torch.cuda.synchronize()
+        assert all(torch.isfinite(t).all() for t in got)
+        assert not got[0][:, 40 * n:40 * n + 70].any() and not got[1][:, 40 * n:40 * n + 70].any()
+        assert all(torch.equal(a, b) for a, b in zip(got, step()))
+    check_attention(*(t.detach() for t in leaves), do, q_doc=qd, k_doc=kd, causal=True)
